@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-enum { LOLLM_BF16 = 0, LOLLM_F32 = 1 };
+enum { LOLLM_BF16 = 0, LOLLM_F32 = 1, LOLLM_F8 = 2 /* OCP e4m3 */ };
 enum { LOLLM_OK = 0, LOLLM_EINVAL = 1, LOLLM_EUNSUPPORTED = 2, LOLLM_EHIP_BASE = 1000 };
 
 const char* lollm_strerror(int code);
@@ -93,6 +93,29 @@ int lollm_attn_verify(const void* q, const void* k_cache, const void* v_cache,
                       long long workspace_bytes, int B, int T, int Hq, int Hkv, int D,
                       int max_len, long long seq_stride, long long head_stride, int grid,
                       float scale, void* stream);
+
+/* The same attention over a paged cache.  Key j of sequence b is row j % page of page
+ * table[b * table_stride + j / page]; an entry < 0 or >= n_pages is unmapped and its keys do
+ * not exist (a query that sees no key gets zeros).  Nothing of a row past kv_len or in an
+ * unmapped page is used, whatever it holds.  No reference counterpart (kv.py:20-58 holds one
+ * contiguous tensor per layer).
+ *
+ *   k_pages, v_pages  (n_pages, Hkv, page, D), kv_dtype LOLLM_BF16 or LOLLM_F8: e4m3 codes,
+ *            their value the code times the page's scale
+ *   k_scale, v_scale  (n_pages, Hkv) fp32 powers of two (8-bit pages; else NULL)
+ *   table    (B, table_width) int32, rows table_stride apart; it holds table_width * page keys
+ *   gate     element d of (token bt, head h) at gate + bt * gate_row + h * gate_head + d (so it
+ *            can be read where the fused projection wrote it), or NULL
+ *   kv_len, q, out, grid, scale  as lollm_attn_verify, which says when a call with grid 0 takes
+ *            query tiles instead of the split-K; the workspace is required either way
+ * Supported: D == 256, page 16, 32, 64 or 128, Hq / Hkv <= 32, B <= 512. */
+long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int grid);
+int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
+                     const float* v_scale, int kv_dtype, const int32_t* table, long long table_stride,
+                     int table_width, int n_pages, int page, const int32_t* kv_len, const void* gate,
+                     long long gate_row, int gate_head, void* out, void* workspace,
+                     long long workspace_bytes, int B, int T, int Hq, int Hkv, int D, int grid,
+                     float scale, void* stream);
 
 /* Speculative-sampling acceptance over the full vocabulary for B sequences with k
  * drafts each, and the residual / bonus draw.
@@ -224,6 +247,27 @@ int lollm_attn_prologue(const void* qkv, const void* q_norm_w, const void* k_nor
                         int rope_per_token, int B, int T, int Hq,
                         int Hkv, int D, int rotary_dim, float eps, void* q_out, void* gate_out,
                         void* k_cache, void* v_cache, int max_len, void* stream);
+
+/* lollm_attn_prologue over a paged cache (lollm_attn_paged's pools and table): q (B, T, Hq, D)
+ * after QK-norm and RoPE, and k (normed, roped) / v into row (lengths[b] + t) % page of page
+ * table[b][(lengths[b] + t) / page]; the gate stays in qkv, for lollm_attn_paged to read there
+ * (gate_row the row of qkv, gate_head 2 D, gate = qkv + D).  Rows before 0, past the table or in
+ * unmapped pages are not stored.  Computed in fp32, angles in fp64, and rounded once, where
+ * lollm_attn_prologue rounds at every tensor of the reference.
+ *
+ * 8-bit pages: a page's scale becomes the least power of two s with amax <= 448 s over the
+ * finite values of its new rows (K and V each, per KV head; at least 2^-64), or stays the larger
+ * one that it has while it keeps rows (the call's first row is not the page's first); kept rows
+ * are rounded to a larger scale again, which changes subnormal codes only.  Values that are not
+ * finite become NaN.  k_scale and v_scale are read and written.
+ * A page written by a call may be in one sequence's table only.  inv_freq, rope_pos and
+ * rope_per_token as in lollm_attn_prologue.  Supported: D == 256, page 16, 32, 64 or 128. */
+int lollm_attn_append(const void* qkv, const void* q_norm_w, const void* k_norm_w, const float* inv_freq,
+                      const int32_t* lengths, const int32_t* rope_pos, int rope_per_token,
+                      const int32_t* table, long long table_stride, int table_width, int n_pages, int page,
+                      int kv_dtype, int B, int T, int Hq, int Hkv, int D, int rotary_dim, float eps,
+                      void* q_out, void* k_pages, void* v_pages, float* k_scale, float* v_scale,
+                      void* stream);
 
 /* Gated attention of one new token per sequence over a short cache, prologue fused
  * (GatedAttention.forward, blocks.py:208-235, for the MTP head's draft block with the

@@ -6,12 +6,15 @@
 namespace lollm {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void_t;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
 
 constexpr int AT_D = 256;            // head dim
 constexpr int AT_ROWS = 32;          // MFMA rows per pair (n_rep x QB)
@@ -21,17 +24,109 @@ struct AttnArgs {
   const uint16_t* kc;      // K cache
   const uint16_t* vc;      // V cache
   const int32_t* kv_len;   // (B) keys per sequence, the T new ones included
-  const uint16_t* gate;    // (B, T, Hq * D) or null
+  const uint16_t* gate;    // (B, T, Hq, D), strided, or null
   uint16_t* out;           // (B, T, Hq * D)
   float* ws;               // partials: (nw + pairs) x AT_PART, then the combine table
   long long seq_stride, head_stride;  // cache strides in elements
   int B, T, Hq, Hkv, n_rep, QB, qblocks, max_len, nw;
   float cl2;               // scale * log2(e)
+  // strides of gate in elements: of a token, of a head (Hq * D and D where it is dense)
+  long long gate_row;
+  int gate_head;
 };
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ float sigmoidf_(float x) { return 1.f / (1.f + __expf(-x)); }
+
+// A pair of fp32 weights as bf16 hi and lo, x = hi + lo to 16 bits.  hi is cut and not rounded, so
+// that lo is never negative, and lo is at least 2^-126 where hi is not 0: an infinite V then takes
+// the sum of both products to infinity as a single product does, not to infinity - infinity or
+// 0 x infinity.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void at_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+  hi = __builtin_amdgcn_perm(yb, xb, 0x07060302u);   // the upper halves
+  const bf16x2 l = {(__bf16)(x - __uint_as_float(xb & 0xffff0000u)), (__bf16)(y - __uint_as_float(yb & 0xffff0000u))};
+  const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, hi), u16x2{0x0080, 0x0080});
+  lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, l), least));
+}
+
+constexpr int AW_WAVES = 4;
+constexpr int AW_THREADS = 64 * AW_WAVES;
+constexpr int AT_BLOCK = 128;        // keys per block
+constexpr int AT_MAXB = 512;         // sequences per call (prefix table in LDS)
+constexpr int AT_PART = 2 * AT_ROWS + AT_ROWS * AT_D;  // floats per partial
+
+// Balanced split-K over 128-key blocks: helpers of the kernels that deal the blocks of all pairs
+// out to a fixed grid of 4-wave workgroups.
+__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
+  return min(max(a.kv_len[b], 0), a.max_len);  // never past the cache capacity
+}
+
+__device__ __forceinline__ int nblk_of(int L) { return (L + AT_BLOCK - 1) / AT_BLOCK; }
+
+// First unit of workgroup w and the workgroup that owns unit u, for U units dealt
+// out to nw workgroups in equal contiguous ranges: w owns [U w / nw, U (w+1) / nw).
+__device__ __forceinline__ long long unit_begin(long long U, int w, int nw) {
+  return U * w / nw;
+}
+__device__ __forceinline__ int unit_owner(long long U, long long u, int nw) {
+  return (int)(((u + 1) * nw - 1) / U);
+}
+
+// pre[b] = blocks of sequences 0..b-1 (pre[0] = 0), for b = 0..B, and len[b] = the
+// clamped key count of sequence b, built in LDS by the whole workgroup (so the main
+// loop never waits on a global load to address the next block).  Returns pre[B].
+__device__ __forceinline__ int build_prefix(const AttnArgs& a, int* pre, int* len, int* tmp) {
+  constexpr int WAVES = AW_WAVES;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int carry = 0;
+  if (tid == 0) pre[0] = 0;
+  for (int base = 0; base < a.B; base += AW_THREADS) {
+    const int b = base + tid;
+    const int Lb = b < a.B ? seq_len(a, b) : 0;
+    if (b < a.B) len[b] = Lb;
+    int v = nblk_of(Lb);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(v, d, 64);
+      if (lane >= d) v += o;
+    }
+    if (lane == 63) tmp[wave] = v;
+    __syncthreads();
+    int before = carry, all = carry;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) before += tmp[w];
+      all += tmp[w];
+    }
+    if (b < a.B) pre[b + 1] = before + v;
+    carry = all;
+    __syncthreads();
+  }
+  return carry;
+}
+
+// Workgroup barrier after this wave's LDS accesses complete; the compiler sees a memory
+// clobber (no LDS access moves across it) but no fence, so global loads and LDS DMA in
+// flight are not drained.
+__device__ __forceinline__ void aw_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// log2 of a cache page's rows (16, 32, 64 or 128), -1 for another size.
+inline int attn_page_shift(int page) {
+  for (int s = 4; s <= 7; ++s)
+    if (page == 1 << s) return s;
+  return -1;
+}
+
+// Merges the pieces of every pair (one per row), with the gate.
+int attn_combine_launch(const AttnArgs& a, hipStream_t st);
+// Sizes of a split-K call and its workspace; workgroups of the balanced grid (`grid` if positive,
+// else one per CU of the current device), -1 where the device is not known.
+int attn_geometry(int B, int T, int Hq, int Hkv, int D, int max_len, int* n_rep, int* QB, int* qblocks);
+long long attn_ws_bytes(long long nw, long long pairs);
+int attn_grid(int grid);
 
 // Row groups per wave of the long-call kernel (attn_prefill.hip) for this geometry on a device
 // with `cus` CUs, or 0 where the split-K kernels are the faster ones.

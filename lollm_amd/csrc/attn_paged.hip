@@ -1,0 +1,485 @@
+// Gated GQA attention over a paged KV cache, pages in bf16 or in 8 bits (gfx950).
+//
+// Math: as attn_verify.hip (offset-causal GQA, query i of the T new positions of sequence b at
+// position kv_len[b] - T + i, output o * sigmoid(gate)), with key j of sequence b in row
+// j % page of page table[b][j / page]: rows of D values, (n_pages, Hkv, page, D).  A key whose
+// page is unmapped (an entry < 0 or >= n_pages) does not exist.  8-bit pages hold e4m3 codes c
+// and one power-of-two scale s for each (page, KV head) of K and of V: the value is c s, which
+// bf16 holds exactly, so both kinds of page go through the same bf16 products.
+//
+// Work decomposition: attn_verify.hip's balanced split-K (128-key blocks of all (sequence, KV
+// head x query block) pairs dealt out evenly, one partial per workgroup and pair, the combine
+// kernel).  What differs is how a wave finds its rows.  Each of the four waves owns 32
+// consecutive keys of a block, which lie in one page, or in two pages of 16.  Every 62 blocks
+// each lane looks up one block of the range ahead -- its sequence and pair by binary search, its
+// page ids, its scales -- and the loop takes them with readlane two blocks before it needs them,
+// so no load of a page waits for a load of the table.
+//   K: 16 bytes a lane straight into the S MFMA A operand (64-bit addresses: a pool may pass
+//      4 GB).  Rows of unmapped pages read page 0 and are masked.
+//   V: LDS DMA through a descriptor of the page's valid rows; the others become zeros, so that
+//      nothing that an unmapped or unwritten row holds meets a weight of 0.
+//   8 bits: a lane's 16 bytes of K are two k-steps (Q's columns are read in the same order);
+//      V is read with the transposing 8-bit LDS read; both become bf16 with
+//      v_cvt_scalef32_pk_bf16_fp8, which applies the scale.
+// Weights enter the product with V as hi + lo bf16 (attn_prefill.hip): the kernel waits for
+// memory, and the second product costs it nothing.
+#include "attn_common.h"
+
+namespace lollm {
+
+struct PagedArgs {
+  AttnArgs a;                 // kc, vc: the pools
+  const int32_t* table;       // (B, table_stride)
+  const float* ks;            // (n_pages, Hkv) scales, 8-bit pages
+  const float* vs;
+  long long table_stride;
+  int n_pages, pshift;        // page = 1 << pshift
+};
+
+constexpr int PG_WKEYS = AT_BLOCK / AW_WAVES;   // 32 keys of each block per wave
+constexpr int PG_QROW = AT_D * 2 + 16;          // padded Q row in LDS
+constexpr int PG_OROW = AT_D / 2 + 4;           // padded floats per row of an O half-dump
+constexpr int PG_DUMP = AW_WAVES * AT_ROWS * PG_OROW * 4;
+
+template <bool F8>
+struct PagedSet {   // the V rows of a block in LDS
+  static constexpr int ROW = F8 ? AT_D : AT_D * 2;
+  // bf16: two rows (one DMA) + 64 bytes, so that the transposing reads of 8 rows touch every bank
+  // at most twice; 8 bits: four rows a DMA, the 16-byte chunk c of row r at c ^ (r % 16)
+  static constexpr int PAIR = F8 ? 2 * AT_D : 2 * AT_D * 2 + 64;
+  static constexpr int WAVE = PG_WKEYS / 2 * PAIR;
+  static constexpr int SET = AW_WAVES * WAVE;
+};
+
+// One block of a workgroup's range, uniform across the wave.
+struct PgUnit {
+  int b, ph, j, L;
+  int page[2];                // of the wave's keys 0..15 and 16..31, -1 unmapped or past the end
+  float ks[2], vs[2];
+};
+
+__device__ __forceinline__ bf16x8 pg_bf16(uint32_t w0, uint32_t w1, float scale) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
+  return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+template <bool F8>
+__global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) {
+  using Set = PagedSet<F8>;
+  const AttnArgs& a = p.a;
+  __shared__ __attribute__((aligned(16))) unsigned char vs0[Set::SET];   // V of even blocks
+  __shared__ __attribute__((aligned(16))) unsigned char vs1[Set::SET];   // V of odd blocks
+  __shared__ __attribute__((aligned(16))) unsigned char own_dump[F8 ? PG_DUMP : 16];
+  __shared__ __attribute__((aligned(16))) unsigned char qs[AT_ROWS * PG_QROW];   // Q of the pair
+  __shared__ float mx[AW_WAVES][32], lx[AW_WAVES][32];
+  __shared__ int pre[AT_MAXB + 1], len[AT_MAXB], tmp[AW_WAVES];
+  static_assert(F8 || PG_DUMP <= Set::SET, "the O dump fits a V set");
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, h = lane >> 5;
+  const int w = blockIdx.x;
+  const int PH = a.Hkv * a.qblocks;
+
+  const long long U = (long long)PH * build_prefix(a, pre, len, tmp);
+  {
+    const int npairs = a.B * PH;
+    int4* tab = reinterpret_cast<int4*>(a.ws + (size_t)(a.nw + npairs) * AT_PART);
+    for (int pr = w * AW_THREADS + tid; pr < npairs; pr += a.nw * AW_THREADS) {
+      const int pb = pr / PH, pph = pr % PH, pnb = pre[pb + 1] - pre[pb];
+      int wf = -1, wl = -1;
+      if (pnb > 0) {
+        const long long first = (long long)PH * pre[pb] + (long long)pph * pnb;
+        wf = unit_owner(U, first, a.nw);
+        wl = unit_owner(U, first + pnb - 1, a.nw);
+      }
+      tab[pr] = make_int4(wf, wl, (int)(uint32_t)U, (int)(uint32_t)(U >> 32));
+    }
+  }
+  const long long u0 = unit_begin(U, w, a.nw), u1 = unit_begin(U, w + 1, a.nw);
+  if (u0 >= u1) return;
+
+  // The lane's block of the 64 from tbase on.
+  long long tbase = u0;
+  int tb = 0, tph = 0, tj = 0, tL = 0, tp[2];
+  float tks[2] = {1.f, 1.f}, tvs[2] = {1.f, 1.f};
+  auto look_up = [&]() {
+    const long long u = min(tbase + lane, u1 - 1);
+    int lo = 0, hi = a.B - 1;   // the last sequence that begins at or before u: not an empty one
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((long long)PH * pre[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    const int nb = pre[lo + 1] - pre[lo];
+    const long long r = u - (long long)PH * pre[lo];
+    tb = lo;
+    tph = (int)(r / nb);
+    tj = (int)(r - (long long)tph * nb);
+    tL = len[lo];
+    const int kvh = tph / a.qblocks;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key = tj * AT_BLOCK + PG_WKEYS * wave + 16 * g;
+      const bool in = key >= 0 && key < tL;   // (a table of 2^31 rows: a last block's keys may wrap)
+      const int id = in ? p.table[(long long)lo * p.table_stride + (key >> p.pshift)] : -1;
+      tp[g] = id >= 0 && id < p.n_pages ? id : -1;
+      if constexpr (F8) {
+        const size_t s = (size_t)max(tp[g], 0) * a.Hkv + kvh;
+        tks[g] = p.ks[s];
+        tvs[g] = p.vs[s];
+      }
+    }
+  };
+  auto unit = [&](long long u) {
+    const int i = (int)(u - tbase);
+    const bool live = u < u1;
+    PgUnit X;
+    X.b = __builtin_amdgcn_readlane(tb, i);
+    X.ph = __builtin_amdgcn_readlane(tph, i);
+    X.j = __builtin_amdgcn_readlane(tj, i);
+    X.L = __builtin_amdgcn_readlane(tL, i);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      X.page[g] = live ? __builtin_amdgcn_readlane(tp[g], i) : -1;
+      X.ks[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(tks[g]), i));
+      X.vs[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(tvs[g]), i));
+    }
+    return X;
+  };
+
+  // Loads of a block (all unconditional; past the range no page is mapped).
+  constexpr int KL = Set::ROW / 32;   // 16-byte loads of a key's row per lane (two lanes a row)
+  u32x4_t kr[KL], qr[4];
+  const int pmask = (1 << p.pshift) - 1;
+  auto row_of = [&](const PgUnit& X, int page, int key) {   // the pool's row of a key in that page
+    const int kvh = X.ph / a.qblocks;
+    return (((long long)page * a.Hkv + kvh) << p.pshift) + (key & pmask);
+  };
+  auto issue_k = [&](const PgUnit& X) {
+    const int key0 = X.j * AT_BLOCK + PG_WKEYS * wave;
+    const long long r0 = row_of(X, max(X.page[0], 0), key0), r1 = row_of(X, max(X.page[1], 0), key0 + 16);
+    const unsigned char* src = reinterpret_cast<const unsigned char*>(a.kc) +
+                               (l32 < 16 ? r0 : r1) * Set::ROW + (l32 & 15) * Set::ROW + 16 * h;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) kr[i] = *reinterpret_cast<const u32x4_t*>(src + 32 * i);
+  };
+  auto issue_v = [&](unsigned char* vset, const PgUnit& X) {
+    unsigned char* dst = vset + wave * Set::WAVE;
+    const int key0 = X.j * AT_BLOCK + PG_WKEYS * wave;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key = key0 + 16 * g;
+      const int rows = X.page[g] >= 0 ? min(X.L - key, 16) : 0;   // (a mapped group begins before L)
+      const __amdgpu_buffer_rsrc_t rs =
+          buf_rsrc(reinterpret_cast<const unsigned char*>(a.vc) + row_of(X, max(X.page[g], 0), key) * Set::ROW,
+                   (uint32_t)(rows * Set::ROW));
+      if constexpr (F8) {
+        // four rows a DMA: lane -> row 4 i + lane / 16, chunk (lane % 16) ^ row
+        const uint32_t vo = 256u * (lane >> 4) + 16u * ((lane & 15) ^ (lane >> 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(dst + 4096 * g + 1024 * i), 16,
+                                                   1024u * i + (vo ^ (64u * i)), 0, 0, 2);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(dst + Set::PAIR * (8 * g + i)), 16,
+                                                   1024u * i + 16u * lane, 0, 0, 2);
+      }
+    }
+  };
+  auto issue_q = [&](const PgUnit& X, bool load) {
+    const int kvh = load ? X.ph / a.qblocks : 0, qb = load ? X.ph % a.qblocks : 0;
+    const int q0_ = qb * a.QB, QB_ = min(a.QB, a.T - q0_), rows_ = a.n_rep * QB_;
+    // (the descriptor spans the query block's tokens: a sequence's may pass 4 GB)
+    const uint32_t bytes = load ? (uint32_t)QB_ * (uint32_t)a.Hq * (AT_D * 2) : 0u;
+    const uint16_t* base = a.q + (load ? ((size_t)X.b * a.T + q0_) * a.Hq * AT_D : 0);
+    const __amdgpu_buffer_rsrc_t rs = buf_rsrc(base, bytes);
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) {
+      const int r = (tid >> 5) + 8 * ii, c = tid & 31;
+      const int hr = r / QB_, i = r % QB_;
+      const uint32_t qo = r < rows_ ? ((uint32_t)i * (uint32_t)a.Hq + (uint32_t)(kvh * a.n_rep + hr)) *
+                                          (AT_D * 2) + 16u * c
+                                    : 0x80000000u;
+      qr[ii] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, qo, 0, 0));
+    }
+  };
+
+  look_up();
+  PgUnit C = unit(u0), X1 = unit(u0 + 1), X2 = unit(u0 + 2);
+  issue_q(C, true);
+  issue_k(C);
+  issue_v(vs0, C);
+  issue_v(vs1, X1);
+
+  f32x16 O[8];            // O^T: d-tile dt (32 columns) x the 32 rows; lane row = l32
+  float m_ref = -INFINITY, l_s = 0.f;
+  int qpos = 0;
+
+  for (long long ub = u0; ub < u1; ub += 2) {
+#pragma unroll
+    for (int set = 0; set < 2; ++set) {
+      unsigned char* vset = set ? vs1 : vs0;
+      const long long u = ub + set;
+      const bool live = u < u1;
+      const int nb = nblk_of(C.L);
+      const bool seg_first = live && ((u == u0) || (C.j == 0));
+      const bool seg_last = live && ((u == u1 - 1) || (C.j == nb - 1));
+      if (seg_first) {
+        const int qb = C.ph % a.qblocks;
+        const int q0 = qb * a.QB, QB = min(a.QB, a.T - q0);
+        qpos = C.L - a.T + q0 + l32 % QB;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
+        m_ref = -INFINITY;
+        l_s = 0.f;
+        // (the previous pair's last block ended with barriers: no wave still reads qs)
+#pragma unroll
+        for (int ii = 0; ii < 4; ++ii)
+          *reinterpret_cast<u32x4_t*>(qs + ((tid >> 5) + 8 * ii) * PG_QROW + 16 * (tid & 31)) = qr[ii];
+        aw_barrier();
+      }
+      // Q of the next block's pair (staged at that block's start)
+      issue_q(X1, u + 1 < u1 && (X1.j == 0));
+
+      // S^T (32 keys x 32 rows) = K Q^T
+      f32x16 S;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[r] = 0.f;
+      if (live) {
+        if constexpr (F8) {
+          const float sc = l32 < 16 ? C.ks[0] : C.ks[1];
+          const unsigned char* qp = qs + l32 * PG_QROW + 32 * h;   // columns 32 i + 16 h ..
+#pragma unroll
+          for (int i = 0; i < KL; ++i) {
+            const bf16x8 k0 = pg_bf16(kr[i].x, kr[i].y, sc), k1 = pg_bf16(kr[i].z, kr[i].w, sc);
+            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, *reinterpret_cast<const bf16x8*>(qp + 64 * i), S, 0, 0, 0);
+            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, *reinterpret_cast<const bf16x8*>(qp + 64 * i + 16), S, 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < KL; ++i) {
+            const bf16x8 qv = *reinterpret_cast<const bf16x8*>(qs + l32 * PG_QROW + 16 * h + 32 * i);
+            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[i]), qv, S, 0, 0, 0);
+          }
+        }
+      }
+      issue_k(X1);   // K of the next block into the registers S consumed
+
+      if (live) {
+        // mask: acc r holds key 32 wave + 8 (r / 4) + 4 h + r % 4 of the block
+        const int kb = C.j * AT_BLOCK + PG_WKEYS * wave + 4 * h;
+        const int lim = min(C.L - 1, qpos) - kb;
+        const int lim0 = C.page[0] >= 0 ? lim : -1, lim1 = C.page[1] >= 0 ? lim : -1;
+        float bm = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int kk = 8 * (r >> 2) + (r & 3);
+          S[r] = kk <= (r < 8 ? lim0 : lim1) ? S[r] : -INFINITY;
+          bm = fmaxf(bm, S[r]);
+        }
+        bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+        // the reference max moves (and l, O are rescaled) only when a row's block max exceeds it
+        // by more than 16 in the exponent: attn_verify's rule, each row's own decision
+        const bool big = (bm - m_ref) * a.cl2 > 16.f;
+        if (__builtin_amdgcn_readfirstlane((int)(__ballot(big) != 0))) {
+          const float mn = big ? fmaxf(m_ref, bm) : m_ref;
+          const float alpha = (!big || mn == -INFINITY) ? 1.f : fast_exp2((m_ref - mn) * a.cl2);
+          m_ref = mn;
+          l_s *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt) O[dt] *= alpha;
+        }
+        const float base = m_ref == -INFINITY ? 0.f : m_ref * a.cl2;
+        float e[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) e[r] = fast_exp2(__builtin_fmaf(S[r], a.cl2, -base));
+        float ps = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ps += e[r];
+        l_s += ps;
+        bf16x8 Ph[2], Pl[2];
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+          u32x4_t hw, lw;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t hi, lo;
+            at_split(e[8 * k2 + 2 * q], e[8 * k2 + 2 * q + 1], hi, lo);
+            hw[q] = hi;
+            lw[q] = lo;
+          }
+          Ph[k2] = __builtin_bit_cast(bf16x8, hw);
+          Pl[k2] = __builtin_bit_cast(bf16x8, lw);
+        }
+
+        // O^T += V^T P^T: A = V^T from LDS by transposing reads (lane: column 32 dt + l32, keys
+        // 16 ks + 4 h + 0..3 and 16 ks + 8 + 4 h + 0..3, the order P holds them in)
+        if constexpr (F8) {
+          // the 16 lanes of a group read 8 rows x 16 bytes: lane i row i / 2 of the order above,
+          // bytes 8 (i % 2) of the group's chunk 2 dt + (group % 2), swizzled by the row
+          const int i2 = (lane & 15) >> 1, key = (i2 & 3) + 4 * h + 8 * (i2 >> 2);
+          const unsigned char* vw = vset + wave * Set::WAVE + 256 * key + 8 * (lane & 1);
+          const int ch = ((lane >> 4) & 1) ^ key;
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              const i32x2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                  (lds_i32x2_t*)(vw + 4096 * ks + 16 * (ch ^ (2 * dt))));
+              const bf16x8 vA = pg_bf16((uint32_t)v.x, (uint32_t)v.y, C.vs[ks]);
+              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Ph[ks], O[dt], 0, 0, 0);
+              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[ks], O[dt], 0, 0, 0);
+            }
+          }
+        } else {
+          const int x = 4 * h + ((lane & 15) >> 2);
+          const unsigned char* vw = vset + wave * Set::WAVE + (x >> 1) * Set::PAIR + (x & 1) * (AT_D * 2) +
+                                    32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds_s16x4_t*)(vw + 8 * ks * Set::PAIR + 64 * dt));
+              const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds_s16x4_t*)(vw + (8 * ks + 4) * Set::PAIR + 64 * dt));
+              const u32x2_t w0 = __builtin_bit_cast(u32x2_t, v0), w1 = __builtin_bit_cast(u32x2_t, v1);
+              const bf16x8 vA = __builtin_bit_cast(bf16x8, u32x4_t{w0.x, w0.y, w1.x, w1.y});
+              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Ph[ks], O[dt], 0, 0, 0);
+              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[ks], O[dt], 0, 0, 0);
+            }
+          }
+        }
+      }
+
+      if (seg_last) {
+        // merge the four waves' (m, l, O) of this pair into the workgroup's piece, in two halves
+        // of d: each wave dumps its O (straight from the accumulators), then every thread sums
+        // one row's 16 columns with the waves' weights exp(m_w - M)
+        const float lrow = l_s + __shfl_xor(l_s, 32, 64);
+        aw_barrier();   // every wave is done reading this set
+        if (h == 0) {
+          mx[wave][l32] = m_ref;
+          lx[wave][l32] = lrow;
+        }
+        const int pair = C.b * PH + C.ph;
+        float* part = a.ws + ((size_t)w + pair) * AT_PART;
+        float* dump = reinterpret_cast<float*>(F8 ? own_dump : vset);
+        const int srow = tid >> 3, sc8 = tid & 7;
+        float wgt[AW_WAVES];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<float4*>(dump + (wave * AT_ROWS + l32) * PG_OROW + 32 * dt + 8 * q + 4 * h) =
+                  make_float4(O[4 * half + dt][4 * q], O[4 * half + dt][4 * q + 1], O[4 * half + dt][4 * q + 2],
+                              O[4 * half + dt][4 * q + 3]);
+          aw_barrier();
+          if (half == 0) {
+            float M = mx[0][srow];
+#pragma unroll
+            for (int ww = 1; ww < AW_WAVES; ++ww) M = fmaxf(M, mx[ww][srow]);
+            float Lsum = 0.f;
+#pragma unroll
+            for (int ww = 0; ww < AW_WAVES; ++ww) {
+              const float mw = mx[ww][srow];
+              wgt[ww] = mw == -INFINITY ? 0.f : fast_exp2((mw - M) * a.cl2);
+              Lsum += lx[ww][srow] * wgt[ww];
+            }
+            if (sc8 == 0) {
+              part[srow] = M;
+              part[AT_ROWS + srow] = Lsum;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int ww = 0; ww < AW_WAVES; ++ww) {
+              const float4 v = *reinterpret_cast<const float4*>(dump + (ww * AT_ROWS + srow) * PG_OROW + 16 * sc8 + 4 * k);
+              acc.x += wgt[ww] * v.x; acc.y += wgt[ww] * v.y; acc.z += wgt[ww] * v.z; acc.w += wgt[ww] * v.w;
+            }
+            *reinterpret_cast<float4*>(part + 2 * AT_ROWS + srow * AT_D + 128 * half + 16 * sc8 + 4 * k) = acc;
+          }
+          aw_barrier();   // the dump is read before it is overwritten (and the set refilled)
+        }
+      }
+      // V of block u + 2 into this set
+      issue_v(vset, X2);
+      C = X1;
+      X1 = X2;
+      if (u + 3 - tbase >= 64) {   // the lanes' blocks are used up
+        tbase = u + 1;
+        look_up();
+      }
+      X2 = unit(u + 3);
+    }
+  }
+}
+
+}  // namespace lollm
+
+using namespace lollm;
+
+LOLLM_API long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int grid) {
+  int n_rep, QB, qblocks;
+  if (attn_geometry(B, T, Hq, Hkv, D, 1, &n_rep, &QB, &qblocks)) return -1;
+  const int nw = attn_grid(grid);
+  if (nw <= 0 || nw > 1024) return -1;
+  return attn_ws_bytes(nw, (long long)B * Hkv * qblocks);
+}
+
+LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages,
+                               const float* k_scale, const float* v_scale, int kv_dtype,
+                               const int32_t* table, long long table_stride, int table_width, int n_pages,
+                               int page, const int32_t* kv_len, const void* gate, long long gate_row,
+                               int gate_head, void* out, void* workspace, long long workspace_bytes, int B,
+                               int T, int Hq, int Hkv, int D, int grid, float scale, void* stream) {
+  if (!q || !k_pages || !v_pages || !table || !kv_len || !out) return LOLLM_EINVAL;
+  if (kv_dtype != LOLLM_BF16 && kv_dtype != LOLLM_F8) return LOLLM_EUNSUPPORTED;
+  const bool f8 = kv_dtype == LOLLM_F8;
+  if (f8 && (!k_scale || !v_scale)) return LOLLM_EINVAL;
+  if (table_width <= 0 || n_pages <= 0 || table_stride < table_width) return LOLLM_EINVAL;
+  const int pshift = attn_page_shift(page);
+  if (pshift < 0) return LOLLM_EUNSUPPORTED;
+  const long long rows = (long long)table_width << pshift;
+  if (rows > 0x7fffff00LL) return LOLLM_EUNSUPPORTED;
+  int n_rep, QB, qblocks;
+  int rc = attn_geometry(B, T, Hq, Hkv, D, (int)rows, &n_rep, &QB, &qblocks);
+  if (rc) return rc;
+  if (grid < 0 || grid > 1024) return LOLLM_EINVAL;  // pieces per pair <= combine table
+  if (gate && (gate_head < D || gate_row < (Hq - 1LL) * gate_head + D)) return LOLLM_EINVAL;
+  if (gate && (gate_row % 8 || gate_head % 8)) return LOLLM_EINVAL;
+  const long long pairs = (long long)B * Hkv * qblocks;
+  if (pairs > 65535) return LOLLM_EUNSUPPORTED;      // the combine's grid
+  const int nw = attn_grid(grid);
+  if (nw <= 0 || nw > 1024) return LOLLM_EUNSUPPORTED;
+  if (!workspace || workspace_bytes < attn_ws_bytes(nw, pairs)) return LOLLM_EINVAL;
+  PagedArgs p;
+  AttnArgs& a = p.a;
+  a.q = (const uint16_t*)q; a.kc = (const uint16_t*)k_pages; a.vc = (const uint16_t*)v_pages;
+  a.kv_len = kv_len; a.gate = (const uint16_t*)gate; a.out = (uint16_t*)out;
+  a.ws = (float*)workspace; a.seq_stride = 0; a.head_stride = 0;
+  a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.n_rep = n_rep; a.QB = QB; a.qblocks = qblocks;
+  a.max_len = (int)rows; a.nw = nw;
+  a.cl2 = scale * 1.4426950408889634f;
+  a.gate_row = gate_row; a.gate_head = gate_head;
+  p.table = table; p.ks = k_scale; p.vs = v_scale; p.table_stride = table_stride;
+  p.n_pages = n_pages; p.pshift = pshift;
+  hipStream_t st = (hipStream_t)stream;
+  if (f8)
+    hipLaunchKernelGGL(attn_paged_kernel<true>, dim3(nw), dim3(AW_THREADS), 0, st, p);
+  else
+    hipLaunchKernelGGL(attn_paged_kernel<false>, dim3(nw), dim3(AW_THREADS), 0, st, p);
+  if ((rc = launch_status())) return rc;
+  return attn_combine_launch(a, st);
+}

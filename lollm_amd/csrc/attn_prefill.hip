@@ -46,8 +46,6 @@ constexpr int AP_KEYS = 32;                    // keys per block
 constexpr int AP_AHEAD = 3;                    // operands read ahead of their products
 constexpr int AP_SET = AP_KEYS * AT_D * 2;     // 16 KB: K or V rows of a block
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
 struct ApArgs {
   const uint16_t* q;       // (B, T, Hq, D)
   const uint16_t* kc;      // K cache
@@ -74,18 +72,6 @@ __device__ __forceinline__ void ap_mfma(f32x16& s, bf16x8 k, bf16x8 q) {
 // the wait states between the last product and the first VALU access of its result
 __device__ __forceinline__ void ap_mfma_done(f32x16& s) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s)); }
 
-// A pair of fp32 weights as bf16 hi and lo, x = hi + lo to 16 bits.  hi is cut and not rounded, so
-// that lo is never negative, and lo is at least 2^-126 where hi is not 0: an infinite V then takes
-// the sum of both products to infinity as a single product does, not to infinity - infinity or
-// 0 x infinity.
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ void ap_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
-  hi = __builtin_amdgcn_perm(yb, xb, 0x07060302u);   // the upper halves
-  const bf16x2 l = {(__bf16)(x - __uint_as_float(xb & 0xffff0000u)), (__bf16)(y - __uint_as_float(yb & 0xffff0000u))};
-  const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, hi), u16x2{0x0080, 0x0080});
-  lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, l), least));
-}
 __device__ __forceinline__ int ap_div(int r, uint32_t mul) { return (int)(((uint32_t)r * mul) >> 16); }
 
 template <int RG>
@@ -302,7 +288,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
         const float p = fast_exp2(__builtin_fmaf(S[rg][n], a.cl2, -base[rg]));
         if (n & 1) {   // (pinned here: the compiler would sink them all past the rescale)
           uint32_t hi, lo;
-          ap_split(pe[rg], p, hi, lo);
+          at_split(pe[rg], p, hi, lo);
           l_s[rg] += pe[rg] + p;
           asm volatile("" : "+v"(hi), "+v"(lo), "+v"(l_s[rg]));
           Pn[rg][n >> 3][(n & 7) >> 1] = hi;
@@ -334,7 +320,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
         const float p0 = fast_exp2(__builtin_fmaf(S[rg][r], a.cl2, -base[rg]));
         const float p1 = fast_exp2(__builtin_fmaf(S[rg][r + 1], a.cl2, -base[rg]));
         uint32_t hi, lo;
-        ap_split(p0, p1, hi, lo);
+        at_split(p0, p1, hi, lo);
         l_s[rg] += p0 + p1;
         Pn[r >> 3][(r & 7) >> 1] = hi;
         Pm[r >> 3][(r & 7) >> 1] = lo;

@@ -42,25 +42,6 @@
 
 namespace lollm {
 
-constexpr int AT_BLOCK = 128;        // keys per block
-constexpr int AT_MAXB = 512;         // sequences per call (prefix table in LDS)
-constexpr int AT_PART = 2 * AT_ROWS + AT_ROWS * AT_D;  // floats per partial
-
-__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
-  return min(max(a.kv_len[b], 0), a.max_len);  // never past the cache capacity
-}
-
-__device__ __forceinline__ int nblk_of(int L) { return (L + AT_BLOCK - 1) / AT_BLOCK; }
-
-// First unit of workgroup w and the workgroup that owns unit u, for U units dealt
-// out to nw workgroups in equal contiguous ranges: w owns [U w / nw, U (w+1) / nw).
-__device__ __forceinline__ long long unit_begin(long long U, int w, int nw) {
-  return U * w / nw;
-}
-__device__ __forceinline__ int unit_owner(long long U, long long u, int nw) {
-  return (int)(((u + 1) * nw - 1) / U);
-}
-
 // Buffer loads through a descriptor over [base, base + bytes): offsets past the end read
 // zeros without touching memory.  AUX = 2 is the non-temporal hint.
 template <int AUX>
@@ -74,8 +55,6 @@ struct AtCursor {
   int b, ph, j, nb;
 };
 
-constexpr int AW_WAVES = 4;
-constexpr int AW_THREADS = 64 * AW_WAVES;
 constexpr int AW_WKEYS = AT_BLOCK / AW_WAVES;        // 32 keys of each block per wave
 constexpr int AW_VPAIR = 2 * AT_D * 2 + 64;          // two V rows (one DMA) + 64 bytes of padding
 constexpr int AW_VWAVE = AW_WKEYS / 2 * AW_VPAIR;     // 17 KB: one wave's V rows of a block
@@ -83,44 +62,6 @@ constexpr int AW_VSET = AW_WAVES * AW_VWAVE;          // the V rows of one block
 constexpr int AW_QROW = AT_D * 2 + 16;                // padded Q row in LDS
 constexpr int AW_OROW = AT_D / 2 + 4;                 // padded floats per row of an O half-dump
 static_assert(AW_WAVES * AT_ROWS * AW_OROW * 4 <= AW_VSET, "the O dump fits a V set");
-
-// pre[b] = blocks of sequences 0..b-1 (pre[0] = 0), for b = 0..B, and len[b] = the
-// clamped key count of sequence b, built in LDS by the whole workgroup (so the main
-// loop never waits on a global load to address the next block).  Returns pre[B].
-__device__ int build_prefix(const AttnArgs& a, int* pre, int* len, int* tmp) {
-  constexpr int WAVES = AW_WAVES;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int carry = 0;
-  if (tid == 0) pre[0] = 0;
-  for (int base = 0; base < a.B; base += AW_THREADS) {
-    const int b = base + tid;
-    const int Lb = b < a.B ? seq_len(a, b) : 0;
-    if (b < a.B) len[b] = Lb;
-    int v = nblk_of(Lb);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(v, d, 64);
-      if (lane >= d) v += o;
-    }
-    if (lane == 63) tmp[wave] = v;
-    __syncthreads();
-    int before = carry, all = carry;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) before += tmp[w];
-      all += tmp[w];
-    }
-    if (b < a.B) pre[b + 1] = before + v;
-    carry = all;
-    __syncthreads();
-  }
-  return carry;
-}
-
-// Workgroup barrier after this wave's LDS accesses complete; the compiler sees a memory
-// clobber (no LDS access moves across it) but no fence, so global loads and LDS DMA in
-// flight are not drained.
-__device__ __forceinline__ void aw_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __global__ __launch_bounds__(AW_THREADS, 1) void attn_verify_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned char vs0[AW_VSET];   // V of even units
@@ -444,7 +385,8 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs a) {
   if (r >= a.n_rep * QB) return;
   const int hr = r / QB, i = r % QB, h = kvh * a.n_rep + hr;
   const size_t o = ((size_t)b * a.T + q0 + i) * a.Hq * AT_D + (size_t)h * AT_D + tid;
-  const float gl = a.gate ? bf16_to_f32(a.gate[o]) : 0.f;   // in flight from the start
+  const size_t go = ((size_t)b * a.T + q0 + i) * a.gate_row + (size_t)h * a.gate_head + tid;
+  const float gl = a.gate ? bf16_to_f32(a.gate[go]) : 0.f;   // in flight from the start
   const int4 te = reinterpret_cast<const int4*>(a.ws + (size_t)(a.nw + a.B * PH) * AT_PART)[pair];
   const int wf = te.x, wl = te.y;
   const long long U = (long long)(((uint64_t)(uint32_t)te.w << 32) | (uint32_t)te.z);
@@ -504,18 +446,19 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs a) {
   a.out[o] = f32_to_bf16(val);
 }
 
-}  // namespace lollm
-
-using namespace lollm;
+int attn_combine_launch(const AttnArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL(attn_combine_kernel, dim3(AT_ROWS, a.B * a.Hkv * a.qblocks), dim3(256), 0, st, a);
+  return launch_status();
+}
 
 // Workspace: one fp32 piece per workgroup plus one per pair, then the combine's table
 // (one int4 per pair).
-static long long attn_ws_bytes(long long nw, long long pairs) {
+long long attn_ws_bytes(long long nw, long long pairs) {
   return (nw + pairs) * AT_PART * (long long)sizeof(float) + pairs * 16;
 }
 
-static int attn_geometry(int B, int T, int Hq, int Hkv, int D, int max_len, int* n_rep, int* QB,
-                         int* qblocks) {
+int attn_geometry(int B, int T, int Hq, int Hkv, int D, int max_len, int* n_rep, int* QB,
+                  int* qblocks) {
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_len <= 0) return LOLLM_EINVAL;
   if (D != AT_D) return LOLLM_EUNSUPPORTED;
   if (B > AT_MAXB) return LOLLM_EUNSUPPORTED;
@@ -528,7 +471,7 @@ static int attn_geometry(int B, int T, int Hq, int Hkv, int D, int max_len, int*
 
 // Workgroups of the balanced grid: `grid` if positive, else one per CU of the current
 // device.  A piece count per pair above the combine's table size is refused.
-static int attn_grid(int grid) {
+int attn_grid(int grid) {
   if (grid > 0) return grid;
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess) return -1;
@@ -536,6 +479,10 @@ static int attn_grid(int grid) {
     return -1;
   return cus > 0 ? cus : -1;
 }
+
+}  // namespace lollm
+
+using namespace lollm;
 
 LOLLM_API long long lollm_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D,
                                                int max_len, int grid) {
@@ -569,6 +516,7 @@ LOLLM_API int lollm_attn_verify(const void* q, const void* k_cache, const void* 
   a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.n_rep = n_rep; a.QB = QB; a.qblocks = qblocks;
   a.max_len = max_len; a.nw = nw;
   a.cl2 = scale * 1.4426950408889634f;
+  a.gate_row = (long long)Hq * D; a.gate_head = D;
   hipStream_t st = (hipStream_t)stream;
   if (grid == 0) {
     const int groups = attn_prefill_groups(B, T, Hkv, n_rep, nw);
@@ -576,6 +524,5 @@ LOLLM_API int lollm_attn_verify(const void* q, const void* k_cache, const void* 
   }
   hipLaunchKernelGGL(attn_verify_kernel, dim3(nw), dim3(AW_THREADS), 0, st, a);
   if ((rc = launch_status())) return rc;
-  hipLaunchKernelGGL(attn_combine_kernel, dim3(AT_ROWS, B * Hkv * qblocks), dim3(256), 0, st, a);
-  return launch_status();
+  return attn_combine_launch(a, st);
 }

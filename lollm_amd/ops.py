@@ -188,6 +188,150 @@ def attn_verify(q, k_cache, v_cache, kv_len, gate=None, *, grid=0, scale=None,
 
 
 # ------------------------------------------------------------------------------------
+# paged KV cache, pages in bf16 or in 8 bits
+# ------------------------------------------------------------------------------------
+F8 = 2
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+def _here(*tensors):
+    """The kernels run on the current device's stream: refuse tensors of another device."""
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors must be on the current device, {dev}, got one on {t.device}")
+
+
+def _pages(k_pages, v_pages, k_scale, v_scale, table, B):
+    """(pages in the pool, KV heads, rows of a page, dtype code, table stride) of a checked paged
+    cache layer."""
+    if k_pages.dim() != 4:
+        raise ValueError("k_pages must be (n_pages, Hkv, page, D)")
+    n, Hkv, page, _ = k_pages.shape
+    if n < 1 or Hkv < 1 or page not in PAGE_SIZES:
+        raise ValueError(f"a page holds {PAGE_SIZES} rows and the pool at least one page, got "
+                         f"{tuple(k_pages.shape)}")
+    code = F8 if k_pages.dtype is torch.float8_e4m3fn else BF16
+    dt = torch.float8_e4m3fn if code == F8 else torch.bfloat16
+    _need(k_pages, "k_pages", dt)
+    _need(v_pages, "v_pages", dt, k_pages.shape)
+    if code == F8:
+        if k_scale is None or v_scale is None:
+            raise ValueError("8-bit pages need k_scale and v_scale")
+        _need(k_scale, "k_scale", torch.float32, (n, Hkv))
+        _need(v_scale, "v_scale", torch.float32, (n, Hkv))
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("bf16 pages have no scales")
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B or not table.is_cuda \
+            or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"table must be ({B}, pages) int32 on the device with unit column stride")
+    stride = table.stride(0) if B > 1 else table.shape[1]
+    if stride < table.shape[1]:
+        raise ValueError("table rows overlap")
+    _here(k_pages, v_pages, k_scale, v_scale, table)
+    return n, Hkv, page, code, stride
+
+
+def attn_append(qkv, q_norm_w, k_norm_w, inv_freq, lengths, table, k_pages, v_pages, Hq, rotary_dim,
+                eps, *, k_scale=None, v_scale=None, rope_pos=None, q_out=None):
+    """attn_prologue over a paged cache: QK-norm and RoPE of the fused projection's output qkv
+    (B, T, Hq*2D + 2*Hkv*D) bf16, keys and values of token t into row lengths[b] + t of sequence
+    b's pages.  table (B, width) int32 page ids (< 0 or past the pool: unmapped, nothing stored);
+    k_pages / v_pages (n_pages, Hkv, page, D) bf16, or float8_e4m3fn with k_scale / v_scale
+    (n_pages, Hkv) fp32, which it updates (include/lollm_amd.h).  rope_pos: None (the cache rows),
+    (B,) int32 start positions, or (B, T) int32.  Returns (q (B, T, Hq, D), the gates
+    (B, T, Hq, D) as a view of qkv)."""
+    if qkv.dim() != 3:
+        raise ValueError("qkv must be (B, T, Hq*2D + 2*Hkv*D)")
+    B, T, width = qkv.shape
+    n, Hkv, page, code, stride = _pages(k_pages, v_pages, k_scale, v_scale, table, B)
+    D = k_pages.shape[3]
+    if B < 1 or T < 1 or Hq < 1 or width != Hq * 2 * D + 2 * Hkv * D:
+        raise ValueError(f"qkv is {tuple(qkv.shape)}, expected (B, T, {Hq * 2 * D + 2 * Hkv * D})")
+    _need(qkv, "qkv", torch.bfloat16)
+    _need(q_norm_w, "q_norm_w", torch.bfloat16, (D,))
+    _need(k_norm_w, "k_norm_w", torch.bfloat16, (D,))
+    if rotary_dim:
+        _need(inv_freq, "inv_freq", torch.float32, (rotary_dim // 2,))
+    _need(lengths, "lengths", torch.int32, (B,))
+    per_token = rope_pos is not None and rope_pos.dim() == 2
+    if rope_pos is not None:
+        _need(rope_pos, "rope_pos", torch.int32, (B, T) if per_token else (B,))
+    if q_out is None:
+        q_out = torch.empty(B, T, Hq, D, dtype=torch.bfloat16, device=qkv.device)
+    _need(q_out, "q_out", torch.bfloat16, (B, T, Hq, D))
+    _here(qkv, q_norm_w, k_norm_w, inv_freq, lengths, rope_pos, q_out)
+    rc = _lib.lib().lollm_attn_append(
+        _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(inv_freq), _ptr(lengths), _ptr(rope_pos),
+        int(per_token), _ptr(table), stride, table.shape[1], n, page, code, B, T, Hq, Hkv, D, rotary_dim,
+        float(eps), _ptr(q_out), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), _stream())
+    _lib.check(rc, "lollm_attn_append")
+    return q_out, qkv.as_strided((B, T, Hq, D), (T * width, width, 2 * D, 1), qkv.storage_offset() + D)
+
+
+def attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid=0):
+    """Bytes of attn_paged's workspace for `grid` workgroups (0: one per CU)."""
+    return _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid, torch._C._cuda_getDevice() if grid <= 0 else -1)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid, device):
+    n = _lib.lib().lollm_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid)
+    if n < 0:
+        raise ValueError("unsupported attention geometry")
+    return n
+
+
+def _gate_strides(gate, B, T, Hq, D):
+    """(row, head) strides of a gate (B, T, Hq*D) or (B, T, Hq, D) whose rows are evenly strided."""
+    if gate.dtype is not torch.bfloat16 or not gate.is_cuda:
+        raise TypeError("gate must be bf16 on the device")
+    if gate.dim() == 3:
+        _need(gate, "gate", torch.bfloat16, (B, T, Hq * D))
+        return Hq * D, D
+    if gate.shape != (B, T, Hq, D):
+        raise ValueError(f"gate has shape {tuple(gate.shape)}, expected {(B, T, Hq, D)}")
+    head = gate.stride(2) if Hq > 1 else D
+    row = gate.stride(1) if T > 1 else (gate.stride(0) if B > 1 else Hq * head)
+    if gate.stride(3) != 1 or (B > 1 and T > 1 and gate.stride(0) != T * row) or head < D \
+            or row < (Hq - 1) * head + D or row % 8 or head % 8 or gate.data_ptr() % 16:
+        raise ValueError("gate rows must be evenly strided, 16-byte aligned and not overlap")
+    return row, head
+
+
+def attn_paged(q, k_pages, v_pages, table, kv_len, gate=None, *, k_scale=None, v_scale=None, grid=0,
+               scale=None, workspace=None, out=None):
+    """attn_verify over a paged cache: q (B, T, Hq, D) bf16, keys and values in the pages that
+    table (B, width) int32 names (as attn_append writes them; keys of unmapped pages do not
+    exist), kv_len (B,) int32 with the T new ones included; gate (B, T, Hq, D) bf16, which may be
+    attn_append's view, or (B, T, Hq*D), or None.  Returns (B, T, Hq*D) bf16."""
+    if q.dim() != 4:
+        raise ValueError("q must be (B, T, Hq, D)")
+    B, T, Hq, D = q.shape
+    n, Hkv, page, code, stride = _pages(k_pages, v_pages, k_scale, v_scale, table, B)
+    if k_pages.shape[3] != D or min(B, T, Hq) < 1 or Hq % Hkv:
+        raise ValueError(f"q {tuple(q.shape)} does not fit pages {tuple(k_pages.shape)}")
+    _need(q, "q", torch.bfloat16)
+    _need(kv_len, "kv_len", torch.int32, (B,))
+    row, head = _gate_strides(gate, B, T, Hq, D) if gate is not None else (0, 0)
+    if out is None:
+        out = torch.empty(B, T, Hq * D, dtype=torch.bfloat16, device=q.device)
+    _need(out, "out", torch.bfloat16, (B, T, Hq * D))
+    if workspace is None:
+        workspace = torch.empty(attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid), dtype=torch.uint8,
+                                device=q.device)
+    _need(workspace, "workspace")
+    _here(q, kv_len, gate, out, workspace)
+    rc = _lib.lib().lollm_attn_paged(
+        _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), code, _ptr(table), stride,
+        table.shape[1], n, page, _ptr(kv_len), _ptr(gate), row, head, _ptr(out), _ptr(workspace),
+        workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, D, grid,
+        D ** -0.5 if scale is None else float(scale), _stream())
+    _lib.check(rc, "lollm_attn_paged")
+    return out
+
+
+# ------------------------------------------------------------------------------------
 # few-row weight-streaming GEMM
 # ------------------------------------------------------------------------------------
 GEMM_NONE, GEMM_SWIGLU = 0, 1
