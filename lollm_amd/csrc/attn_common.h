@@ -35,6 +35,16 @@ struct AttnArgs {
   int gate_head;
 };
 
+struct PagedArgs {
+  AttnArgs a;                 // kc, vc: the pools; max_len: the rows that the table can name
+  const int32_t* table;       // (B, table_stride)
+  const float* ks;            // (n_pages, Hkv) scales, 8-bit pages
+  const float* vs;
+  long long table_stride;
+  int n_pages, pshift;        // page = 1 << pshift
+  uint32_t rep_mul;           // ceil(2^16 / n_rep): r / n_rep = r * rep_mul >> 16 for r < 256
+};
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ float sigmoidf_(float x) { return 1.f / (1.f + __expf(-x)); }
@@ -50,6 +60,15 @@ __device__ __forceinline__ void at_split(float x, float y, uint32_t& hi, uint32_
   const bf16x2 l = {(__bf16)(x - __uint_as_float(xb & 0xffff0000u)), (__bf16)(y - __uint_as_float(yb & 0xffff0000u))};
   const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, hi), u16x2{0x0080, 0x0080});
   lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, l), least));
+}
+
+// Eight e4m3 codes as bf16, times their scale (a power of two: exact).
+__device__ __forceinline__ bf16x8 at_bf16(uint32_t w0, uint32_t w1, float scale) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
+  return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
 constexpr int AW_WAVES = 4;
@@ -120,8 +139,6 @@ inline int attn_page_shift(int page) {
   return -1;
 }
 
-// Merges the pieces of every pair (one per row), with the gate.
-int attn_combine_launch(const AttnArgs& a, hipStream_t st);
 // Sizes of a split-K call and its workspace; workgroups of the balanced grid (`grid` if positive,
 // else one per CU of the current device), -1 where the device is not known.
 int attn_geometry(int B, int T, int Hq, int Hkv, int D, int max_len, int* n_rep, int* QB, int* qblocks);
@@ -131,6 +148,6 @@ int attn_grid(int grid);
 // Row groups per wave of the long-call kernel (attn_prefill.hip) for this geometry on a device
 // with `cus` CUs, or 0 where the split-K kernels are the faster ones.
 int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus);
-int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st);
+int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st, const PagedArgs* paged = nullptr);
 
 }  // namespace lollm

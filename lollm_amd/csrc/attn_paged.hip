@@ -27,15 +27,6 @@
 
 namespace lollm {
 
-struct PagedArgs {
-  AttnArgs a;                 // kc, vc: the pools
-  const int32_t* table;       // (B, table_stride)
-  const float* ks;            // (n_pages, Hkv) scales, 8-bit pages
-  const float* vs;
-  long long table_stride;
-  int n_pages, pshift;        // page = 1 << pshift
-};
-
 constexpr int PG_WKEYS = AT_BLOCK / AW_WAVES;   // 32 keys of each block per wave
 constexpr int PG_QROW = AT_D * 2 + 16;          // padded Q row in LDS
 constexpr int PG_OROW = AT_D / 2 + 4;           // padded floats per row of an O half-dump
@@ -58,20 +49,45 @@ struct PgUnit {
   float ks[2], vs[2];
 };
 
-__device__ __forceinline__ bf16x8 pg_bf16(uint32_t w0, uint32_t w1, float scale) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
-  return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+__device__ __forceinline__ uint32_t lds_at(const unsigned char* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)p;
+}
+
+// A wave's V operands of a block by transposing reads, landed when they return.  8 bits: column
+// tile d at `at` with the chunk bits (5 .. 7: rows begin at multiples of 256) flipped by 2 d, keys
+// 16 .. 31 4 KB further.
+__device__ __forceinline__ void pg_read_codes(uint32_t at, i32x2_t (&v)[16]) {
+#define RD2(i, j, a) "ds_read_b64_tr_b8 %" #i ", %" #a "\n\tds_read_b64_tr_b8 %" #j ", %" #a " offset:4096\n\t"
+  asm volatile(RD2(0, 1, 16) RD2(2, 3, 17) RD2(4, 5, 18) RD2(6, 7, 19) RD2(8, 9, 20) RD2(10, 11, 21) RD2(12, 13, 22)
+                   RD2(14, 15, 23) "s_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]),
+                 "=&v"(v[7]), "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]),
+                 "=&v"(v[14]), "=&v"(v[15])
+               : "v"(at), "v"(at ^ 32u), "v"(at ^ 64u), "v"(at ^ 96u), "v"(at ^ 128u), "v"(at ^ 160u), "v"(at ^ 192u),
+                 "v"(at ^ 224u)
+               : "memory");
+#undef RD2
+}
+
+// bf16: two column tiles 64 bytes apart, rows in pairs of PAIR bytes.
+template <int PAIR>
+__device__ __forceinline__ void pg_read_rows(uint32_t at, u32x2_t (&v)[8]) {
+#define RD(i, off) "ds_read_b64_tr_b16 %" #i ", %8 offset:%" #off "\n\t"
+  asm volatile(RD(0, 9) RD(1, 10) RD(2, 11) RD(3, 12) RD(4, 13) RD(5, 14) RD(6, 15) RD(7, 16)
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+               : "v"(at), "n"(0), "n"(4 * PAIR), "n"(8 * PAIR), "n"(12 * PAIR), "n"(64), "n"(64 + 4 * PAIR),
+                 "n"(64 + 8 * PAIR), "n"(64 + 12 * PAIR)
+               : "memory");
+#undef RD
 }
 
 template <bool F8>
 __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) {
   using Set = PagedSet<F8>;
   const AttnArgs& a = p.a;
-  __shared__ __attribute__((aligned(16))) unsigned char vs0[Set::SET];   // V of even blocks
-  __shared__ __attribute__((aligned(16))) unsigned char vs1[Set::SET];   // V of odd blocks
+  __shared__ __attribute__((aligned(256))) unsigned char vs0[Set::SET];   // V of even blocks
+  __shared__ __attribute__((aligned(256))) unsigned char vs1[Set::SET];   // V of odd blocks
   __shared__ __attribute__((aligned(16))) unsigned char own_dump[F8 ? PG_DUMP : 16];
   __shared__ __attribute__((aligned(16))) unsigned char qs[AT_ROWS * PG_QROW];   // Q of the pair
   __shared__ float mx[AW_WAVES][32], lx[AW_WAVES][32];
@@ -85,22 +101,27 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   const int PH = a.Hkv * a.qblocks;
 
   const long long U = (long long)PH * build_prefix(a, pre, len, tmp);
-  {
+  // one block a workgroup where there are fewer blocks: no workgroup between a pair's has none
+  const int nw = (int)min((long long)a.nw, U);
+  const long long u0 = w < nw ? unit_begin(U, w, nw) : 0, u1 = w < nw ? unit_begin(U, w + 1, nw) : 0;
+  auto build_table = [&]() {
     const int npairs = a.B * PH;
-    int4* tab = reinterpret_cast<int4*>(a.ws + (size_t)(a.nw + npairs) * AT_PART);
-    for (int pr = w * AW_THREADS + tid; pr < npairs; pr += a.nw * AW_THREADS) {
+    int2* tab = reinterpret_cast<int2*>(a.ws + (size_t)(a.nw + npairs) * AT_PART);
+    for (int pr = w * AW_THREADS + tid; pr < npairs; pr += (U ? nw : a.nw) * AW_THREADS) {
       const int pb = pr / PH, pph = pr % PH, pnb = pre[pb + 1] - pre[pb];
       int wf = -1, wl = -1;
       if (pnb > 0) {
         const long long first = (long long)PH * pre[pb] + (long long)pph * pnb;
-        wf = unit_owner(U, first, a.nw);
-        wl = unit_owner(U, first + pnb - 1, a.nw);
+        wf = unit_owner(U, first, nw);
+        wl = unit_owner(U, first + pnb - 1, nw);
       }
-      tab[pr] = make_int4(wf, wl, (int)(uint32_t)U, (int)(uint32_t)(U >> 32));
+      tab[pr] = make_int2(wf, wl);
     }
+  };
+  if (u0 >= u1) {   // no work for this one; with no keys at all the table says so
+    if (U == 0) build_table();
+    return;
   }
-  const long long u0 = unit_begin(U, w, a.nw), u1 = unit_begin(U, w + 1, a.nw);
-  if (u0 >= u1) return;
 
   // The lane's block of the 64 from tbase on.
   long long tbase = u0;
@@ -128,10 +149,12 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       tp[g] = id >= 0 && id < p.n_pages ? id : -1;
       if constexpr (F8) {
         const size_t s = (size_t)max(tp[g], 0) * a.Hkv + kvh;
-        tks[g] = p.ks[s];
-        tvs[g] = p.vs[s];
+        tks[g] = tp[g] >= 0 ? p.ks[s] : 1.f;
+        tvs[g] = tp[g] >= 0 ? p.vs[s] : 1.f;   // (V's rows are zeros there: no NaN may meet them)
       }
     }
+    // (waited for here: else the compiler drains every load of the loop where it reads these)
+    asm volatile("" : "+v"(tp[0]), "+v"(tp[1]), "+v"(tks[0]), "+v"(tks[1]), "+v"(tvs[0]), "+v"(tvs[1]));
   };
   auto unit = [&](long long u) {
     const int i = (int)(u - tbase);
@@ -191,34 +214,38 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       }
     }
   };
-  auto issue_q = [&](const PgUnit& X, bool load) {
-    const int kvh = load ? X.ph / a.qblocks : 0, qb = load ? X.ph % a.qblocks : 0;
-    const int q0_ = qb * a.QB, QB_ = min(a.QB, a.T - q0_), rows_ = a.n_rep * QB_;
-    // (the descriptor spans the query block's tokens: a sequence's may pass 4 GB)
-    const uint32_t bytes = load ? (uint32_t)QB_ * (uint32_t)a.Hq * (AT_D * 2) : 0u;
-    const uint16_t* base = a.q + (load ? ((size_t)X.b * a.T + q0_) * a.Hq * AT_D : 0);
-    const __amdgpu_buffer_rsrc_t rs = buf_rsrc(base, bytes);
+  // Row r of a pair is position r / n_rep of its query block, head r % n_rep; this thread's rows
+  // tid / 32 + 8 i of Q, 16 bytes each.
+  uint32_t qoff[4];
+  int qi[4];
 #pragma unroll
-    for (int ii = 0; ii < 4; ++ii) {
-      const int r = (tid >> 5) + 8 * ii, c = tid & 31;
-      const int hr = r / QB_, i = r % QB_;
-      const uint32_t qo = r < rows_ ? ((uint32_t)i * (uint32_t)a.Hq + (uint32_t)(kvh * a.n_rep + hr)) *
-                                          (AT_D * 2) + 16u * c
-                                    : 0x80000000u;
-      qr[ii] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, qo, 0, 0));
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int r = (tid >> 5) + 8 * i;
+    qi[i] = (int)(((uint32_t)r * p.rep_mul) >> 16);
+    qoff[i] = ((uint32_t)qi[i] * a.Hq + (r - qi[i] * a.n_rep)) * (AT_D * 2) + 16u * (tid & 31);
+  }
+  auto issue_q = [&](const PgUnit& X) {
+    const int kvh = X.ph / a.qblocks, q0 = (X.ph - kvh * a.qblocks) * a.QB, QB = min(a.QB, a.T - q0);
+    const uint16_t* base = a.q + (((size_t)X.b * a.T + q0) * a.Hq + kvh * a.n_rep) * AT_D;
+    const __amdgpu_buffer_rsrc_t rs = buf_rsrc(base, (uint32_t)((QB - 1) * a.Hq + a.n_rep) * (AT_D * 2));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                              rs, qi[i] < QB ? qoff[i] : 0x80000000u, 0, 0));
   };
 
   look_up();
   PgUnit C = unit(u0), X1 = unit(u0 + 1), X2 = unit(u0 + 2);
-  issue_q(C, true);
-  issue_k(C);
+  issue_q(C);
   issue_v(vs0, C);
+  issue_k(C);
   issue_v(vs1, X1);
+  build_table();
 
   f32x16 O[8];            // O^T: d-tile dt (32 columns) x the 32 rows; lane row = l32
   float m_ref = -INFINITY, l_s = 0.f;
-  int qpos = 0;
+  const int lq = (int)(((uint32_t)l32 * p.rep_mul) >> 16);   // the lane's position in its query block
+  int qpos = 0, rows = 0;
 
   for (long long ub = u0; ub < u1; ub += 2) {
 #pragma unroll
@@ -226,13 +253,14 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       unsigned char* vset = set ? vs1 : vs0;
       const long long u = ub + set;
       const bool live = u < u1;
+      const bool any = live && (C.page[0] & C.page[1]) != -1;   // keys of this wave to look at
       const int nb = nblk_of(C.L);
       const bool seg_first = live && ((u == u0) || (C.j == 0));
       const bool seg_last = live && ((u == u1 - 1) || (C.j == nb - 1));
       if (seg_first) {
-        const int qb = C.ph % a.qblocks;
-        const int q0 = qb * a.QB, QB = min(a.QB, a.T - q0);
-        qpos = C.L - a.T + q0 + l32 % QB;
+        const int q0 = (C.ph % a.qblocks) * a.QB;
+        qpos = C.L - a.T + q0 + lq;
+        rows = a.n_rep * min(a.QB, a.T - q0);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
@@ -245,20 +273,17 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
           *reinterpret_cast<u32x4_t*>(qs + ((tid >> 5) + 8 * ii) * PG_QROW + 16 * (tid & 31)) = qr[ii];
         aw_barrier();
       }
-      // Q of the next block's pair (staged at that block's start)
-      issue_q(X1, u + 1 < u1 && (X1.j == 0));
-
       // S^T (32 keys x 32 rows) = K Q^T
       f32x16 S;
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[r] = 0.f;
-      if (live) {
+      if (any) {
         if constexpr (F8) {
           const float sc = l32 < 16 ? C.ks[0] : C.ks[1];
           const unsigned char* qp = qs + l32 * PG_QROW + 32 * h;   // columns 32 i + 16 h ..
 #pragma unroll
           for (int i = 0; i < KL; ++i) {
-            const bf16x8 k0 = pg_bf16(kr[i].x, kr[i].y, sc), k1 = pg_bf16(kr[i].z, kr[i].w, sc);
+            const bf16x8 k0 = at_bf16(kr[i].x, kr[i].y, sc), k1 = at_bf16(kr[i].z, kr[i].w, sc);
             S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, *reinterpret_cast<const bf16x8*>(qp + 64 * i), S, 0, 0, 0);
             S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, *reinterpret_cast<const bf16x8*>(qp + 64 * i + 16), S, 0, 0, 0);
           }
@@ -270,9 +295,17 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
           }
         }
       }
+      // Q of the next block's pair (staged at that block's start)
+      if (u + 1 < u1 && X1.j == 0) issue_q(X1);
       issue_k(X1);   // K of the next block into the registers S consumed
+      // V of this block has landed: at least V and K of the next one were asked for after it.
+      // (Counted here and V read by hand: where the compiler cannot tell the sets apart it waits
+      // for both, and nothing is on its way while the products run.)
+      if constexpr (F8) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
+      static_assert(KL + PG_WKEYS * Set::ROW / 1024 == (F8 ? 16 : 32), "the counts above");
 
-      if (live) {
+      if (any) {
         // mask: acc r holds key 32 wave + 8 (r / 4) + 4 h + r % 4 of the block
         const int kb = C.j * AT_BLOCK + PG_WKEYS * wave + 4 * h;
         const int lim = min(C.L - 1, qpos) - kb;
@@ -321,39 +354,34 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 
         // O^T += V^T P^T: A = V^T from LDS by transposing reads (lane: column 32 dt + l32, keys
         // 16 ks + 4 h + 0..3 and 16 ks + 8 + 4 h + 0..3, the order P holds them in)
+        const uint32_t set_at = lds_at(vset) + (uint32_t)(wave * Set::WAVE);
         if constexpr (F8) {
           // the 16 lanes of a group read 8 rows x 16 bytes: lane i row i / 2 of the order above,
           // bytes 8 (i % 2) of the group's chunk 2 dt + (group % 2), swizzled by the row
           const int i2 = (lane & 15) >> 1, key = (i2 & 3) + 4 * h + 8 * (i2 >> 2);
-          const unsigned char* vw = vset + wave * Set::WAVE + 256 * key + 8 * (lane & 1);
-          const int ch = ((lane >> 4) & 1) ^ key;
+          const uint32_t at = set_at + (uint32_t)(256 * key + 16 * (((lane >> 4) & 1) ^ key) + 8 * (lane & 1));
+          i32x2_t v[16];   // column tile i / 2, keys 16 (i % 2) ..
+          pg_read_codes(at, v);
 #pragma unroll
-          for (int dt = 0; dt < 8; ++dt) {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const i32x2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                  (lds_i32x2_t*)(vw + 4096 * ks + 16 * (ch ^ (2 * dt))));
-              const bf16x8 vA = pg_bf16((uint32_t)v.x, (uint32_t)v.y, C.vs[ks]);
-              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Ph[ks], O[dt], 0, 0, 0);
-              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[ks], O[dt], 0, 0, 0);
-            }
+          for (int i = 0; i < 16; ++i) {
+            const bf16x8 vA = at_bf16((uint32_t)v[i].x, (uint32_t)v[i].y, C.vs[i & 1]);
+            O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Ph[i & 1], O[i >> 1], 0, 0, 0);
+            O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[i & 1], O[i >> 1], 0, 0, 0);
           }
         } else {
           const int x = 4 * h + ((lane & 15) >> 2);
-          const unsigned char* vw = vset + wave * Set::WAVE + (x >> 1) * Set::PAIR + (x & 1) * (AT_D * 2) +
-                                    32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+          const uint32_t at = set_at + (uint32_t)((x >> 1) * Set::PAIR + (x & 1) * (AT_D * 2) +
+                                                  32 * ((lane >> 4) & 1) + 8 * (lane & 3));
 #pragma unroll
-          for (int dt = 0; dt < 8; ++dt) {
+          for (int two = 0; two < 4; ++two) {
+            u32x2_t v[8];   // column tile 2 two + i / 4, keys 16 (i / 2 % 2) + 8 (i % 2) ..
+            pg_read_rows<Set::PAIR>(at + 128 * two, v);
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (lds_s16x4_t*)(vw + 8 * ks * Set::PAIR + 64 * dt));
-              const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (lds_s16x4_t*)(vw + (8 * ks + 4) * Set::PAIR + 64 * dt));
-              const u32x2_t w0 = __builtin_bit_cast(u32x2_t, v0), w1 = __builtin_bit_cast(u32x2_t, v1);
-              const bf16x8 vA = __builtin_bit_cast(bf16x8, u32x4_t{w0.x, w0.y, w1.x, w1.y});
-              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Ph[ks], O[dt], 0, 0, 0);
-              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[ks], O[dt], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+              const bf16x8 vA = __builtin_bit_cast(bf16x8, u32x4_t{v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y});
+              const int dt = 2 * two + (i >> 1);
+              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Ph[i & 1], O[dt], 0, 0, 0);
+              O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[i & 1], O[dt], 0, 0, 0);
             }
           }
         }
@@ -376,6 +404,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         float wgt[AW_WAVES];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
+          if (l32 < rows) {   // (few tokens leave most of the 32 rows empty)
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -383,6 +412,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
               *reinterpret_cast<float4*>(dump + (wave * AT_ROWS + l32) * PG_OROW + 32 * dt + 8 * q + 4 * h) =
                   make_float4(O[4 * half + dt][4 * q], O[4 * half + dt][4 * q + 1], O[4 * half + dt][4 * q + 2],
                               O[4 * half + dt][4 * q + 3]);
+          }
           aw_barrier();
           if (half == 0) {
             float M = mx[0][srow];
@@ -400,6 +430,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
               part[AT_ROWS + srow] = Lsum;
             }
           }
+          if (srow < rows) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -410,6 +441,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
             }
             *reinterpret_cast<float4*>(part + 2 * AT_ROWS + srow * AT_D + 128 * half + 16 * sc8 + 4 * k) = acc;
           }
+          }
           aw_barrier();   // the dump is read before it is overwritten (and the set refilled)
         }
       }
@@ -417,13 +449,70 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       issue_v(vset, X2);
       C = X1;
       X1 = X2;
-      if (u + 3 - tbase >= 64) {   // the lanes' blocks are used up
+      if (set && u + 4 - tbase >= 64) {   // the lanes' blocks are used up
         tbase = u + 1;
         look_up();
       }
       X2 = unit(u + 3);
     }
   }
+}
+
+// Merges the pieces of pair blockIdx.y for its row blockIdx.x and applies the gate: thread d owns
+// column d.  The pieces are those of workgroups wf .. wl of the table, in that order; every wave
+// forms the weights of 64 pieces in its lanes while the first columns are on their way.
+__global__ __launch_bounds__(AT_D) void attn_paged_combine_kernel(PagedArgs p) {
+  const AttnArgs& a = p.a;
+  const int r = blockIdx.x, pair = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int PH = a.Hkv * a.qblocks;
+  const int2 te = reinterpret_cast<const int2*>(a.ws + (size_t)(a.nw + a.B * PH) * AT_PART)[pair];
+  const int b = pair / PH, ph = pair - b * PH, kvh = ph / a.qblocks;
+  const int q0 = (ph - kvh * a.qblocks) * a.QB;
+  const int i = (int)(((uint32_t)r * p.rep_mul) >> 16), h = kvh * a.n_rep + r - i * a.n_rep;
+  if (i >= min(a.QB, a.T - q0)) return;
+  const size_t bt = (size_t)b * a.T + q0 + i;
+  const float gl = a.gate ? bf16_to_f32(a.gate[bt * a.gate_row + (size_t)h * a.gate_head + tid]) : 0.f;
+  const int wf = te.x, np = wf < 0 ? 0 : te.y - wf + 1;
+  const float* base = a.ws + ((size_t)max(wf, 0) + pair) * AT_PART;
+  const float* col = base + 2 * AT_ROWS + r * AT_D + tid;
+  constexpr int AHEAD = 8;
+  float M = -INFINITY, l = 0.f, acc = 0.f;
+  for (int c = 0; c < np; c += 64) {
+    const int n = min(np - c, 64);
+    const float* piece = base + (size_t)(c + min(lane, n - 1)) * AT_PART;
+    float m = piece[r], ls = piece[AT_ROWS + r];
+    float v[AHEAD];
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) v[s] = col[(size_t)(c + min(s, n - 1)) * AT_PART];
+    if (lane >= n) {
+      m = -INFINITY;
+      ls = 0.f;
+    }
+    float mn = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
+    mn = fmaxf(mn, M);
+    const float shrink = M == -INFINITY ? 0.f : fast_exp2((M - mn) * a.cl2);
+    const float wgt = m == -INFINITY ? 0.f : fast_exp2((m - mn) * a.cl2);
+    ls *= wgt;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o, 64);
+    l = l * shrink + ls;
+    acc *= shrink;
+    M = mn;
+    for (int s = 0; s < n; s += AHEAD) {
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e)
+        if (s + e < n) acc += v[e] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), s + e));
+      if (s + AHEAD < n) {
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) v[e] = col[(size_t)(c + min(s + AHEAD + e, n - 1)) * AT_PART];
+      }
+    }
+  }
+  float val = l == 0.f ? 0.f : acc / l;   // no key seen: zeros
+  if (a.gate) val *= sigmoidf_(gl);
+  a.out[(bt * a.Hq + h) * AT_D + tid] = f32_to_bf16(val);
 }
 
 }  // namespace lollm
@@ -456,13 +545,15 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   int n_rep, QB, qblocks;
   int rc = attn_geometry(B, T, Hq, Hkv, D, (int)rows, &n_rep, &QB, &qblocks);
   if (rc) return rc;
+  if (Hkv > 65535) return LOLLM_EUNSUPPORTED;        // 32-bit offsets in a query block's tokens
   if (grid < 0 || grid > 1024) return LOLLM_EINVAL;  // pieces per pair <= combine table
   if (gate && (gate_head < D || gate_row < (Hq - 1LL) * gate_head + D)) return LOLLM_EINVAL;
   if (gate && (gate_row % 8 || gate_head % 8)) return LOLLM_EINVAL;
   const long long pairs = (long long)B * Hkv * qblocks;
-  if (pairs > 65535) return LOLLM_EUNSUPPORTED;      // the combine's grid
   const int nw = attn_grid(grid);
   if (nw <= 0 || nw > 1024) return LOLLM_EUNSUPPORTED;
+  const int groups = grid == 0 ? attn_prefill_groups(B, T, Hkv, n_rep, nw) : 0;   // lollm_attn_verify's rule
+  if (!groups && pairs > 65535) return LOLLM_EUNSUPPORTED;                        // the combine's grid
   if (!workspace || workspace_bytes < attn_ws_bytes(nw, pairs)) return LOLLM_EINVAL;
   PagedArgs p;
   AttnArgs& a = p.a;
@@ -475,11 +566,14 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   a.gate_row = gate_row; a.gate_head = gate_head;
   p.table = table; p.ks = k_scale; p.vs = v_scale; p.table_stride = table_stride;
   p.n_pages = n_pages; p.pshift = pshift;
+  p.rep_mul = (uint32_t)((65536 + n_rep - 1) / n_rep);
   hipStream_t st = (hipStream_t)stream;
+  if (groups) return attn_prefill_launch(a, groups, st, &p);
   if (f8)
     hipLaunchKernelGGL(attn_paged_kernel<true>, dim3(nw), dim3(AW_THREADS), 0, st, p);
   else
     hipLaunchKernelGGL(attn_paged_kernel<false>, dim3(nw), dim3(AW_THREADS), 0, st, p);
   if ((rc = launch_status())) return rc;
-  return attn_combine_launch(a, st);
+  hipLaunchKernelGGL(attn_paged_combine_kernel, dim3(n_rep * QB, (unsigned)pairs), dim3(AT_D), 0, st, p);
+  return launch_status();
 }

@@ -44,17 +44,26 @@ constexpr int AP_MIN_T = 16;                   // new positions per sequence
 constexpr int AP_FEW_ROWS = 64;                // tokens of a call that keeps the split-K kernels
 constexpr int AP_KEYS = 32;                    // keys per block
 constexpr int AP_AHEAD = 3;                    // operands read ahead of their products
-constexpr int AP_SET = AP_KEYS * AT_D * 2;     // 16 KB: K or V rows of a block
+constexpr int AP_DUMP = 32 * AT_D * 2;         // 16 KB: half of a wave's O on its way out
+
+// Where the keys are: AP_ROWS one slab per (sequence, KV head); AP_PAGES, AP_PAGES8 pages that a
+// table names (attn_paged.hip), in bf16 or as e4m3 codes with scales.
+enum { AP_ROWS, AP_PAGES, AP_PAGES8 };
 
 struct ApArgs {
   const uint16_t* q;       // (B, T, Hq, D)
   const uint16_t* kc;      // K cache
   const uint16_t* vc;      // V cache
   const int32_t* kv_len;   // (B) keys per sequence, the T new ones included
-  const uint16_t* gate;    // (B, T, Hq * D) or null
+  const uint16_t* gate;    // (B, T, Hq, D), strided, or null
   uint16_t* out;           // (B, T, Hq * D)
   long long seq_stride, head_stride;
   int B, T, Hq, Hkv, n_rep, QB, qtiles, max_len;
+  const int32_t* table;    // pages: (B, table_stride)
+  const float* ks;         // 8-bit pages: (n_pages, Hkv) scales
+  const float* vs;
+  long long table_stride, gate_row;
+  int gate_head, n_pages, pshift;
   uint32_t rep_mul;        // ceil(2^16 / n_rep): r / n_rep = r * rep_mul >> 16 for r < 256
   float cl2;
 };
@@ -74,11 +83,22 @@ __device__ __forceinline__ void ap_mfma_done(f32x16& s) { asm volatile("s_nop 15
 
 __device__ __forceinline__ int ap_div(int r, uint32_t mul) { return (int)(((uint32_t)r * mul) >> 16); }
 
-template <int RG>
+// A value that every lane loads from the same address, through the scalar cache: nothing that the
+// kernel writes is read so.
+template <typename T>
+__device__ __forceinline__ T ap_sload(const T* p, long long i) {
+  return ((const __attribute__((address_space(4))) T*)p)[i];
+}
+
+template <int RG, int KV>
 __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a) {
+  constexpr bool F8 = KV == AP_PAGES8;
+  constexpr int ROW = F8 ? AT_D : AT_D * 2;      // bytes of a key's row
+  constexpr int AP_SET = AP_KEYS * ROW;          // K or V rows of a block
   // separate arrays, so that the reads of one set are not ordered after the DMA into another
   __shared__ __attribute__((aligned(16))) unsigned char ks0[AP_SET], ks1[AP_SET], ks2[AP_SET];
   __shared__ __attribute__((aligned(16))) unsigned char vs0[AP_SET], vs1[AP_SET], vs2[AP_SET];
+  __shared__ __attribute__((aligned(16))) unsigned char dumps[F8 ? AP_WAVES * AP_DUMP : 16];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -97,11 +117,38 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // Loads of a block: wave w brings rows 8 w .. 8 w + 7 of K and of V, two rows (1 KB) per
   // instruction; the lane's source chunk undoes the swizzle of the place it writes.  Rows
   // past the sequence's end touch no memory.
+  // Pages: the wave's 8 rows of a block lie in one page, which a descriptor of their own covers
+  // (none of its bytes where the page is unmapped: zeros).  Page ids come through the scalar
+  // cache a block before they are needed, and two bits a block say which halves are mapped.
   constexpr int WR = AP_KEYS / AP_WAVES;
   static_assert(WR == 8, "the swizzles below take the row of the wave's 8");
-  const size_t cbase = (size_t)b * a.seq_stride + (size_t)kvh * a.head_stride;
-  const __amdgpu_buffer_rsrc_t krs = buf_rsrc(a.kc + cbase, (uint32_t)L * (AT_D * 2));
-  const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(a.vc + cbase, (uint32_t)L * (AT_D * 2));
+  const size_t cbase = KV == AP_ROWS ? (size_t)b * a.seq_stride + (size_t)kvh * a.head_stride : 0;
+  const __amdgpu_buffer_rsrc_t krs = buf_rsrc(a.kc + cbase, KV == AP_ROWS ? (uint32_t)L * (AT_D * 2) : 0u);
+  const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(a.vc + cbase, KV == AP_ROWS ? (uint32_t)L * (AT_D * 2) : 0u);
+  // page of keys 16 g .. of block j, -1: unmapped or past the end
+  auto page_at = [&](int j, int g) {
+    const uint32_t key = (uint32_t)(j * AP_KEYS + 16 * g);   // (no branch: O lives in all of them)
+    const int id = ap_sload(a.table, b * a.table_stride + (min(key, (uint32_t)max(L - 1, 0)) >> a.pshift));
+    return key < (uint32_t)L && (uint32_t)id < (uint32_t)a.n_pages ? id : -1;
+  };
+  auto mapped = [&](int j) { return (page_at(j, 0) >= 0 ? 1u : 0u) | (page_at(j, 1) >= 0 ? 2u : 0u); };
+  auto page_rsrc = [&](const uint16_t* pool, int id, int j) {
+    const int key = j * AP_KEYS + WR * wave;
+    const long long row = (((long long)max(id, 0) * a.Hkv + kvh) << a.pshift) + (key & ((1 << a.pshift) - 1));
+    const int rows = id >= 0 ? min(max(L - key, 0), WR) : 0;
+    return buf_rsrc((const unsigned char*)pool + row * ROW, (uint32_t)(rows * ROW));
+  };
+  // 8 bits: four rows a load, the 16-byte chunk c of row r at c ^ (r & 15)
+  const uint32_t l8 = 256u * (lane >> 4) + 16u * ((lane & 15) ^ (8 * (wave & 1) + (lane >> 4)));
+  auto issue_page = [&](unsigned char* d, const uint16_t* pool, int id, int j, uint32_t x, uint32_t swz) {
+    asm volatile("" : "+v"(x));
+    const __amdgpu_buffer_rsrc_t rs = page_rsrc(pool, id, j);
+    constexpr int N = F8 ? WR / 4 : WR / 2;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(d + ROW * WR * wave + 1024 * i), 16,
+                                               1024u * i + (x ^ (swz * i)) + (F8 ? 0u : (uint32_t)(ROW * h)), 0, 0, 0);
+  };
   // (row = 8 w + 2 i + h: its swizzle is the lane's part ^ that of 2 i; one register per cache,
   // the rest formed per load -- registers are what this kernel is short of)
   const uint32_t rl = (uint32_t)(WR * wave + h) * (AT_D * 2);
@@ -124,6 +171,16 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
       __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void_t*)(vd + 512 * WR * wave + 1024 * i), 16,
                                                blk + 1024u * i + (x ^ (64u * i)), 0, 0, 0);
   };
+  auto load_k = [&](unsigned char* kd, int id, int j) {
+    if constexpr (KV == AP_ROWS) issue_k(kd, j);
+    else if constexpr (F8) issue_page(kd, a.kc, id, j, l8, 64u);
+    else issue_page(kd, a.kc, id, j, kl, 32u);
+  };
+  auto load_v = [&](unsigned char* vd, int id, int j) {
+    if constexpr (KV == AP_ROWS) issue_v(vd, j);
+    else if constexpr (F8) issue_page(vd, a.vc, id, j, l8, 64u);
+    else issue_page(vd, a.vc, id, j, vl, 64u);
+  };
   // this wave's loads up to the last N have landed and its LDS accesses are complete, then
   // every wave's
 #define AP_BARRIER(N) asm volatile("s_waitcnt vmcnt(" #N ") lgkmcnt(0)\n\ts_barrier" ::: "memory")
@@ -143,17 +200,36 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     const int r = 32 * (RG * wave + rg) + l32, qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
     const bool live = qi < QB;
     qpos[rg] = live ? p0 + qi : -1;
-    const uint16_t* src = a.q + (((size_t)b * a.T + q0 + (live ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D + 8 * h;
+    const uint16_t* src = a.q + (((size_t)b * a.T + q0 + (live ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D;
 #pragma unroll
-    for (int ks = 0; ks < 16; ++ks)
-      Q[rg][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(src + 16 * ks));
+    for (int ks = 0; ks < 16; ++ks)   // (8 bits: a lane's 16 codes of K are two k-steps)
+      Q[rg][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(
+                                                 src + (F8 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1) : 16 * ks + 8 * h)));
   }
+  const int wg = wave >> 1;   // the half of a block that holds the wave's rows
+  int pg[3] = {-1, -1, -1}, pn = -1;   // pages of the wave's rows of blocks 0 .. 2, then 3
+  uint32_t vm = 3;                     // mapped halves: 2 bits from block j + 1 on
+  float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f};   // scales of the next block's K, of this one's V
+  auto scales = [&](const float* sc, int j, float (&to)[2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int id = page_at(j, g);
+      const float s = ap_sload(sc, (long long)max(id, 0) * a.Hkv + kvh);
+      to[g] = id >= 0 ? s : 1.f;
+    }
+  };
+  if constexpr (KV != AP_ROWS) {
+#pragma unroll
+    for (int j = 0; j < 3; ++j) pg[j] = page_at(j, wg);
+    pn = page_at(3, wg);
+  }
+  const uint32_t vm0 = KV == AP_ROWS ? 3u : mapped(0);
   AP_BARRIER(0);   // the zeroed sets, before any DMA into them (and Q: the counts below are the DMA's)
-  issue_k(ks0, 0);
-  issue_k(ks1, 1);
-  issue_v(vs0, 0);
-  issue_k(ks2, 2);
-  issue_v(vs1, 1);
+  load_k(ks0, pg[0], 0);
+  load_k(ks1, pg[1], 1);
+  load_v(vs0, pg[0], 0);
+  load_k(ks2, pg[2], 2);
+  load_v(vs1, pg[1], 1);
 
   // the positions this wave's rows span: the key blocks it sees, and which need a mask
   const int wq0 = ap_div(32 * RG * wave, a.rep_mul);
@@ -163,10 +239,12 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
 
   // LDS offsets of the operand reads: K row l32 at chunk 2 ks + h, V row x = 4 h + (lane % 16) / 4
   // at chunk 4 dt + 2 ((lane / 16) % 2) + (lane % 4) / 2; the k-step and the column tile
-  // enter by xor
-  const int ko = l32 * (AT_D * 2) + 16 * (h ^ (l32 & 15));
-  const int vxr = 4 * h + ((lane & 15) >> 2);
-  const int vo = vxr * (AT_D * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (2 * vxr)) + 8 * (lane & 1);
+  // enter by xor.  8 bits: V row 4 h + (r & 3) + 8 (r >> 2), r = (lane % 16) / 2, at chunk
+  // 2 dt + (lane / 16) % 2
+  const int ko = l32 * ROW + 16 * (h ^ (l32 & 15));
+  const int vxr = F8 ? 4 * h + ((lane & 7) >> 1) + (lane & 8) : 4 * h + ((lane & 15) >> 2);
+  const int vo = F8 ? vxr * ROW + 16 * (((lane >> 4) & 1) ^ vxr) + 8 * (lane & 1)
+                    : vxr * (AT_D * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (2 * vxr)) + 8 * (lane & 1);
 
   f32x16 O[RG][8];   // O^T: 32 columns x 32 rows per tile; lane's row = l32
   float m_ref[RG], l_s[RG];
@@ -185,9 +263,26 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   float base[RG], alpha[RG];
   bool moved;
   // S^T (32 keys x 32 rows) = K Q^T of block j, masked, and the row maxima
-  auto scores = [&](const unsigned char* kset, int j) {
+  auto scores = [&](const unsigned char* kset, int j, uint32_t there) {
     int kof = ko;
     asm volatile("" : "+v"(kof));
+    if constexpr (F8) {
+      const float sc = l32 < 16 ? ksc[0] : ksc[1];
+      u32x4_t kw[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kw[i] = *reinterpret_cast<const u32x4_t*>(kset + (kof ^ (32 * i)));
+#pragma unroll
+      for (int ks = 0; ks < 16; ++ks) {
+        const u32x4_t c = kw[(ks >> 1) & 1];
+        const bf16x8 kf = ks & 1 ? at_bf16(c.z, c.w, sc) : at_bf16(c.x, c.y, sc);
+#pragma unroll
+        for (int rg = 0; rg < RG; ++rg)
+          if (ks == 0) ap_mfma_first(S[rg], kf, Q[rg][0]); else ap_mfma(S[rg], kf, Q[rg][ks]);
+        const int kn = (ks >> 1) + 2;
+        if ((ks & 1) && kn < 8) kw[kn & 1] = *reinterpret_cast<const u32x4_t*>(kset + (kof ^ (32 * kn)));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
     bf16x8 kf[AP_AHEAD];
 #pragma unroll
     for (int i = 0; i < AP_AHEAD; ++i)
@@ -202,15 +297,17 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
         kf[ks % AP_AHEAD] = *reinterpret_cast<const bf16x8*>(kset + (kof ^ (32 * (kn & 7))) + 256 * (kn >> 3));
       __builtin_amdgcn_sched_barrier(0);   // no more operands ahead than the registers hold
     }
+    }
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) ap_mfma_done(S[rg]);
     const int key0 = j * AP_KEYS;
-    if (key0 + AP_KEYS - 1 > wmin) {   // acc r holds key 8 (r / 4) + 4 h + r % 4 of the block
+    if (key0 + AP_KEYS - 1 > wmin || (KV != AP_ROWS && there != 3)) {   // acc r holds key 8 (r / 4) + 4 h + r % 4
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg) {
         const int lim = qpos[rg] - key0 - 4 * h;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) S[rg][r] = 8 * (r >> 2) + (r & 3) <= lim ? S[rg][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r)
+          S[rg][r] = 8 * (r >> 2) + (r & 3) <= (KV == AP_ROWS || there & (r < 8 ? 1u : 2u) ? lim : -1) ? S[rg][r] : -INFINITY;
       }
     }
     bool any = false;
@@ -258,30 +355,38 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // are all masked.
   auto step = [&](const unsigned char* knext, const unsigned char* vset, int j) {
     if (j >= wblk) return;
-    scores(knext, j + 1);
+    scores(knext, j + 1, vm & 3);
     int vof = vo;
     asm volatile("" : "+v"(vof));
     auto read_v = [&](int n) {   // operand n = 2 dt + k2, by transposing reads (attn_verify's key order)
       const int dt = n >> 1, k2 = n & 1;
+      if constexpr (F8) {   // 8 codes, converted when their product comes
+        const i32x2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_i32x2_t*)(vset + (vof ^ (32 * dt)) + 16 * ROW * k2));
+        return __builtin_bit_cast(u32x2_t, v);
+      } else {
       const unsigned char* vp = vset + (vof ^ (64 * (dt & 3))) + 256 * (dt >> 2) + 16 * (AT_D * 2) * k2;
       const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)vp);
       const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vp + 8 * (AT_D * 2)));
       const u32x2_t w0 = __builtin_bit_cast(u32x2_t, v0), w1 = __builtin_bit_cast(u32x2_t, v1);
       return __builtin_bit_cast(bf16x8, u32x4_t{w0.x, w0.y, w1.x, w1.y});
+      }
     };
-    bf16x8 vf[AP_AHEAD];
+    decltype(read_v(0)) vf[AP_AHEAD];
     u32x4_t Pn[RG][2], Pm[RG][2];
     float pe[RG];
 #pragma unroll
     for (int i = 0; i < AP_AHEAD; ++i) vf[i] = read_v(i);
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
+      bf16x8 vA;
+      if constexpr (F8) vA = at_bf16(vf[n % AP_AHEAD].x, vf[n % AP_AHEAD].y, vsc[n & 1]); else vA = vf[n % AP_AHEAD];
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg)
-        O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AP_AHEAD], P[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+        O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, P[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg)
-        O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AP_AHEAD], Pl[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+        O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
       if (n + AP_AHEAD < 16) vf[n % AP_AHEAD] = read_v(n + AP_AHEAD);
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg) {
@@ -309,9 +414,14 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     rescale();
   };
 
-  AP_BARRIER(16);   // block 0 of K, the first 4 of the 20 loads
+  if constexpr (F8) {
+    scales(a.ks, 0, ksc);
+    AP_BARRIER(8);    // block 0 of K, the first 2 of the 10 loads
+  } else {
+    AP_BARRIER(16);   // block 0 of K, the first 4 of the 20 loads
+  }
   if (wblk > 0) {
-    scores(ks0, 0);
+    scores(ks0, 0, vm0);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
       u32x4_t Pn[2], Pm[2];
@@ -333,22 +443,44 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     }
     rescale();
   }
-  // Barrier before step j: blocks j + 1 of K and j of V have landed (the 8 loads after them may
-  // be in flight), and every wave is done with K of block j and V of block j - 1, whose sets
-  // the loads of blocks j + 3 and j + 2 take.
+  // Barrier before step j: blocks j + 1 of K and j of V have landed (the 8 loads after them, 4 of
+  // 8-bit pages, may be in flight), and every wave is done with K of block j and V of block j - 1,
+  // whose sets the loads of blocks j + 3 and j + 2 take.
+  if constexpr (F8) {
+    scales(a.ks, 1, ksc);
+    scales(a.vs, 0, vsc);
+  }
+  if constexpr (KV != AP_ROWS) vm = mapped(1);
+  auto turn = [&](unsigned char* kfree, unsigned char* vfree, const unsigned char* knext, const unsigned char* vset,
+                  int j) {
+    if constexpr (F8) AP_BARRIER(4); else AP_BARRIER(8);
+    load_k(kfree, pn, j + 3);
+    load_v(vfree, pg[2], j + 2);
+    float kn[2], vn[2];
+    uint32_t mn = 3;
+    if constexpr (KV != AP_ROWS) {   // what the next step needs, on its way during this one
+      pg[2] = pn;
+      pn = page_at(j + 4, wg);
+      mn = mapped(j + 2);
+    }
+    if constexpr (F8) {
+      scales(a.ks, j + 2, kn);
+      scales(a.vs, j + 1, vn);
+    }
+    step(knext, vset, j);
+    vm = mn;
+    if constexpr (F8) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        ksc[g] = kn[g];
+        vsc[g] = vn[g];
+      }
+    }
+  };
   for (int j = 0; j < nblk; j += 3) {
-    AP_BARRIER(8);
-    issue_k(ks0, j + 3);
-    issue_v(vs2, j + 2);
-    step(ks1, vs0, j);
-    AP_BARRIER(8);
-    issue_k(ks1, j + 4);
-    issue_v(vs0, j + 3);
-    step(ks2, vs1, j + 1);
-    AP_BARRIER(8);
-    issue_k(ks2, j + 5);
-    issue_v(vs1, j + 4);
-    step(ks0, vs2, j + 2);
+    turn(ks0, vs2, ks1, vs0, j);
+    turn(ks1, vs0, ks2, vs1, j + 1);
+    turn(ks2, vs1, ks0, vs2, j + 2);
   }
   AP_BARRIER(0);   // no load in flight, every wave done with the sets: the dumps take them
 #undef AP_BARRIER
@@ -356,7 +488,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // Epilogue in two halves of the columns: O / l through the wave's own 16 KB (fp32, chunk c
   // of row r at c ^ (r & 15)), then whole half rows with the gate: 8 columns per lane,
   // 16-byte loads and stores.
-  unsigned char* dump = wave == 0 ? ks0 : (wave == 1 ? ks1 : (wave == 2 ? ks2 : vs0));
+  unsigned char* dump = F8 ? dumps + AP_DUMP * wave : wave == 0 ? ks0 : (wave == 1 ? ks1 : (wave == 2 ? ks2 : vs0));
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_s[rg]), __float_as_uint(l_s[rg]), false, false);
@@ -374,7 +506,9 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
         const int r = 32 * (RG * wave + rg) + 4 * it + (lane >> 4), qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
         live[it] = qi < QB;
         oo[it] = (((size_t)b * a.T + q0 + (live[it] ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D + 128 * half + 8 * c8;
-        if (a.gate) g[it] = *reinterpret_cast<const u32x4_t*>(a.gate + oo[it]);
+        if (a.gate)
+          g[it] = *reinterpret_cast<const u32x4_t*>(a.gate + ((size_t)b * a.T + q0 + (live[it] ? qi : 0)) * a.gate_row +
+                                                    (size_t)(kvh * a.n_rep + hr) * a.gate_head + 128 * half + 8 * c8);
       }
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
@@ -433,21 +567,37 @@ int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus) {
   return 0;
 }
 
-int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st) {
+template <int KV>
+static void prefill_start(const ApArgs& a, int rg, unsigned n, hipStream_t st) {
+  if (rg == 2)
+    hipLaunchKernelGGL((attn_prefill_kernel<2, KV>), dim3(n), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_prefill_kernel<1, KV>), dim3(n), dim3(256), 0, st, a);
+}
+
+int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st, const PagedArgs* paged) {
   ApArgs a;
   a.q = v.q; a.kc = v.kc; a.vc = v.vc; a.kv_len = v.kv_len; a.gate = v.gate; a.out = v.out;
   a.seq_stride = v.seq_stride; a.head_stride = v.head_stride;
+  a.gate_row = v.gate_row; a.gate_head = v.gate_head;
   a.B = v.B; a.T = v.T; a.Hq = v.Hq; a.Hkv = v.Hkv; a.n_rep = v.n_rep; a.max_len = v.max_len;
   a.cl2 = v.cl2;
   a.rep_mul = (uint32_t)((65536 + v.n_rep - 1) / v.n_rep);
   a.QB = 128 * rg / v.n_rep < v.T ? 128 * rg / v.n_rep : v.T;
   a.qtiles = (v.T + a.QB - 1) / a.QB;
+  a.table = nullptr; a.ks = a.vs = nullptr; a.table_stride = 0; a.n_pages = a.pshift = 0;
   const long long n = (long long)a.qtiles * v.B * v.Hkv;
   if (n > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;
-  if (rg == 2)
-    hipLaunchKernelGGL(attn_prefill_kernel<2>, dim3((unsigned)n), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL(attn_prefill_kernel<1>, dim3((unsigned)n), dim3(256), 0, st, a);
+  if (!paged) {
+    prefill_start<AP_ROWS>(a, rg, (unsigned)n, st);
+  } else {
+    a.table = paged->table; a.ks = paged->ks; a.vs = paged->vs; a.table_stride = paged->table_stride;
+    a.n_pages = paged->n_pages; a.pshift = paged->pshift;
+    if (paged->ks)
+      prefill_start<AP_PAGES8>(a, rg, (unsigned)n, st);
+    else
+      prefill_start<AP_PAGES>(a, rg, (unsigned)n, st);
+  }
   return launch_status();
 }
 

@@ -385,8 +385,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs a) {
   if (r >= a.n_rep * QB) return;
   const int hr = r / QB, i = r % QB, h = kvh * a.n_rep + hr;
   const size_t o = ((size_t)b * a.T + q0 + i) * a.Hq * AT_D + (size_t)h * AT_D + tid;
-  const size_t go = ((size_t)b * a.T + q0 + i) * a.gate_row + (size_t)h * a.gate_head + tid;
-  const float gl = a.gate ? bf16_to_f32(a.gate[go]) : 0.f;   // in flight from the start
+  const float gl = a.gate ? bf16_to_f32(a.gate[o]) : 0.f;   // in flight from the start
   const int4 te = reinterpret_cast<const int4*>(a.ws + (size_t)(a.nw + a.B * PH) * AT_PART)[pair];
   const int wf = te.x, wl = te.y;
   const long long U = (long long)(((uint64_t)(uint32_t)te.w << 32) | (uint32_t)te.z);
@@ -444,11 +443,6 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnArgs a) {
   float val = lsum > 0.f ? acc / lsum : 0.f;
   if (a.gate) val *= sigmoidf_(gl);
   a.out[o] = f32_to_bf16(val);
-}
-
-int attn_combine_launch(const AttnArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(attn_combine_kernel, dim3(AT_ROWS, a.B * a.Hkv * a.qblocks), dim3(256), 0, st, a);
-  return launch_status();
 }
 
 // Workspace: one fp32 piece per workgroup plus one per pair, then the combine's table
@@ -524,5 +518,6 @@ LOLLM_API int lollm_attn_verify(const void* q, const void* k_cache, const void* 
   }
   hipLaunchKernelGGL(attn_verify_kernel, dim3(nw), dim3(AW_THREADS), 0, st, a);
   if ((rc = launch_status())) return rc;
-  return attn_combine_launch(a, st);
+  hipLaunchKernelGGL(attn_combine_kernel, dim3(AT_ROWS, B * Hkv * qblocks), dim3(256), 0, st, a);
+  return launch_status();
 }

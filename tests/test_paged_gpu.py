@@ -31,9 +31,10 @@ def attend_case(seed, B, T, Hq, Hkv, lens, P, bits, holes=(), spare=2):
     g = gen(seed)
     width = max(1, max(-(-L // P) for L in lens))
     n = sum(-(-L // P) for L in lens) + spare
+    first = lens[0] == 0 or (0, 0) in holes            # page 0 of the pool is nobody's now and then
     k, ks = pool(g, n, Hkv, P, bits)
     v, vs = pool(g, n, Hkv, P, bits)
-    perm = torch.randperm(n, generator=g).tolist()
+    perm = [p for p in torch.randperm(n, generator=g).tolist() if not first or p]
     table = torch.full((B, width), -1, dtype=torch.int32)
     dead = torch.ones(n, P, dtype=torch.bool)
     for b, L in enumerate(lens):
@@ -44,6 +45,9 @@ def attend_case(seed, B, T, Hq, Hkv, lens, P, bits, holes=(), spare=2):
             p = perm.pop()
             table[b, i] = p
             dead[p, :max(0, min(P, L - i * P))] = False
+    if bits == 8:                                      # pages of nobody have no scale either
+        nobody = dead.all(1)
+        ks[nobody], vs[nobody] = float("nan"), float("nan")
     nan = torch.tensor(float("nan"))
     for x in (k, v):
         x.view(torch.uint8 if bits == 8 else torch.bfloat16).masked_fill_(
@@ -76,6 +80,11 @@ def check_attention(case, Hq, **kw):
     qd, kd, vd, td, ld, gd, ksd, vsd = cuda(q, k, v, table, lens, qkv, ks, vs)
     out = ops.attn_paged(qd, kd, vd, td, ld, gates(gd, Hq), k_scale=ksd, v_scale=vsd, **kw)
     torch.cuda.synchronize()
+    # nothing of what lay in the workspace counts
+    ws = torch.full((ops.attn_paged_workspace_bytes(*q.shape[:3], k.shape[1], D, kw.get("grid", 0)),), 255,
+                    dtype=torch.uint8, device="cuda")
+    again = ops.attn_paged(qd, kd, vd, td, ld, gates(gd, Hq), k_scale=ksd, v_scale=vsd, workspace=ws, **kw)
+    assert torch.equal(again, out)
     got = out.cpu().double()
     assert got.isfinite().all()
     worst = ((got - ref).abs() - tol).max()
