@@ -100,20 +100,27 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   const int w = blockIdx.x;
   const int PH = a.Hkv * a.qblocks;
 
-  const long long U = (long long)PH * build_prefix(a, pre, len, tmp);
-  // one block a workgroup where there are fewer blocks: no workgroup between a pair's has none
-  const int nw = (int)min((long long)a.nw, U);
-  const long long u0 = w < nw ? unit_begin(U, w, nw) : 0, u1 = w < nw ? unit_begin(U, w + 1, nw) : 0;
+  // All pairs' blocks, dealt out in equal ranges, the first `more` of them one block longer (the
+  // host keeps U below 2^31); one block a workgroup where there are fewer blocks, so that no
+  // workgroup between a pair's has none.
+  const uint32_t U = (uint32_t)PH * (uint32_t)build_prefix(a, pre, len, tmp);
+  const uint32_t nw = min((uint32_t)a.nw, U), each = U / max(nw, 1u), more = U - each * nw;
+  auto owner = [&](uint32_t u) {
+    const uint32_t cut = more * (each + 1);
+    return (int)(u < cut ? u / (each + 1) : more + (u - cut) / each);
+  };
+  const uint32_t u0 = min((uint32_t)w, nw) * each + min((uint32_t)w, more);
+  const uint32_t u1 = (uint32_t)w < nw ? u0 + each + ((uint32_t)w < more) : u0;
   auto build_table = [&]() {
     const int npairs = a.B * PH;
     int2* tab = reinterpret_cast<int2*>(a.ws + (size_t)(a.nw + npairs) * AT_PART);
-    for (int pr = w * AW_THREADS + tid; pr < npairs; pr += (U ? nw : a.nw) * AW_THREADS) {
+    for (int pr = w * AW_THREADS + tid; pr < npairs; pr += (U ? (int)nw : a.nw) * AW_THREADS) {
       const int pb = pr / PH, pph = pr % PH, pnb = pre[pb + 1] - pre[pb];
       int wf = -1, wl = -1;
       if (pnb > 0) {
-        const long long first = (long long)PH * pre[pb] + (long long)pph * pnb;
-        wf = unit_owner(U, first, nw);
-        wl = unit_owner(U, first + pnb - 1, nw);
+        const uint32_t first = (uint32_t)PH * pre[pb] + (uint32_t)pph * pnb;
+        wf = owner(first);
+        wl = owner(first + pnb - 1);
       }
       tab[pr] = make_int2(wf, wl);
     }
@@ -124,21 +131,20 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   }
 
   // The lane's block of the 64 from tbase on.
-  long long tbase = u0;
+  uint32_t tbase = u0;
   int tb = 0, tph = 0, tj = 0, tL = 0, tp[2];
   float tks[2] = {1.f, 1.f}, tvs[2] = {1.f, 1.f};
   auto look_up = [&]() {
-    const long long u = min(tbase + lane, u1 - 1);
+    const uint32_t u = min(tbase + lane, u1 - 1);
     int lo = 0, hi = a.B - 1;   // the last sequence that begins at or before u: not an empty one
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if ((long long)PH * pre[mid] <= u) lo = mid; else hi = mid - 1;
+      if ((uint32_t)PH * pre[mid] <= u) lo = mid; else hi = mid - 1;
     }
-    const int nb = pre[lo + 1] - pre[lo];
-    const long long r = u - (long long)PH * pre[lo];
+    const uint32_t nb = pre[lo + 1] - pre[lo], r = u - (uint32_t)PH * pre[lo];
     tb = lo;
     tph = (int)(r / nb);
-    tj = (int)(r - (long long)tph * nb);
+    tj = (int)(r - tph * nb);
     tL = len[lo];
     const int kvh = tph / a.qblocks;
 #pragma unroll
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
     // (waited for here: else the compiler drains every load of the loop where it reads these)
     asm volatile("" : "+v"(tp[0]), "+v"(tp[1]), "+v"(tks[0]), "+v"(tks[1]), "+v"(tvs[0]), "+v"(tvs[1]));
   };
-  auto unit = [&](long long u) {
+  auto unit = [&](uint32_t u) {
     const int i = (int)(u - tbase);
     const bool live = u < u1;
     PgUnit X;
@@ -175,19 +181,20 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 
   // Loads of a block (all unconditional; past the range no page is mapped).
   constexpr int KL = Set::ROW / 32;   // 16-byte loads of a key's row per lane (two lanes a row)
-  u32x4_t kr[KL], qr[4];
+  constexpr int KAHEAD = F8 ? 2 : 1;  // blocks that K is asked for ahead of its products
+  u32x4_t kr[KAHEAD][KL], qr[4];
   const int pmask = (1 << p.pshift) - 1;
   auto row_of = [&](const PgUnit& X, int page, int key) {   // the pool's row of a key in that page
     const int kvh = X.ph / a.qblocks;
     return (((long long)page * a.Hkv + kvh) << p.pshift) + (key & pmask);
   };
-  auto issue_k = [&](const PgUnit& X) {
+  auto issue_k = [&](u32x4_t (&to)[KL], const PgUnit& X) {
     const int key0 = X.j * AT_BLOCK + PG_WKEYS * wave;
     const long long r0 = row_of(X, max(X.page[0], 0), key0), r1 = row_of(X, max(X.page[1], 0), key0 + 16);
     const unsigned char* src = reinterpret_cast<const unsigned char*>(a.kc) +
                                (l32 < 16 ? r0 : r1) * Set::ROW + (l32 & 15) * Set::ROW + 16 * h;
 #pragma unroll
-    for (int i = 0; i < KL; ++i) kr[i] = *reinterpret_cast<const u32x4_t*>(src + 32 * i);
+    for (int i = 0; i < KL; ++i) to[i] = *reinterpret_cast<const u32x4_t*>(src + 32 * i);
   };
   auto issue_v = [&](unsigned char* vset, const PgUnit& X) {
     unsigned char* dst = vset + wave * Set::WAVE;
@@ -237,8 +244,10 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   look_up();
   PgUnit C = unit(u0), X1 = unit(u0 + 1), X2 = unit(u0 + 2);
   issue_q(C);
+  // (in the loop's own order, for the counts of its waits)
+  if constexpr (F8) issue_k(kr[0], C);
   issue_v(vs0, C);
-  issue_k(C);
+  issue_k(kr[KAHEAD - 1], F8 ? X1 : C);
   issue_v(vs1, X1);
   build_table();
 
@@ -247,11 +256,11 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   const int lq = (int)(((uint32_t)l32 * p.rep_mul) >> 16);   // the lane's position in its query block
   int qpos = 0, rows = 0;
 
-  for (long long ub = u0; ub < u1; ub += 2) {
+  for (uint32_t ub = u0; ub < u1; ub += 2) {
 #pragma unroll
     for (int set = 0; set < 2; ++set) {
       unsigned char* vset = set ? vs1 : vs0;
-      const long long u = ub + set;
+      const uint32_t u = ub + set;
       const bool live = u < u1;
       const bool any = live && (C.page[0] & C.page[1]) != -1;   // keys of this wave to look at
       const int nb = nblk_of(C.L);
@@ -283,7 +292,8 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
           const unsigned char* qp = qs + l32 * PG_QROW + 32 * h;   // columns 32 i + 16 h ..
 #pragma unroll
           for (int i = 0; i < KL; ++i) {
-            const bf16x8 k0 = at_bf16(kr[i].x, kr[i].y, sc), k1 = at_bf16(kr[i].z, kr[i].w, sc);
+            const u32x4_t c = kr[set][i];
+            const bf16x8 k0 = at_bf16(c.x, c.y, sc), k1 = at_bf16(c.z, c.w, sc);
             S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, *reinterpret_cast<const bf16x8*>(qp + 64 * i), S, 0, 0, 0);
             S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, *reinterpret_cast<const bf16x8*>(qp + 64 * i + 16), S, 0, 0, 0);
           }
@@ -291,19 +301,24 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 #pragma unroll
           for (int i = 0; i < KL; ++i) {
             const bf16x8 qv = *reinterpret_cast<const bf16x8*>(qs + l32 * PG_QROW + 16 * h + 32 * i);
-            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[i]), qv, S, 0, 0, 0);
+            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[0][i]), qv, S, 0, 0, 0);
           }
         }
       }
       // Q of the next block's pair (staged at that block's start)
       if (u + 1 < u1 && X1.j == 0) issue_q(X1);
-      issue_k(X1);   // K of the next block into the registers S consumed
-      // V of this block has landed: at least V and K of the next one were asked for after it.
-      // (Counted here and V read by hand: where the compiler cannot tell the sets apart it waits
-      // for both, and nothing is on its way while the products run.)
-      if constexpr (F8) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
-      static_assert(KL + PG_WKEYS * Set::ROW / 1024 == (F8 ? 16 : 32), "the counts above");
+      // K into the registers S consumed, V of this block landed: after it at least V of the next
+      // block and K of the next KAHEAD were asked for.  (Counted here and V read by hand: where
+      // the compiler cannot tell the sets apart it waits for both, and nothing is on its way while
+      // the products run.)
+      if constexpr (F8) {
+        issue_k(kr[set], X2);
+        asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
+      } else {
+        issue_k(kr[0], X1);
+        asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
+      }
+      static_assert(KAHEAD * KL + PG_WKEYS * Set::ROW / 1024 == (F8 ? 24 : 32), "the counts above");
 
       if (any) {
         // mask: acc r holds key 32 wave + 8 (r / 4) + 4 h + r % 4 of the block
@@ -321,14 +336,23 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         // the reference max moves (and l, O are rescaled) only when a row's block max exceeds it
         // by more than 16 in the exponent: attn_verify's rule, each row's own decision
         const bool big = (bm - m_ref) * a.cl2 > 16.f;
-        if (__builtin_amdgcn_readfirstlane((int)(__ballot(big) != 0))) {
-          const float mn = big ? fmaxf(m_ref, bm) : m_ref;
-          const float alpha = (!big || mn == -INFINITY) ? 1.f : fast_exp2((m_ref - mn) * a.cl2);
-          m_ref = mn;
+        const bool had = m_ref != -INFINITY;   // (nothing to rescale at a row's first block)
+        if (__builtin_amdgcn_readfirstlane((int)(__ballot(big && had) != 0))) {
+          const float alpha = big && had ? fast_exp2((m_ref - bm) * a.cl2) : 1.f;
           l_s *= alpha;
 #pragma unroll
-          for (int dt = 0; dt < 8; ++dt) O[dt] *= alpha;
+          for (int dt = 0; dt < 8; ++dt) {
+            // (O stays in accumulator registers but for the tile at hand: without the pins the
+            // compiler copies all of it to vector registers and back in every block)
+            asm volatile("" : "+a"(O[dt]));
+            O[dt] *= alpha;
+            asm volatile("" : "+a"(O[dt]));
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) asm volatile("" : "+a"(O[dt]));
+        m_ref = big ? bm : m_ref;
         const float base = m_ref == -INFINITY ? 0.f : m_ref * a.cl2;
         float e[16];
 #pragma unroll
@@ -554,6 +578,7 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   if (nw <= 0 || nw > 1024) return LOLLM_EUNSUPPORTED;
   const int groups = grid == 0 ? attn_prefill_groups(B, T, Hkv, n_rep, nw) : 0;   // lollm_attn_verify's rule
   if (!groups && pairs > 65535) return LOLLM_EUNSUPPORTED;                        // the combine's grid
+  if (!groups && pairs * (rows / AT_BLOCK + 1) > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;   // 32-bit block numbers
   if (!workspace || workspace_bytes < attn_ws_bytes(nw, pairs)) return LOLLM_EINVAL;
   PagedArgs p;
   AttnArgs& a = p.a;
