@@ -23,14 +23,15 @@
 //      v_cvt_scalef32_pk_bf16_fp8, which applies the scale.
 // Weights enter the product with V as hi + lo bf16 (attn_prefill.hip): the kernel waits for
 // memory, and the second product costs it nothing.
+#include <type_traits>
+
 #include "attn_common.h"
 
 namespace lollm {
 
 constexpr int PG_WKEYS = AT_BLOCK / AW_WAVES;   // 32 keys of each block per wave
 constexpr int PG_QROW = AT_D * 2 + 16;          // padded Q row in LDS
-constexpr int PG_OROW = AT_D / 2 + 4;           // padded floats per row of an O half-dump
-constexpr int PG_DUMP = AW_WAVES * AT_ROWS * PG_OROW * 4;
+constexpr int PG_DUMP = AW_WAVES * AT_ROWS * (AT_D / 2 + 4) * 4;   // half of a pair's O of four waves
 
 template <bool F8>
 struct PagedSet {   // the V rows of a block in LDS
@@ -146,21 +147,35 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
     tph = (int)(r / nb);
     tj = (int)(r - tph * nb);
     tL = len[lo];
-    const int kvh = tph / a.qblocks;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int key = tj * AT_BLOCK + PG_WKEYS * wave + 16 * g;
       const bool in = key >= 0 && key < tL;   // (a table of 2^31 rows: a last block's keys may wrap)
       const int id = in ? p.table[(long long)lo * p.table_stride + (key >> p.pshift)] : -1;
       tp[g] = id >= 0 && id < p.n_pages ? id : -1;
-      if constexpr (F8) {
+    }
+  };
+  auto look_up_scales = [&]() {
+    if constexpr (F8) {
+      const int kvh = tph / a.qblocks;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
         const size_t s = (size_t)max(tp[g], 0) * a.Hkv + kvh;
-        tks[g] = tp[g] >= 0 ? p.ks[s] : 1.f;
-        tvs[g] = tp[g] >= 0 ? p.vs[s] : 1.f;   // (V's rows are zeros there: no NaN may meet them)
+        tks[g] = p.ks[s];
+        tvs[g] = p.vs[s];
       }
     }
-    // (waited for here: else the compiler drains every load of the loop where it reads these)
-    asm volatile("" : "+v"(tp[0]), "+v"(tp[1]), "+v"(tks[0]), "+v"(tks[1]), "+v"(tvs[0]), "+v"(tvs[1]));
+  };
+  // (an unmapped page's rows of V are zeros: no NaN for a scale may meet them)
+  auto unit_scales = [&](PgUnit& X, uint32_t u) {
+    const int i = (int)(u - tbase);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int k = __builtin_amdgcn_readlane(__float_as_int(tks[g]), i);
+      const int v = __builtin_amdgcn_readlane(__float_as_int(tvs[g]), i);
+      X.ks[g] = __int_as_float(X.page[g] >= 0 ? k : 0x3f800000);
+      X.vs[g] = __int_as_float(X.page[g] >= 0 ? v : 0x3f800000);
+    }
   };
   auto unit = [&](uint32_t u) {
     const int i = (int)(u - tbase);
@@ -173,8 +188,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       X.page[g] = live ? __builtin_amdgcn_readlane(tp[g], i) : -1;
-      X.ks[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(tks[g]), i));
-      X.vs[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(tvs[g]), i));
+      X.ks[g] = X.vs[g] = 1.f;
     }
     return X;
   };
@@ -243,12 +257,18 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 
   look_up();
   PgUnit C = unit(u0), X1 = unit(u0 + 1), X2 = unit(u0 + 2);
+  look_up_scales();   // before the rows: here when these are
   issue_q(C);
   // (in the loop's own order, for the counts of its waits)
   if constexpr (F8) issue_k(kr[0], C);
   issue_v(vs0, C);
   issue_k(kr[KAHEAD - 1], F8 ? X1 : C);
   issue_v(vs1, X1);
+  if constexpr (F8) {
+    unit_scales(C, u0);
+    unit_scales(X1, u0 + 1);
+    unit_scales(X2, u0 + 2);
+  }
   build_table();
 
   f32x16 O[8];            // O^T: d-tile dt (32 columns) x the 32 rows; lane row = l32
@@ -283,9 +303,9 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         aw_barrier();
       }
       // S^T (32 keys x 32 rows) = K Q^T
-      f32x16 S;
+      f32x16 S, S1;   // two chains: a product waits for the one before the last
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[r] = 0.f;
+      for (int r = 0; r < 16; ++r) S[r] = S1[r] = 0.f;
       if (any) {
         if constexpr (F8) {
           const float sc = l32 < 16 ? C.ks[0] : C.ks[1];
@@ -295,13 +315,14 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
             const u32x4_t c = kr[set][i];
             const bf16x8 k0 = at_bf16(c.x, c.y, sc), k1 = at_bf16(c.z, c.w, sc);
             S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, *reinterpret_cast<const bf16x8*>(qp + 64 * i), S, 0, 0, 0);
-            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, *reinterpret_cast<const bf16x8*>(qp + 64 * i + 16), S, 0, 0, 0);
+            S1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, *reinterpret_cast<const bf16x8*>(qp + 64 * i + 16), S1, 0, 0, 0);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < KL; ++i) {
             const bf16x8 qv = *reinterpret_cast<const bf16x8*>(qs + l32 * PG_QROW + 16 * h + 32 * i);
-            S = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[0][i]), qv, S, 0, 0, 0);
+            f32x16& s = i & 1 ? S1 : S;
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kr[0][i]), qv, s, 0, 0, 0);
           }
         }
       }
@@ -329,7 +350,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int kk = 8 * (r >> 2) + (r & 3);
-          S[r] = kk <= (r < 8 ? lim0 : lim1) ? S[r] : -INFINITY;
+          S[r] = kk <= (r < 8 ? lim0 : lim1) ? S[r] + S1[r] : -INFINITY;
           bm = fmaxf(bm, S[r]);
         }
         bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
@@ -412,61 +433,68 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       }
 
       if (seg_last) {
-        // merge the four waves' (m, l, O) of this pair into the workgroup's piece, in two halves
-        // of d: each wave dumps its O (straight from the accumulators), then every thread sums
-        // one row's 16 columns with the waves' weights exp(m_w - M)
+        // merge the four waves' (m, l, O) of this pair into the workgroup's piece: each wave dumps
+        // its O straight from the accumulators, then every thread sums 16 columns of a row with
+        // the waves' weights exp(m_w - M).  Up to 16 rows (few tokens have no more) go in one
+        // turn, more in two turns of half the columns.
         const float lrow = l_s + __shfl_xor(l_s, 32, 64);
         aw_barrier();   // every wave is done reading this set
         if (h == 0) {
           mx[wave][l32] = m_ref;
           lx[wave][l32] = lrow;
         }
-        const int pair = C.b * PH + C.ph;
-        float* part = a.ws + ((size_t)w + pair) * AT_PART;
+        float* part = a.ws + ((size_t)w + C.b * PH + C.ph) * AT_PART;
         float* dump = reinterpret_cast<float*>(F8 ? own_dump : vset);
-        const int srow = tid >> 3, sc8 = tid & 7;
-        float wgt[AW_WAVES];
+        // columns D0 .. of the rows that the wave has, WIDE of them, then their sum
+        auto turn = [&](auto first, auto wide) {
+          constexpr int D0 = decltype(first)::value, WIDE = decltype(wide)::value;
+          constexpr int ROWS = WIDE == AT_D ? 16 : AT_ROWS, OROW = WIDE + 4, TPR = AW_THREADS / ROWS;
+          static_assert(AW_WAVES * ROWS * OROW * 4 <= PG_DUMP, "a turn fits the dump");
+          if (l32 < rows) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (l32 < rows) {   // (few tokens leave most of the 32 rows empty)
+            for (int dt = 0; dt < WIDE / 32; ++dt)
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<float4*>(dump + (wave * AT_ROWS + l32) * PG_OROW + 32 * dt + 8 * q + 4 * h) =
-                  make_float4(O[4 * half + dt][4 * q], O[4 * half + dt][4 * q + 1], O[4 * half + dt][4 * q + 2],
-                              O[4 * half + dt][4 * q + 3]);
+              for (int q = 0; q < 4; ++q) {
+                const f32x16& o = O[D0 / 32 + dt];
+                *reinterpret_cast<float4*>(dump + (wave * ROWS + l32) * OROW + 32 * dt + 8 * q + 4 * h) =
+                    make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+              }
           }
           aw_barrier();
-          if (half == 0) {
-            float M = mx[0][srow];
+          const int row = tid / TPR, c4 = 4 * (tid % TPR);
+          if (row < rows) {
+            float M = mx[0][row], Lsum = 0.f, wgt[AW_WAVES];
 #pragma unroll
-            for (int ww = 1; ww < AW_WAVES; ++ww) M = fmaxf(M, mx[ww][srow]);
-            float Lsum = 0.f;
+            for (int ww = 1; ww < AW_WAVES; ++ww) M = fmaxf(M, mx[ww][row]);
 #pragma unroll
             for (int ww = 0; ww < AW_WAVES; ++ww) {
-              const float mw = mx[ww][srow];
+              const float mw = mx[ww][row];
               wgt[ww] = mw == -INFINITY ? 0.f : fast_exp2((mw - M) * a.cl2);
-              Lsum += lx[ww][srow] * wgt[ww];
+              Lsum += lx[ww][row] * wgt[ww];
             }
-            if (sc8 == 0) {
-              part[srow] = M;
-              part[AT_ROWS + srow] = Lsum;
+            if (D0 == 0 && c4 == 0) {
+              part[row] = M;
+              part[AT_ROWS + row] = Lsum;
             }
-          }
-          if (srow < rows) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < 4; ++k) {
+              const int c = c4 + 4 * TPR * k;
+              float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int ww = 0; ww < AW_WAVES; ++ww) {
-              const float4 v = *reinterpret_cast<const float4*>(dump + (ww * AT_ROWS + srow) * PG_OROW + 16 * sc8 + 4 * k);
-              acc.x += wgt[ww] * v.x; acc.y += wgt[ww] * v.y; acc.z += wgt[ww] * v.z; acc.w += wgt[ww] * v.w;
+              for (int ww = 0; ww < AW_WAVES; ++ww) {
+                const float4 v = *reinterpret_cast<const float4*>(dump + (ww * ROWS + row) * OROW + c);
+                acc.x += wgt[ww] * v.x; acc.y += wgt[ww] * v.y; acc.z += wgt[ww] * v.z; acc.w += wgt[ww] * v.w;
+              }
+              *reinterpret_cast<float4*>(part + 2 * AT_ROWS + row * AT_D + D0 + c) = acc;
             }
-            *reinterpret_cast<float4*>(part + 2 * AT_ROWS + srow * AT_D + 128 * half + 16 * sc8 + 4 * k) = acc;
-          }
           }
           aw_barrier();   // the dump is read before it is overwritten (and the set refilled)
+        };
+        if (rows <= 16) {
+          turn(std::integral_constant<int, 0>{}, std::integral_constant<int, AT_D>{});
+        } else {
+          turn(std::integral_constant<int, 0>{}, std::integral_constant<int, AT_D / 2>{});
+          turn(std::integral_constant<int, AT_D / 2>{}, std::integral_constant<int, AT_D / 2>{});
         }
       }
       // V of block u + 2 into this set
@@ -476,8 +504,12 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       if (set && u + 4 - tbase >= 64) {   // the lanes' blocks are used up
         tbase = u + 1;
         look_up();
+        look_up_scales();
+        // (waited for here: else the compiler drains the loop's loads where it reads these)
+        asm volatile("" : "+v"(tp[0]), "+v"(tp[1]), "+v"(tks[0]), "+v"(tks[1]), "+v"(tvs[0]), "+v"(tvs[1]));
       }
       X2 = unit(u + 3);
+      if constexpr (F8) unit_scales(X2, u + 3);
     }
   }
 }
