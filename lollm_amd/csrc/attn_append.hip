@@ -17,10 +17,13 @@
 // but for codes that become subnormal, which are rounded again.  Values that are not finite
 // become NaN.
 //
-// One workgroup per (sequence, page touched, KV head, K or V): it owns the page's scale.  A head
-// vector per half-wave, 8 values a lane, 16-byte loads; an 8-bit page's rows stay in registers
-// between their maximum and their rounding.  Query heads: one workgroup per token, or per token
-// and 8 heads where tokens are few.  Bound by memory for prompts, by the launch for few tokens.
+// One workgroup per (sequence, page touched, KV head, K or V) for 8-bit pages, whose scale it
+// owns, per 16 or 32 rows of a bf16 page; up to 4 rows per half-wave, 8 values a lane, 16-byte
+// loads.  An 8-bit page's rows stay in registers as they came and are formed twice, for their
+// maximum and for their rounding (in fp32 they would take the registers of two waves in three).
+// Query heads: a workgroup per token and as many heads as its half-waves take at once where
+// tokens are few, up to 32 heads otherwise.  Bound by memory for prompts, by the launch for few
+// tokens.
 #include "attn_common.h"
 
 namespace lollm {
@@ -40,14 +43,14 @@ struct AppendArgs {
   float* vs;
   long long table_stride;
   int per_token, T, Hq, Hkv, rd, table_width, n_pages, pshift;
-  int npg;                   // pages that T rows can touch
+  int gshift;                // rows of a workgroup's piece of a page: 1 << gshift
+  int npg;                   // pieces that T rows can touch
   int kv_items, q_chunks;    // workgroups of K and V; query-head chunks of a token
   int chunk_heads;           // heads of a chunk
   float eps;
 };
 
-constexpr int AA_THREADS = 256;
-constexpr int AA_HALVES = AA_THREADS / 32;   // head vectors at a time
+constexpr int AA_CHUNK = 32;                 // query heads of a workgroup at most
 
 __device__ __forceinline__ void aa_unpack(u32x4_t w, float (&x)[8]) {
 #pragma unroll
@@ -79,8 +82,9 @@ __device__ __forceinline__ void aa_angles(const float* inv_freq, int half, int p
   }
 }
 
-// The half-wave's head vector (8 values a lane) normalised and rotated; xs: 256 floats of its own.
-__device__ __forceinline__ void aa_norm_rotate(float (&x)[8], const float (&w)[8], int rd, float eps, int l,
+// The half-wave's head vector (8 values a lane) normalised, w1 = 1 + w, and rotated; xs: 256 floats
+// of its own.
+__device__ __forceinline__ void aa_norm_rotate(float (&x)[8], const float (&w1)[8], int rd, float eps, int l,
                                                const float* cs, const float* sn, float* xs) {
   float ss = 0.f;
 #pragma unroll
@@ -89,7 +93,7 @@ __device__ __forceinline__ void aa_norm_rotate(float (&x)[8], const float (&w)[8
   ss += __shfl_xor(ss, 16, 64);
   const float r = rsqrtf(ss / (float)AT_D + eps);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (1.f + w[e]);
+  for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w1[e];
   const int half = rd / 2;
   if (8 * l < rd) {
 #pragma unroll
@@ -97,7 +101,20 @@ __device__ __forceinline__ void aa_norm_rotate(float (&x)[8], const float (&w)[8
       *reinterpret_cast<float4*>(xs + 8 * l + 4 * u) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read by the same wave
-  if (8 * l < rd) {
+  if (half % 8 == 0) {   // the lane's partners, cosines and sines are 8 in a row
+    if (8 * l < rd) {
+      const int f = 8 * l < half ? 8 * l : 8 * l - half, at = 8 * l < half ? 8 * l + half : f;
+      float o[8], c[8], s[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        *reinterpret_cast<float4*>(o + 4 * u) = *reinterpret_cast<const float4*>(xs + at + 4 * u);
+        *reinterpret_cast<float4*>(c + 4 * u) = *reinterpret_cast<const float4*>(cs + f + 4 * u);
+        *reinterpret_cast<float4*>(s + 4 * u) = *reinterpret_cast<const float4*>(sn + f + 4 * u);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * c[e] + (8 * l < half ? -o[e] : o[e]) * s[e];
+    }
+  } else if (8 * l < rd) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int d = 8 * l + e;
@@ -126,35 +143,58 @@ __device__ __forceinline__ uint2 aa_codes(const float (&y)[8], float inv) {
   return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
-// RPH: rows of a page per half-wave.
-template <bool F8, int RPH>
-__global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
+// Query heads of item `item`: a token and a chunk of its heads.
+template <int THREADS>
+__device__ __forceinline__ void aa_queries(const AppendArgs& a, int item, float (&xs)[THREADS / 32][AT_D],
+                                           float* cs, float* sn) {
+  constexpr int D = AT_D, HALVES = THREADS / 32, QN = AA_CHUNK / HALVES;   // query heads per half-wave
+  const int tid = threadIdx.x, l = tid & 31, hw = tid >> 5;
+  const int bt = item / a.q_chunks, b = bt / a.T, t = bt - b * a.T;
+  const long long row_w = (long long)a.Hq * 2 * D + 2LL * a.Hkv * D;
+  const int h0 = (item - bt * a.q_chunks) * a.chunk_heads, h1 = min(h0 + a.chunk_heads, a.Hq);
+  const int p = a.per_token ? a.rope_pos[bt] : (a.rope_pos ? a.rope_pos[b] : a.lengths[b]) + t;
+  u32x4_t raw[QN];   // the half-wave's heads, on their way together
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    const int hd = h0 + hw + HALVES * i;
+    raw[i] = u32x4_t{0, 0, 0, 0};
+    if (hd < h1) raw[i] = reinterpret_cast<const u32x4_t*>(a.qkv + bt * row_w + (long long)hd * 2 * D)[l];
+  }
+  float w1[8];
+  aa_unpack(reinterpret_cast<const u32x4_t*>(a.qw)[l], w1);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w1[e] += 1.f;
+  aa_angles(a.inv_freq, a.rd / 2, p, tid, THREADS, cs, sn);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    const int hd = h0 + hw + HALVES * i;
+    if (h0 + HALVES * i >= h1) break;
+    float x[8];
+    aa_unpack(raw[i], x);
+    aa_norm_rotate(x, w1, a.rd, a.eps, l, cs, sn, xs[hw]);
+    if (hd < h1) reinterpret_cast<u32x4_t*>(a.q_out + ((long long)bt * a.Hq + hd) * D)[l] = aa_pack(x);
+  }
+}
+
+// RPH: rows of a piece per half-wave.
+template <bool F8, int THREADS, int RPH>
+__global__ __launch_bounds__(THREADS, THREADS == 512 ? 6 : 5) void attn_append_kernel(AppendArgs a) {
   constexpr int D = AT_D;
+  constexpr int AA_THREADS = THREADS, AA_HALVES = THREADS / 32;   // head vectors at a time
   __shared__ __attribute__((aligned(16))) float xs[AA_HALVES][D];
-  __shared__ float cs[AA_HALVES][D / 2], sn[AA_HALVES][D / 2];
+  __shared__ __attribute__((aligned(16))) float cs[AA_HALVES][D / 2], sn[AA_HALVES][D / 2];
   __shared__ float red[AA_THREADS / 64];
   const int tid = threadIdx.x, l = tid & 31, hw = tid >> 5;
   const long long row_w = (long long)a.Hq * 2 * D + 2LL * a.Hkv * D;
   const int half = a.rd / 2;
 
-  if ((int)blockIdx.x >= a.kv_items) {   // query heads
-    const int item = blockIdx.x - a.kv_items, bt = item / a.q_chunks, b = bt / a.T, t = bt - b * a.T;
-    const int h0 = (item - bt * a.q_chunks) * a.chunk_heads, h1 = min(h0 + a.chunk_heads, a.Hq);
-    const int p = a.per_token ? a.rope_pos[bt] : (a.rope_pos ? a.rope_pos[b] : a.lengths[b]) + t;
-    float w[8];
-    aa_unpack(reinterpret_cast<const u32x4_t*>(a.qw)[l], w);
-    aa_angles(a.inv_freq, half, p, tid, AA_THREADS, cs[0], sn[0]);
-    __syncthreads();
-    for (int hd = h0 + hw; hd < h1; hd += AA_HALVES) {
-      float x[8];
-      aa_unpack(reinterpret_cast<const u32x4_t*>(a.qkv + bt * row_w + (long long)hd * 2 * D)[l], x);
-      aa_norm_rotate(x, w, a.rd, a.eps, l, cs[0], sn[0], xs[hw]);
-      reinterpret_cast<u32x4_t*>(a.q_out + ((long long)bt * a.Hq + hd) * D)[l] = aa_pack(x);
-    }
+  if ((int)blockIdx.x >= a.kv_items) {
+    aa_queries<THREADS>(a, blockIdx.x - a.kv_items, xs, cs[0], sn[0]);
     return;
   }
 
-  // K or V of one KV head in one page
+  // K or V of one KV head in a piece of a page
   int item = blockIdx.x;
   const bool is_k = !(item & 1);
   item >>= 1;
@@ -162,8 +202,8 @@ __global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
   item /= a.Hkv;
   const int b = item / a.npg, pi = item - b * a.npg;
   const long long len = a.lengths[b];
-  const long long idx = (max(len, 0LL) >> a.pshift) + pi;
-  const long long lo = max(max(len, 0LL), idx << a.pshift), hi = min(len + a.T, (idx + 1) << a.pshift);
+  const long long piece = (max(len, 0LL) >> a.gshift) + pi, idx = (piece << a.gshift) >> a.pshift;
+  const long long lo = max(max(len, 0LL), piece << a.gshift), hi = min(len + a.T, (piece + 1) << a.gshift);
   if (lo >= hi || idx >= a.table_width) return;
   const int id = a.table[b * a.table_stride + idx];
   if (id < 0 || id >= a.n_pages) return;
@@ -179,8 +219,10 @@ __global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
     raw[i] = u32x4_t{0, 0, 0, 0};
     if (s < s1 - s0) raw[i] = reinterpret_cast<const u32x4_t*>(src + s * row_w)[l];
   }
-  float w[8];
-  aa_unpack(reinterpret_cast<const u32x4_t*>(a.kw)[l], w);
+  float w1[8];
+  aa_unpack(reinterpret_cast<const u32x4_t*>(a.kw)[l], w1);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w1[e] += 1.f;
   const int start = a.rope_pos && !a.per_token ? a.rope_pos[b] : (int)len;
   auto form = [&](int i, float (&x)[8]) {   // row i's values, in fp32
     const int s = hw + AA_HALVES * i;
@@ -189,7 +231,7 @@ __global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
       const int t = (int)t0 + min(s, s1 - s0 - 1);
       const int p = a.per_token ? a.rope_pos[(long long)b * a.T + t] : start + t;
       aa_angles(a.inv_freq, half, p, l, 32, cs[hw], sn[hw]);
-      aa_norm_rotate(x, w, a.rd, a.eps, l, cs[hw], sn[hw], xs[hw]);
+      aa_norm_rotate(x, w1, a.rd, a.eps, l, cs[hw], sn[hw], xs[hw]);
     }
   };
   if constexpr (!F8) {
@@ -203,17 +245,17 @@ __global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
       if (s < s1 - s0) reinterpret_cast<u32x4_t*>(dst + (long long)s * D)[l] = aa_pack(x);
     }
   } else {
-    float y[RPH][8];
     float* scale = (is_k ? a.ks : a.vs) + (long long)id * a.Hkv + kvh;
     const float old = s0 > 0 ? *scale : 0.f;
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < RPH; ++i) {
       if (AA_HALVES * i >= s1 - s0) break;
-      form(i, y[i]);
+      float y[8];
+      form(i, y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float m = fabsf(y[i][e]);
+        const float m = fabsf(y[e]);
         amax = fmaxf(amax, m < INFINITY ? m : 0.f);
       }
     }
@@ -221,7 +263,8 @@ __global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
     for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
     if ((tid & 63) == 0) red[tid >> 6] = amax;
     __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int w = 0; w < AA_THREADS / 64; ++w) amax = fmaxf(amax, red[w]);
     const float now = fmaxf(old, aa_scale_for(amax));
     const float inv = 1.f / now;   // (exact: a power of two)
     uint8_t* page = (uint8_t*)(is_k ? a.kp : a.vp) + first_row * D;
@@ -243,7 +286,10 @@ __global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
 #pragma unroll
     for (int i = 0; i < RPH; ++i) {
       const int s = hw + AA_HALVES * i;
-      if (s < s1 - s0) reinterpret_cast<uint2*>(page + (s0 + s) * D)[l] = aa_codes(y[i], inv);
+      if (AA_HALVES * i >= s1 - s0) break;
+      float y[8];
+      form(i, y);   // again: the rows as they came are half of what they are in fp32
+      if (s < s1 - s0) reinterpret_cast<uint2*>(page + (s0 + s) * D)[l] = aa_codes(y, inv);
     }
     if (tid == 0) *scale = now;
   }
@@ -253,14 +299,18 @@ __global__ __launch_bounds__(AA_THREADS) void attn_append_kernel(AppendArgs a) {
 
 using namespace lollm;
 
-template <bool F8>
-static void append_launch(const AppendArgs& a, unsigned n, hipStream_t st) {
-  switch (a.pshift) {
-    case 4: hipLaunchKernelGGL((attn_append_kernel<F8, 2>), dim3(n), dim3(AA_THREADS), 0, st, a); break;
-    case 5: hipLaunchKernelGGL((attn_append_kernel<F8, 4>), dim3(n), dim3(AA_THREADS), 0, st, a); break;
-    case 6: hipLaunchKernelGGL((attn_append_kernel<F8, 8>), dim3(n), dim3(AA_THREADS), 0, st, a); break;
-    default: hipLaunchKernelGGL((attn_append_kernel<F8, 16>), dim3(n), dim3(AA_THREADS), 0, st, a); break;
-  }
+template <bool F8, int THREADS, int RPH>
+static void append_start(AppendArgs a, int B, int* too_many, hipStream_t st) {
+  constexpr int halves = THREADS / 32;
+  static_assert(halves * RPH >= 16, "a piece of 16 rows or more");
+  a.npg = (int)(((long long)a.T + (1 << a.gshift) - 2) >> a.gshift) + 1;
+  // few tokens: no half-wave has a second head to wait for
+  a.chunk_heads = (long long)B * a.T < 1024 ? halves : AA_CHUNK;
+  a.q_chunks = (a.Hq + a.chunk_heads - 1) / a.chunk_heads;
+  const long long kv = 2LL * B * a.npg * a.Hkv, n = kv + (long long)B * a.T * a.q_chunks;
+  if ((*too_many = n > 0x7fffffffLL)) return;
+  a.kv_items = (int)kv;
+  hipLaunchKernelGGL((attn_append_kernel<F8, THREADS, RPH>), dim3((unsigned)n), dim3(THREADS), 0, st, a);
 }
 
 LOLLM_API int lollm_attn_append(const void* qkv, const void* q_norm_w, const void* k_norm_w,
@@ -287,17 +337,25 @@ LOLLM_API int lollm_attn_append(const void* qkv, const void* q_norm_w, const voi
   a.table_stride = table_stride; a.per_token = rope_per_token ? 1 : 0;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.rd = rotary_dim; a.table_width = table_width; a.n_pages = n_pages;
   a.pshift = pshift; a.eps = eps;
-  a.npg = (int)(((long long)T + page - 2) / page) + 1;
-  const long long kv = 2LL * B * a.npg * Hkv;
-  // few tokens: a workgroup per 8 heads, so that no half-wave has a second head to wait for
-  a.chunk_heads = (long long)B * T < 1024 ? AA_HALVES : Hq;
-  a.q_chunks = (Hq + a.chunk_heads - 1) / a.chunk_heads;
-  const long long n = kv + (long long)B * T * a.q_chunks;
-  if (n > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;
-  a.kv_items = (int)kv;
-  if (kv_dtype == LOLLM_F8)
-    append_launch<true>(a, (unsigned)n, (hipStream_t)stream);
-  else
-    append_launch<false>(a, (unsigned)n, (hipStream_t)stream);
-  return launch_status();
+  const bool f8 = kv_dtype == LOLLM_F8;
+  a.gshift = f8 || pshift < 5 ? pshift : 5;
+  int too_many = 0;
+  hipStream_t st = (hipStream_t)stream;
+  // New rows of a page at most: as many threads as bring it to 4 rows a half-wave.  A page of 128
+  // takes 1024, which leave the query heads, most of the work of many tokens, a CU half empty: from
+  // 2560 tokens on 512 with 8 rows (us, 1024 / 512 threads: 512 tokens 13 / 21, 1800 22 / 27, 3998
+  // 42 / 37; a second launch for the query heads costs 5).
+  const int rows = T < page ? T : page;
+  if (f8) {
+    if (rows <= 16) append_start<true, 256, 2>(a, B, &too_many, st);
+    else if (rows <= 32) append_start<true, 256, 4>(a, B, &too_many, st);
+    else if (rows <= 64) append_start<true, 512, 4>(a, B, &too_many, st);
+    else if ((long long)B * T < 2560) append_start<true, 1024, 4>(a, B, &too_many, st);
+    else append_start<true, 512, 8>(a, B, &too_many, st);
+  } else if (rows <= 16) {
+    append_start<false, 256, 2>(a, B, &too_many, st);
+  } else {
+    append_start<false, 256, 4>(a, B, &too_many, st);
+  }
+  return too_many ? LOLLM_EUNSUPPORTED : launch_status();
 }
