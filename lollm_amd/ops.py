@@ -194,42 +194,51 @@ F8 = 2
 PAGE_SIZES = (16, 32, 64, 128)
 
 
-def _here(*tensors):
-    """The kernels run on the current device's stream: refuse tensors of another device."""
-    dev = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"tensors must be on the current device, {dev}, got one on {t.device}")
+def _arg(t, name, dtype, shape, dev):
+    """The address of a tensor that _need accepts and that lies on device `dev` (the kernels run on
+    the current device's stream); one look at each property (a call of few tokens is host time)."""
+    if t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        p = t.data_ptr()
+        if not p & 15:
+            return p
+    _need(t, name, dtype, shape)
+    raise ValueError(f"{name} must be on the current device, {dev}, not on {t.device}")
 
 
-def _pages(k_pages, v_pages, k_scale, v_scale, table, B):
-    """(pages in the pool, KV heads, rows of a page, dtype code, table stride) of a checked paged
-    cache layer."""
+def _pages(k_pages, v_pages, k_scale, v_scale, table, B, dev):
+    """(shape of the pools, dtype code, table stride and width, addresses of k_pages, v_pages,
+    k_scale, v_scale and table) of a checked paged cache layer."""
     if k_pages.dim() != 4:
         raise ValueError("k_pages must be (n_pages, Hkv, page, D)")
-    n, Hkv, page, _ = k_pages.shape
+    shape = k_pages.shape
+    n, Hkv, page, _ = shape
     if n < 1 or Hkv < 1 or page not in PAGE_SIZES:
         raise ValueError(f"a page holds {PAGE_SIZES} rows and the pool at least one page, got "
-                         f"{tuple(k_pages.shape)}")
-    code = F8 if k_pages.dtype is torch.float8_e4m3fn else BF16
-    dt = torch.float8_e4m3fn if code == F8 else torch.bfloat16
-    _need(k_pages, "k_pages", dt)
-    _need(v_pages, "v_pages", dt, k_pages.shape)
-    if code == F8:
+                         f"{tuple(shape)}")
+    code, dt, ks, vs = BF16, torch.bfloat16, None, None
+    if k_pages.dtype is torch.float8_e4m3fn:
+        code, dt = F8, torch.float8_e4m3fn
         if k_scale is None or v_scale is None:
             raise ValueError("8-bit pages need k_scale and v_scale")
-        _need(k_scale, "k_scale", torch.float32, (n, Hkv))
-        _need(v_scale, "v_scale", torch.float32, (n, Hkv))
+        ks = _arg(k_scale, "k_scale", torch.float32, (n, Hkv), dev)
+        vs = _arg(v_scale, "v_scale", torch.float32, (n, Hkv), dev)
+    elif k_pages.dtype is not dt:
+        raise TypeError(f"pages are bf16 or float8_e4m3fn, not {k_pages.dtype}")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("bf16 pages have no scales")
-    if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B or not table.is_cuda \
-            or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"table must be ({B}, pages) int32 on the device with unit column stride")
-    stride = table.stride(0) if B > 1 else table.shape[1]
-    if stride < table.shape[1]:
+    kp = _arg(k_pages, "k_pages", dt, shape, dev)
+    vp = _arg(v_pages, "v_pages", dt, shape, dev)
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.get_device() != dev:
+        raise ValueError(f"table must be ({B}, pages) int32 on the current device, {dev}")
+    rows, width = table.shape
+    stride, col = table.stride()
+    if rows != B or width < 1 or (width > 1 and col != 1):
+        raise ValueError(f"table must be ({B}, pages) with unit column stride")
+    if B == 1:
+        stride = width
+    if stride < width:
         raise ValueError("table rows overlap")
-    _here(k_pages, v_pages, k_scale, v_scale, table)
-    return n, Hkv, page, code, stride
+    return n, Hkv, page, code, stride, width, kp, vp, ks, vs, table.data_ptr()
 
 
 def attn_append(qkv, q_norm_w, k_norm_w, inv_freq, lengths, table, k_pages, v_pages, Hq, rotary_dim,
@@ -243,29 +252,30 @@ def attn_append(qkv, q_norm_w, k_norm_w, inv_freq, lengths, table, k_pages, v_pa
     (B, T, Hq, D) as a view of qkv)."""
     if qkv.dim() != 3:
         raise ValueError("qkv must be (B, T, Hq*2D + 2*Hkv*D)")
+    dev = torch._C._cuda_getDevice()
     B, T, width = qkv.shape
-    n, Hkv, page, code, stride = _pages(k_pages, v_pages, k_scale, v_scale, table, B)
+    n, Hkv, page, code, stride, cols, kp, vp, ks, vs, tab = _pages(k_pages, v_pages, k_scale, v_scale,
+                                                                   table, B, dev)
     D = k_pages.shape[3]
     if B < 1 or T < 1 or Hq < 1 or width != Hq * 2 * D + 2 * Hkv * D:
         raise ValueError(f"qkv is {tuple(qkv.shape)}, expected (B, T, {Hq * 2 * D + 2 * Hkv * D})")
-    _need(qkv, "qkv", torch.bfloat16)
-    _need(q_norm_w, "q_norm_w", torch.bfloat16, (D,))
-    _need(k_norm_w, "k_norm_w", torch.bfloat16, (D,))
-    if rotary_dim:
-        _need(inv_freq, "inv_freq", torch.float32, (rotary_dim // 2,))
-    _need(lengths, "lengths", torch.int32, (B,))
-    per_token = rope_pos is not None and rope_pos.dim() == 2
+    x = _arg(qkv, "qkv", torch.bfloat16, (B, T, width), dev)
+    qw = _arg(q_norm_w, "q_norm_w", torch.bfloat16, (D,), dev)
+    kw = _arg(k_norm_w, "k_norm_w", torch.bfloat16, (D,), dev)
+    freq = _arg(inv_freq, "inv_freq", torch.float32, (rotary_dim // 2,), dev) if rotary_dim else None
+    ln = _arg(lengths, "lengths", torch.int32, (B,), dev)
+    pos, per_token = None, False
     if rope_pos is not None:
-        _need(rope_pos, "rope_pos", torch.int32, (B, T) if per_token else (B,))
+        per_token = rope_pos.dim() == 2
+        pos = _arg(rope_pos, "rope_pos", torch.int32, (B, T) if per_token else (B,), dev)
     if q_out is None:
-        q_out = torch.empty(B, T, Hq, D, dtype=torch.bfloat16, device=qkv.device)
-    _need(q_out, "q_out", torch.bfloat16, (B, T, Hq, D))
-    _here(qkv, q_norm_w, k_norm_w, inv_freq, lengths, rope_pos, q_out)
+        q_out = qkv.new_empty((B, T, Hq, D))
+    q = _arg(q_out, "q_out", torch.bfloat16, (B, T, Hq, D), dev)
     rc = _lib.lib().lollm_attn_append(
-        _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(inv_freq), _ptr(lengths), _ptr(rope_pos),
-        int(per_token), _ptr(table), stride, table.shape[1], n, page, code, B, T, Hq, Hkv, D, rotary_dim,
-        float(eps), _ptr(q_out), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), _stream())
-    _lib.check(rc, "lollm_attn_append")
+        x, qw, kw, freq, ln, pos, per_token, tab, stride, cols, n, page, code, B, T, Hq, Hkv, D, rotary_dim,
+        eps, q, kp, vp, ks, vs, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, "lollm_attn_append")
     return q_out, qkv.as_strided((B, T, Hq, D), (T * width, width, 2 * D, 1), qkv.storage_offset() + D)
 
 
@@ -282,21 +292,25 @@ def _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid, device):
     return n
 
 
-def _gate_strides(gate, B, T, Hq, D):
-    """(row, head) strides of a gate (B, T, Hq*D) or (B, T, Hq, D) whose rows are evenly strided."""
-    if gate.dtype is not torch.bfloat16 or not gate.is_cuda:
-        raise TypeError("gate must be bf16 on the device")
+def _gate_arg(gate, B, T, Hq, D, dev):
+    """(address, row stride, head stride) of a gate (B, T, Hq*D) or (B, T, Hq, D) whose rows are
+    evenly strided."""
     if gate.dim() == 3:
-        _need(gate, "gate", torch.bfloat16, (B, T, Hq * D))
-        return Hq * D, D
+        return _arg(gate, "gate", torch.bfloat16, (B, T, Hq * D), dev), Hq * D, D
+    if gate.dtype is not torch.bfloat16 or gate.get_device() != dev:
+        raise TypeError(f"gate must be bf16 on the current device, {dev}")
     if gate.shape != (B, T, Hq, D):
         raise ValueError(f"gate has shape {tuple(gate.shape)}, expected {(B, T, Hq, D)}")
-    head = gate.stride(2) if Hq > 1 else D
-    row = gate.stride(1) if T > 1 else (gate.stride(0) if B > 1 else Hq * head)
-    if gate.stride(3) != 1 or (B > 1 and T > 1 and gate.stride(0) != T * row) or head < D \
-            or row < (Hq - 1) * head + D or row % 8 or head % 8 or gate.data_ptr() % 16:
+    seq, row, head, one = gate.stride()
+    if Hq == 1:
+        head = D
+    if T == 1:
+        row = seq if B > 1 else Hq * head
+    p = gate.data_ptr()
+    if one != 1 or (B > 1 and T > 1 and seq != T * row) or head < D or row < (Hq - 1) * head + D \
+            or row % 8 or head % 8 or p & 15:
         raise ValueError("gate rows must be evenly strided, 16-byte aligned and not overlap")
-    return row, head
+    return p, row, head
 
 
 def attn_paged(q, k_pages, v_pages, table, kv_len, gate=None, *, k_scale=None, v_scale=None, grid=0,
@@ -307,27 +321,28 @@ def attn_paged(q, k_pages, v_pages, table, kv_len, gate=None, *, k_scale=None, v
     attn_append's view, or (B, T, Hq*D), or None.  Returns (B, T, Hq*D) bf16."""
     if q.dim() != 4:
         raise ValueError("q must be (B, T, Hq, D)")
+    dev = torch._C._cuda_getDevice()
     B, T, Hq, D = q.shape
-    n, Hkv, page, code, stride = _pages(k_pages, v_pages, k_scale, v_scale, table, B)
+    n, Hkv, page, code, stride, cols, kp, vp, ks, vs, tab = _pages(k_pages, v_pages, k_scale, v_scale,
+                                                                   table, B, dev)
     if k_pages.shape[3] != D or min(B, T, Hq) < 1 or Hq % Hkv:
         raise ValueError(f"q {tuple(q.shape)} does not fit pages {tuple(k_pages.shape)}")
-    _need(q, "q", torch.bfloat16)
-    _need(kv_len, "kv_len", torch.int32, (B,))
-    row, head = _gate_strides(gate, B, T, Hq, D) if gate is not None else (0, 0)
+    x = _arg(q, "q", torch.bfloat16, (B, T, Hq, D), dev)
+    ln = _arg(kv_len, "kv_len", torch.int32, (B,), dev)
+    g, row, head = _gate_arg(gate, B, T, Hq, D, dev) if gate is not None else (None, 0, 0)
     if out is None:
-        out = torch.empty(B, T, Hq * D, dtype=torch.bfloat16, device=q.device)
-    _need(out, "out", torch.bfloat16, (B, T, Hq * D))
+        out = q.new_empty((B, T, Hq * D))
+    o = _arg(out, "out", torch.bfloat16, (B, T, Hq * D), dev)
     if workspace is None:
         workspace = torch.empty(attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid), dtype=torch.uint8,
                                 device=q.device)
-    _need(workspace, "workspace")
-    _here(q, kv_len, gate, out, workspace)
+    ws = _arg(workspace, "workspace", workspace.dtype, workspace.shape, dev)
     rc = _lib.lib().lollm_attn_paged(
-        _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), code, _ptr(table), stride,
-        table.shape[1], n, page, _ptr(kv_len), _ptr(gate), row, head, _ptr(out), _ptr(workspace),
+        x, kp, vp, ks, vs, code, tab, stride, cols, n, page, ln, g, row, head, o, ws,
         workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, D, grid,
-        D ** -0.5 if scale is None else float(scale), _stream())
-    _lib.check(rc, "lollm_attn_paged")
+        D ** -0.5 if scale is None else scale, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, "lollm_attn_paged")
     return out
 
 
