@@ -106,10 +106,13 @@ int lollm_attn_verify(const void* q, const void* k_cache, const void* v_cache,
  *   table    (B, table_width) int32, rows table_stride apart; it holds table_width * page keys
  *   gate     element d of (token bt, head h) at gate + bt * gate_row + h * gate_head + d (so it
  *            can be read where the fused projection wrote it), or NULL
- *   kv_len, q, out, grid, scale  as lollm_attn_verify, which says when a call with grid 0 takes
- *            query tiles instead of the split-K; the workspace is required either way
+ *   kv_len, q, out, scale  as lollm_attn_verify
+ *   grid     as lollm_attn_verify; with 0, calls of more than 64 tokens in all and 16 or more a
+ *            sequence run on query tiles of one KV head, the keys of few tiles divided between
+ *            workgroups (few tiles of 8-bit pages keep the split-K)
+ *   workspace  lollm_attn_paged_workspace_bytes() bytes (required), used only within the call
  * Supported: D == 256, page 16, 32, 64 or 128, Hq / Hkv <= 32, B <= 512. */
-long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int grid);
+long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype, int grid);
 int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
                      const float* v_scale, int kv_dtype, const int32_t* table, long long table_stride,
                      int table_width, int n_pages, int page, const int32_t* kv_len, const void* gate,

@@ -32,7 +32,7 @@ SIGNATURES = {
     "lollm_attn_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _I], ctypes.c_longlong),
     "lollm_attn_verify": ([_P, _P, _P, _P, _P, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _I,
                            _I, ctypes.c_longlong, ctypes.c_longlong, _I, _F, _P], _I),
-    "lollm_attn_paged_workspace_bytes": ([_I, _I, _I, _I, _I, _I], ctypes.c_longlong),
+    "lollm_attn_paged_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _I], ctypes.c_longlong),
     "lollm_attn_paged": ([_P, _P, _P, _P, _P, _I, _P, ctypes.c_longlong, _I, _I, _I, _P, _P,
                           ctypes.c_longlong, _I, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _I, _I, _F,
                           _P], _I),

@@ -148,6 +148,11 @@ int attn_grid(int grid);
 // Row groups per wave of the long-call kernel (attn_prefill.hip) for this geometry on a device
 // with `cus` CUs, or 0 where the split-K kernels are the faster ones.
 int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus);
-int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st, const PagedArgs* paged = nullptr);
+int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st, const PagedArgs* paged = nullptr,
+                        int parts = 1);
+// The same for pages, and the workgroups that a tile's keys are dealt out to, with the bytes of
+// workspace that takes.
+int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts);
+long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts);
 
 }  // namespace lollm

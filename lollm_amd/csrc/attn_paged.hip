@@ -575,12 +575,20 @@ __global__ __launch_bounds__(AT_D) void attn_paged_combine_kernel(PagedArgs p) {
 
 using namespace lollm;
 
-LOLLM_API long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int grid) {
-  int n_rep, QB, qblocks;
+// Workspace of a call: the split-K's pieces, or the parts' of query tiles.
+static long long paged_ws_bytes(int B, int T, int Hkv, int n_rep, int qblocks, int nw, int groups, int parts) {
+  const long long n = groups ? attn_parts_bytes(B, T, Hkv, n_rep, parts) : attn_ws_bytes(nw, (long long)B * Hkv * qblocks);
+  return n > 16 ? n : 16;
+}
+
+LOLLM_API long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype,
+                                                     int grid) {
+  int n_rep, QB, qblocks, parts = 1;
   if (attn_geometry(B, T, Hq, Hkv, D, 1, &n_rep, &QB, &qblocks)) return -1;
   const int nw = attn_grid(grid);
-  if (nw <= 0 || nw > 1024) return -1;
-  return attn_ws_bytes(nw, (long long)B * Hkv * qblocks);
+  if (nw <= 0 || nw > 1024 || (kv_dtype != LOLLM_BF16 && kv_dtype != LOLLM_F8)) return -1;
+  const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, kv_dtype == LOLLM_F8, &parts) : 0;
+  return paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts);
 }
 
 LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages,
@@ -608,10 +616,11 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   const long long pairs = (long long)B * Hkv * qblocks;
   const int nw = attn_grid(grid);
   if (nw <= 0 || nw > 1024) return LOLLM_EUNSUPPORTED;
-  const int groups = grid == 0 ? attn_prefill_groups(B, T, Hkv, n_rep, nw) : 0;   // lollm_attn_verify's rule
+  int parts = 1;
+  const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, f8, &parts) : 0;
   if (!groups && pairs > 65535) return LOLLM_EUNSUPPORTED;                        // the combine's grid
   if (!groups && pairs * (rows / AT_BLOCK + 1) > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;   // 32-bit block numbers
-  if (!workspace || workspace_bytes < attn_ws_bytes(nw, pairs)) return LOLLM_EINVAL;
+  if (!workspace || workspace_bytes < paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts)) return LOLLM_EINVAL;
   PagedArgs p;
   AttnArgs& a = p.a;
   a.q = (const uint16_t*)q; a.kc = (const uint16_t*)k_pages; a.vc = (const uint16_t*)v_pages;
@@ -625,7 +634,7 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   p.n_pages = n_pages; p.pshift = pshift;
   p.rep_mul = (uint32_t)((65536 + n_rep - 1) / n_rep);
   hipStream_t st = (hipStream_t)stream;
-  if (groups) return attn_prefill_launch(a, groups, st, &p);
+  if (groups) return attn_prefill_launch(a, groups, st, &p, parts);
   if (f8)
     hipLaunchKernelGGL(attn_paged_kernel<true>, dim3(nw), dim3(AW_THREADS), 0, st, p);
   else

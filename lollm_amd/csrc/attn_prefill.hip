@@ -44,6 +44,9 @@ constexpr int AP_MIN_T = 16;                   // new positions per sequence
 constexpr int AP_FEW_ROWS = 64;                // tokens of a call that keeps the split-K kernels
 constexpr int AP_KEYS = 32;                    // keys per block
 constexpr int AP_AHEAD = 3;                    // operands read ahead of their products
+constexpr int AP_PART_BLOCKS = 8;              // blocks of a part of a tile's keys at least
+constexpr int AP_MAX_PARTS = 64;
+constexpr int AP_PIECE = 2 * 128 + 128 * AT_D; // floats: maxima, sums and O of a part of a 128-row tile
 constexpr int AP_DUMP = 32 * AT_D * 2;         // 16 KB: half of a wave's O on its way out
 
 // Where the keys are: AP_ROWS one slab per (sequence, KV head); AP_PAGES, AP_PAGES8 pages that a
@@ -63,7 +66,8 @@ struct ApArgs {
   const float* ks;         // 8-bit pages: (n_pages, Hkv) scales
   const float* vs;
   long long table_stride, gate_row;
-  int gate_head, n_pages, pshift;
+  float* ws;               // pieces of tiles whose keys are dealt out to several workgroups
+  int gate_head, n_pages, pshift, parts;
   uint32_t rep_mul;        // ceil(2^16 / n_rep): r / n_rep = r * rep_mul >> 16 for r < 256
   float cl2;
 };
@@ -106,13 +110,45 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // the longest tiles first (they end last), (sequence, KV head) fastest: with a multiple of
   // 8 pairs, one pair's tiles all run on one XCD and share its L2
   const int pairs = a.B * a.Hkv;
-  const int qt = a.qtiles - 1 - blockIdx.x / pairs, pair = blockIdx.x % pairs;
+  constexpr bool PARTS = KV != AP_ROWS && RG == 1;   // a tile's keys may go to a.parts workgroups
+  const int turn_ = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+  const int part = PARTS ? turn_ % a.parts : 0;
+  const int qt = a.qtiles - 1 - (PARTS ? turn_ / a.parts : turn_);
   const int b = pair / a.Hkv, kvh = pair % a.Hkv;
   const int q0 = qt * a.QB, QB = min(a.QB, a.T - q0);
   const int L = min(max(a.kv_len[b], 0), a.max_len);
   const int p0 = L - a.T + q0;                       // position of the tile's first query
   const int keys = min(max(p0 + QB, 0), L);          // keys any row of the tile sees
-  const int nblk = (keys + AP_KEYS - 1) / AP_KEYS;
+  const int nall = (keys + AP_KEYS - 1) / AP_KEYS;
+
+  // The blocks of this workgroup: from the first page that is mapped on (a window leaves none
+  // before it), and of these one of `parts` equal parts.  Parts of 8 blocks (10 us) or more, from
+  // 24 blocks on: what a division saves has to pay for the pieces and their merge, some 10 us.
+  int j0 = 0, nblk = nall, parts = 1;
+  if constexpr (KV != AP_ROWS) {
+    const int32_t* row = a.table + b * a.table_stride;
+    const int entries = (int)(((long long)keys + (1 << a.pshift) - 1) >> a.pshift);
+    if (entries > 0 && (uint32_t)ap_sload(row, 0) >= (uint32_t)a.n_pages) {
+      int e = entries;
+      for (int at = 0; at < entries; at += 64) {
+        const bool there = at + lane < entries && (uint32_t)row[at + lane] < (uint32_t)a.n_pages;
+        const uint64_t m = __ballot(there);
+        if (m) {
+          e = at + __builtin_ctzll(m);
+          break;
+        }
+      }
+      j0 = min((int)(((long long)e << a.pshift) / AP_KEYS), nall);
+    }
+    if constexpr (PARTS) {
+      const int n = nall - j0;
+      parts = n < 3 * AP_PART_BLOCKS ? 1 : min(a.parts, n / AP_PART_BLOCKS);
+      if (part >= parts) return;
+      nblk = j0 + (int)((long long)n * (part + 1) / parts);
+      j0 += (int)((long long)n * part / parts);
+    }
+  }
+  const int Lend = (int)min((long long)L, (long long)nblk * AP_KEYS);
 
   // Loads of a block: wave w brings rows 8 w .. 8 w + 7 of K and of V, two rows (1 KB) per
   // instruction; the lane's source chunk undoes the swizzle of the place it writes.  Rows
@@ -125,11 +161,11 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   const size_t cbase = KV == AP_ROWS ? (size_t)b * a.seq_stride + (size_t)kvh * a.head_stride : 0;
   const __amdgpu_buffer_rsrc_t krs = buf_rsrc(a.kc + cbase, KV == AP_ROWS ? (uint32_t)L * (AT_D * 2) : 0u);
   const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(a.vc + cbase, KV == AP_ROWS ? (uint32_t)L * (AT_D * 2) : 0u);
-  // page of keys 16 g .. of block j, -1: unmapped or past the end
+  // page of keys 16 g .. of block j, -1: unmapped or past this workgroup's blocks
   auto page_at = [&](int j, int g) {
     const uint32_t key = (uint32_t)(j * AP_KEYS + 16 * g);   // (no branch: O lives in all of them)
     const int id = ap_sload(a.table, b * a.table_stride + (min(key, (uint32_t)max(L - 1, 0)) >> a.pshift));
-    return key < (uint32_t)L && (uint32_t)id < (uint32_t)a.n_pages ? id : -1;
+    return key < (uint32_t)Lend && (uint32_t)id < (uint32_t)a.n_pages ? id : -1;
   };
   auto mapped = [&](int j) { return (page_at(j, 0) >= 0 ? 1u : 0u) | (page_at(j, 1) >= 0 ? 2u : 0u); };
   auto page_rsrc = [&](const uint16_t* pool, int id, int j) {
@@ -220,22 +256,22 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   };
   if constexpr (KV != AP_ROWS) {
 #pragma unroll
-    for (int j = 0; j < 3; ++j) pg[j] = page_at(j, wg);
-    pn = page_at(3, wg);
+    for (int j = 0; j < 3; ++j) pg[j] = page_at(j0 + j, wg);
+    pn = page_at(j0 + 3, wg);
   }
-  const uint32_t vm0 = KV == AP_ROWS ? 3u : mapped(0);
+  const uint32_t vm0 = KV == AP_ROWS ? 3u : mapped(j0);
   AP_BARRIER(0);   // the zeroed sets, before any DMA into them (and Q: the counts below are the DMA's)
-  load_k(ks0, pg[0], 0);
-  load_k(ks1, pg[1], 1);
-  load_v(vs0, pg[0], 0);
-  load_k(ks2, pg[2], 2);
-  load_v(vs1, pg[1], 1);
+  load_k(ks0, pg[0], j0);
+  load_k(ks1, pg[1], j0 + 1);
+  load_v(vs0, pg[0], j0);
+  load_k(ks2, pg[2], j0 + 2);
+  load_v(vs1, pg[1], j0 + 1);
 
   // the positions this wave's rows span: the key blocks it sees, and which need a mask
   const int wq0 = ap_div(32 * RG * wave, a.rep_mul);
   const int wq1 = min(ap_div(32 * RG * wave + 32 * RG - 1, a.rep_mul), QB - 1);
   const int wmin = p0 + wq0, wmax = wq0 < QB ? p0 + wq1 : -1;
-  const int wblk = wmax < 0 ? 0 : wmax / AP_KEYS + 1;
+  const int wblk = min(wmax < 0 ? 0 : wmax / AP_KEYS + 1, KV == AP_ROWS ? INT32_MAX : nblk);
 
   // LDS offsets of the operand reads: K row l32 at chunk 2 ks + h, V row x = 4 h + (lane % 16) / 4
   // at chunk 4 dt + 2 ((lane / 16) % 2) + (lane % 4) / 2; the k-step and the column tile
@@ -415,13 +451,13 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   };
 
   if constexpr (F8) {
-    scales(a.ks, 0, ksc);
+    scales(a.ks, j0, ksc);
     AP_BARRIER(8);    // block 0 of K, the first 2 of the 10 loads
   } else {
     AP_BARRIER(16);   // block 0 of K, the first 4 of the 20 loads
   }
-  if (wblk > 0) {
-    scores(ks0, 0, vm0);
+  if (wblk > j0) {
+    scores(ks0, j0, vm0);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
       u32x4_t Pn[2], Pm[2];
@@ -447,10 +483,10 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // 8-bit pages, may be in flight), and every wave is done with K of block j and V of block j - 1,
   // whose sets the loads of blocks j + 3 and j + 2 take.
   if constexpr (F8) {
-    scales(a.ks, 1, ksc);
-    scales(a.vs, 0, vsc);
+    scales(a.ks, j0 + 1, ksc);
+    scales(a.vs, j0, vsc);
   }
-  if constexpr (KV != AP_ROWS) vm = mapped(1);
+  if constexpr (KV != AP_ROWS) vm = mapped(j0 + 1);
   auto turn = [&](unsigned char* kfree, unsigned char* vfree, const unsigned char* knext, const unsigned char* vset,
                   int j) {
     if constexpr (F8) AP_BARRIER(4); else AP_BARRIER(8);
@@ -477,7 +513,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
       }
     }
   };
-  for (int j = 0; j < nblk; j += 3) {
+  for (int j = j0; j < nblk; j += 3) {
     turn(ks0, vs2, ks1, vs0, j);
     turn(ks1, vs0, ks2, vs1, j + 1);
     turn(ks2, vs1, ks0, vs2, j + 2);
@@ -493,7 +529,21 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   for (int rg = 0; rg < RG; ++rg) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_s[rg]), __float_as_uint(l_s[rg]), false, false);
     const float l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-    const float inv = l == 0.f ? 0.f : 1.f / l;   // no key seen: zeros
+    const bool whole = !PARTS || parts == 1;
+    const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);   // no key seen: zeros
+    float* piece = nullptr;
+    if constexpr (PARTS) {
+      if (!whole) {
+        const int tile = qt * pairs + pair;
+        piece = a.ws + ((size_t)tile * a.parts + part) * AP_PIECE;
+        if (h == 0) {
+          piece[32 * wave + l32] = m_ref[0];
+          piece[128 + 32 * wave + l32] = l;
+        }
+      }
+      if (tid == 0 && part == 0 && a.parts > 1)
+        reinterpret_cast<int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[qt * pairs + pair] = parts;
+    }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       // this lane's 8 half rows 4 it + lane / 16, columns 8 (lane % 16) ..; gates first
@@ -506,7 +556,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
         const int r = 32 * (RG * wave + rg) + 4 * it + (lane >> 4), qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
         live[it] = qi < QB;
         oo[it] = (((size_t)b * a.T + q0 + (live[it] ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D + 128 * half + 8 * c8;
-        if (a.gate)
+        if (a.gate && whole)
           g[it] = *reinterpret_cast<const u32x4_t*>(a.gate + ((size_t)b * a.T + q0 + (live[it] ? qi : 0)) * a.gate_row +
                                                     (size_t)(kvh * a.n_rep + hr) * a.gate_head + 128 * half + 8 * c8);
       }
@@ -529,6 +579,14 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
           const float4 f = *reinterpret_cast<const float4*>(dump + rr * 512 + 16 * ((2 * c8 + u) ^ (rr & 15)));
           y[4 * u] = f.x; y[4 * u + 1] = f.y; y[4 * u + 2] = f.z; y[4 * u + 3] = f.w;
         }
+        if (!whole) {
+          if (live[it]) {
+            float* to = piece + 256 + (32 * wave + rr) * AT_D + 128 * half + 8 * c8;
+            *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4*>(to + 4) = make_float4(y[4], y[5], y[6], y[7]);
+          }
+          continue;
+        }
         if (a.gate) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -549,6 +607,62 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   }
 }
 
+// Merges the parts of a tile, a wave per row (4 columns a lane), with the gate; tiles of one part
+// are finished already.
+__global__ __launch_bounds__(256) void attn_parts_combine_kernel(ApArgs a) {
+  const int pairs = a.B * a.Hkv, tile = blockIdx.x >> 5, lane = threadIdx.x & 63;
+  const int r = 4 * (blockIdx.x & 31) + (threadIdx.x >> 6);
+  const int n = reinterpret_cast<const int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[tile];
+  if (n == 1) return;
+  const int qt = tile / pairs, pair = tile - qt * pairs, b = pair / a.Hkv, kvh = pair - b * a.Hkv;
+  const int qi = ap_div(r, a.rep_mul), q0 = qt * a.QB;
+  if (qi >= min(a.QB, a.T - q0)) return;
+  const int head = kvh * a.n_rep + r - qi * a.n_rep;
+  const size_t bt = (size_t)b * a.T + q0 + qi;
+  const float* piece = a.ws + (size_t)tile * a.parts * AP_PIECE;
+  const float* mine = piece + (size_t)min(lane, n - 1) * AP_PIECE;
+  const float m = mine[r], ls = lane < n ? mine[128 + r] : 0.f;
+  const float* col = piece + 256 + r * AT_D + 4 * lane;
+  float4 v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float4*>(col + (size_t)min(e, n - 1) * AP_PIECE);
+  uint2 gv = make_uint2(0, 0);
+  if (a.gate)
+    gv = *reinterpret_cast<const uint2*>(a.gate + bt * a.gate_row + (size_t)head * a.gate_head + 4 * lane);
+  float M = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float wgt = m == -INFINITY ? 0.f : fast_exp2((m - M) * a.cl2);
+  float l = ls * wgt;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < n; s += 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (s + e < n) {
+        const float x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), s + e));
+        acc[0] += x * v[e].x; acc[1] += x * v[e].y; acc[2] += x * v[e].z; acc[3] += x * v[e].w;
+      }
+    }
+    if (s + 4 < n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = *reinterpret_cast<const float4*>(col + (size_t)min(s + 4 + e, n - 1) * AP_PIECE);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;   // no key seen: zeros
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = acc[e] * inv;
+    if (a.gate) y[e] *= sigmoidf_(__uint_as_float(e & 1 ? (e < 2 ? gv.x : gv.y) & 0xffff0000u : (e < 2 ? gv.x : gv.y) << 16));
+  }
+  const bf16x2 lo = {(__bf16)y[0], (__bf16)y[1]}, hi = {(__bf16)y[2], (__bf16)y[3]};
+  *reinterpret_cast<uint2*>(a.out + (bt * a.Hq + head) * AT_D + 4 * lane) =
+      make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
 int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus) {
   // A sequence's numbers do not depend on how its tokens are divided into calls of up to 64 (the
   // few-row GEMMs' limit): those keep the split-K kernels, whose rows do not depend on T.  Nor do
@@ -567,6 +681,49 @@ int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus) {
   return 0;
 }
 
+static int prefill_tiles(int B, int T, int Hkv, int n_rep, int rg, int* QB) {
+  *QB = 128 * rg / n_rep < T ? 128 * rg / n_rep : T;
+  return (T + *QB - 1) / *QB;
+}
+
+int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts) {
+  *parts = 1;
+  const int rg = attn_prefill_groups(B, T, Hkv, n_rep, cus);
+  if (rg == 2 || T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS) return rg;
+  // Fewer tiles than CUs divide their keys: as many parts as the chip holds at once, or a few more
+  // where their rounds come out a tenth shorter (160 tiles: 3 parts take 2 rounds of a third).
+  // With that tiles are the faster form at any number of them (us, tiles / split-K, bf16: 20 tiles
+  // of 2070 keys 36 / 43, of 30000 138 / 304; 64 of 8256 130 / 229; 128 of 8289 234 / 436), but
+  // for few tiles of 8-bit pages, whose codes a tile converts for 32 rows at a time as the split-K
+  // does, without its depth of loads (20 of 2070 keys 40 / 33, of 8000 64 / 61; 128 of 8289 265 /
+  // 298; 64 x 136 rows of 8017 257 / 232): from 80 full tiles on.
+  const long long pairs = (long long)B * Hkv;
+  if (f8 && 16 * pairs * T * n_rep < 5LL * cus * 128) return 0;
+  int QB;
+  const long long tiles = prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * pairs;
+  if (tiles < cus) {
+    int best = cus / (int)tiles;
+    best = best > AP_MAX_PARTS ? AP_MAX_PARTS : best;
+    double cost = 0.9 / best;   // (one round)
+    for (int n = best + 1; n <= best + 4 && n <= AP_MAX_PARTS; ++n) {
+      const double c = (double)((tiles * n + cus - 1) / cus) / n;
+      if (c < cost) {
+        cost = c;
+        best = n;
+      }
+    }
+    *parts = best;
+  }
+  return 1;
+}
+
+long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts) {
+  int QB;
+  if (parts <= 1) return 0;
+  const long long tiles = (long long)prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * B * Hkv;
+  return tiles * parts * AP_PIECE * (long long)sizeof(float) + tiles * 4;
+}
+
 template <int KV>
 static void prefill_start(const ApArgs& a, int rg, unsigned n, hipStream_t st) {
   if (rg == 2)
@@ -575,7 +732,7 @@ static void prefill_start(const ApArgs& a, int rg, unsigned n, hipStream_t st) {
     hipLaunchKernelGGL((attn_prefill_kernel<1, KV>), dim3(n), dim3(256), 0, st, a);
 }
 
-int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st, const PagedArgs* paged) {
+int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st, const PagedArgs* paged, int parts) {
   ApArgs a;
   a.q = v.q; a.kc = v.kc; a.vc = v.vc; a.kv_len = v.kv_len; a.gate = v.gate; a.out = v.out;
   a.seq_stride = v.seq_stride; a.head_stride = v.head_stride;
@@ -583,10 +740,10 @@ int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st, const PagedAr
   a.B = v.B; a.T = v.T; a.Hq = v.Hq; a.Hkv = v.Hkv; a.n_rep = v.n_rep; a.max_len = v.max_len;
   a.cl2 = v.cl2;
   a.rep_mul = (uint32_t)((65536 + v.n_rep - 1) / v.n_rep);
-  a.QB = 128 * rg / v.n_rep < v.T ? 128 * rg / v.n_rep : v.T;
-  a.qtiles = (v.T + a.QB - 1) / a.QB;
+  a.qtiles = prefill_tiles(v.B, v.T, v.Hkv, v.n_rep, rg, &a.QB);
+  a.parts = parts; a.ws = v.ws;
   a.table = nullptr; a.ks = a.vs = nullptr; a.table_stride = 0; a.n_pages = a.pshift = 0;
-  const long long n = (long long)a.qtiles * v.B * v.Hkv;
+  const long long n = (long long)a.qtiles * v.B * v.Hkv * parts;
   if (n > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;
   if (!paged) {
     prefill_start<AP_ROWS>(a, rg, (unsigned)n, st);
@@ -597,6 +754,11 @@ int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st, const PagedAr
       prefill_start<AP_PAGES8>(a, rg, (unsigned)n, st);
     else
       prefill_start<AP_PAGES>(a, rg, (unsigned)n, st);
+  }
+  if (parts > 1) {
+    const int rc = launch_status();
+    if (rc) return rc;
+    hipLaunchKernelGGL(attn_parts_combine_kernel, dim3((unsigned)(n / parts) * 32), dim3(256), 0, st, a);
   }
   return launch_status();
 }

@@ -279,14 +279,15 @@ def attn_append(qkv, q_norm_w, k_norm_w, inv_freq, lengths, table, k_pages, v_pa
     return q_out, qkv.as_strided((B, T, Hq, D), (T * width, width, 2 * D, 1), qkv.storage_offset() + D)
 
 
-def attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid=0):
-    """Bytes of attn_paged's workspace for `grid` workgroups (0: one per CU)."""
-    return _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid, torch._C._cuda_getDevice() if grid <= 0 else -1)
+def attn_paged_workspace_bytes(B, T, Hq, Hkv, D, dtype=torch.bfloat16, grid=0):
+    """Bytes of attn_paged's workspace over pages of `dtype`, for `grid` workgroups (0: one per CU)."""
+    return _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, F8 if dtype is torch.float8_e4m3fn else BF16, grid,
+                                       torch._C._cuda_getDevice() if grid <= 0 else -1)
 
 
 @functools.lru_cache(maxsize=4096)
-def _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid, device):
-    n = _lib.lib().lollm_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid)
+def _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, code, grid, device):
+    n = _lib.lib().lollm_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, code, grid)
     if n < 0:
         raise ValueError("unsupported attention geometry")
     return n
@@ -334,7 +335,7 @@ def attn_paged(q, k_pages, v_pages, table, kv_len, gate=None, *, k_scale=None, v
         out = q.new_empty((B, T, Hq * D))
     o = _arg(out, "out", torch.bfloat16, (B, T, Hq * D), dev)
     if workspace is None:
-        workspace = torch.empty(attn_paged_workspace_bytes(B, T, Hq, Hkv, D, grid), dtype=torch.uint8,
+        workspace = torch.empty(attn_paged_workspace_bytes(B, T, Hq, Hkv, D, k_pages.dtype, grid), dtype=torch.uint8,
                                 device=q.device)
     ws = _arg(workspace, "workspace", workspace.dtype, workspace.shape, dev)
     rc = _lib.lib().lollm_attn_paged(

@@ -48,9 +48,10 @@ def test_attn_append_refuses(kw, rc):
 
 
 def test_workspace_bytes():
-    L = _lib.lib()
+    f = _lib.lib().lollm_attn_paged_workspace_bytes
     # one fp32 piece of 32 x 256 values and 2 x 32 sums per workgroup and pair, 16 bytes a pair
-    assert L.lollm_attn_paged_workspace_bytes(2, 1, 8, 2, 256, 7) == (7 + 4) * (64 + 8192) * 4 + 4 * 16
-    assert L.lollm_attn_paged_workspace_bytes(2, 1, 8, 3, 256, 7) == -1
-    assert L.lollm_attn_paged_workspace_bytes(2, 1, 8, 2, 128, 7) == -1
-    assert L.lollm_attn_paged_workspace_bytes(2, 1, 8, 2, 256, 1025) == -1
+    assert f(2, 1, 8, 2, 256, 0, 7) == (7 + 4) * (64 + 8192) * 4 + 4 * 16 == f(2, 1, 8, 2, 256, 2, 7)
+    assert f(2, 1, 8, 3, 256, 0, 7) == -1
+    assert f(2, 1, 8, 2, 128, 0, 7) == -1
+    assert f(2, 1, 8, 2, 256, 1, 7) == -1
+    assert f(2, 1, 8, 2, 256, 0, 1025) == -1

@@ -81,7 +81,7 @@ def check_attention(case, Hq, **kw):
     out = ops.attn_paged(qd, kd, vd, td, ld, gates(gd, Hq), k_scale=ksd, v_scale=vsd, **kw)
     torch.cuda.synchronize()
     # nothing of what lay in the workspace counts
-    ws = torch.full((ops.attn_paged_workspace_bytes(*q.shape[:3], k.shape[1], D, kw.get("grid", 0)),), 255,
+    ws = torch.full((ops.attn_paged_workspace_bytes(*q.shape[:3], k.shape[1], D, k.dtype, kw.get("grid", 0)),), 255,
                     dtype=torch.uint8, device="cuda")
     again = ops.attn_paged(qd, kd, vd, td, ld, gates(gd, Hq), k_scale=ksd, v_scale=vsd, workspace=ws, **kw)
     assert torch.equal(again, out)
@@ -107,7 +107,11 @@ CASES = [
     (1, 1, 32, 1, [9000], 128, 1),                   # more blocks than a lookup holds
     (2, 3, 6, 2, [77, 4100], 64, 2),                 # 3 query heads a KV head
     (1, 33, 4, 2, [50], 32, 0),
-    (2, 70, 8, 2, [70, 213], 16, 0),
+    (2, 70, 8, 2, [70, 213], 16, 0),                 # query tiles
+    (1, 100, 8, 2, [1501], 16, 0),                   # their keys in parts
+    (2, 67, 32, 4, [2100, 67], 64, 0),               # one sequence in parts, one whole
+    (3, 65, 6, 2, [700, 0, 65], 32, 0),              # an idle slot; 3 query heads a KV head
+    (1, 600, 32, 4, [1111], 128, 0),                 # several tiles a part
 ]
 
 
@@ -127,6 +131,19 @@ def test_attention_unmapped_pages(P, bits):
     holes = {(0, 1), (0, 4), (0, 5), (0, 6), (0, 7), (1, 0), (2, 0), (2, 1), (3, 0)}
     out = check_attention(attend_case(P, 4, 2, 8, 2, lens, P, bits, holes), 8)
     assert (out[2] == 0).all() and (out[3] == 0).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("P", [16, 64])
+def test_attention_window_of_a_chunk(P, bits):
+    """Query tiles over a window: the early pages given back, of one sequence to the last of them
+    that no query sees, of one all; a hole inside."""
+    print(f"case window page {P} bits {bits}", flush=True)
+    lens = [1900, 1300, 700]
+    holes = {(0, i) for i in range(1000 // P)} | {(1, i) for i in range(1300 // P - 1)} | {(2, i) for i in range(-(-700 // P))}
+    holes |= {(0, 1200 // P), (0, 1300 // P + 1)}
+    out = check_attention(attend_case(P, 3, 72, 8, 2, lens, P, bits, holes), 8)
+    assert (out[2] == 0).all()
 
 
 @pytest.mark.parametrize("bits", [16, 8])
@@ -349,7 +366,7 @@ def test_other_stream_and_caller_workspace():
     want = ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs)
     torch.cuda.synchronize()
     st = torch.cuda.Stream()
-    ws = torch.empty(ops.attn_paged_workspace_bytes(4, 2, 8, 2, D), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(ops.attn_paged_workspace_bytes(4, 2, 8, 2, D, k.dtype), dtype=torch.uint8, device="cuda")
     with torch.cuda.stream(st):
         got = ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs, workspace=ws)
     st.synchronize()
