@@ -61,13 +61,14 @@ def sample_next(logits, temperature, top_k, top_p, repetition_penalty=1.0, prev_
 
 @torch.no_grad()
 def generate(model, ids, decode, stop_ids, device="cuda", *, max_new_tokens=128,
-             temperature=0.7, top_k=20, top_p=0.8, repetition_penalty=1.1):
+             temperature=0.7, top_k=20, top_p=0.8, repetition_penalty=1.1, **cache):
     """generate.py:40-62: prefill, then one token per forward; yields text pieces.  The
-    cache holds the prompt plus max_new_tokens (the reference's grows without bound)."""
+    cache holds the prompt plus max_new_tokens (the reference's grows without bound); further
+    keywords go to model.new_cache (page, kv_dtype: keys and values in pages)."""
     input_ids = torch.tensor([ids], device=device)
     context = list(ids)
     eos = set(stop_ids)
-    past = model.new_cache(1, len(ids) + max_new_tokens + 1)
+    past = model.new_cache(1, len(ids) + max_new_tokens + 1, **cache)
     logits, past = model(input_ids, past)
     nxt = sample_next(logits[0, -1], temperature, top_k, top_p, repetition_penalty, context)
     generated, prev = [], ""

@@ -4,7 +4,7 @@ Registration mirrors src/qwen3_5/__init__.py:20-23 (model types and sampling def
 """
 
 from .config import Qwen3_5Config, build_config  # noqa: F401
-from .kv import Qwen3_5Cache  # noqa: F401
+from .kv import Qwen3_5Cache, Qwen3_5PagedCache  # noqa: F401
 from .modeling_qwen3_5 import Qwen3_5Model  # noqa: F401
 from .mtp import MTP, SpecDecoder, generate_mtp, load_mtp, speculate  # noqa: F401
 from .weights import load, to_raw  # noqa: F401

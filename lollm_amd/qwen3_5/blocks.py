@@ -265,12 +265,20 @@ class GatedAttention:
         return [self.qkv, self.o_proj]
 
     def core(self, x, k_cache, v_cache, lengths, kv_len, rope_pos=None, grid=0,
-             workspace=None):
+             workspace=None, table=None, k_scale=None, v_scale=None):
         """Everything before o_proj (blocks.py:208-235).  rope_pos: None (RoPE at the cache
-        rows), (B,) int32 start positions, or (B, T) int32 per-token positions."""
+        rows), (B,) int32 start positions, or (B, T) int32 per-token positions.  table: the caches
+        are pages that it names (ops.attn_append, ops.attn_paged), with their scales where they
+        hold 8 bits."""
         B, T, _ = x.shape
         cfg = self.cfg
         qkv = self.qkv(x)
+        if table is not None:
+            q, gate = ops.attn_append(qkv, self.q_norm, self.k_norm, self.inv_freq, lengths, table, k_cache,
+                                      v_cache, cfg.num_attention_heads, cfg.rotary_dim, cfg.rms_norm_eps,
+                                      k_scale=k_scale, v_scale=v_scale, rope_pos=rope_pos)
+            return ops.attn_paged(q, k_cache, v_cache, table, kv_len, gate, k_scale=k_scale,
+                                  v_scale=v_scale, grid=grid, workspace=workspace)
         if T == 1 and k_cache.shape[2] <= ops.ATTN_SMALL_MAXL:
             # one token over a short cache (the MTP head's draft block): prologue fused
             return ops.attn_small(qkv, self.q_norm, self.k_norm, self.inv_freq, lengths, kv_len, B,

@@ -20,6 +20,9 @@ for the MI355X kernels:
     states, so rolling back to `a` accepted drafts only rewrites four small integers per
     sequence (`lollm_spec_commit`) -- the reference instead deep-copies the whole cache
     before every verify (kv.py:49-54, mtp.py:141) and re-runs on reject (mtp.py:156-162).
+
+Qwen3_5PagedCache holds the full-attention layers' keys and values in pages instead, in bf16
+or in 8 bits: a sequence takes the pages it fills, and gives them back.
 """
 
 from __future__ import annotations
@@ -46,9 +49,7 @@ class Qwen3_5Cache:
         K = cfg.linear_conv_kernel_dim
         for i in range(n):
             if cfg.layer_type(i) == "full_attention":
-                shape = (batch, cfg.num_key_value_heads, max_len, cfg.head_dim)
-                self.layers[i] = {"k": torch.zeros(shape, dtype=torch.bfloat16, device=device),
-                                  "v": torch.zeros(shape, dtype=torch.bfloat16, device=device)}
+                self.layers[i] = self._kv_layer()
             else:
                 self.layers[i] = {
                     "win": torch.zeros(batch, 2 * self.win_rows, cfg.conv_dim,
@@ -69,6 +70,16 @@ class Qwen3_5Cache:
         # host-side upper bound of max(lengths): every forward or speculative step adds
         # its T, rollbacks leave it, so capacity is checked without reading the device
         self.len_bound = 0
+
+    def _kv_layer(self):
+        cfg = self.cfg
+        shape = (self.batch, cfg.num_key_value_heads, self.max_len, cfg.head_dim)
+        return {"k": torch.zeros(shape, dtype=torch.bfloat16, device=self.device),
+                "v": torch.zeros(shape, dtype=torch.bfloat16, device=self.device)}
+
+    def kv_args(self, layer):
+        """What GatedAttention.core takes beside the layer's "k" and "v"."""
+        return {}
 
     @property
     def win_rows(self):
@@ -208,3 +219,133 @@ class Qwen3_5Cache:
             for t in s.values():
                 tot += t.numel() * t.element_size()
         return tot
+
+
+class Qwen3_5PagedCache(Qwen3_5Cache):
+    """The same cache with the full-attention layers' keys and values in pages of `page` rows
+    (16, 32, 64 or 128) that sequences take from one pool as they grow: `table` (batch,
+    ceil(max_len / page)) int32 on the device names each sequence's pages, the same ones in every
+    layer's pools "k", "v" (n_pages, n_kv, page, head_dim).  kv_dtype torch.float8_e4m3fn holds
+    them in 8 bits with one power-of-two scale per page and KV head ("ks", "vs"; ops.attn_append):
+    half the memory and half of what a long context's attention reads.
+
+    n_pages: pages of the pool, by default enough for every sequence at max_len.  `reserve` hands
+    them out on the host, before the forward or step that fills them (a captured step is replayed
+    over the same table); `release` takes a finished sequence's back."""
+
+    def __init__(self, cfg: Qwen3_5Config, batch: int, max_len: int, spec_slots: int = 4,
+                 device="cuda", page: int = 64, kv_dtype=torch.bfloat16, n_pages=None):
+        if page not in ops.PAGE_SIZES:
+            raise ValueError(f"page must be one of {ops.PAGE_SIZES}, got {page}")
+        if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise TypeError(f"kv_dtype must be bfloat16 or float8_e4m3fn, got {kv_dtype}")
+        self.page, self.kv_dtype = page, kv_dtype
+        width = -(-max_len // page)
+        self.n_pages = batch * width if n_pages is None else n_pages
+        if self.n_pages < 1:
+            raise ValueError("n_pages must be positive")
+        super().__init__(cfg, batch, max_len, spec_slots, device)
+        self.table = torch.full((batch, width), -1, dtype=torch.int32, device=self.device)
+        self._host_table = torch.full((batch, width), -1, dtype=torch.int32)
+        self.free = list(range(self.n_pages - 1, -1, -1))
+        self.held = [0] * batch          # pages of each sequence
+        self.live = [True] * batch       # released sequences take no more
+
+    def _kv_layer(self):
+        cfg = self.cfg
+        shape = (self.n_pages, cfg.num_key_value_heads, self.page, cfg.head_dim)
+        kv = {n: torch.zeros(shape, dtype=self.kv_dtype, device=self.device) for n in ("k", "v")}
+        if self.kv_dtype != torch.bfloat16:
+            kv.update({n: torch.ones(shape[:2], dtype=torch.float32, device=self.device)
+                       for n in ("ks", "vs")})
+        return kv
+
+    def kv_args(self, layer):
+        s = self.layers[layer]
+        return {"table": self.table, "k_scale": s.get("ks"), "v_scale": s.get("vs")}
+
+    def reserve(self, T: int):
+        """Raise RuntimeError unless T more rows fit max_len and the pool; name their pages.  Goes
+        by the host-side bound of the lengths, and by the lengths themselves (a host sync) only
+        where the pool cannot give every sequence that many."""
+        super().reserve(T)
+
+        def short(lengths):
+            return [0 if not live else max(0, -(-(n + T) // self.page) - held)
+                    for n, held, live in zip(lengths, self.held, self.live)]
+
+        want = short([self.len_bound] * self.batch)
+        if not any(want):
+            return
+        if capturing():
+            raise RuntimeError("pages cannot be handed out under capture: reserve() before it")
+        if sum(want) > len(self.free):
+            lengths = self.lengths.tolist()
+            self.len_bound = max(lengths)
+            want = short(lengths)
+            if sum(want) > len(self.free):
+                raise RuntimeError(f"KV page pool exhausted: {sum(want)} pages needed, {len(self.free)} of "
+                                   f"{self.n_pages} free")
+        for b, n in enumerate(want):
+            for _ in range(n):
+                self._host_table[b, self.held[b]] = self.free.pop()
+                self.held[b] += 1
+        self.table.copy_(self._host_table)
+
+    def release(self, b: int):
+        """Give back the pages of a finished sequence: it holds no keys from now on, takes no more
+        pages, and its rows of later calls mean nothing."""
+        self.free += self._host_table[b, :self.held[b]].tolist()
+        self._host_table[b] = -1
+        self.held[b], self.live[b] = 0, False
+        self.lengths[b] = 0
+        self.table.copy_(self._host_table)
+
+    # -- the reference cache API -------------------------------------------------------
+    def _rows(self, L):
+        at = torch.arange(L, device=self.device)
+        return self.table[:, at // self.page].long(), at % self.page
+
+    def append_kv(self, layer, k, v):
+        """Write k, v (B, n_kv, t, D) at the current length; return the full (K, V)."""
+        s = self.layers[layer]
+        if "ks" in s:
+            raise RuntimeError("8-bit pages are written by ops.attn_append, which keeps their scales")
+        L, t = self._uniform_length(), k.shape[2]
+        if L + t > self.max_len:
+            raise RuntimeError("KV cache capacity exceeded")
+        if t:
+            self.reserve(t)
+            page, slot = self._rows(L + t)
+            s["k"][page[:, L:], :, slot[L:]] = k.transpose(1, 2).to(torch.bfloat16)
+            s["v"][page[:, L:], :, slot[L:]] = v.transpose(1, 2).to(torch.bfloat16)
+        return self._read(layer, L + t)
+
+    def _read(self, layer, L):
+        s = self.layers[layer]
+        page, slot = self._rows(L)
+        out = []
+        for n, sn in (("k", "ks"), ("v", "vs")):
+            if sn in s:
+                x = s[n].view(torch.uint8)[page, :, slot].view(self.kv_dtype).float()
+                x = (x * s[sn][page][..., None]).to(torch.bfloat16)   # exact
+            else:
+                x = s[n][page, :, slot]
+            out.append(x.transpose(1, 2))
+        return tuple(out)
+
+    def read_kv(self, layer):
+        s = self.layers[layer]
+        if s is None or "k" not in s:
+            return None
+        return self._read(layer, self._uniform_length())
+
+    def clone(self):
+        new = super().clone()
+        new.__class__ = Qwen3_5PagedCache
+        new.table, new._host_table = self.table.clone(), self._host_table.clone()
+        new.free, new.held, new.live = list(self.free), list(self.held), list(self.live)
+        return new
+
+    def nbytes(self):
+        return super().nbytes() + self.table.numel() * self.table.element_size()

@@ -19,7 +19,7 @@ import torch.nn.functional as F
 from .. import ops
 from .blocks import MLP, GatedAttention, GatedDeltaNet, Projection, RMSNorm, _cus, rope_inv_freq
 from .config import Qwen3_5Config
-from .kv import Qwen3_5Cache
+from .kv import Qwen3_5Cache, Qwen3_5PagedCache
 
 __all__ = ["DecoderLayer", "Qwen3_5Model", "Qwen3_5Cache"]
 
@@ -80,8 +80,14 @@ class Qwen3_5Model:
         return out
 
     # ---------------------------------------------------------------------------------
-    def new_cache(self, batch, max_len, spec_slots=4):
-        return Qwen3_5Cache(self.cfg, batch, max_len, spec_slots, self.device)
+    def new_cache(self, batch, max_len, spec_slots=4, page=None, kv_dtype=None, n_pages=None):
+        """A cache of `batch` sequences of up to max_len tokens: one slab per sequence, or, with
+        any of page (rows of a page, 64), kv_dtype (bfloat16, or float8_e4m3fn for 8 bits) and
+        n_pages (of the pool) given, keys and values in pages (Qwen3_5PagedCache)."""
+        if page is None and kv_dtype is None and n_pages is None:
+            return Qwen3_5Cache(self.cfg, batch, max_len, spec_slots, self.device)
+        return Qwen3_5PagedCache(self.cfg, batch, max_len, spec_slots, self.device, page or 64,
+                                 kv_dtype or torch.bfloat16, n_pages)
 
     def attn_workspace(self, B, T, max_len, keep=True):
         """Split-K partials buffer of the attention layers (shared by all layers of a
@@ -130,7 +136,9 @@ class Qwen3_5Model:
         else:
             x, h_first, kv_len = inputs
         # (the calls that repeat a shape: one token, the verify block)
-        ws = self.attn_workspace(B, T, cache.max_len, keep=T <= max(cache.spec_slots, 1))
+        # (pages: of the size that the call's form needs, from the allocator)
+        ws = (None if isinstance(cache, Qwen3_5PagedCache) else
+              self.attn_workspace(B, T, cache.max_len, keep=T <= max(cache.spec_slots, 1)))
         # a call that can be rolled back (the verify block, as the GDN layers tell it) asks for
         # the split-K attention at any size, where a row's bits do not depend on T
         grid = self.attn_grid or (_cus() if T <= cache.spec_slots else 0)
@@ -146,7 +154,7 @@ class Qwen3_5Model:
                 s = cache.layers[i]
                 mixer = layer.self_attn
                 core = mixer.core(h_in, s["k"], s["v"], lengths, kv_len,
-                                  grid=grid, workspace=ws)
+                                  grid=grid, workspace=ws, **cache.kv_args(i))
             else:
                 mixer = layer.linear_attn
                 core = mixer.core(h_in, cache, i)

@@ -141,11 +141,15 @@ class SpecDecoder:
     Capacity: a step adds at most k + 1 tokens to a sequence; step() and replay() raise
     RuntimeError before a step whose tokens might not fit the cache (max_len) or the
     output buffer (out_capacity), from host-side upper bounds (exact values are read
-    from the device only when a bound says the step might not fit)."""
+    from the device only when a bound says the step might not fit).
+
+    page, kv_dtype, n_pages: keys and values in pages, in bf16 or 8 bits, as
+    Qwen3_5Model.new_cache; a step's pages are handed out before it."""
 
     def __init__(self, model: Qwen3_5Model, mtp: MTP, batch: int, max_len: int, k: int = 3,
                  temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, seed: int = 0,
-                 draft: str = "argmax", out_capacity: int = 4096, repetition_penalty: float = 1.0):
+                 draft: str = "argmax", out_capacity: int = 4096, repetition_penalty: float = 1.0,
+                 page=None, kv_dtype=None, n_pages=None):
         if draft not in ("argmax", "sample"):
             raise ValueError("draft must be 'argmax' or 'sample'")
         if not repetition_penalty or repetition_penalty <= 0:
@@ -156,7 +160,8 @@ class SpecDecoder:
         self.penalty = float(repetition_penalty)
         self.draft_mode = draft if temperature > 0 else "argmax"
         cfg, dev = model.cfg, model.device
-        self.cache = model.new_cache(batch, max_len, spec_slots=k + 1)
+        self.cache = model.new_cache(batch, max_len, spec_slots=k + 1, page=page, kv_dtype=kv_dtype,
+                                     n_pages=n_pages)
         self.mkc, self.mvc = mtp.scratch_cache(batch, max(k, 1))
         i32 = dict(dtype=torch.int32, device=dev)
         self.pending = torch.zeros(batch, **i32)
@@ -371,16 +376,18 @@ class SpecDecoder:
 
 @torch.no_grad()
 def generate_mtp(model, mtp: MTP, ids, decode, stop_ids, device="cuda", *, max_new_tokens=128,
-                 temperature=0.7, top_k=20, top_p=0.8, repetition_penalty=1.1, k=1, seed=0):
+                 temperature=0.7, top_k=20, top_p=0.8, repetition_penalty=1.1, k=1, seed=0,
+                 page=None, kv_dtype=None):
     """Drop-in for the reference's generate_mtp (mtp.py:92-162): yields text pieces.
     Runs the batched decoder with B = 1 and k drafts (k = 1 by default, as the
     reference), with the reference's sampling arguments (run.py passes the family
-    defaults, repetition_penalty 1.05 included)."""
+    defaults, repetition_penalty 1.05 included); page, kv_dtype as SpecDecoder."""
     eos = set(stop_ids)
     pen = 1.0 if repetition_penalty is None else float(repetition_penalty)
     dec = SpecDecoder(model, mtp, 1, len(ids) + max_new_tokens + 2 * k + 8, k=k,
                       temperature=temperature, top_k=top_k, top_p=top_p, seed=seed,
-                      out_capacity=max_new_tokens + 2 * k + 2, repetition_penalty=pen)
+                      out_capacity=max_new_tokens + 2 * k + 2, repetition_penalty=pen, page=page,
+                      kv_dtype=kv_dtype)
     dec.prefill(torch.tensor([ids], device=model.device))
     generated, prev = [], ""
     while True:

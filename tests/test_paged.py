@@ -1,10 +1,14 @@
-"""The paged cache's C entry points refuse what they do not take before any launch (no GPU)."""
+"""The paged cache without a GPU: its C entry points refuse what they do not take before any
+launch; Qwen3_5PagedCache hands pages out and takes them back on the host."""
 
 import ctypes
 
 import pytest
+import torch
 
 from lollm_amd import _lib
+from lollm_amd.qwen3_5 import Qwen3_5Config, Qwen3_5PagedCache
+from lollm_amd.qwen3_5.config import micro_config_dict
 
 P = ctypes.c_void_p(4096)   # never dereferenced: every call below is refused on the host
 Z = None
@@ -55,3 +59,80 @@ def test_workspace_bytes():
     assert f(2, 1, 8, 2, 128, 0, 7) == -1
     assert f(2, 1, 8, 2, 256, 1, 7) == -1
     assert f(2, 1, 8, 2, 256, 0, 1025) == -1
+
+
+def cache(batch=3, max_len=100, **kw):
+    return Qwen3_5PagedCache(Qwen3_5Config.from_hf(micro_config_dict()), batch, max_len, device="cpu", **kw)
+
+
+def pages_of(c):
+    return [[int(p) for p in row if p >= 0] for row in c.table]
+
+
+def test_cache_hands_pages_out_as_sequences_grow():
+    c = cache(page=16)
+    assert c.table.shape == (3, 7) and c.n_pages == 21 and pages_of(c) == [[], [], []]
+    c.advance(16)
+    assert [len(p) for p in pages_of(c)] == [1, 1, 1]
+    c.advance(1)
+    assert [len(p) for p in pages_of(c)] == [2, 2, 2]
+    c.reserve(15)                                    # what is held suffices
+    assert [len(p) for p in pages_of(c)] == [2, 2, 2]
+    c.advance(83)
+    every = sum(pages_of(c), [])
+    assert len(every) == len(set(every)) == 21 and not c.free and c.seen_tokens == 100
+    with pytest.raises(RuntimeError, match="capacity"):
+        c.reserve(1)
+
+
+def test_cache_pool_smaller_than_every_sequence_at_max_len():
+    c = cache(page=16, n_pages=7)
+    c.advance(20)                                    # 2 pages each, 1 free
+    with pytest.raises(RuntimeError, match="pool exhausted"):
+        c.reserve(13)
+    before = pages_of(c)
+    c.release(1)
+    assert pages_of(c) == [before[0], [], before[2]] and len(c.free) == 3 and int(c.lengths[1]) == 0
+    c.reserve(13)                                    # the released one takes none
+    assert [len(p) for p in pages_of(c)] == [3, 0, 3] and len(c.free) == 1
+
+
+def test_cache_goes_by_the_lengths_where_the_bound_is_short_of_pages():
+    c = cache(page=16, n_pages=7)
+    c.advance(20)
+    c.lengths.copy_(torch.tensor([20, 5, 9], dtype=torch.int32))   # rolled back since
+    c.len_bound = 40                                 # the bound would take 9 pages
+    c.reserve(10)
+    assert [len(p) for p in pages_of(c)] == [2, 2, 2] and c.len_bound == 20
+
+
+def test_cache_append_read_and_clone():
+    g = torch.Generator().manual_seed(1)
+    c = cache(page=16)
+    k, v = (torch.randn(3, 2, 37, 256, generator=g).bfloat16() for _ in range(2))
+    layer = 3
+    assert c.read_kv(0) is None
+    for a, b in ((0, 5), (5, 20), (20, 37)):
+        kk, vv = c.append_kv(layer, k[:, :, a:b], v[:, :, a:b])
+        assert torch.equal(kk, k[:, :, :b]) and torch.equal(vv, v[:, :, :b])
+        c.advance(b - a)
+    d = c.clone()
+    assert type(d) is Qwen3_5PagedCache and d.nbytes() == c.nbytes()
+    d.append_kv(layer, k[:, :, :20], v[:, :, :20])
+    d.advance(20)
+    assert len(c.free) == 12 and len(d.free) == 9 and c.seen_tokens == 37
+    assert torch.equal(c.read_kv(layer)[0], k) and torch.equal(d.read_kv(layer)[1][:, :, 37:], v[:, :, :20])
+
+
+def test_cache_refusals():
+    with pytest.raises(ValueError):
+        cache(page=48)
+    with pytest.raises(TypeError):
+        cache(kv_dtype=torch.float16)
+    with pytest.raises(ValueError):
+        cache(n_pages=0)
+    c = cache(page=32, kv_dtype=torch.float8_e4m3fn)
+    x = torch.zeros(3, 2, 1, 256, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="attn_append"):
+        c.append_kv(3, x, x)
+    assert set(c.layers[3]) == {"k", "v", "ks", "vs"} and set(c.layers[0]) == {"win", "rec", "rep"}
