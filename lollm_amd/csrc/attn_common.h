@@ -7,6 +7,8 @@ namespace lollm {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -70,6 +72,25 @@ __device__ __forceinline__ bf16x8 at_bf16(uint32_t w0, uint32_t w1, float scale)
   const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
   return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
+
+// Eight e4m3 codes as fp16, times a power of two of at most 1.  With 8-bit values the weights enter
+// their product as fp16, 11 bits of them, in one product, where bf16 values (whose range fp16 lacks)
+// take two of hi + lo bf16 weights.  So that no value leaves fp16's range, a tile of O counts in
+// units of the largest scale it has met: codes enter times their page's scale over that, and O is
+// rescaled where a larger one comes.  Scales are compared and divided as the bits of powers of two;
+// 0 is no scale (an unmapped page).
+__device__ __forceinline__ f16x8 at_f16(uint32_t w0, uint32_t w1, float ratio) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, ratio, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, ratio, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, ratio, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, ratio, true);
+  return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// a / b of two powers of two a <= b, or 1 where b is no scale; 2^-126 where it is less.
+__device__ __forceinline__ float at_ratio(int a, int b) {
+  return __int_as_float(b == 0 ? 0x3f800000 : max(a - b + 0x3f800000, 0x00800000));
+}
+__device__ __forceinline__ int at_scale_bits(float s) { return __float_as_int(s) & 0x7f800000; }
 
 constexpr int AW_WAVES = 4;
 constexpr int AW_THREADS = 64 * AW_WAVES;

@@ -5,7 +5,7 @@
 // j % page of page table[b][j / page]: rows of D values, (n_pages, Hkv, page, D).  A key whose
 // page is unmapped (an entry < 0 or >= n_pages) does not exist.  8-bit pages hold e4m3 codes c
 // and one power-of-two scale s for each (page, KV head) of K and of V: the value is c s, which
-// bf16 holds exactly, so both kinds of page go through the same bf16 products.
+// bf16 holds exactly.
 //
 // Work decomposition: attn_verify.hip's balanced split-K (128-key blocks of all (sequence, KV
 // head x query block) pairs dealt out evenly, one partial per workgroup and pair, the combine
@@ -18,11 +18,10 @@
 //      4 GB).  Rows of unmapped pages read page 0 and are masked.
 //   V: LDS DMA through a descriptor of the page's valid rows; the others become zeros, so that
 //      nothing that an unmapped or unwritten row holds meets a weight of 0.
-//   8 bits: a lane's 16 bytes of K are two k-steps (Q's columns are read in the same order);
-//      V is read with the transposing 8-bit LDS read; both become bf16 with
-//      v_cvt_scalef32_pk_bf16_fp8, which applies the scale.
-// Weights enter the product with V as hi + lo bf16 (attn_prefill.hip): the kernel waits for
-// memory, and the second product costs it nothing.
+//   8 bits: a lane's 16 bytes of K are two k-steps (Q's columns are read in the same order) and
+//      become bf16 with v_cvt_scalef32_pk_bf16_fp8, which applies the scale; V is read with the
+//      transposing 8-bit LDS read and becomes fp16 (at_f16).
+// Weights enter the product with V as hi + lo bf16 (attn_prefill.hip), with 8-bit V as fp16.
 #include <type_traits>
 
 #include "attn_common.h"
@@ -47,7 +46,8 @@ struct PagedSet {   // the V rows of a block in LDS
 struct PgUnit {
   int b, ph, j, L;
   int page[2];                // of the wave's keys 0..15 and 16..31, -1 unmapped or past the end
-  float ks[2], vs[2];
+  float ks[2];
+  int vs[2];                  // bits of V's scales, 0 unmapped
 };
 
 __device__ __forceinline__ uint32_t lds_at(const unsigned char* p) {
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   __shared__ __attribute__((aligned(256))) unsigned char vs1[Set::SET];   // V of odd blocks
   __shared__ __attribute__((aligned(16))) unsigned char own_dump[F8 ? PG_DUMP : 16];
   __shared__ __attribute__((aligned(16))) unsigned char qs[AT_ROWS * PG_QROW];   // Q of the pair
-  __shared__ float mx[AW_WAVES][32], lx[AW_WAVES][32];
+  __shared__ float mx[AW_WAVES][32], lx[AW_WAVES][32], vx[AW_WAVES];
   __shared__ int pre[AT_MAXB + 1], len[AT_MAXB], tmp[AW_WAVES];
   static_assert(F8 || PG_DUMP <= Set::SET, "the O dump fits a V set");
 
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       }
     }
   };
-  // (an unmapped page's rows of V are zeros: no NaN for a scale may meet them)
+  // (an unmapped page's scale is not there: whatever lies in page 0's may not meet its zeros)
   auto unit_scales = [&](PgUnit& X, uint32_t u) {
     const int i = (int)(u - tbase);
 #pragma unroll
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       const int k = __builtin_amdgcn_readlane(__float_as_int(tks[g]), i);
       const int v = __builtin_amdgcn_readlane(__float_as_int(tvs[g]), i);
       X.ks[g] = __int_as_float(X.page[g] >= 0 ? k : 0x3f800000);
-      X.vs[g] = __int_as_float(X.page[g] >= 0 ? v : 0x3f800000);
+      X.vs[g] = X.page[g] >= 0 ? v & 0x7f800000 : 0;
     }
   };
   auto unit = [&](uint32_t u) {
@@ -188,7 +188,8 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       X.page[g] = live ? __builtin_amdgcn_readlane(tp[g], i) : -1;
-      X.ks[g] = X.vs[g] = 1.f;
+      X.ks[g] = 1.f;
+      X.vs[g] = 0;
     }
     return X;
   };
@@ -273,6 +274,8 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 
   f32x16 O[8];            // O^T: d-tile dt (32 columns) x the 32 rows; lane row = l32
   float m_ref = -INFINITY, l_s = 0.f;
+  int v_ref = 0;          // 8 bits: O counts in units of this scale (bits), the largest met
+  constexpr float LAG = F8 ? 15.f : 16.f;   // (fp16 weights end at 2^16)
   const int lq = (int)(((uint32_t)l32 * p.rep_mul) >> 16);   // the lane's position in its query block
   int qpos = 0, rows = 0;
 
@@ -296,6 +299,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
           for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
         m_ref = -INFINITY;
         l_s = 0.f;
+        v_ref = 0;
         // (the previous pair's last block ended with barriers: no wave still reads qs)
 #pragma unroll
         for (int ii = 0; ii < 4; ++ii)
@@ -355,12 +359,15 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         }
         bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
         // the reference max moves (and l, O are rescaled) only when a row's block max exceeds it
-        // by more than 16 in the exponent: attn_verify's rule, each row's own decision
-        const bool big = (bm - m_ref) * a.cl2 > 16.f;
+        // by more than LAG in the exponent: attn_verify's rule, each row's own decision
+        const bool big = (bm - m_ref) * a.cl2 > LAG;
         const bool had = m_ref != -INFINITY;   // (nothing to rescale at a row's first block)
-        if (__builtin_amdgcn_readfirstlane((int)(__ballot(big && had) != 0))) {
-          const float alpha = big && had ? fast_exp2((m_ref - bm) * a.cl2) : 1.f;
+        const int v_now = F8 ? max(v_ref, max(C.vs[0], C.vs[1])) : 0;
+        const bool units = F8 && v_ref != 0 && v_now != v_ref;
+        if (__builtin_amdgcn_readfirstlane((int)(__ballot(big && had) != 0 || units))) {
+          float alpha = big && had ? fast_exp2((m_ref - bm) * a.cl2) : 1.f;
           l_s *= alpha;
+          if (units) alpha *= at_ratio(v_ref, v_now);
 #pragma unroll
           for (int dt = 0; dt < 8; ++dt) {
             // (O stays in accumulator registers but for the tile at hand: without the pins the
@@ -374,6 +381,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) asm volatile("" : "+a"(O[dt]));
         m_ref = big ? bm : m_ref;
+        v_ref = v_now;
         const float base = m_ref == -INFINITY ? 0.f : m_ref * a.cl2;
         float e[16];
 #pragma unroll
@@ -383,6 +391,11 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         for (int r = 0; r < 16; ++r) ps += e[r];
         l_s += ps;
         bf16x8 Ph[2], Pl[2];
+        f16x8 Pf[2];
+        if constexpr (F8) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) Pf[r >> 3][r & 7] = (_Float16)e[r];
+        } else
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
           u32x4_t hw, lw;
@@ -405,13 +418,13 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
           // bytes 8 (i % 2) of the group's chunk 2 dt + (group % 2), swizzled by the row
           const int i2 = (lane & 15) >> 1, key = (i2 & 3) + 4 * h + 8 * (i2 >> 2);
           const uint32_t at = set_at + (uint32_t)(256 * key + 16 * (((lane >> 4) & 1) ^ key) + 8 * (lane & 1));
+          const float ratio[2] = {at_ratio(C.vs[0], v_ref), at_ratio(C.vs[1], v_ref)};
           i32x2_t v[16];   // column tile i / 2, keys 16 (i % 2) ..
           pg_read_codes(at, v);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const bf16x8 vA = at_bf16((uint32_t)v[i].x, (uint32_t)v[i].y, C.vs[i & 1]);
-            O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Ph[i & 1], O[i >> 1], 0, 0, 0);
-            O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[i & 1], O[i >> 1], 0, 0, 0);
+            const f16x8 vA = at_f16((uint32_t)v[i].x, (uint32_t)v[i].y, ratio[i & 1]);
+            O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vA, Pf[i & 1], O[i >> 1], 0, 0, 0);
           }
         } else {
           const int x = 4 * h + ((lane & 15) >> 2);
@@ -442,6 +455,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         if (h == 0) {
           mx[wave][l32] = m_ref;
           lx[wave][l32] = lrow;
+          if (F8 && l32 == 0) vx[wave] = __int_as_float(v_ref);
         }
         float* part = a.ws + ((size_t)w + C.b * PH + C.ph) * AT_PART;
         float* dump = reinterpret_cast<float*>(F8 ? own_dump : vset);
@@ -471,6 +485,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
               const float mw = mx[ww][row];
               wgt[ww] = mw == -INFINITY ? 0.f : fast_exp2((mw - M) * a.cl2);
               Lsum += lx[ww][row] * wgt[ww];
+              if constexpr (F8) wgt[ww] *= vx[ww];
             }
             if (D0 == 0 && c4 == 0) {
               part[row] = M;

@@ -245,14 +245,22 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   const int wg = wave >> 1;   // the half of a block that holds the wave's rows
   int pg[3] = {-1, -1, -1}, pn = -1;   // pages of the wave's rows of blocks 0 .. 2, then 3
   uint32_t vm = 3;                     // mapped halves: 2 bits from block j + 1 on
-  float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f};   // scales of the next block's K, of this one's V
+  float ksc[2] = {1.f, 1.f};           // scales of the next block's K
+  int vsc[2] = {0, 0}, v_ref = 0;      // of this block's V (bits), and the units of O (at_f16)
+  constexpr float LAG = F8 ? 15.f : 16.f;   // (fp16 weights end at 2^16)
   auto scales = [&](const float* sc, int j, float (&to)[2]) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int id = page_at(j, g);
       const float s = ap_sload(sc, (long long)max(id, 0) * a.Hkv + kvh);
-      to[g] = id >= 0 ? s : 1.f;
+      to[g] = id >= 0 ? s : 0.f;
     }
+  };
+  auto scale_bits = [&](const float* sc, int j, int (&to)[2]) {
+    float f[2];
+    scales(sc, j, f);
+    to[0] = at_scale_bits(f[0]);
+    to[1] = at_scale_bits(f[1]);
   };
   if constexpr (KV != AP_ROWS) {
 #pragma unroll
@@ -284,7 +292,9 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
 
   f32x16 O[RG][8];   // O^T: 32 columns x 32 rows per tile; lane's row = l32
   float m_ref[RG], l_s[RG];
-  bf16x8 P[RG][2], Pl[RG][2];   // exp of the block whose V comes next, hi and lo
+  // exp of the block whose V comes next: hi and lo bf16, or fp16
+  bf16x8 P[RG][2], Pl[RG][2];
+  f16x8 Pf[RG][2];
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     m_ref[rg] = -INFINITY;
@@ -303,7 +313,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     int kof = ko;
     asm volatile("" : "+v"(kof));
     if constexpr (F8) {
-      const float sc = l32 < 16 ? ksc[0] : ksc[1];
+      const float sc = l32 < 16 ? ksc[0] : ksc[1];   // (0, an exponent like any, where K is masked)
       u32x4_t kw[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) kw[i] = *reinterpret_cast<const u32x4_t*>(kset + (kof ^ (32 * i)));
@@ -355,8 +365,8 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
       const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(bm), __float_as_uint(bm), false, false);
       bm = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
       // the reference max moves (and l, O are rescaled) only when a row's block max exceeds it
-      // by more than 16 in the exponent: attn_verify's rule, each row's own decision
-      const bool big = (bm - m_ref[rg]) * a.cl2 > 16.f;
+      // by more than LAG in the exponent: attn_verify's rule, each row's own decision
+      const bool big = (bm - m_ref[rg]) * a.cl2 > LAG;
       const float mn = big ? fmaxf(m_ref[rg], bm) : m_ref[rg];
       alpha[rg] = (!big || mn == -INFINITY) ? 1.f : fast_exp2((m_ref[rg] - mn) * a.cl2);
       m_ref[rg] = mn;
@@ -366,8 +376,9 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     }
     moved = __builtin_amdgcn_readfirstlane((int)(__ballot(any) != 0)) != 0;
   };
-  auto rescale = [&]() {
-    if (moved) {
+  // (factor: of the units of O, by which the next block's V counts)
+  auto rescale = [&](float factor, bool units) {
+    if (moved || units) {
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
@@ -375,7 +386,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
           // (O stays in accumulator registers but for the tile at hand: without the pins the
           // compiler copies all of it to vector registers around this branch)
           asm volatile("" : "+a"(O[rg][dt]));
-          O[rg][dt] *= alpha[rg];
+          O[rg][dt] *= F8 ? alpha[rg] * factor : alpha[rg];
           asm volatile("" : "+a"(O[rg][dt]));
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -389,7 +400,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // block j + 1 between its products (the matrix pipe is busy 32 cycles per product, the
   // wave's VALU work of one product about as long).  Past the wave's last block the scores
   // are all masked.
-  auto step = [&](const unsigned char* knext, const unsigned char* vset, int j) {
+  auto step = [&](const unsigned char* knext, const unsigned char* vset, int j, const int (&v_coming)[2]) {
     if (j >= wblk) return;
     scores(knext, j + 1, vm & 3);
     int vof = vo;
@@ -411,25 +422,32 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     decltype(read_v(0)) vf[AP_AHEAD];
     u32x4_t Pn[RG][2], Pm[RG][2];
     float pe[RG];
+    const float ratio[2] = {at_ratio(vsc[0], v_ref), at_ratio(vsc[1], v_ref)};   // (8 bits)
 #pragma unroll
     for (int i = 0; i < AP_AHEAD; ++i) vf[i] = read_v(i);
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
-      bf16x8 vA;
-      if constexpr (F8) vA = at_bf16(vf[n % AP_AHEAD].x, vf[n % AP_AHEAD].y, vsc[n & 1]); else vA = vf[n % AP_AHEAD];
+      if constexpr (F8) {
+        const f16x8 vA = at_f16(vf[n % AP_AHEAD].x, vf[n % AP_AHEAD].y, ratio[n & 1]);
 #pragma unroll
-      for (int rg = 0; rg < RG; ++rg)
-        O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, P[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+        for (int rg = 0; rg < RG; ++rg)
+          O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vA, Pf[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+      } else {
 #pragma unroll
-      for (int rg = 0; rg < RG; ++rg)
-        O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vA, Pl[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+        for (int rg = 0; rg < RG; ++rg)
+          O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AP_AHEAD], P[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+#pragma unroll
+        for (int rg = 0; rg < RG; ++rg)
+          O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AP_AHEAD], Pl[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+      }
       if (n + AP_AHEAD < 16) vf[n % AP_AHEAD] = read_v(n + AP_AHEAD);
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg) {
         const float p = fast_exp2(__builtin_fmaf(S[rg][n], a.cl2, -base[rg]));
         if (n & 1) {   // (pinned here: the compiler would sink them all past the rescale)
-          uint32_t hi, lo;
-          at_split(pe[rg], p, hi, lo);
+          uint32_t hi, lo = 0;
+          if constexpr (F8) hi = __builtin_bit_cast(uint32_t, f16x2{(_Float16)pe[rg], (_Float16)p});
+          else at_split(pe[rg], p, hi, lo);
           l_s[rg] += pe[rg] + p;
           asm volatile("" : "+v"(hi), "+v"(lo), "+v"(l_s[rg]));
           Pn[rg][n >> 3][(n & 7) >> 1] = hi;
@@ -444,10 +462,16 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
-        P[rg][k2] = __builtin_bit_cast(bf16x8, Pn[rg][k2]);
-        Pl[rg][k2] = __builtin_bit_cast(bf16x8, Pm[rg][k2]);
+        if constexpr (F8) {
+          Pf[rg][k2] = __builtin_bit_cast(f16x8, Pn[rg][k2]);
+        } else {
+          P[rg][k2] = __builtin_bit_cast(bf16x8, Pn[rg][k2]);
+          Pl[rg][k2] = __builtin_bit_cast(bf16x8, Pm[rg][k2]);
+        }
       }
-    rescale();
+    const int v_next = F8 ? max(v_ref, max(v_coming[0], v_coming[1])) : 0;
+    rescale(F8 ? at_ratio(v_ref, v_next) : 1.f, F8 && v_next != v_ref);
+    if constexpr (F8) v_ref = v_next;
   };
 
   if constexpr (F8) {
@@ -465,26 +489,32 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
       for (int r = 0; r < 16; r += 2) {
         const float p0 = fast_exp2(__builtin_fmaf(S[rg][r], a.cl2, -base[rg]));
         const float p1 = fast_exp2(__builtin_fmaf(S[rg][r + 1], a.cl2, -base[rg]));
-        uint32_t hi, lo;
-        at_split(p0, p1, hi, lo);
+        uint32_t hi, lo = 0;
+        if constexpr (F8) hi = __builtin_bit_cast(uint32_t, f16x2{(_Float16)p0, (_Float16)p1});
+        else at_split(p0, p1, hi, lo);
         l_s[rg] += p0 + p1;
         Pn[r >> 3][(r & 7) >> 1] = hi;
         Pm[r >> 3][(r & 7) >> 1] = lo;
       }
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
-        P[rg][k2] = __builtin_bit_cast(bf16x8, Pn[k2]);
-        Pl[rg][k2] = __builtin_bit_cast(bf16x8, Pm[k2]);
+        if constexpr (F8) {
+          Pf[rg][k2] = __builtin_bit_cast(f16x8, Pn[k2]);
+        } else {
+          P[rg][k2] = __builtin_bit_cast(bf16x8, Pn[k2]);
+          Pl[rg][k2] = __builtin_bit_cast(bf16x8, Pm[k2]);
+        }
       }
     }
-    rescale();
+    rescale(1.f, false);
   }
   // Barrier before step j: blocks j + 1 of K and j of V have landed (the 8 loads after them, 4 of
   // 8-bit pages, may be in flight), and every wave is done with K of block j and V of block j - 1,
   // whose sets the loads of blocks j + 3 and j + 2 take.
   if constexpr (F8) {
     scales(a.ks, j0 + 1, ksc);
-    scales(a.vs, j0, vsc);
+    scale_bits(a.vs, j0, vsc);
+    v_ref = max(vsc[0], vsc[1]);
   }
   if constexpr (KV != AP_ROWS) vm = mapped(j0 + 1);
   auto turn = [&](unsigned char* kfree, unsigned char* vfree, const unsigned char* knext, const unsigned char* vset,
@@ -492,7 +522,8 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     if constexpr (F8) AP_BARRIER(4); else AP_BARRIER(8);
     load_k(kfree, pn, j + 3);
     load_v(vfree, pg[2], j + 2);
-    float kn[2], vn[2];
+    float kn[2];
+    int vn[2] = {0, 0};
     uint32_t mn = 3;
     if constexpr (KV != AP_ROWS) {   // what the next step needs, on its way during this one
       pg[2] = pn;
@@ -501,9 +532,9 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     }
     if constexpr (F8) {
       scales(a.ks, j + 2, kn);
-      scales(a.vs, j + 1, vn);
+      scale_bits(a.vs, j + 1, vn);
     }
-    step(knext, vset, j);
+    step(knext, vset, j, vn);
     vm = mn;
     if constexpr (F8) {
 #pragma unroll
@@ -530,7 +561,8 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_s[rg]), __float_as_uint(l_s[rg]), false, false);
     const float l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     const bool whole = !PARTS || parts == 1;
-    const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);   // no key seen: zeros
+    float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);   // no key seen: zeros
+    if constexpr (F8) inv *= __int_as_float(v_ref);
     float* piece = nullptr;
     if constexpr (PARTS) {
       if (!whole) {

@@ -23,9 +23,12 @@ def pow2_scale(amax):
 
 
 def attention(q, k_pages, v_pages, table, kv_len, gate, k_scale=None, v_scale=None, scale=None):
-    """(out (B, T, Hq*D), tolerance of a bf16 result): half a bf16 step of the value (2^-8), the
-    weights' 16 bits (2^-15 for the weight and the sum) and the fp32 scores (258 roundings of
-    2^-24 on the absolute products, doubled for the sum), on the weighted mean of |v|."""
+    """(out (B, T, Hq*D), tolerance of a bf16 result): half a bf16 step of the value (2^-8); on the
+    weighted mean of |v| half a step of the weights' type (bf16 pages: hi + lo, 16 bits, 2^-15 for
+    the weight and the sum; 8-bit pages: fp16, 2^-11) and the fp32 scores (258 roundings of 2^-24 on
+    the absolute products, doubled for the sum); and for fp16 weights, whose step ends at 2^-24, half
+    of that (2^-25) on the sum of |v| beside a largest weight of 1 or more."""
+    weight = 2.0 ** -14 if k_scale is None else 2.0 ** -11
     B, T, Hq, _ = q.shape
     n, Hkv, P, _ = k_pages.shape
     s = D ** -0.5 if scale is None else scale
@@ -47,7 +50,9 @@ def attention(q, k_pages, v_pages, table, kv_len, gate, k_scale=None, v_scale=No
             p = torch.softmax(x, -1).nan_to_num(0.0)
             out[b, :, h] = p @ vb
             ds = 258 * 2.0 ** -24 * (qb.abs() @ kb.abs().T * s).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
-            tol[b, :, h] = (2.0 ** -14 + 2 * ds) * (p @ vb.abs())
+            tol[b, :, h] = (weight + 2 * ds) * (p @ vb.abs())
+            if k_scale is not None:
+                tol[b, :, h] += 2.0 ** -25 * p.amax(-1, keepdim=True) * ((~hidden).double() @ vb.abs())
     if gate is not None:
         g = torch.sigmoid(gate.double().reshape(B, T, Hq, D))
         out, tol = out * g, tol * g
