@@ -162,12 +162,13 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   const __amdgpu_buffer_rsrc_t krs = buf_rsrc(a.kc + cbase, KV == AP_ROWS ? (uint32_t)L * (AT_D * 2) : 0u);
   const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(a.vc + cbase, KV == AP_ROWS ? (uint32_t)L * (AT_D * 2) : 0u);
   // page of keys 16 g .. of block j, -1: unmapped or past this workgroup's blocks
-  auto page_at = [&](int j, int g) {
-    const uint32_t key = (uint32_t)(j * AP_KEYS + 16 * g);   // (no branch: O lives in all of them)
-    const int id = ap_sload(a.table, b * a.table_stride + (min(key, (uint32_t)max(L - 1, 0)) >> a.pshift));
-    return key < (uint32_t)Lend && (uint32_t)id < (uint32_t)a.n_pages ? id : -1;
+  auto entry = [&](int j, int g) {   // (no branch: O lives in all of them)
+    const uint32_t key = (uint32_t)(j * AP_KEYS + 16 * g);
+    return ap_sload(a.table, b * a.table_stride + (min(key, (uint32_t)max(L - 1, 0)) >> a.pshift));
   };
-  auto mapped = [&](int j) { return (page_at(j, 0) >= 0 ? 1u : 0u) | (page_at(j, 1) >= 0 ? 2u : 0u); };
+  auto page_of = [&](int id, int j, int g) {
+    return (uint32_t)(j * AP_KEYS + 16 * g) < (uint32_t)Lend && (uint32_t)id < (uint32_t)a.n_pages ? id : -1;
+  };
   auto page_rsrc = [&](const uint16_t* pool, int id, int j) {
     const int key = j * AP_KEYS + WR * wave;
     const long long row = (((long long)max(id, 0) * a.Hkv + kvh) << a.pshift) + (key & ((1 << a.pshift) - 1));
@@ -242,38 +243,37 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
       Q[rg][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(
                                                  src + (F8 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1) : 16 * ks + 8 * h)));
   }
-  const int wg = wave >> 1;   // the half of a block that holds the wave's rows
-  int pg[3] = {-1, -1, -1}, pn = -1;   // pages of the wave's rows of blocks 0 .. 2, then 3
-  uint32_t vm = 3;                     // mapped halves: 2 bits from block j + 1 on
-  float ksc[2] = {1.f, 1.f};           // scales of the next block's K
-  int vsc[2] = {0, 0}, v_ref = 0;      // of this block's V (bits), and the units of O (at_f16)
+  // Pages (two halves of a block): of blocks j + 1, j + 2 and j + 3 before step j, and the entry of
+  // block j + 4; the scales of block j + 1's K and of block j's V.  What a step asks the scalar
+  // cache for, the next one uses.
+  const int wg = wave >> 1;            // the half of a block that holds the wave's rows
+  int pg[3][2], raw[2] = {-1, -1}, pg0[2] = {-1, -1};
+  float ksc[2] = {0.f, 0.f};
+  int vsc[2] = {0, 0}, v_ref = 0;      // (bits; v_ref: the units of O, at_f16)
   constexpr float LAG = F8 ? 15.f : 16.f;   // (fp16 weights end at 2^16)
-  auto scales = [&](const float* sc, int j, float (&to)[2]) {
+  auto scale_at = [&](const float* sc, int id) {
+    const float s = ap_sload(sc, (long long)max(id, 0) * a.Hkv + kvh);
+    return id >= 0 ? s : 0.f;
+  };
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int id = page_at(j, g);
-      const float s = ap_sload(sc, (long long)max(id, 0) * a.Hkv + kvh);
-      to[g] = id >= 0 ? s : 0.f;
+  for (int g = 0; g < 2; ++g) {
+    pg[0][g] = pg[1][g] = pg[2][g] = -1;
+    if constexpr (KV != AP_ROWS) {
+      pg0[g] = page_of(entry(j0, g), j0, g);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) pg[n][g] = page_of(entry(j0 + 1 + n, g), j0 + 1 + n, g);
+      raw[g] = entry(j0 + 4, g);
     }
-  };
-  auto scale_bits = [&](const float* sc, int j, int (&to)[2]) {
-    float f[2];
-    scales(sc, j, f);
-    to[0] = at_scale_bits(f[0]);
-    to[1] = at_scale_bits(f[1]);
-  };
-  if constexpr (KV != AP_ROWS) {
-#pragma unroll
-    for (int j = 0; j < 3; ++j) pg[j] = page_at(j0 + j, wg);
-    pn = page_at(j0 + 3, wg);
   }
-  const uint32_t vm0 = KV == AP_ROWS ? 3u : mapped(j0);
+  auto both = [&](const int (&id)[2]) {   // mapped halves
+    return KV == AP_ROWS ? 3u : (id[0] >= 0 ? 1u : 0u) | (id[1] >= 0 ? 2u : 0u);
+  };
   AP_BARRIER(0);   // the zeroed sets, before any DMA into them (and Q: the counts below are the DMA's)
-  load_k(ks0, pg[0], j0);
-  load_k(ks1, pg[1], j0 + 1);
-  load_v(vs0, pg[0], j0);
-  load_k(ks2, pg[2], j0 + 2);
-  load_v(vs1, pg[1], j0 + 1);
+  load_k(ks0, pg0[wg], j0);
+  load_k(ks1, pg[0][wg], j0 + 1);
+  load_v(vs0, pg0[wg], j0);
+  load_k(ks2, pg[1][wg], j0 + 2);
+  load_v(vs1, pg[0][wg], j0 + 1);
 
   // the positions this wave's rows span: the key blocks it sees, and which need a mask
   const int wq0 = ap_div(32 * RG * wave, a.rep_mul);
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // are all masked.
   auto step = [&](const unsigned char* knext, const unsigned char* vset, int j, const int (&v_coming)[2]) {
     if (j >= wblk) return;
-    scores(knext, j + 1, vm & 3);
+    scores(knext, j + 1, both(pg[0]));
     int vof = vo;
     asm volatile("" : "+v"(vof));
     auto read_v = [&](int n) {   // operand n = 2 dt + k2, by transposing reads (attn_verify's key order)
@@ -475,13 +475,14 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   };
 
   if constexpr (F8) {
-    scales(a.ks, j0, ksc);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) ksc[g] = scale_at(a.ks, pg0[g]);
     AP_BARRIER(8);    // block 0 of K, the first 2 of the 10 loads
   } else {
     AP_BARRIER(16);   // block 0 of K, the first 4 of the 20 loads
   }
   if (wblk > j0) {
-    scores(ks0, j0, vm0);
+    scores(ks0, j0, both(pg0));
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
       u32x4_t Pn[2], Pm[2];
@@ -512,36 +513,37 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   // 8-bit pages, may be in flight), and every wave is done with K of block j and V of block j - 1,
   // whose sets the loads of blocks j + 3 and j + 2 take.
   if constexpr (F8) {
-    scales(a.ks, j0 + 1, ksc);
-    scale_bits(a.vs, j0, vsc);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      ksc[g] = scale_at(a.ks, pg[0][g]);
+      vsc[g] = at_scale_bits(scale_at(a.vs, pg0[g]));
+    }
     v_ref = max(vsc[0], vsc[1]);
   }
-  if constexpr (KV != AP_ROWS) vm = mapped(j0 + 1);
   auto turn = [&](unsigned char* kfree, unsigned char* vfree, const unsigned char* knext, const unsigned char* vset,
                   int j) {
     if constexpr (F8) AP_BARRIER(4); else AP_BARRIER(8);
-    load_k(kfree, pn, j + 3);
-    load_v(vfree, pg[2], j + 2);
-    float kn[2];
-    int vn[2] = {0, 0};
-    uint32_t mn = 3;
-    if constexpr (KV != AP_ROWS) {   // what the next step needs, on its way during this one
-      pg[2] = pn;
-      pn = page_at(j + 4, wg);
-      mn = mapped(j + 2);
-    }
-    if constexpr (F8) {
-      scales(a.ks, j + 2, kn);
-      scale_bits(a.vs, j + 1, vn);
+    load_k(kfree, pg[2][wg], j + 3);
+    load_v(vfree, pg[1][wg], j + 2);
+    float kn[2] = {0.f, 0.f};
+    int vn[2] = {0, 0}, rn[2] = {-1, -1};
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      if constexpr (KV != AP_ROWS) rn[g] = entry(j + 5, g);
+      if constexpr (F8) {
+        kn[g] = scale_at(a.ks, pg[1][g]);
+        vn[g] = at_scale_bits(scale_at(a.vs, pg[0][g]));
+      }
     }
     step(knext, vset, j, vn);
-    vm = mn;
-    if constexpr (F8) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        ksc[g] = kn[g];
-        vsc[g] = vn[g];
-      }
+    for (int g = 0; g < 2; ++g) {
+      pg[0][g] = pg[1][g];
+      pg[1][g] = pg[2][g];
+      if constexpr (KV != AP_ROWS) pg[2][g] = page_of(raw[g], j + 4, g);
+      raw[g] = rn[g];
+      ksc[g] = kn[g];
+      vsc[g] = vn[g];
     }
   };
   for (int j = j0; j < nblk; j += 3) {
