@@ -73,12 +73,12 @@ __device__ __forceinline__ bf16x8 at_bf16(uint32_t w0, uint32_t w1, float scale)
   return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Eight e4m3 codes as fp16, times a power of two of at most 1.  With 8-bit values the weights enter
+// Eight e4m3 codes as fp16, times a power of two of at most 2^7.  With 8-bit values the weights enter
 // their product as fp16, 11 bits of them, in one product, where bf16 values (whose range fp16 lacks)
 // take two of hi + lo bf16 weights.  So that no value leaves fp16's range, a tile of O counts in
-// units of the largest scale it has met: codes enter times their page's scale over that, and O is
-// rescaled where a larger one comes.  Scales are compared and divided as the bits of powers of two;
-// 0 is no scale (an unmapped page).
+// units of a scale that it has met: codes enter times their page's scale over that (448 * 2^7 is
+// below 2^16), and O is rescaled where one comes that is more than 2^7 of it.  Scales are compared
+// and divided as the bits of powers of two; 0 is no scale (an unmapped page).
 __device__ __forceinline__ f16x8 at_f16(uint32_t w0, uint32_t w1, float ratio) {
   const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, ratio, false);
   const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, ratio, true);
@@ -86,7 +86,11 @@ __device__ __forceinline__ f16x8 at_f16(uint32_t w0, uint32_t w1, float ratio) {
   const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, ratio, true);
   return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
-// a / b of two powers of two a <= b, or 1 where b is no scale; 2^-126 where it is less.
+__device__ __forceinline__ int at_units(int units, int a, int b) {   // for a block of these scales
+  const int m = max(a, b);
+  return units == 0 || m > units + (7 << 23) ? max(m, units) : units;
+}
+// a / b of two powers of two, or 1 where b is no scale; 2^-126 where it is less.
 __device__ __forceinline__ float at_ratio(int a, int b) {
   return __int_as_float(b == 0 ? 0x3f800000 : max(a - b + 0x3f800000, 0x00800000));
 }

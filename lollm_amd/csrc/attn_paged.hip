@@ -274,7 +274,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 
   f32x16 O[8];            // O^T: d-tile dt (32 columns) x the 32 rows; lane row = l32
   float m_ref = -INFINITY, l_s = 0.f;
-  int v_ref = 0;          // 8 bits: O counts in units of this scale (bits), the largest met
+  int v_ref = 0;          // 8 bits: O counts in units of this scale (bits), at_f16
   constexpr float LAG = F8 ? 15.f : 16.f;   // (fp16 weights end at 2^16)
   const int lq = (int)(((uint32_t)l32 * p.rep_mul) >> 16);   // the lane's position in its query block
   int qpos = 0, rows = 0;
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         // by more than LAG in the exponent: attn_verify's rule, each row's own decision
         const bool big = (bm - m_ref) * a.cl2 > LAG;
         const bool had = m_ref != -INFINITY;   // (nothing to rescale at a row's first block)
-        const int v_now = F8 ? max(v_ref, max(C.vs[0], C.vs[1])) : 0;
+        const int v_now = F8 ? at_units(v_ref, C.vs[0], C.vs[1]) : 0;
         const bool units = F8 && v_ref != 0 && v_now != v_ref;
         if (__builtin_amdgcn_readfirstlane((int)(__ballot(big && had) != 0 || units))) {
           float alpha = big && had ? fast_exp2((m_ref - bm) * a.cl2) : 1.f;

@@ -169,17 +169,17 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   auto page_of = [&](int id, int j, int g) {
     return (uint32_t)(j * AP_KEYS + 16 * g) < (uint32_t)Lend && (uint32_t)id < (uint32_t)a.n_pages ? id : -1;
   };
-  auto page_rsrc = [&](const uint16_t* pool, int id, int j) {
+  struct Rows { long long at; uint32_t bytes; };   // the wave's rows of a block, the same in both pools
+  auto rows_of = [&](int id, int j) {
     const int key = j * AP_KEYS + WR * wave;
     const long long row = (((long long)max(id, 0) * a.Hkv + kvh) << a.pshift) + (key & ((1 << a.pshift) - 1));
-    const int rows = id >= 0 ? min(max(L - key, 0), WR) : 0;
-    return buf_rsrc((const unsigned char*)pool + row * ROW, (uint32_t)(rows * ROW));
+    return Rows{row * ROW, id >= 0 ? (uint32_t)(min(max(L - key, 0), WR) * ROW) : 0u};
   };
   // 8 bits: four rows a load, the 16-byte chunk c of row r at c ^ (r & 15)
   const uint32_t l8 = 256u * (lane >> 4) + 16u * ((lane & 15) ^ (8 * (wave & 1) + (lane >> 4)));
-  auto issue_page = [&](unsigned char* d, const uint16_t* pool, int id, int j, uint32_t x, uint32_t swz) {
+  auto issue_page = [&](unsigned char* d, const uint16_t* pool, const Rows& r, uint32_t x, uint32_t swz) {
     asm volatile("" : "+v"(x));
-    const __amdgpu_buffer_rsrc_t rs = page_rsrc(pool, id, j);
+    const __amdgpu_buffer_rsrc_t rs = buf_rsrc((const unsigned char*)pool + r.at, r.bytes);
     constexpr int N = F8 ? WR / 4 : WR / 2;
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -208,15 +208,15 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
       __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void_t*)(vd + 512 * WR * wave + 1024 * i), 16,
                                                blk + 1024u * i + (x ^ (64u * i)), 0, 0, 0);
   };
-  auto load_k = [&](unsigned char* kd, int id, int j) {
+  auto load_k = [&](unsigned char* kd, const Rows& r, int j) {
     if constexpr (KV == AP_ROWS) issue_k(kd, j);
-    else if constexpr (F8) issue_page(kd, a.kc, id, j, l8, 64u);
-    else issue_page(kd, a.kc, id, j, kl, 32u);
+    else if constexpr (F8) issue_page(kd, a.kc, r, l8, 64u);
+    else issue_page(kd, a.kc, r, kl, 32u);
   };
-  auto load_v = [&](unsigned char* vd, int id, int j) {
+  auto load_v = [&](unsigned char* vd, const Rows& r, int j) {
     if constexpr (KV == AP_ROWS) issue_v(vd, j);
-    else if constexpr (F8) issue_page(vd, a.vc, id, j, l8, 64u);
-    else issue_page(vd, a.vc, id, j, vl, 64u);
+    else if constexpr (F8) issue_page(vd, a.vc, r, l8, 64u);
+    else issue_page(vd, a.vc, r, vl, 64u);
   };
   // this wave's loads up to the last N have landed and its LDS accesses are complete, then
   // every wave's
@@ -269,11 +269,13 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
     return KV == AP_ROWS ? 3u : (id[0] >= 0 ? 1u : 0u) | (id[1] >= 0 ? 2u : 0u);
   };
   AP_BARRIER(0);   // the zeroed sets, before any DMA into them (and Q: the counts below are the DMA's)
-  load_k(ks0, pg0[wg], j0);
-  load_k(ks1, pg[0][wg], j0 + 1);
-  load_v(vs0, pg0[wg], j0);
-  load_k(ks2, pg[1][wg], j0 + 2);
-  load_v(vs1, pg[0][wg], j0 + 1);
+  const Rows first = rows_of(pg0[wg], j0), second = rows_of(pg[0][wg], j0 + 1);
+  Rows coming = rows_of(pg[1][wg], j0 + 2);   // of block j + 2 before step j
+  load_k(ks0, first, j0);
+  load_k(ks1, second, j0 + 1);
+  load_v(vs0, first, j0);
+  load_k(ks2, coming, j0 + 2);
+  load_v(vs1, second, j0 + 1);
 
   // the positions this wave's rows span: the key blocks it sees, and which need a mask
   const int wq0 = ap_div(32 * RG * wave, a.rep_mul);
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
           Pl[rg][k2] = __builtin_bit_cast(bf16x8, Pm[rg][k2]);
         }
       }
-    const int v_next = F8 ? max(v_ref, max(v_coming[0], v_coming[1])) : 0;
+    const int v_next = F8 ? at_units(v_ref, v_coming[0], v_coming[1]) : 0;
     rescale(F8 ? at_ratio(v_ref, v_next) : 1.f, F8 && v_next != v_ref);
     if constexpr (F8) v_ref = v_next;
   };
@@ -523,8 +525,10 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   auto turn = [&](unsigned char* kfree, unsigned char* vfree, const unsigned char* knext, const unsigned char* vset,
                   int j) {
     if constexpr (F8) AP_BARRIER(4); else AP_BARRIER(8);
-    load_k(kfree, pg[2][wg], j + 3);
-    load_v(vfree, pg[1][wg], j + 2);
+    const Rows next = rows_of(pg[2][wg], j + 3);
+    load_k(kfree, next, j + 3);
+    load_v(vfree, F8 ? coming : rows_of(pg[1][wg], j + 2), j + 2);
+    coming = next;
     float kn[2] = {0.f, 0.f};
     int vn[2] = {0, 0}, rn[2] = {-1, -1};
 #pragma unroll
