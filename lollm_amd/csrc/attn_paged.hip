@@ -206,8 +206,10 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   auto issue_k = [&](u32x4_t (&to)[KL], const PgUnit& X) {
     const int key0 = X.j * AT_BLOCK + PG_WKEYS * wave;
     const long long r0 = row_of(X, max(X.page[0], 0), key0), r1 = row_of(X, max(X.page[1], 0), key0 + 16);
-    const unsigned char* src = reinterpret_cast<const unsigned char*>(a.kc) +
-                               (l32 < 16 ? r0 : r1) * Set::ROW + (l32 & 15) * Set::ROW + 16 * h;
+    // (without a page all lanes read the pool's first bytes, one line an instruction)
+    const long long at = (l32 < 16 ? r0 : r1) * Set::ROW + (l32 & 15) * Set::ROW + 16 * h;
+    const unsigned char* src =
+        reinterpret_cast<const unsigned char*>(a.kc) + ((l32 < 16 ? X.page[0] : X.page[1]) >= 0 ? at : 0);
 #pragma unroll
     for (int i = 0; i < KL; ++i) to[i] = *reinterpret_cast<const u32x4_t*>(src + 32 * i);
   };
