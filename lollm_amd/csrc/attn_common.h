@@ -96,6 +96,19 @@ __device__ __forceinline__ float at_ratio(int a, int b) {
 }
 __device__ __forceinline__ int at_scale_bits(float s) { return __float_as_int(s) & 0x7f800000; }
 
+// Four columns of a finished row: acc / l (inv = 1 / l, 0 where no key was seen) times sigmoid(gate).
+__device__ __forceinline__ void at_store4(uint16_t* out, const float (&acc)[4], float inv, bool gated, uint2 gate) {
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t g = e < 2 ? gate.x : gate.y;
+    y[e] = acc[e] * inv;
+    if (gated) y[e] *= sigmoidf_(__uint_as_float(e & 1 ? g & 0xffff0000u : g << 16));
+  }
+  const bf16x2 lo = {(__bf16)y[0], (__bf16)y[1]}, hi = {(__bf16)y[2], (__bf16)y[3]};
+  *reinterpret_cast<uint2*>(out) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
 constexpr int AW_WAVES = 4;
 constexpr int AW_THREADS = 64 * AW_WAVES;
 constexpr int AT_BLOCK = 128;        // keys per block

@@ -531,12 +531,12 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   }
 }
 
-// Merges the pieces of pair blockIdx.y for its row blockIdx.x and applies the gate: thread d owns
-// column d.  The pieces are those of workgroups wf .. wl of the table, in that order; every wave
-// forms the weights of 64 pieces in its lanes while the first columns are on their way.
-__global__ __launch_bounds__(AT_D) void attn_paged_combine_kernel(PagedArgs p) {
+// Merges the pieces of pair blockIdx.y for its rows 4 blockIdx.x .., a wave per row with 4 columns a
+// lane, and applies the gate.  The pieces are those of workgroups wf .. wl of the table, in that
+// order; the weights of 64 of them are formed in the lanes while the first columns are on their way.
+__global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedArgs p) {
   const AttnArgs& a = p.a;
-  const int r = blockIdx.x, pair = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int r = 4 * blockIdx.x + (threadIdx.x >> 6), pair = blockIdx.y, lane = threadIdx.x & 63;
   const int PH = a.Hkv * a.qblocks;
   const int2 te = reinterpret_cast<const int2*>(a.ws + (size_t)(a.nw + a.B * PH) * AT_PART)[pair];
   const int b = pair / PH, ph = pair - b * PH, kvh = ph / a.qblocks;
@@ -544,19 +544,21 @@ __global__ __launch_bounds__(AT_D) void attn_paged_combine_kernel(PagedArgs p) {
   const int i = (int)(((uint32_t)r * p.rep_mul) >> 16), h = kvh * a.n_rep + r - i * a.n_rep;
   if (i >= min(a.QB, a.T - q0)) return;
   const size_t bt = (size_t)b * a.T + q0 + i;
-  const float gl = a.gate ? bf16_to_f32(a.gate[bt * a.gate_row + (size_t)h * a.gate_head + tid]) : 0.f;
+  uint2 gv = make_uint2(0, 0);
+  if (a.gate) gv = *reinterpret_cast<const uint2*>(a.gate + bt * a.gate_row + (size_t)h * a.gate_head + 4 * lane);
   const int wf = te.x, np = wf < 0 ? 0 : te.y - wf + 1;
   const float* base = a.ws + ((size_t)max(wf, 0) + pair) * AT_PART;
-  const float* col = base + 2 * AT_ROWS + r * AT_D + tid;
-  constexpr int AHEAD = 8;
-  float M = -INFINITY, l = 0.f, acc = 0.f;
+  const float* col = base + 2 * AT_ROWS + r * AT_D + 4 * lane;
+  constexpr int AHEAD = 6;
+  float M = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
   for (int c = 0; c < np; c += 64) {
     const int n = min(np - c, 64);
     const float* piece = base + (size_t)(c + min(lane, n - 1)) * AT_PART;
     float m = piece[r], ls = piece[AT_ROWS + r];
-    float v[AHEAD];
+    float4 v[AHEAD];
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s) v[s] = col[(size_t)(c + min(s, n - 1)) * AT_PART];
+    for (int s = 0; s < AHEAD; ++s)
+      v[s] = *reinterpret_cast<const float4*>(col + (size_t)(c + min(s, n - 1)) * AT_PART);
     if (lane >= n) {
       m = -INFINITY;
       ls = 0.f;
@@ -571,21 +573,25 @@ __global__ __launch_bounds__(AT_D) void attn_paged_combine_kernel(PagedArgs p) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o, 64);
     l = l * shrink + ls;
-    acc *= shrink;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= shrink;
     M = mn;
     for (int s = 0; s < n; s += AHEAD) {
 #pragma unroll
-      for (int e = 0; e < AHEAD; ++e)
-        if (s + e < n) acc += v[e] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), s + e));
+      for (int e = 0; e < AHEAD; ++e) {
+        if (s + e < n) {
+          const float x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), s + e));
+          acc[0] += x * v[e].x; acc[1] += x * v[e].y; acc[2] += x * v[e].z; acc[3] += x * v[e].w;
+        }
+      }
       if (s + AHEAD < n) {
 #pragma unroll
-        for (int e = 0; e < AHEAD; ++e) v[e] = col[(size_t)(c + min(s + AHEAD + e, n - 1)) * AT_PART];
+        for (int e = 0; e < AHEAD; ++e)
+          v[e] = *reinterpret_cast<const float4*>(col + (size_t)(c + min(s + AHEAD + e, n - 1)) * AT_PART);
       }
     }
   }
-  float val = l == 0.f ? 0.f : acc / l;   // no key seen: zeros
-  if (a.gate) val *= sigmoidf_(gl);
-  a.out[(bt * a.Hq + h) * AT_D + tid] = f32_to_bf16(val);
+  at_store4(a.out + (bt * a.Hq + h) * AT_D + 4 * lane, acc, l == 0.f ? 0.f : 1.f / l, a.gate != nullptr, gv);
 }
 
 }  // namespace lollm
@@ -657,6 +663,6 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   else
     hipLaunchKernelGGL(attn_paged_kernel<false>, dim3(nw), dim3(AW_THREADS), 0, st, p);
   if ((rc = launch_status())) return rc;
-  hipLaunchKernelGGL(attn_paged_combine_kernel, dim3(n_rep * QB, (unsigned)pairs), dim3(AT_D), 0, st, p);
+  hipLaunchKernelGGL(attn_paged_combine_kernel, dim3((n_rep * QB + 3) / 4, (unsigned)pairs), dim3(256), 0, st, p);
   return launch_status();
 }

@@ -689,16 +689,7 @@ __global__ __launch_bounds__(256) void attn_parts_combine_kernel(ApArgs a) {
         v[e] = *reinterpret_cast<const float4*>(col + (size_t)min(s + 4 + e, n - 1) * AP_PIECE);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;   // no key seen: zeros
-  float y[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    y[e] = acc[e] * inv;
-    if (a.gate) y[e] *= sigmoidf_(__uint_as_float(e & 1 ? (e < 2 ? gv.x : gv.y) & 0xffff0000u : (e < 2 ? gv.x : gv.y) << 16));
-  }
-  const bf16x2 lo = {(__bf16)y[0], (__bf16)y[1]}, hi = {(__bf16)y[2], (__bf16)y[3]};
-  *reinterpret_cast<uint2*>(a.out + (bt * a.Hq + head) * AT_D + 4 * lane) =
-      make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+  at_store4(a.out + (bt * a.Hq + head) * AT_D + 4 * lane, acc, l == 0.f ? 0.f : 1.f / l, a.gate != nullptr, gv);
 }
 
 int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus) {
