@@ -27,7 +27,9 @@ def attention(q, k_pages, v_pages, table, kv_len, gate, k_scale=None, v_scale=No
     weighted mean of |v| half a step of the weights' type (bf16 pages: hi + lo, 16 bits, 2^-15 for
     the weight and the sum; 8-bit pages: fp16, 2^-11) and the fp32 scores (258 roundings of 2^-24 on
     the absolute products, doubled for the sum); and for fp16 weights, whose step ends at 2^-24, half
-    of that (2^-25) on the sum of |v| beside a largest weight of 1 or more."""
+    of that (2^-25) on the sum of |v| beside a largest weight of 1 or more.  8-bit values enter as fp16 in
+    units of at most the largest scale among the sequence's pages: half of fp16's least step in these
+    units, 2^-25 of that scale, on each value, so on their mean."""
     weight = 2.0 ** -14 if k_scale is None else 2.0 ** -11
     B, T, Hq, _ = q.shape
     n, Hkv, P, _ = k_pages.shape
@@ -53,6 +55,7 @@ def attention(q, k_pages, v_pages, table, kv_len, gate, k_scale=None, v_scale=No
             tol[b, :, h] = (weight + 2 * ds) * (p @ vb.abs())
             if k_scale is not None:
                 tol[b, :, h] += 2.0 ** -25 * p.amax(-1, keepdim=True) * ((~hidden).double() @ vb.abs())
+                tol[b, :, h] += 2.0 ** -25 * float(v_scale[page, h // (Hq // Hkv)].max()) * (~hidden).any(-1, keepdim=True)
     if gate is not None:
         g = torch.sigmoid(gate.double().reshape(B, T, Hq, D))
         out, tol = out * g, tol * g

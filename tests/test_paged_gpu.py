@@ -154,6 +154,45 @@ def test_attention_scale_and_large_values(bits):
     check_attention((q, k, v, table, lens, qkv, ks, vs), 8, scale=0.11)
 
 
+@pytest.mark.parametrize("T", [2, 72])
+@pytest.mark.parametrize("P", [16, 64])
+@pytest.mark.parametrize("spread", [4, 12, 40])
+def test_attention_scales_far_apart(spread, P, T):
+    """Pages whose values lie up to 2^(2 spread) apart, in both directions along a sequence."""
+    print(f"case spread {spread} page {P} T {T}", flush=True)
+    q, k, v, table, lens, qkv, ks, vs = attend_case(20 + spread, 3, T, 8, 2, [1030, 300, 75], P, 8)
+    vs = vs * torch.exp2(torch.randint(-spread, spread + 1, vs.shape, generator=gen(spread)).float())
+    check_attention((q, k, v, table, lens, qkv, ks, vs), 8)
+
+
+@pytest.mark.parametrize("T", [15, 72])
+def test_attention_far_scale_of_a_later_page(T):
+    """The last page's values are 2^20 of the others': rows before it see none of that but the
+    units of its scale."""
+    q, k, v, table, lens, qkv, ks, vs = attend_case(31, 2, T, 8, 2, [1030, 75], 16, 8)
+    for b, L in enumerate(lens.tolist()):
+        vs[table[b, (L - 1) // 16]] *= 2.0 ** 20
+    check_attention((q, k, v, table, lens, qkv, ks, vs), 8)
+
+
+@pytest.mark.parametrize("T", [1, 80])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_light_weights_add_up(bits, T):
+    """One key of value 0 outweighs each of the others by 2^16 or more: what they add up to counts."""
+    print(f"case light T {T} bits {bits}", flush=True)
+    q, k, v, table, lens, qkv, ks, vs = attend_case(30, 1, T, 8, 2, [2000], 64, bits)
+    q = torch.zeros_like(q)
+    q[..., 0] = 16.0                                  # the scores: k's first column
+    k, v = torch.zeros_like(k.float()), torch.ones_like(v.float())
+    first = int(table[0, 0])
+    k[first, :, 3, 0] = 11.5                          # e^11.5 = 2^16.6
+    v[first, :, 3] = 0.0
+    k, v = (x.to(torch.bfloat16 if bits == 16 else torch.float8_e4m3fn) for x in (k, v))
+    if bits == 8:
+        ks, vs = torch.ones_like(ks), torch.ones_like(vs)
+    check_attention((q, k, v, table, lens, qkv, ks, vs), 8)
+
+
 def test_attention_gate_forms_and_strided_table():
     from lollm_amd import ops
     q, k, v, table, lens, qkv, ks, vs = cuda(*attend_case(4, 3, 2, 8, 2, [40, 1, 333], 16, 8))
