@@ -97,16 +97,19 @@ int lollm_attn_verify(const void* q, const void* k_cache, const void* v_cache,
 /* The same attention over a paged cache.  Key j of sequence b is row j % page of page
  * table[b * table_stride + j / page]; an entry < 0 or >= n_pages is unmapped and its keys do
  * not exist (a query that sees no key gets zeros).  Nothing of a row past kv_len or in an
- * unmapped page is used, whatever it holds.  No reference counterpart (kv.py:20-58 holds one
+ * unmapped page is used, whatever it holds; of the T new keys, those after a query enter its sum
+ * with weight 0, so their values have to be finite.  No reference counterpart (kv.py:20-58 holds one
  * contiguous tensor per layer).
  *
  *   k_pages, v_pages  (n_pages, Hkv, page, D), kv_dtype LOLLM_BF16 or LOLLM_F8: e4m3 codes,
  *            their value the code times the page's scale
- *   k_scale, v_scale  (n_pages, Hkv) fp32 powers of two (8-bit pages; else NULL)
+ *   k_scale, v_scale  (n_pages, Hkv) fp32 powers of two (8-bit pages; else NULL).  Beside the
+ *            output's rounding a result is off by up to 2^-11 of the weighted mean of |V|, and by
+ *            2^-25 of the largest V scale among the sequence's pages
  *   table    (B, table_width) int32, rows table_stride apart; it holds table_width * page keys
  *   gate     element d of (token bt, head h) at gate + bt * gate_row + h * gate_head + d (so it
  *            can be read where the fused projection wrote it), or NULL
- *   kv_len, q, out, scale  as lollm_attn_verify
+ *   kv_len, q, out, scale  as lollm_attn_verify; scale positive
  *   grid     as lollm_attn_verify; with 0, calls of more than 64 tokens in all and 16 or more a
  *            sequence run on query tiles of one KV head, the keys of few tiles divided between
  *            workgroups (few tiles of 8-bit pages keep the split-K)
@@ -263,7 +266,7 @@ int lollm_attn_prologue(const void* qkv, const void* q_norm_w, const void* k_nor
  * one that it has while it keeps rows (the call's first row is not the page's first); kept rows
  * are rounded to a larger scale again, which changes subnormal codes only.  Values that are not
  * finite become NaN.  k_scale and v_scale are read and written.
- * A page written by a call may be in one sequence's table only.  inv_freq, rope_pos and
+ * A page that a call writes may be named by one entry of the table only.  inv_freq, rope_pos and
  * rope_per_token as in lollm_attn_prologue.  Supported: D == 256, page 16, 32, 64 or 128. */
 int lollm_attn_append(const void* qkv, const void* q_norm_w, const void* k_norm_w, const float* inv_freq,
                       const int32_t* lengths, const int32_t* rope_pos, int rope_per_token,

@@ -324,6 +324,7 @@ LOLLM_API int lollm_attn_append(const void* qkv, const void* q_norm_w, const voi
   if (rope_per_token && !rope_pos) return LOLLM_EINVAL;
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0) return LOLLM_EINVAL;
   if (table_width <= 0 || n_pages <= 0 || table_stride < table_width) return LOLLM_EINVAL;
+  if (Hq > 32 * 65535 || Hkv > 65535) return LOLLM_EUNSUPPORTED;   // (32-bit offsets in a token)
   if (D != AT_D || rotary_dim < 0 || rotary_dim > D || rotary_dim % 2) return LOLLM_EUNSUPPORTED;
   if (rotary_dim > 0 && !inv_freq) return LOLLM_EINVAL;
   if (kv_dtype != LOLLM_BF16 && kv_dtype != LOLLM_F8) return LOLLM_EUNSUPPORTED;

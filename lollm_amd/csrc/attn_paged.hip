@@ -633,6 +633,7 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   int rc = attn_geometry(B, T, Hq, Hkv, D, (int)rows, &n_rep, &QB, &qblocks);
   if (rc) return rc;
   if (Hkv > 65535) return LOLLM_EUNSUPPORTED;        // 32-bit offsets in a query block's tokens
+  if (!(scale > 0.f) || !(scale < INFINITY)) return LOLLM_EINVAL;   // the maxima are of unscaled scores
   if (grid < 0 || grid > 1024) return LOLLM_EINVAL;  // pieces per pair <= combine table
   if (gate && (gate_head < D || gate_row < (Hq - 1LL) * gate_head + D)) return LOLLM_EINVAL;
   if (gate && (gate_row % 8 || gate_head % 8)) return LOLLM_EINVAL;

@@ -295,6 +295,8 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
     def release(self, b: int):
         """Give back the pages of a finished sequence: it holds no keys from now on, takes no more
         pages, and its rows of later calls mean nothing."""
+        if capturing():
+            raise RuntimeError("release() under capture")
         self.free += self._host_table[b, :self.held[b]].tolist()
         self._host_table[b] = -1
         self.held[b], self.live[b] = 0, False
@@ -303,6 +305,8 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
 
     # -- the reference cache API -------------------------------------------------------
     def _rows(self, L):
+        if not all(self.live):
+            raise RuntimeError("a released sequence has no rows")
         at = torch.arange(L, device=self.device)
         return self.table[:, at // self.page].long(), at % self.page
 

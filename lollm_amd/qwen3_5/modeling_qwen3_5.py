@@ -86,8 +86,9 @@ class Qwen3_5Model:
         n_pages (of the pool) given, keys and values in pages (Qwen3_5PagedCache)."""
         if page is None and kv_dtype is None and n_pages is None:
             return Qwen3_5Cache(self.cfg, batch, max_len, spec_slots, self.device)
-        return Qwen3_5PagedCache(self.cfg, batch, max_len, spec_slots, self.device, page or 64,
-                                 kv_dtype or torch.bfloat16, n_pages)
+        return Qwen3_5PagedCache(self.cfg, batch, max_len, spec_slots, self.device,
+                                 64 if page is None else page,
+                                 torch.bfloat16 if kv_dtype is None else kv_dtype, n_pages)
 
     def attn_workspace(self, B, T, max_len, keep=True):
         """Split-K partials buffer of the attention layers (shared by all layers of a

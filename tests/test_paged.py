@@ -35,6 +35,7 @@ def append(**kw):
     (dict(B=0), 1), (dict(T=0), 1), (dict(Hq=7), 1), (dict(D=128), 2), (dict(B=513), 2), (dict(Hq=66), 2),
     (dict(grid=-1), 1), (dict(grid=1025), 1), (dict(gate=P, gr=100, gh=256), 1), (dict(gate=P, gr=2048, gh=128), 1),
     (dict(gate=P, gr=2049, gh=256), 1), (dict(T=2 ** 20), 2), (dict(wsb=10 ** 9), 1), (dict(ws=P, wsb=100), 1),
+    (dict(scale=0.0), 1), (dict(scale=-1.0), 1), (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1),
 ])
 def test_attn_paged_refuses(kw, rc):
     assert attn(**kw) == rc
@@ -46,6 +47,7 @@ def test_attn_paged_refuses(kw, rc):
     (dict(n=0), 1), (dict(page=8), 2), (dict(page=256), 2), (dict(dt=1), 2), (dict(dt=2), 1), (dict(dt=2, ks=P), 1),
     (dict(B=0), 1), (dict(T=0), 1), (dict(Hq=0), 1), (dict(Hkv=0), 1), (dict(D=128), 2), (dict(rd=63), 2),
     (dict(rd=258), 2), (dict(rd=-2), 2), (dict(ts=2 ** 28, tw=2 ** 28), 2), (dict(B=2 ** 16, T=2 ** 16), 2),
+    (dict(Hkv=65536), 2), (dict(Hq=2 ** 22), 2),
 ])
 def test_attn_append_refuses(kw, rc):
     assert append(**kw) == rc
@@ -136,3 +138,30 @@ def test_cache_refusals():
     with pytest.raises(RuntimeError, match="attn_append"):
         c.append_kv(3, x, x)
     assert set(c.layers[3]) == {"k", "v", "ks", "vs"} and set(c.layers[0]) == {"win", "rec", "rep"}
+
+
+def test_cache_refuses_rows_of_a_released_sequence():
+    c = cache(batch=1, page=16)
+    x = torch.zeros(1, 2, 5, 256, dtype=torch.bfloat16)
+    c.append_kv(3, x, x)
+    c.release(0)
+    c.release(0)                                     # again: nothing to give back
+    assert len(c.free) == 7
+    for call in (lambda: c.append_kv(3, x, x), lambda: c.read_kv(3)):
+        with pytest.raises(RuntimeError, match="released"):
+            call()
+
+
+def test_new_cache_takes_what_it_is_given():
+    from lollm_amd.qwen3_5 import Qwen3_5Cache, Qwen3_5Model
+
+    class Model:
+        cfg, device = Qwen3_5Config.from_hf(micro_config_dict()), torch.device("cpu")
+        new_cache = Qwen3_5Model.new_cache
+
+    assert type(Model().new_cache(1, 50)) is Qwen3_5Cache
+    c = Model().new_cache(1, 50, kv_dtype=torch.float8_e4m3fn)
+    assert (c.page, c.kv_dtype, c.n_pages) == (64, torch.float8_e4m3fn, 1)
+    assert Model().new_cache(1, 50, n_pages=3).kv_dtype == torch.bfloat16
+    with pytest.raises(ValueError):
+        Model().new_cache(1, 50, page=0)

@@ -208,6 +208,53 @@ def test_attention_gate_forms_and_strided_table():
     torch.testing.assert_close(want.float(), plain * torch.sigmoid(dense.float().view(3, 2, -1)), rtol=2 ** -6, atol=1e-6)
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("T", [2, 70])
+def test_attention_shared_pages(T, bits):
+    """Two sequences over the pages of a common prompt, and a page named twice in one table."""
+    print(f"case shared T {T} bits {bits}", flush=True)
+    q, k, v, table, lens, qkv, ks, vs = attend_case(32, 3, T, 8, 2, [500, 333, 200], 32, bits)
+    table[1, :6] = table[0, :6]
+    table[2, 2] = table[2, 0]
+    check_attention((q, k, v, table, lens, qkv, ks, vs), 8)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_largest_batch(bits):
+    print(f"case 512 sequences bits {bits}", flush=True)
+    lens = [(37 * b) % 150 for b in range(512)]
+    check_attention(attend_case(33, 512, 1, 4, 2, lens, 16, bits), 4)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_pools_past_4_gb(bits):
+    """Pages whose bytes begin past 2^32, where neither 32 bits of bytes nor 31 of values reach."""
+    from lollm_amd import ops
+    print(f"case large pool bits {bits}", flush=True)
+    Hkv, P = 2, 128
+    n = (2 ** 32 + 2 ** 28) // (Hkv * P * D * bits // 8)
+    for T in (3, 80):
+        q, k, v, table, lens, qkv, ks, vs = cuda(*attend_case(34, 2, T, 8, Hkv, [700, 333], P, bits))
+        want = ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs)
+        m = k.shape[0]
+        far = torch.where(table >= 0, table + (n - m), table)
+
+        def grown(x):
+            y = torch.empty((n, *x.shape[1:]), dtype=x.dtype, device="cuda")
+            y[n - m:].view(torch.uint8).copy_(x.view(torch.uint8))
+            return y
+
+        big = [None if x is None else grown(x) for x in (k, v, ks, vs)]
+        assert torch.equal(ops.attn_paged(q, big[0], big[1], far, lens, gates(qkv, 8), k_scale=big[2], v_scale=big[3]), want)
+        w, inv = torch.zeros(D, dtype=torch.bfloat16, device="cuda"), torch.ones(32, device="cuda")
+        for pools, tb in (((k, v, ks, vs), table), (big, far)):
+            ops.attn_append(qkv, w, w, inv, lens - T, tb, pools[0], pools[1], 8, 64, EPS, k_scale=pools[2], v_scale=pools[3])
+        torch.cuda.synchronize()
+        for x, y in zip((k, v, ks, vs), big):
+            assert x is None or torch.equal(x.view(torch.uint8), y[n - m:].view(torch.uint8))
+        del big
+
+
 def test_attention_repeats_bit_for_bit():
     from lollm_amd import ops
     q, k, v, table, lens, qkv, ks, vs = cuda(*attend_case(5, 4, 4, 16, 2, [900, 40, 2000, 333], 64, 8))
@@ -410,6 +457,55 @@ def test_other_stream_and_caller_workspace():
         got = ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs, workspace=ws)
     st.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T", [2, 72])
+def test_two_streams_at_once(T):
+    from lollm_amd import ops
+    cases = [cuda(*attend_case(40 + i, 3, T, 8, 2, [900, 77, 300 + i], 32, 8)) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def call(c):
+        q, k, v, table, lens, qkv, ks, vs = c
+        return ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs)
+
+    want = [call(c) for c in cases]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(call(cases[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])
+
+
+@pytest.mark.parametrize("T", [2, 72])
+def test_two_graphs_share_a_workspace(T):
+    """Replayed in turn on one stream, over lengths that move between the replays."""
+    from lollm_amd import ops
+    cases = [cuda(*attend_case(50 + i, 3, T, 8, 2, [900, 80, 300 + i], 32, 8)) for i in range(2)]
+    ws = torch.empty(ops.attn_paged_workspace_bytes(3, T, 8, 2, D, cases[0][1].dtype), dtype=torch.uint8, device="cuda")
+
+    def call(c, workspace):
+        q, k, v, table, lens, qkv, ks, vs = c
+        return ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs, workspace=workspace)
+
+    graphs, outs = [], []
+    for c in cases:
+        call(c, None)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(c, ws))
+        graphs.append(g)
+    for i in range(5):
+        for c in cases:
+            c[4].sub_(i)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for c, out in zip(cases, outs):
+            assert torch.equal(out, call(c, None))
 
 
 def test_refusals():
