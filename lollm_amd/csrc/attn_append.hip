@@ -22,8 +22,11 @@
 // loads.  An 8-bit page's rows stay in registers as they came and are formed twice, for their
 // maximum and for their rounding (in fp32 they would take the registers of two waves in three).
 // Query heads: a workgroup per token and as many heads as its half-waves take at once where
-// tokens are few, up to 32 heads otherwise.  Bound by memory for prompts, by the launch for few
-// tokens.
+// tokens are few, up to 32 heads otherwise.
+//
+// What bounds it: memory for prompts (32 / 4 heads, us and TB/s: 3 x 1500 tokens into bf16 pages 31,
+// 5.9; 2 x 1999 28, 5.8; into 8-bit pages of 16 / 64 / 128 rows 31 / 33 / 37, 5.1 / 4.8 / 4.2, as the
+// rows that a workgroup holds take its registers), the launch for few tokens (4 to 5 us at 1 to 64).
 #include "attn_common.h"
 
 namespace lollm {

@@ -10,18 +10,26 @@
 // Work decomposition: attn_verify.hip's balanced split-K (128-key blocks of all (sequence, KV
 // head x query block) pairs dealt out evenly, one partial per workgroup and pair, the combine
 // kernel).  What differs is how a wave finds its rows.  Each of the four waves owns 32
-// consecutive keys of a block, which lie in one page, or in two pages of 16.  Every 62 blocks
+// consecutive keys of a block, which lie in one page, or in two pages of 16.  Every 64 blocks
 // each lane looks up one block of the range ahead -- its sequence and pair by binary search, its
 // page ids, its scales -- and the loop takes them with readlane two blocks before it needs them,
 // so no load of a page waits for a load of the table.
 //   K: 16 bytes a lane straight into the S MFMA A operand (64-bit addresses: a pool may pass
-//      4 GB).  Rows of unmapped pages read page 0 and are masked.
+//      4 GB).  Without a page it is masked, and the lanes read the pool's first line.
 //   V: LDS DMA through a descriptor of the page's valid rows; the others become zeros, so that
 //      nothing that an unmapped or unwritten row holds meets a weight of 0.
 //   8 bits: a lane's 16 bytes of K are two k-steps (Q's columns are read in the same order) and
 //      become bf16 with v_cvt_scalef32_pk_bf16_fp8, which applies the scale; V is read with the
 //      transposing 8-bit LDS read and becomes fp16 (at_f16).
 // Weights enter the product with V as hi + lo bf16 (attn_prefill.hip), with 8-bit V as fp16.
+//
+// What bounds it: the KV stream from some ten blocks a workgroup on, a fixed 13 us before.  16 x 4
+// tokens, 32 / 4 heads (us, TB/s of K and V): 128 keys 17.0 (8 bits 15.2), 1024 25.9, 2.6 (21.1,
+// 1.6), 4096 53, 5.0 (35, 3.8), 16384 182, 5.9 (93, 5.7), 65536 665, 6.5 (354, 6.1); pages of 16 to
+// 128 rows alike.  Of the fixed part the two launches are 5, the table and the scales' round trips
+// before the first load 2, the last block's products and the merge of the waves 4.  8-bit blocks
+// are half the bytes: K is asked for two blocks ahead, of bf16 one, as a wave has at most 63 loads on
+// its way.
 #include <type_traits>
 
 #include "attn_common.h"

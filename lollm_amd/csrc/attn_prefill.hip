@@ -3,7 +3,8 @@
 // Same math and operands as attn_verify.hip (src/qwen3_5/blocks.py:226-235 +
 // src/attention.py:43-51: offset-causal GQA over the cache, output o * sigmoid(gate)),
 // for calls whose query rows alone fill the chip, where splitting keys between workgroups
-// (and the fp32 pieces and the second launch that go with it) buys nothing.
+// (and the fp32 pieces and the second launch that go with it) buys nothing; and for long calls
+// over pages at any number of tiles.
 //
 // Tile.  A workgroup owns 128 RG query rows of one (sequence, KV head): the n_rep query
 // heads x QB consecutive positions, packed position-major (row r = position r / n_rep,
@@ -30,6 +31,16 @@
 // Measured (us, causal, T = kv length, split-K kernels / RG = 1 / RG = 2): 2 x 1999,
 // 32 q / 4 kv heads 1020 / 247 / 222 (591 TFLOP/s); 1 x 4096 1822 / 407 / 372 (740 TFLOP/s);
 // 3 x 1500 1110 / 216 / 217; 32 x 128 over 1128 keys 903 / 260 / 244.
+//
+// Pages (attn_paged.hip).  A block's rows lie in one page, or two of 16 rows; a wave's eight in one,
+// which a descriptor of their own covers.  Page ids and scales are the same for every lane and come
+// through the scalar cache, a block ahead of the loads that need them.  8 bits: K becomes bf16 and V
+// fp16 as they are read, once for every 32 rows, and weights are fp16, one product in the place of
+// two.  2 x 1999 tokens: bf16 pages 240 us, 8 bits 197 (with RG = 2 a block
+// has 680 VALU instructions beside its 64 products, which take 2048 of its 7150 cycles); slabs 221.
+// Where tiles are fewer than CUs (RG = 1 over pages), a tile's keys are dealt out to `parts`
+// workgroups, whose pieces a second kernel merges: 512 tokens over 8289 keys, 128 tiles, 423 us
+// on the split-K kernel, 237 in two parts (a slab's tiles, undivided, 368).
 //
 // Rows of K and V are 512 bytes in LDS with no padding (the DMA writes 1 KB runs); the
 // 16-byte chunk c of row r sits at c ^ (r & 15) for K and c ^ (2 (r & 7)) for V, so the

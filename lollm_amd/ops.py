@@ -270,7 +270,9 @@ def attn_append(qkv, q_norm_w, k_norm_w, inv_freq, lengths, table, k_pages, v_pa
         pos = _arg(rope_pos, "rope_pos", torch.int32, (B, T) if per_token else (B,), dev)
     if q_out is None:
         q_out = qkv.new_empty((B, T, Hq, D))
-    q = _arg(q_out, "q_out", torch.bfloat16, (B, T, Hq, D), dev)
+        q = q_out.data_ptr()
+    else:
+        q = _arg(q_out, "q_out", torch.bfloat16, (B, T, Hq, D), dev)
     rc = _lib.lib().lollm_attn_append(
         x, qw, kw, freq, ln, pos, per_token, tab, stride, cols, n, page, code, B, T, Hq, Hkv, D, rotary_dim,
         eps, q, kp, vp, ks, vs, torch._C._cuda_getCurrentRawStream(dev))
@@ -333,14 +335,18 @@ def attn_paged(q, k_pages, v_pages, table, kv_len, gate=None, *, k_scale=None, v
     g, row, head = _gate_arg(gate, B, T, Hq, D, dev) if gate is not None else (None, 0, 0)
     if out is None:
         out = q.new_empty((B, T, Hq * D))
-    o = _arg(out, "out", torch.bfloat16, (B, T, Hq * D), dev)
+        o = out.data_ptr()
+    else:
+        o = _arg(out, "out", torch.bfloat16, (B, T, Hq * D), dev)
     if workspace is None:
-        workspace = torch.empty(attn_paged_workspace_bytes(B, T, Hq, Hkv, D, k_pages.dtype, grid), dtype=torch.uint8,
-                                device=q.device)
-    ws = _arg(workspace, "workspace", workspace.dtype, workspace.shape, dev)
+        wbytes = attn_paged_workspace_bytes(B, T, Hq, Hkv, D, k_pages.dtype, grid)
+        workspace = q.new_empty(wbytes, dtype=torch.uint8)
+        ws = workspace.data_ptr()
+    else:
+        wbytes = workspace.numel() * workspace.element_size()
+        ws = _arg(workspace, "workspace", workspace.dtype, workspace.shape, dev)
     rc = _lib.lib().lollm_attn_paged(
-        x, kp, vp, ks, vs, code, tab, stride, cols, n, page, ln, g, row, head, o, ws,
-        workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, D, grid,
+        x, kp, vp, ks, vs, code, tab, stride, cols, n, page, ln, g, row, head, o, ws, wbytes, B, T, Hq, Hkv, D, grid,
         D ** -0.5 if scale is None else scale, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, "lollm_attn_paged")
