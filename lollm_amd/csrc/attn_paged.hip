@@ -291,14 +291,13 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 
   for (uint32_t ub = u0; ub < u1; ub += 2) {
 #pragma unroll
-    for (int set = 0; set < 2; ++set) {
+    for (int set = 0; set < 2; ++set) {   // (left from the inside after the last block)
       unsigned char* vset = set ? vs1 : vs0;
       const uint32_t u = ub + set;
-      const bool live = u < u1;
-      const bool any = live && (C.page[0] & C.page[1]) != -1;   // keys of this wave to look at
+      const bool any = (C.page[0] & C.page[1]) != -1;   // keys of this wave to look at
       const int nb = nblk_of(C.L);
-      const bool seg_first = live && ((u == u0) || (C.j == 0));
-      const bool seg_last = live && ((u == u1 - 1) || (C.j == nb - 1));
+      const bool seg_first = u == u0 || C.j == 0;
+      const bool seg_last = u == u1 - 1 || C.j == nb - 1;
       if (seg_first) {
         const int q0 = (C.ph % a.qblocks) * a.QB;
         qpos = C.L - a.T + q0 + lq;
@@ -522,6 +521,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
           turn(std::integral_constant<int, AT_D / 2>{}, std::integral_constant<int, AT_D / 2>{});
         }
       }
+      if (u + 1 >= u1) break;   // the last block: nothing is to come
       // V of block u + 2 into this set
       issue_v(vset, X2);
       C = X1;
