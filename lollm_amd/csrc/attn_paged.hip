@@ -112,7 +112,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   // All pairs' blocks, dealt out in equal ranges, the first `more` of them one block longer (the
   // host keeps U below 2^31); one block a workgroup where there are fewer blocks, so that no
   // workgroup between a pair's has none.
-  const uint32_t U = (uint32_t)PH * (uint32_t)build_prefix(a, pre, len, tmp);
+  const uint32_t U = (uint32_t)PH * (uint32_t)__builtin_amdgcn_readfirstlane(build_prefix(a, pre, len, tmp));
   const uint32_t nw = min((uint32_t)a.nw, U), each = U / max(nw, 1u), more = U - each * nw;
   auto owner = [&](uint32_t u) {
     const uint32_t cut = more * (each + 1);
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
 
   for (uint32_t ub = u0; ub < u1; ub += 2) {
 #pragma unroll
-    for (int set = 0; set < 2; ++set) {   // (left from the inside after the last block)
+    for (int set = 0; set < 2; ++set) {   // (ended from the inside)
       unsigned char* vset = set ? vs1 : vs0;
       const uint32_t u = ub + set;
       const bool any = (C.page[0] & C.page[1]) != -1;   // keys of this wave to look at
@@ -521,7 +521,9 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
           turn(std::integral_constant<int, AT_D / 2>{}, std::integral_constant<int, AT_D / 2>{});
         }
       }
-      if (u + 1 >= u1) break;   // the last block: nothing is to come
+      // The last block: nothing is to come.  (By hand: as a branch of the compiler's this is an edge
+      // over which no V follows K, and its waits for K in the next block then wait for all.)
+      asm volatile("s_cmp_lt_u32 %0, %1\n\ts_cbranch_scc1 1f\n\ts_endpgm\n1:" ::"s"(u + 1), "s"(u1) : "scc", "memory");
       // V of block u + 2 into this set
       issue_v(vset, X2);
       C = X1;
