@@ -58,7 +58,6 @@ constexpr int AP_AHEAD = 3;                    // operands read ahead of their p
 constexpr int AP_PART_BLOCKS = 8;              // blocks of a part of a tile's keys at least
 constexpr int AP_MAX_PARTS = 64;
 constexpr int AP_PIECE = 2 * 128 + 128 * AT_D; // floats: maxima, sums and O of a part of a 128-row tile
-constexpr int AP_DUMP = 32 * AT_D * 2;         // 16 KB: half of a wave's O on its way out
 
 // Where the keys are: AP_ROWS one slab per (sequence, KV head); AP_PAGES, AP_PAGES8 pages that a
 // table names (attn_paged.hip), in bf16 or as e4m3 codes with scales.
@@ -106,14 +105,13 @@ __device__ __forceinline__ T ap_sload(const T* p, long long i) {
 }
 
 template <int RG, int KV>
-__global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a) {
+__global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) void attn_prefill_kernel(ApArgs a) {
   constexpr bool F8 = KV == AP_PAGES8;
   constexpr int ROW = F8 ? AT_D : AT_D * 2;      // bytes of a key's row
   constexpr int AP_SET = AP_KEYS * ROW;          // K or V rows of a block
   // separate arrays, so that the reads of one set are not ordered after the DMA into another
   __shared__ __attribute__((aligned(16))) unsigned char ks0[AP_SET], ks1[AP_SET], ks2[AP_SET];
   __shared__ __attribute__((aligned(16))) unsigned char vs0[AP_SET], vs1[AP_SET], vs2[AP_SET];
-  __shared__ __attribute__((aligned(16))) unsigned char dumps[F8 ? AP_WAVES * AP_DUMP : 16];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -569,10 +567,11 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
   AP_BARRIER(0);   // no load in flight, every wave done with the sets: the dumps take them
 #undef AP_BARRIER
 
-  // Epilogue in two halves of the columns: O / l through the wave's own 16 KB (fp32, chunk c
-  // of row r at c ^ (r & 15)), then whole half rows with the gate: 8 columns per lane,
-  // 16-byte loads and stores.
-  unsigned char* dump = F8 ? dumps + AP_DUMP * wave : wave == 0 ? ks0 : (wave == 1 ? ks1 : (wave == 2 ? ks2 : vs0));
+  // Epilogue in two or four parts of the columns: O / l through a set as the wave's own (fp32, chunk
+  // c of row r at c ^ (r & 15)), then runs of whole rows with the gate: 8 columns per lane, 16-byte
+  // loads and stores.
+  constexpr int COLS = AP_SET / 128, LPR = COLS / 8, RPI = 64 / LPR;   // lanes of a row, rows at a time
+  unsigned char* dump = wave == 0 ? ks0 : (wave == 1 ? ks1 : (wave == 2 ? ks2 : vs0));
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_s[rg]), __float_as_uint(l_s[rg]), false, false);
@@ -594,43 +593,43 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
         reinterpret_cast<int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[qt * pairs + pair] = parts;
     }
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      // this lane's 8 half rows 4 it + lane / 16, columns 8 (lane % 16) ..; gates first
-      const int c8 = lane & 15;
-      u32x4_t g[8];
-      size_t oo[8];
-      bool live[8];
+    for (int cp = 0; cp < AT_D / COLS; ++cp) {
+      // this lane's rows RPI it + lane / LPR, columns 8 (lane % LPR) ..; gates first
+      const int c8 = lane & (LPR - 1);
+      u32x4_t g[32 / RPI];
+      size_t oo[32 / RPI];
+      bool live[32 / RPI];
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int r = 32 * (RG * wave + rg) + 4 * it + (lane >> 4), qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
+      for (int it = 0; it < 32 / RPI; ++it) {
+        const int r = 32 * (RG * wave + rg) + RPI * it + lane / LPR, qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
         live[it] = qi < QB;
-        oo[it] = (((size_t)b * a.T + q0 + (live[it] ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D + 128 * half + 8 * c8;
+        oo[it] = (((size_t)b * a.T + q0 + (live[it] ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D + COLS * cp + 8 * c8;
         if (a.gate && whole)
           g[it] = *reinterpret_cast<const u32x4_t*>(a.gate + ((size_t)b * a.T + q0 + (live[it] ? qi : 0)) * a.gate_row +
-                                                    (size_t)(kvh * a.n_rep + hr) * a.gate_head + 128 * half + 8 * c8);
+                                                    (size_t)(kvh * a.n_rep + hr) * a.gate_head + COLS * cp + 8 * c8);
       }
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
+      for (int dt = 0; dt < COLS / 32; ++dt)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int c = (8 * dt + 2 * q + h) ^ (l32 & 15);
-          const f32x16& o = O[rg][4 * half + dt];
-          *reinterpret_cast<float4*>(dump + l32 * 512 + 16 * c) =
+          const f32x16& o = O[rg][COLS / 32 * cp + dt];
+          *reinterpret_cast<float4*>(dump + l32 * (COLS * 4) + 16 * c) =
               make_float4(o[4 * q] * inv, o[4 * q + 1] * inv, o[4 * q + 2] * inv, o[4 * q + 3] * inv);
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own dump, read by the wave only
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int rr = 4 * it + (lane >> 4);
+      for (int it = 0; it < 32 / RPI; ++it) {
+        const int rr = RPI * it + lane / LPR;
         float y[8];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float4 f = *reinterpret_cast<const float4*>(dump + rr * 512 + 16 * ((2 * c8 + u) ^ (rr & 15)));
+          const float4 f = *reinterpret_cast<const float4*>(dump + rr * (COLS * 4) + 16 * ((2 * c8 + u) ^ (rr & 15)));
           y[4 * u] = f.x; y[4 * u + 1] = f.y; y[4 * u + 2] = f.z; y[4 * u + 3] = f.w;
         }
         if (!whole) {
           if (live[it]) {
-            float* to = piece + 256 + (32 * wave + rr) * AT_D + 128 * half + 8 * c8;
+            float* to = piece + 256 + (32 * wave + rr) * AT_D + COLS * cp + 8 * c8;
             *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
             *reinterpret_cast<float4*>(to + 4) = make_float4(y[4], y[5], y[6], y[7]);
           }
@@ -651,7 +650,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, 1) void attn_prefill_kernel(ApArgs a
         }
         if (live[it]) *reinterpret_cast<u32x4_t*>(a.out + oo[it]) = w;
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next half's dump
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next dump
     }
   }
 }
@@ -729,7 +728,7 @@ static int prefill_tiles(int B, int T, int Hkv, int n_rep, int rg, int* QB) {
 int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts) {
   *parts = 1;
   const int rg = attn_prefill_groups(B, T, Hkv, n_rep, cus);
-  if (rg == 2 || T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS) return rg;
+  if ((rg == 2 && !f8) || T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS) return rg;
   // Fewer tiles than CUs divide their keys: as many parts as the chip holds at once, or a few more
   // where their rounds come out a tenth shorter (160 tiles: 3 parts take 2 rounds of a third).
   // With that tiles are the faster form at any number of them (us, tiles / split-K, bf16: 20 tiles
@@ -741,12 +740,13 @@ int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* p
   if (f8 && 16 * pairs * T * n_rep < 5LL * cus * 128) return 0;
   int QB;
   const long long tiles = prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * pairs;
-  if (tiles < cus) {
-    int best = cus / (int)tiles;
+  const int slots = f8 ? 2 * cus : cus;   // workgroups that the chip holds
+  if (tiles < slots) {
+    int best = slots / (int)tiles;
     best = best > AP_MAX_PARTS ? AP_MAX_PARTS : best;
     double cost = 0.9 / best;   // (one round)
     for (int n = best + 1; n <= best + 4 && n <= AP_MAX_PARTS; ++n) {
-      const double c = (double)((tiles * n + cus - 1) / cus) / n;
+      const double c = (double)((tiles * n + slots - 1) / slots) / n;
       if (c < cost) {
         cost = c;
         best = n;
