@@ -188,8 +188,8 @@ int attn_grid(int grid);
 int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus);
 int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st, const PagedArgs* paged = nullptr,
                         int parts = 1);
-// The same for pages, and the workgroups that a tile's keys are dealt out to, with the bytes of
-// workspace that takes.
+// For pages: workgroups of 128-row tiles that share a CU, or 0 for the split-K kernels, and the
+// workgroups that a tile's keys are dealt out to, with the bytes of workspace that takes.
 int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts);
 long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts);
 

@@ -35,17 +35,23 @@
 // Pages (attn_paged.hip).  A block's rows lie in one page, or two of 16 rows; a wave's eight in one,
 // which a descriptor of their own covers.  Page ids and scales are the same for every lane and come
 // through the scalar cache, a block ahead of the loads that need them.  8 bits: K becomes bf16 and V
-// fp16 as they are read, once for every 32 rows, and weights are fp16, one product in the place of
-// two.  2 x 1999 tokens: bf16 pages 240 us, 8 bits 197 (with RG = 2 a block
-// has 680 VALU instructions beside its 64 products, which take 2048 of its 7150 cycles); slabs 221.
-// Where tiles are fewer than CUs (RG = 1 over pages), a tile's keys are dealt out to `parts`
-// workgroups, whose pieces a second kernel merges: 512 tokens over 8289 keys, 128 tiles, 423 us
-// on the split-K kernel, 237 in two parts (a slab's tiles, undivided, 368).
+// fp16 as they are read, and weights are fp16, one product in the place of two.  Tiles of 128 rows
+// only, where they can two workgroups a CU: 256 registers a wave, for which bf16 pages leave four of
+// Q's 16 operands in LDS and have two sets of rows (80 KB), and O leaves through the sets.  2 x 1999
+// tokens: bf16 pages 223 us (588 TFLOP/s; one workgroup of 256 rows a CU 240, slabs that way 219), 8
+// bits 183 (717; 197).  1024 tokens over 9024 keys: 383 us (745; 433), 8 bits 317 (902; 412).  What
+// bounds it is the instructions beside the products: 240 of the VALU and 80 of the scalar unit a
+// block and wave of 8-bit pages, half of the former conversions, beside 32 products of 32 cycles.
+// Where tiles are fewer than the chip holds, a tile's keys are dealt out to `parts` workgroups, whose
+// pieces a second kernel merges (512 tokens over 8289 keys, 128 tiles in four parts: 203 us, of
+// which the merge 11; 418 on the split-K kernel).
 //
 // Rows of K and V are 512 bytes in LDS with no padding (the DMA writes 1 KB runs); the
 // 16-byte chunk c of row r sits at c ^ (r & 15) for K and c ^ (2 (r & 7)) for V, so the
 // operand reads (32 rows at one chunk; 8 rows x 4 chunks for the transposing V read) touch
 // every bank equally.
+#include <type_traits>
+
 #include "attn_common.h"
 
 namespace lollm {
@@ -104,14 +110,18 @@ __device__ __forceinline__ T ap_sload(const T* p, long long i) {
   return ((const __attribute__((address_space(4))) T*)p)[i];
 }
 
-template <int RG, int KV>
-__global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) void attn_prefill_kernel(ApArgs a) {
+// SETS: of K and V rows in LDS.  Two for bf16 pages where two workgroups share a CU (K two blocks
+// ahead, V one), else three.
+template <int RG, int KV, int SETS>
+__global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1) void attn_prefill_kernel(ApArgs a) {
   constexpr bool F8 = KV == AP_PAGES8;
   constexpr int ROW = F8 ? AT_D : AT_D * 2;      // bytes of a key's row
   constexpr int AP_SET = AP_KEYS * ROW;          // K or V rows of a block
   // separate arrays, so that the reads of one set are not ordered after the DMA into another
-  __shared__ __attribute__((aligned(16))) unsigned char ks0[AP_SET], ks1[AP_SET], ks2[AP_SET];
-  __shared__ __attribute__((aligned(16))) unsigned char vs0[AP_SET], vs1[AP_SET], vs2[AP_SET];
+  constexpr int AHEAD = SETS == 2 ? 2 : AP_AHEAD;
+  constexpr int THIRD = SETS == 3 ? AP_SET : 16;
+  __shared__ __attribute__((aligned(16))) unsigned char ks0[AP_SET], ks1[AP_SET], ks2[THIRD];
+  __shared__ __attribute__((aligned(16))) unsigned char vs0[AP_SET], vs1[AP_SET], vs2[THIRD];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -119,7 +129,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
   // the longest tiles first (they end last), (sequence, KV head) fastest: with a multiple of
   // 8 pairs, one pair's tiles all run on one XCD and share its L2
   const int pairs = a.B * a.Hkv;
-  constexpr bool PARTS = KV != AP_ROWS && RG == 1;   // a tile's keys may go to a.parts workgroups
+  constexpr bool PARTS = KV != AP_ROWS;   // a tile's keys may go to a.parts workgroups
   const int turn_ = blockIdx.x / pairs, pair = blockIdx.x % pairs;
   const int part = PARTS ? turn_ % a.parts : 0;
   const int qt = a.qtiles - 1 - (PARTS ? turn_ / a.parts : turn_);
@@ -189,11 +199,17 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
   auto issue_page = [&](unsigned char* d, const uint16_t* pool, const Rows& r, uint32_t x, uint32_t swz) {
     asm volatile("" : "+v"(x));
     const __amdgpu_buffer_rsrc_t rs = buf_rsrc((const unsigned char*)pool + r.at, r.bytes);
-    constexpr int N = F8 ? WR / 4 : WR / 2;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(d + ROW * WR * wave + 1024 * i), 16,
-                                               1024u * i + (x ^ (swz * i)) + (F8 ? 0u : (uint32_t)(ROW * h)), 0, 0, 0);
+    // (the instruction's own offset moves both the row's address and its place)
+    auto load = [&](auto at) {
+      constexpr int I = decltype(at)::value;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(d + ROW * WR * wave), 16, x ^ (swz * I), 0, 1024 * I, 0);
+    };
+    load(std::integral_constant<int, 0>{});
+    load(std::integral_constant<int, 1>{});
+    if constexpr (!F8) {
+      load(std::integral_constant<int, 2>{});
+      load(std::integral_constant<int, 3>{});
+    }
   };
   // (row = 8 w + 2 i + h: its swizzle is the lane's part ^ that of 2 i; one register per cache,
   // the rest formed per load -- registers are what this kernel is short of)
@@ -220,12 +236,12 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
   auto load_k = [&](unsigned char* kd, const Rows& r, int j) {
     if constexpr (KV == AP_ROWS) issue_k(kd, j);
     else if constexpr (F8) issue_page(kd, a.kc, r, l8, 64u);
-    else issue_page(kd, a.kc, r, kl, 32u);
+    else issue_page(kd, a.kc, r, kl + (uint32_t)(ROW * h), 32u);
   };
   auto load_v = [&](unsigned char* vd, const Rows& r, int j) {
     if constexpr (KV == AP_ROWS) issue_v(vd, j);
     else if constexpr (F8) issue_page(vd, a.vc, r, l8, 64u);
-    else issue_page(vd, a.vc, r, vl, 64u);
+    else issue_page(vd, a.vc, r, vl + (uint32_t)(ROW * h), 64u);
   };
   // this wave's loads up to the last N have landed and its LDS accesses are complete, then
   // every wave's
@@ -236,8 +252,12 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
   for (int i = tid; i < AP_SET / 16; i += 64 * AP_WAVES) {
     *reinterpret_cast<uint4*>(vs0 + 16 * i) = make_uint4(0, 0, 0, 0);
     *reinterpret_cast<uint4*>(vs1 + 16 * i) = make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(vs2 + 16 * i) = make_uint4(0, 0, 0, 0);
+    if constexpr (SETS == 3) *reinterpret_cast<uint4*>(vs2 + 16 * i) = make_uint4(0, 0, 0, 0);
   }
+  // Q's last QL operands wait in LDS where the registers of two waves a SIMD do not hold them.
+  constexpr int QL = SETS == 2 ? 4 : 0;
+  __shared__ __attribute__((aligned(16))) unsigned char qlate[QL ? AP_WAVES * QL * 1024 : 16];
+  unsigned char* const ql = qlate + (QL ? 1024 * QL * wave + 16 * lane : 0);
   // this lane's rows: position q0 + qi, query head kvh n_rep + hr
   int qpos[RG];
   bf16x8 Q[RG][16];
@@ -251,11 +271,14 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
     for (int ks = 0; ks < 16; ++ks)   // (8 bits: a lane's 16 codes of K are two k-steps)
       Q[rg][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(
                                                  src + (F8 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1) : 16 * ks + 8 * h)));
+#pragma unroll
+    for (int i = 0; i < QL; ++i) *reinterpret_cast<bf16x8*>(ql + 1024 * i) = Q[rg][16 - QL + i];
   }
   // Pages (two halves of a block): of blocks j + 1, j + 2 and j + 3 before step j, and the entry of
   // block j + 4; the scales of block j + 1's K and of block j's V.  What a step asks the scalar
   // cache for, the next one uses.
-  const int wg = wave >> 1;            // the half of a block that holds the wave's rows
+  // the half of a block that holds the wave's rows (a choice: an index is a search of all of them)
+  auto mine = [&](const int (&id)[2]) { return wave >> 1 ? id[1] : id[0]; };
   int pg[3][2], raw[2] = {-1, -1}, pg0[2] = {-1, -1};
   float ksc[2] = {0.f, 0.f};
   int vsc[2] = {0, 0}, v_ref = 0;      // (bits; v_ref: the units of O, at_f16)
@@ -278,13 +301,15 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
     return KV == AP_ROWS ? 3u : (id[0] >= 0 ? 1u : 0u) | (id[1] >= 0 ? 2u : 0u);
   };
   AP_BARRIER(0);   // the zeroed sets, before any DMA into them (and Q: the counts below are the DMA's)
-  const Rows first = rows_of(pg0[wg], j0), second = rows_of(pg[0][wg], j0 + 1);
-  Rows coming = rows_of(pg[1][wg], j0 + 2);   // of block j + 2 before step j
+  const Rows first = rows_of(mine(pg0), j0), second = rows_of(mine(pg[0]), j0 + 1);
+  Rows coming = rows_of(mine(pg[1]), j0 + 2);   // of block j + 2 before step j
   load_k(ks0, first, j0);
   load_k(ks1, second, j0 + 1);
   load_v(vs0, first, j0);
-  load_k(ks2, coming, j0 + 2);
-  load_v(vs1, second, j0 + 1);
+  if constexpr (SETS == 3) {
+    load_k(ks2, coming, j0 + 2);
+    load_v(vs1, second, j0 + 1);
+  }
 
   // the positions this wave's rows span: the key blocks it sees, and which need a mask
   const int wq0 = ap_div(32 * RG * wave, a.rep_mul);
@@ -340,18 +365,23 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-    bf16x8 kf[AP_AHEAD];
+    bf16x8 kf[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AP_AHEAD; ++i)
+    for (int i = 0; i < AHEAD; ++i)
       kf[i] = *reinterpret_cast<const bf16x8*>(kset + (kof ^ (32 * (i & 7))) + 256 * (i >> 3));
+    bf16x8 qn;
 #pragma unroll
     for (int ks = 0; ks < 16; ++ks) {
+      const bf16x8 qv = qn;
+      if (QL && ks + 1 >= 16 - QL && ks + 1 < 16) qn = *reinterpret_cast<const bf16x8*>(ql + 1024 * (ks + 1 - (16 - QL)));
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg)
-        if (ks == 0) ap_mfma_first(S[rg], kf[0], Q[rg][0]); else ap_mfma(S[rg], kf[ks % AP_AHEAD], Q[rg][ks]);
-      const int kn = ks + AP_AHEAD;
+        if (ks == 0) ap_mfma_first(S[rg], kf[0], Q[rg][0]);
+        else ap_mfma(S[rg], kf[ks % AHEAD], QL && ks >= 16 - QL ? qv : Q[rg][ks]);
+      const int kn = ks + AHEAD;
+      if (QL && kn == 8) asm volatile("" : "+v"(kof));   // (or all 8 addresses wait in registers)
       if (kn < 16)
-        kf[ks % AP_AHEAD] = *reinterpret_cast<const bf16x8*>(kset + (kof ^ (32 * (kn & 7))) + 256 * (kn >> 3));
+        kf[ks % AHEAD] = *reinterpret_cast<const bf16x8*>(kset + (kof ^ (32 * (kn & 7))) + 256 * (kn >> 3));
       __builtin_amdgcn_sched_barrier(0);   // no more operands ahead than the registers hold
     }
     }
@@ -430,28 +460,29 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
       return __builtin_bit_cast(bf16x8, u32x4_t{w0.x, w0.y, w1.x, w1.y});
       }
     };
-    decltype(read_v(0)) vf[AP_AHEAD];
+    decltype(read_v(0)) vf[AHEAD];
     u32x4_t Pn[RG][2], Pm[RG][2];
     float pe[RG];
     const float ratio[2] = {at_ratio(vsc[0], v_ref), at_ratio(vsc[1], v_ref)};   // (8 bits)
 #pragma unroll
-    for (int i = 0; i < AP_AHEAD; ++i) vf[i] = read_v(i);
+    for (int i = 0; i < AHEAD; ++i) vf[i] = read_v(i);
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
       if constexpr (F8) {
-        const f16x8 vA = at_f16(vf[n % AP_AHEAD].x, vf[n % AP_AHEAD].y, ratio[n & 1]);
+        const f16x8 vA = at_f16(vf[n % AHEAD].x, vf[n % AHEAD].y, ratio[n & 1]);
 #pragma unroll
         for (int rg = 0; rg < RG; ++rg)
           O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vA, Pf[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
       } else {
 #pragma unroll
         for (int rg = 0; rg < RG; ++rg)
-          O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AP_AHEAD], P[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+          O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AHEAD], P[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
 #pragma unroll
         for (int rg = 0; rg < RG; ++rg)
-          O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AP_AHEAD], Pl[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
+          O[rg][n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n % AHEAD], Pl[rg][n & 1], O[rg][n >> 1], 0, 0, 0);
       }
-      if (n + AP_AHEAD < 16) vf[n % AP_AHEAD] = read_v(n + AP_AHEAD);
+      if (QL && n + AHEAD == 8) asm volatile("" : "+v"(vof));
+      if (n + AHEAD < 16) vf[n % AHEAD] = read_v(n + AHEAD);
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg) {
         const float p = fast_exp2(__builtin_fmaf(S[rg][n], a.cl2, -base[rg]));
@@ -489,6 +520,8 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
 #pragma unroll
     for (int g = 0; g < 2; ++g) ksc[g] = scale_at(a.ks, pg0[g]);
     AP_BARRIER(8);    // block 0 of K, the first 2 of the 10 loads
+  } else if constexpr (SETS == 2) {
+    AP_BARRIER(8);    // the first 4 of 12
   } else {
     AP_BARRIER(16);   // block 0 of K, the first 4 of the 20 loads
   }
@@ -522,7 +555,8 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
   }
   // Barrier before step j: blocks j + 1 of K and j of V have landed (the 8 loads after them, 4 of
   // 8-bit pages, may be in flight), and every wave is done with K of block j and V of block j - 1,
-  // whose sets the loads of blocks j + 3 and j + 2 take.
+  // whose sets the loads of blocks j + 3 and j + 2 take.  With two sets nothing is in flight, and they
+  // are those of blocks j + 2 and j + 1.
   if constexpr (F8) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
@@ -533,11 +567,17 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
   }
   auto turn = [&](unsigned char* kfree, unsigned char* vfree, const unsigned char* knext, const unsigned char* vset,
                   int j) {
-    if constexpr (F8) AP_BARRIER(4); else AP_BARRIER(8);
-    const Rows next = rows_of(pg[2][wg], j + 3);
-    load_k(kfree, next, j + 3);
-    load_v(vfree, F8 ? coming : rows_of(pg[1][wg], j + 2), j + 2);
-    coming = next;
+    if constexpr (SETS == 2) {
+      AP_BARRIER(0);
+      load_k(kfree, rows_of(mine(pg[1]), j + 2), j + 2);
+      load_v(vfree, rows_of(mine(pg[0]), j + 1), j + 1);
+    } else {
+      if constexpr (F8) AP_BARRIER(4); else AP_BARRIER(8);
+      const Rows next = rows_of(mine(pg[2]), j + 3);
+      load_k(kfree, next, j + 3);
+      load_v(vfree, F8 ? coming : rows_of(mine(pg[1]), j + 2), j + 2);
+      coming = next;
+    }
     float kn[2] = {0.f, 0.f};
     int vn[2] = {0, 0}, rn[2] = {-1, -1};
 #pragma unroll
@@ -559,10 +599,15 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
       vsc[g] = vn[g];
     }
   };
-  for (int j = j0; j < nblk; j += 3) {
-    turn(ks0, vs2, ks1, vs0, j);
-    turn(ks1, vs0, ks2, vs1, j + 1);
-    turn(ks2, vs1, ks0, vs2, j + 2);
+  for (int j = j0; j < nblk; j += SETS) {
+    if constexpr (SETS == 2) {
+      turn(ks0, vs1, ks1, vs0, j);
+      turn(ks1, vs0, ks0, vs1, j + 1);
+    } else {
+      turn(ks0, vs2, ks1, vs0, j);
+      turn(ks1, vs0, ks2, vs1, j + 1);
+      turn(ks2, vs1, ks0, vs2, j + 2);
+    }
   }
   AP_BARRIER(0);   // no load in flight, every wave done with the sets: the dumps take them
 #undef AP_BARRIER
@@ -571,7 +616,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, RG == 1 && KV == AP_PAGES8 ? 2 : 1) 
   // c of row r at c ^ (r & 15)), then runs of whole rows with the gate: 8 columns per lane, 16-byte
   // loads and stores.
   constexpr int COLS = AP_SET / 128, LPR = COLS / 8, RPI = 64 / LPR;   // lanes of a row, rows at a time
-  unsigned char* dump = wave == 0 ? ks0 : (wave == 1 ? ks1 : (wave == 2 ? ks2 : vs0));
+  unsigned char* dump = wave == 0 ? ks0 : (wave == 1 ? ks1 : (wave == 2 ? (SETS == 3 ? ks2 : vs1) : vs0));
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_s[rg]), __float_as_uint(l_s[rg]), false, false);
@@ -727,20 +772,25 @@ static int prefill_tiles(int B, int T, int Hkv, int n_rep, int rg, int* QB) {
 
 int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts) {
   *parts = 1;
-  const int rg = attn_prefill_groups(B, T, Hkv, n_rep, cus);
-  if ((rg == 2 && !f8) || T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS) return rg;
-  // Fewer tiles than CUs divide their keys: as many parts as the chip holds at once, or a few more
-  // where their rounds come out a tenth shorter (160 tiles: 3 parts take 2 rounds of a third).
-  // With that tiles are the faster form at any number of them (us, tiles / split-K, bf16: 20 tiles
-  // of 2070 keys 36 / 43, of 30000 138 / 304; 64 of 8256 130 / 229; 128 of 8289 234 / 436), but
-  // for few tiles of 8-bit pages, whose codes a tile converts for 32 rows at a time as the split-K
-  // does, without its depth of loads (20 of 2070 keys 40 / 33, of 8000 64 / 61; 128 of 8289 265 /
-  // 298; 64 x 136 rows of 8017 257 / 232): from 80 full tiles on.
+  if (T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS) return 0;
   const long long pairs = (long long)B * Hkv;
-  if (f8 && 16 * pairs * T * n_rep < 5LL * cus * 128) return 0;
+  // Query tiles, whatever their number (us, tiles / split-K, bf16: 20 tiles of 2070 keys 35 / 38, of
+  // 30000 134 / 308; 64 of 8256 123 / 220; 128 of 8289 203 / 418; but 32 of 256 28 / 20), but for few
+  // tiles of 8-bit pages, whose codes a tile converts for 32 rows at a time as the split-K does,
+  // without its depth of loads: from 64 full tiles on (32 of 1128 42 / 31, of 4128 53 / 53; 64 of
+  // 1256 47 / 37, of 4256 72 / 79, of 16256 164 / 236; 128 of 512 46 / 42, of 8289 166 / 249).
+  if (f8 && 4 * pairs * T * n_rep < 128LL * cus) return 0;
   int QB;
   const long long tiles = prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * pairs;
-  const int slots = f8 ? 2 * cus : cus;   // workgroups that the chip holds
+  // Workgroups of a CU: a wave alone on its SIMD issues a VALU instruction every 8 cycles, two share
+  // it at 4.  8-bit pages have the LDS for two with three sets; bf16 pages with two, which leave a
+  // block's rows one step to arrive: where there are tiles for half of the CUs and rows for keys (us, one / two
+  // a CU: 128 tiles of 8289 keys 237 / 203, 160 of 4640 185 / 151, 256 of 9024 433 / 383; but 32 of
+  // 1128 37 / 43, 128 of 17 20 / 27).
+  const int per_cu = f8 || (2 * tiles >= cus && T >= 256) ? 2 : 1;
+  const int slots = per_cu * cus;
+  // Fewer tiles than these divide their keys: as many parts as the chip holds at once, or a few more
+  // where their rounds come out a tenth shorter (160 tiles: 3 parts take 2 rounds of a third).
   if (tiles < slots) {
     int best = slots / (int)tiles;
     best = best > AP_MAX_PARTS ? AP_MAX_PARTS : best;
@@ -754,7 +804,7 @@ int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* p
     }
     *parts = best;
   }
-  return 1;
+  return per_cu;
 }
 
 long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts) {
@@ -764,15 +814,12 @@ long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts) {
   return tiles * parts * AP_PIECE * (long long)sizeof(float) + tiles * 4;
 }
 
-template <int KV>
-static void prefill_start(const ApArgs& a, int rg, unsigned n, hipStream_t st) {
-  if (rg == 2)
-    hipLaunchKernelGGL((attn_prefill_kernel<2, KV>), dim3(n), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((attn_prefill_kernel<1, KV>), dim3(n), dim3(256), 0, st, a);
+template <int RG, int KV, int SETS>
+static void prefill_start(const ApArgs& a, unsigned n, hipStream_t st) {
+  hipLaunchKernelGGL((attn_prefill_kernel<RG, KV, SETS>), dim3(n), dim3(256), 0, st, a);
 }
 
-int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st, const PagedArgs* paged, int parts) {
+int attn_prefill_launch(const AttnArgs& v, int groups, hipStream_t st, const PagedArgs* paged, int parts) {
   ApArgs a;
   a.q = v.q; a.kc = v.kc; a.vc = v.vc; a.kv_len = v.kv_len; a.gate = v.gate; a.out = v.out;
   a.seq_stride = v.seq_stride; a.head_stride = v.head_stride;
@@ -780,21 +827,20 @@ int attn_prefill_launch(const AttnArgs& v, int rg, hipStream_t st, const PagedAr
   a.B = v.B; a.T = v.T; a.Hq = v.Hq; a.Hkv = v.Hkv; a.n_rep = v.n_rep; a.max_len = v.max_len;
   a.cl2 = v.cl2;
   a.rep_mul = (uint32_t)((65536 + v.n_rep - 1) / v.n_rep);
-  a.qtiles = prefill_tiles(v.B, v.T, v.Hkv, v.n_rep, rg, &a.QB);
+  a.qtiles = prefill_tiles(v.B, v.T, v.Hkv, v.n_rep, paged ? 1 : groups, &a.QB);
   a.parts = parts; a.ws = v.ws;
   a.table = nullptr; a.ks = a.vs = nullptr; a.table_stride = 0; a.n_pages = a.pshift = 0;
   const long long n = (long long)a.qtiles * v.B * v.Hkv * parts;
   if (n > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;
-  if (!paged) {
-    prefill_start<AP_ROWS>(a, rg, (unsigned)n, st);
-  } else {
+  if (paged) {
     a.table = paged->table; a.ks = paged->ks; a.vs = paged->vs; a.table_stride = paged->table_stride;
     a.n_pages = paged->n_pages; a.pshift = paged->pshift;
-    if (paged->ks)
-      prefill_start<AP_PAGES8>(a, rg, (unsigned)n, st);
-    else
-      prefill_start<AP_PAGES>(a, rg, (unsigned)n, st);
   }
+  if (paged && paged->ks) prefill_start<1, AP_PAGES8, 3>(a, (unsigned)n, st);
+  else if (paged && groups == 2) prefill_start<1, AP_PAGES, 2>(a, (unsigned)n, st);
+  else if (paged) prefill_start<1, AP_PAGES, 3>(a, (unsigned)n, st);
+  else if (groups == 2) prefill_start<2, AP_ROWS, 3>(a, (unsigned)n, st);
+  else prefill_start<1, AP_ROWS, 3>(a, (unsigned)n, st);
   if (parts > 1) {
     const int rc = launch_status();
     if (rc) return rc;

@@ -147,6 +147,20 @@ def test_attention_window_of_a_chunk(P, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("B,T,lens,P,given,holes", [
+    (1, 520, [2300], 64, 1000, (19, 25)),            # a window, holes behind it
+    (1, 513, [1501], 16, 0, (3, 40, 41, 60, 92)),    # holes that end inside a block
+    (2, 300, [1300, 0], 32, 200, (38,)),             # an idle slot
+    (2, 257, [140, 3000], 128, 0, (1,)),             # more rows than keys
+])
+def test_attention_many_tiles(B, T, lens, P, given, holes, bits):
+    """Tiles that share a CU two by two, their keys in parts."""
+    print(f"case tiles {B} {T} {lens} page {P} bits {bits}", flush=True)
+    holes = {(0, i) for i in range(given // P)} | {(0, i) for i in holes}
+    check_attention(attend_case(sum(lens) + P, B, T, 32, 4, lens, P, bits, holes), 32)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
 def test_attention_scale_and_large_values(bits):
     """A maximum that moves by more than the rescale threshold between blocks, and a scale."""
     q, k, v, table, lens, qkv, ks, vs = attend_case(3, 2, 2, 8, 2, [900, 300], 32, bits)
