@@ -23,11 +23,11 @@
 //      transposing 8-bit LDS read and becomes fp16 (at_f16).
 // Weights enter the product with V as hi + lo bf16 (attn_prefill.hip), with 8-bit V as fp16.
 //
-// What bounds it: the KV stream from some ten blocks a workgroup on, a fixed 13 us before.  16 x 4
-// tokens, 32 / 4 heads (us, TB/s of K and V): 128 keys 17.0 (8 bits 15.2), 1024 25.9, 2.6 (21.1,
-// 1.6), 4096 53, 5.0 (35, 3.8), 16384 182, 5.9 (93, 5.7), 65536 665, 6.5 (354, 6.1); pages of 16 to
-// 128 rows alike.  Of the fixed part the two launches are 5, the table and the scales' round trips
-// before the first load 2, the last block's products and the merge of the waves 4.  8-bit blocks
+// What bounds it: the KV stream from some ten blocks a workgroup on, a fixed 12 us before.  16 x 4
+// tokens, 32 / 4 heads (us, TB/s of K and V): 128 keys 15.5 (8 bits 14.3), 1024 25.4, 2.6 (21.0,
+// 1.6), 4096 53, 5.0 (35, 3.9), 16384 180, 6.0 (93, 5.8), 65536 663, 6.5 (349, 6.1); pages of 16 to
+// 128 rows alike.  Of the fixed part the two launches are 5, lengths and table before the first
+// load 1.5, the last block's products 1.5, the merge of the waves 1.8.  8-bit blocks
 // are half the bytes: K is asked for two blocks ahead, of bf16 one, as a wave has at most 63 loads on
 // its way.
 #include <type_traits>

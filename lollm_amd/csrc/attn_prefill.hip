@@ -44,7 +44,7 @@
 // block and wave of 8-bit pages, half of the former conversions, beside 32 products of 32 cycles.
 // Where tiles are fewer than the chip holds, a tile's keys are dealt out to `parts` workgroups, whose
 // pieces a second kernel merges (512 tokens over 8289 keys, 128 tiles in four parts: 203 us, of
-// which the merge 11; 418 on the split-K kernel).
+// which the merge 15; 418 on the split-K kernel).
 //
 // Rows of K and V are 512 bytes in LDS with no padding (the DMA writes 1 KB runs); the
 // 16-byte chunk c of row r sits at c ^ (r & 15) for K and c ^ (2 (r & 7)) for V, so the
