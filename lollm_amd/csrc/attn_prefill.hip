@@ -784,7 +784,7 @@ int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* p
   const long long tiles = prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * pairs;
   // Workgroups of a CU: a wave alone on its SIMD issues a VALU instruction every 8 cycles, two share
   // it at 4.  8-bit pages have the LDS for two with three sets; bf16 pages with two, which leave a
-  // block's rows one step to arrive: where there are tiles for half of the CUs and rows for keys (us, one / two
+  // block's rows one step to arrive: for half as many tiles as CUs and 256 tokens a sequence (us, one / two
   // a CU: 128 tiles of 8289 keys 237 / 203, 160 of 4640 185 / 151, 256 of 9024 433 / 383; but 32 of
   // 1128 37 / 43, 128 of 17 20 / 27).
   const int per_cu = f8 || (2 * tiles >= cus && T >= 256) ? 2 : 1;

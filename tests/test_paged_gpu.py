@@ -269,6 +269,36 @@ def test_pools_past_4_gb(bits):
         del big
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("T", [3, 90, 520])
+def test_attention_lengths_outside_the_table(T, bits):
+    """A length past what the table names counts as that much, a negative one as none."""
+    print(f"case lengths T {T} bits {bits}", flush=True)
+    q, k, v, table, lens, qkv, ks, vs = attend_case(35, 3, T, 16, 4, [640, 600, 64], 64, bits)
+    lens = torch.tensor([2 ** 31 - 1, 600, -7], dtype=torch.int32)
+    out = check_attention((q, k, v, table, lens, qkv, ks, vs), 16)
+    assert (out[2] == 0).all()
+
+
+def test_outputs_of_the_caller():
+    from lollm_amd import ops
+    q, k, v, table, lens, qkv, ks, vs = cuda(*attend_case(36, 2, 3, 8, 2, [40, 90], 16, 8))
+    want = ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs)
+    out = torch.full((2, 3, 8 * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert ops.attn_paged(q, k, v, table, lens, gates(qkv, 8), k_scale=ks, v_scale=vs, out=out) is out
+    assert torch.equal(out, want)
+    w, inv = torch.zeros(D, dtype=torch.bfloat16, device="cuda"), torch.ones(32, device="cuda")
+    args = (qkv, w, w, inv, lens - 3, table, k, v, 8, 64, EPS)
+    want, _ = ops.attn_append(*args, k_scale=ks, v_scale=vs)
+    got, _ = ops.attn_append(*args, k_scale=ks, v_scale=vs, q_out=torch.empty_like(q))
+    assert torch.equal(got, want)
+    for bad in (torch.empty_like(q)[:, :2], torch.empty_like(q).float(), torch.empty_like(q).cpu()):
+        with pytest.raises((ValueError, TypeError)):
+            ops.attn_append(*args, k_scale=ks, v_scale=vs, q_out=bad)
+        with pytest.raises((ValueError, TypeError)):
+            ops.attn_paged(q, k, v, table, lens, None, k_scale=ks, v_scale=vs, out=bad)
+
+
 def test_attention_repeats_bit_for_bit():
     from lollm_amd import ops
     q, k, v, table, lens, qkv, ks, vs = cuda(*attend_case(5, 4, 4, 16, 2, [900, 40, 2000, 333], 64, 8))
