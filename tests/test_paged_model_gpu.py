@@ -97,6 +97,26 @@ def test_decoder_out_of_pages_and_released(micro):
     assert d.cache.held[1] == 0 and (d.cache.table[1] == -1).all()
 
 
+def test_rollback_leaves_nothing_in_bf16_pages(micro):
+    """4 tokens of which a + 1 are kept (a = 0 .. 3 over the batch, a page's end among them), then one
+    more: bit for bit the logits of a cache that saw the kept ones only."""
+    model, _, _, cfg = micro
+    g = torch.Generator().manual_seed(7)
+    prompts, blk, nxt = (torch.randint(0, cfg.vocab_size, (4, n), generator=g).cuda() for n in (46, 4, 1))
+    acc = torch.arange(4, device="cuda").int()
+    cache = model.new_cache(4, 80, page=16)
+    model(prompts, cache, logits="last")
+    short = cache.clone()
+    model(blk, cache)
+    cache.rollback(acc)
+    got, _ = model(nxt, cache)
+    for a in range(4):
+        c = short.clone()
+        model(blk[:, :a + 1], c)
+        want, _ = model(nxt, c)
+        assert torch.equal(got[a], want[a])
+
+
 def test_generate_over_8_bit_pages(micro):
     from lollm_amd.generate import generate
     from lollm_amd.qwen3_5 import generate_mtp
