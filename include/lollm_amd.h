@@ -104,8 +104,9 @@ int lollm_attn_verify(const void* q, const void* k_cache, const void* v_cache,
  *   k_pages, v_pages  (n_pages, Hkv, page, D), kv_dtype LOLLM_BF16 or LOLLM_F8: e4m3 codes,
  *            their value the code times the page's scale
  *   k_scale, v_scale  (n_pages, Hkv) fp32 powers of two (8-bit pages; else NULL).  Beside the
- *            output's rounding a result is off by up to 2^-11 of the weighted mean of |V|, and by
- *            2^-25 of the largest V scale among the sequence's pages
+ *            output's rounding a result is off by up to 2^-11 of the weighted mean of |V|, by 2^-35
+ *            of the row's largest weight times the sum of |V| over its keys (the step of fp16
+ *            weights), and by 2^-25 of the largest V scale among the sequence's pages
  *   table    (B, table_width) int32, rows table_stride apart; it holds table_width * page keys
  *   gate     element d of (token bt, head h) at gate + bt * gate_row + h * gate_head + d (so it
  *            can be read where the fused projection wrote it), or NULL

@@ -285,7 +285,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   f32x16 O[8];            // O^T: d-tile dt (32 columns) x the 32 rows; lane row = l32
   float m_ref = -INFINITY, l_s = 0.f;
   int v_ref = 0;          // 8 bits: O counts in units of this scale (bits), at_f16
-  constexpr float LAG = F8 ? 15.f : 16.f;   // (fp16 weights end at 2^16)
+  constexpr float LAG = F8 ? AT_F16_LAG : 16.f, UP = F8 ? AT_F16_UP : 0.f;
   const int lq = (int)(((uint32_t)l32 * p.rep_mul) >> 16);   // the lane's position in its query block
   int qpos = 0, rows = 0;
 
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         for (int dt = 0; dt < 8; ++dt) asm volatile("" : "+a"(O[dt]));
         m_ref = big ? bm : m_ref;
         v_ref = v_now;
-        const float base = m_ref == -INFINITY ? 0.f : m_ref * a.cl2;
+        const float base = m_ref == -INFINITY ? 0.f : m_ref * a.cl2 - UP;
         float e[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) e[r] = fast_exp2(__builtin_fmaf(S[r], a.cl2, -base));

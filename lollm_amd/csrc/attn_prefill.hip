@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
   int pg[3][2], raw[2] = {-1, -1}, pg0[2] = {-1, -1};
   float ksc[2] = {0.f, 0.f};
   int vsc[2] = {0, 0}, v_ref = 0;      // (bits; v_ref: the units of O, at_f16)
-  constexpr float LAG = F8 ? 15.f : 16.f;   // (fp16 weights end at 2^16)
+  constexpr float LAG = F8 ? AT_F16_LAG : 16.f, UP = F8 ? AT_F16_UP : 0.f;
   auto scale_at = [&](const float* sc, int id) {
     const float s = ap_sload(sc, (long long)max(id, 0) * a.Hkv + kvh);
     return id >= 0 ? s : 0.f;
@@ -408,11 +408,14 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
       // the reference max moves (and l, O are rescaled) only when a row's block max exceeds it
       // by more than LAG in the exponent: attn_verify's rule, each row's own decision
       const bool big = (bm - m_ref[rg]) * a.cl2 > LAG;
-      const float mn = big ? fmaxf(m_ref[rg], bm) : m_ref[rg];
-      alpha[rg] = (!big || mn == -INFINITY) ? 1.f : fast_exp2((m_ref[rg] - mn) * a.cl2);
+      // (8 bits, whose LAG is small: with one row every row moves that can, as all of O is rescaled
+      // anyway; alone 195 us for 2 x 1999, so 185)
+      const bool move = F8 ? __ballot(big) != 0 && bm > m_ref[rg] : big;
+      const float mn = move ? fmaxf(m_ref[rg], bm) : m_ref[rg];
+      alpha[rg] = (!move || mn == -INFINITY) ? 1.f : fast_exp2((m_ref[rg] - mn) * a.cl2);
       m_ref[rg] = mn;
       l_s[rg] *= alpha[rg];
-      base[rg] = mn == -INFINITY ? 0.f : mn * a.cl2;
+      base[rg] = mn == -INFINITY ? 0.f : mn * a.cl2 - UP;
       any = any || big;
     }
     moved = __builtin_amdgcn_readfirstlane((int)(__ballot(any) != 0)) != 0;
