@@ -95,10 +95,14 @@ class Qwen3_5Cache:
         if capturing():
             raise RuntimeError(f"KV cache capacity: {self.len_bound} + {T} rows may exceed "
                                f"max_len {self.max_len} (cannot check exactly under capture)")
-        self.len_bound = int(self.lengths.max()) if self.batch else 0
+        self._measure()
         if self.len_bound + T > self.max_len:
             raise RuntimeError(f"KV cache capacity exceeded: a sequence holds {self.len_bound} "
                                f"tokens, {T} more do not fit max_len {self.max_len}")
+
+    def _measure(self):
+        """Set the bound to what it bounds (a host sync)."""
+        self.len_bound = int(self.lengths.max()) if self.batch else 0
 
     def grew(self, T: int):
         """Record that a call may have added up to T tokens to every sequence."""
@@ -264,42 +268,65 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
         s = self.layers[layer]
         return {"table": self.table, "k_scale": s.get("ks"), "v_scale": s.get("vs")}
 
+    @property
+    def len_bound(self):
+        return max(self._bounds, default=0)
+
+    @len_bound.setter
+    def len_bound(self, n):
+        self._bounds = [n] * self.batch      # of each sequence: lengths part as drafts are rejected
+
+    def _measure(self):
+        self._bounds = self.lengths.tolist()
+
+    def grew(self, T: int):
+        self._bounds = [n + T for n in self._bounds]
+
     def reserve(self, T: int):
         """Raise RuntimeError unless T more rows fit max_len and the pool; name their pages.  Goes
-        by the host-side bound of the lengths, and by the lengths themselves (a host sync) only
-        where the pool cannot give every sequence that many."""
+        by the host-side bounds of the lengths, and by the lengths themselves (a host sync) only
+        where the pool is short of that; sequences then give back the pages that they do not need for
+        their rows and T more (an earlier call's, if it reserved more and they were not filled)."""
         super().reserve(T)
 
-        def short(lengths):
-            return [0 if not live else max(0, -(-(n + T) // self.page) - held)
-                    for n, held, live in zip(lengths, self.held, self.live)]
+        def needs():
+            return [-(-(n + T) // self.page) if live else 0 for n, live in zip(self._bounds, self.live)]
 
-        want = short([self.len_bound] * self.batch)
-        if not any(want):
+        def missing(need):
+            return sum(max(0, n - held) for n, held in zip(need, self.held))
+
+        need = needs()
+        if not missing(need):
             return
         if capturing():
             raise RuntimeError("pages cannot be handed out under capture: reserve() before it")
-        if sum(want) > len(self.free):
-            lengths = self.lengths.tolist()
-            self.len_bound = max(lengths)
-            want = short(lengths)
-            if sum(want) > len(self.free):
-                raise RuntimeError(f"KV page pool exhausted: {sum(want)} pages needed, {len(self.free)} of "
-                                   f"{self.n_pages} free")
-        for b, n in enumerate(want):
-            for _ in range(n):
+        if missing(need) > len(self.free):
+            self._measure()
+            need = needs()
+            if sum(need) > self.n_pages:
+                raise RuntimeError(f"KV page pool exhausted: {sum(need)} pages needed, the pool has {self.n_pages}")
+            if missing(need) > len(self.free):
+                for b, n in enumerate(need):   # (past the rows to come: rolled back, or never written)
+                    self._take_back(b, n)
+        for b, n in enumerate(need):
+            while self.held[b] < n:
                 self._host_table[b, self.held[b]] = self.free.pop()
                 self.held[b] += 1
         self.table.copy_(self._host_table)
+
+    def _take_back(self, b: int, keep: int):
+        """Pages of sequence b from its `keep`-th on go back to the pool (the table follows)."""
+        self.free += self._host_table[b, keep:max(keep, self.held[b])].tolist()
+        self._host_table[b, keep:] = -1
+        self.held[b] = min(self.held[b], keep)
 
     def release(self, b: int):
         """Give back the pages of a finished sequence: it holds no keys from now on, takes no more
         pages, and its rows of later calls mean nothing."""
         if capturing():
             raise RuntimeError("release() under capture")
-        self.free += self._host_table[b, :self.held[b]].tolist()
-        self._host_table[b] = -1
-        self.held[b], self.live[b] = 0, False
+        self._take_back(b, 0)
+        self.live[b] = False
         self.lengths[b] = 0
         self.table.copy_(self._host_table)
 
@@ -348,7 +375,8 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
         new = super().clone()
         new.__class__ = Qwen3_5PagedCache
         new.table, new._host_table = self.table.clone(), self._host_table.clone()
-        new.free, new.held, new.live = list(self.free), list(self.held), list(self.live)
+        for n in ("free", "held", "live", "_bounds"):
+            setattr(new, n, list(getattr(self, n)))
         return new
 
     def nbytes(self):

@@ -108,6 +108,63 @@ def test_cache_goes_by_the_lengths_where_the_bound_is_short_of_pages():
     assert [len(p) for p in pages_of(c)] == [2, 2, 2] and c.len_bound == 20
 
 
+def test_cache_takes_idle_pages_back_before_the_pool_is_short():
+    """A long bound gave both sequences four pages; the second fills two when the first needs a fifth."""
+    c = cache(batch=2, page=16, n_pages=8)
+    c.reserve(60)
+    c.lengths.copy_(torch.tensor([60, 28], dtype=torch.int32))
+    c.grew(60)
+    assert c.held == [4, 4] and not c.free
+    mine, other = pages_of(c)
+    c.lengths.copy_(torch.tensor([64, 29], dtype=torch.int32))
+    c.grew(4)
+    c.reserve(4)
+    now = pages_of(c)
+    assert now[0][:4] == mine and len(now[0]) == 5 and now[1] == other[:3] and c.held == [5, 3]
+    assert torch.equal(c.table, c._host_table) and (c.table[1, 3:] == -1).all()
+
+
+@pytest.mark.parametrize("kept", [(4, 1), (1, 4), (4, 4), (2, 3)])
+def test_cache_serves_until_the_real_need_passes_the_pool(kept):
+    """Steps of 4 rows of which a sequence keeps its own number: the first step that is refused is
+    the first whose rows do not fit, and rows that are there keep their pages until then."""
+    c = cache(batch=2, max_len=2000, page=16, n_pages=40)
+    c.advance(32)
+    for step in range(1000):
+        need = [-(-(int(n) + 4) // 16) for n in c.lengths]
+        full = [-(-int(n) // 16) for n in c.lengths]
+        before = pages_of(c)
+        if sum(need) > 40:
+            with pytest.raises(RuntimeError, match="pool exhausted"):
+                c.reserve(4)
+            assert pages_of(c) == before
+            break
+        c.reserve(4)
+        now = pages_of(c)
+        assert all(n[:f] == b[:f] for n, b, f in zip(now, before, full))
+        assert all(len(n) >= m for n, m in zip(now, need)) and [len(n) for n in now] == c.held
+        every = sum(now, [])
+        assert sorted(every + c.free) == list(range(40)) and c.len_bound >= int(c.lengths.max())
+        c.lengths += torch.tensor(kept, dtype=torch.int32)
+        c.grew(4)
+    else:
+        raise AssertionError("never refused")
+
+
+def test_cache_reads_the_lengths_only_where_the_pool_is_short():
+    """Bounds are each sequence's own once read: a page at a time, not all of the batch's longest."""
+    c = cache(batch=2, max_len=2000, page=16, n_pages=41)
+    c.advance(32)
+    reads = []
+    measure = c._measure
+    c._measure = lambda: (reads.append(1), measure())
+    for _ in range(84):
+        c.reserve(4)
+        c.lengths += torch.tensor([4, 1], dtype=torch.int32)
+        c.grew(4)
+    assert c.held[1] < c.held[0] and 1 <= len(reads) <= 4
+
+
 def test_cache_append_read_and_clone():
     g = torch.Generator().manual_seed(1)
     c = cache(page=16)
