@@ -102,7 +102,11 @@ class Qwen3_5Cache:
 
     def _measure(self):
         """Set the bound to what it bounds (a host sync)."""
-        self.len_bound = int(self.lengths.max()) if self.batch else 0
+        self.len_bound = self.longest(self.lengths)
+
+    def longest(self, counts: torch.Tensor) -> int:
+        """The largest of a count per sequence (a host sync)."""
+        return int(counts.max()) if self.batch else 0
 
     def grew(self, T: int):
         """Record that a call may have added up to T tokens to every sequence."""
@@ -244,6 +248,7 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
         if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise TypeError(f"kv_dtype must be bfloat16 or float8_e4m3fn, got {kv_dtype}")
         self.page, self.kv_dtype = page, kv_dtype
+        self.live = [True] * batch       # released sequences take no more
         width = -(-max_len // page)
         self.n_pages = batch * width if n_pages is None else n_pages
         if self.n_pages < 1:
@@ -253,7 +258,7 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
         self._host_table = torch.full((batch, width), -1, dtype=torch.int32)
         self.free = list(range(self.n_pages - 1, -1, -1))
         self.held = [0] * batch          # pages of each sequence
-        self.live = [True] * batch       # released sequences take no more
+        self._dead = torch.zeros(batch, dtype=torch.bool, device=self.device)   # not live
 
     def _kv_layer(self):
         cfg = self.cfg
@@ -270,7 +275,7 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
 
     @property
     def len_bound(self):
-        return max(self._bounds, default=0)
+        return max((n for n, live in zip(self._bounds, self.live) if live), default=0)
 
     @len_bound.setter
     def len_bound(self, n):
@@ -278,6 +283,9 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
 
     def _measure(self):
         self._bounds = self.lengths.tolist()
+
+    def longest(self, counts):
+        return max((n for n, live in zip(counts.tolist(), self.live) if live), default=0)
 
     def grew(self, T: int):
         self._bounds = [n + T for n in self._bounds]
@@ -288,6 +296,8 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
         where the pool is short of that; sequences then give back the pages that they do not need for
         their rows and T more (an earlier call's, if it reserved more and they were not filled)."""
         super().reserve(T)
+        if not all(self.live) and not capturing():
+            self.lengths.masked_fill_(self._dead, 0)   # what calls since have added
 
         def needs():
             return [-(-(n + T) // self.page) if live else 0 for n, live in zip(self._bounds, self.live)]
@@ -322,11 +332,13 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
 
     def release(self, b: int):
         """Give back the pages of a finished sequence: it holds no keys from now on, takes no more
-        pages, and its rows of later calls mean nothing."""
+        pages, and its rows of later calls mean nothing (take a decoder's tokens before).  What calls
+        add to its length is cleared by the next reserve() and counts against no capacity."""
         if capturing():
             raise RuntimeError("release() under capture")
         self._take_back(b, 0)
         self.live[b] = False
+        self._dead[b] = True
         self.lengths[b] = 0
         self.table.copy_(self._host_table)
 
@@ -374,7 +386,8 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
     def clone(self):
         new = super().clone()
         new.__class__ = Qwen3_5PagedCache
-        new.table, new._host_table = self.table.clone(), self._host_table.clone()
+        for n in ("table", "_host_table", "_dead"):
+            setattr(new, n, getattr(self, n).clone())
         for n in ("free", "held", "live", "_bounds"):
             setattr(new, n, list(getattr(self, n)))
         return new

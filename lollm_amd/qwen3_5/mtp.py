@@ -277,7 +277,7 @@ class SpecDecoder:
         if self.out_bound + T > self.out_capacity:
             if capturing():
                 raise RuntimeError("output capacity may be exceeded (cannot check under capture)")
-            self.out_bound = int(self.out_count.max())
+            self.out_bound = self.cache.longest(self.out_count)
             if self.out_bound + T > self.out_capacity:
                 raise RuntimeError(f"output capacity exceeded: a sequence holds {self.out_bound} "
                                    f"tokens, a step may add {T}, out_capacity {self.out_capacity}")

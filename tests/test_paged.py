@@ -209,6 +209,40 @@ def test_cache_refuses_rows_of_a_released_sequence():
             call()
 
 
+def test_released_sequence_takes_no_capacity():
+    """Steps go on adding to a released sequence's length, here more than to the live one's: it is
+    cleared before each, and the live one reaches max_len."""
+    c = cache(batch=2, max_len=64, page=16)
+    c.advance(32)
+    c.release(1)
+    for n in range(32, 61):
+        c.reserve(4)
+        assert c.lengths.tolist() == [n, 0] and c.held[1] == 0
+        c.lengths += torch.tensor([1, 4], dtype=torch.int32)
+        c.grew(4)
+    with pytest.raises(RuntimeError, match="capacity"):
+        c.reserve(4)
+    assert c.len_bound == 61
+    d = c.clone()
+    d.release(0)
+    d.reserve(4)                                     # no one left: nothing to refuse
+    assert d.lengths.tolist() == [0, 0] and d.len_bound == 0 and c.live == [True, False]
+
+
+def test_released_sequence_takes_no_output_capacity():
+    from lollm_amd.qwen3_5 import SpecDecoder
+    d = SpecDecoder.__new__(SpecDecoder)
+    d.k, d.cache, d.out_capacity, d.out_bound = 3, cache(batch=2, max_len=64, page=16), 16, 0
+    d.out_count = torch.tensor([9, 30], dtype=torch.int32)
+    d.cache.release(1)
+    d.out_bound = 14
+    d._reserve()                                     # 9 + 4 <= 16
+    assert d.out_bound == 9
+    d.out_count[0], d.out_bound = 13, 16
+    with pytest.raises(RuntimeError, match="output capacity"):
+        d._reserve()
+
+
 def test_new_cache_takes_what_it_is_given():
     from lollm_amd.qwen3_5 import Qwen3_5Cache, Qwen3_5Model
 

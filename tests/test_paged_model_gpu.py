@@ -127,3 +127,22 @@ def test_generate_over_8_bit_pages(micro):
     assert len("".join(out)) == 9
     out = list(generate_mtp(model, mtp, ids, lambda t: "x" * len(t), [], k=2, **kw))
     assert len("".join(out)) == 9
+
+
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float8_e4m3fn])
+def test_released_sequence_in_a_replayed_decoder(micro, kv):
+    """Released between replays: its length stays a step's, its rows have no page, and the live one
+    goes on to the end of the cache with pages that only it holds."""
+    from lollm_amd.qwen3_5 import SpecDecoder
+    model, mtp = micro[:2]
+    print(f"case released {kv}", flush=True)
+    d = SpecDecoder(model, mtp, 2, 96, k=3, page=16, kv_dtype=kv, n_pages=7)
+    d.prefill(torch.randint(0, 512, (2, 30), generator=torch.Generator().manual_seed(8)).cuda())
+    d.step()
+    d.capture()
+    d.cache.release(1)
+    with pytest.raises(RuntimeError, match="capacity"):
+        for _ in range(80):
+            d.replay()
+            assert int(d.cache.lengths[1]) <= 4 and (d.cache.table[1] == -1).all()
+    assert int(d.cache.lengths[0]) > 92 and d.cache.held == [6, 0]
