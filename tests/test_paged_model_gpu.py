@@ -146,3 +146,43 @@ def test_released_sequence_in_a_replayed_decoder(micro, kv):
             d.replay()
             assert int(d.cache.lengths[1]) <= 4 and (d.cache.table[1] == -1).all()
     assert int(d.cache.lengths[0]) > 92 and d.cache.held == [6, 0]
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_logits_over_8_bit_pages(micro, page, monkeypatch):
+    """A prompt, a token, a verify block and chunks over 8-bit pages, against the same forwards whose
+    attention is the oracle's in 64 bits over what the cache's pages and scales hold: at the model's
+    bf16 bar, which the same with K's scales and V's exchanged does not meet."""
+    from lollm_amd import ops
+    from paged_oracle import attention
+    model, _, (W, W16), cfg = micro
+    print(f"case logits over 8-bit pages of {page}", flush=True)
+    ids = torch.randint(0, cfg.vocab_size, (2, 110), generator=torch.Generator().manual_seed(9))
+    cache = model.new_cache(2, 128, page=page, kv_dtype=torch.float8_e4m3fn)
+    past = p16 = None
+    worst_exchanged = 0.0
+
+    def oracle(c, first, second):
+        def attn(q, k, v, table, kv_len, gate, **kw):
+            s = {n: x.cpu() for n, x in c.layers[ATTN].items()}
+            out, _ = attention(q.cpu(), s["k"], s["v"], c.table.cpu(), kv_len.cpu(), gate.cpu(), s[first], s[second])
+            return out.bfloat16().cuda()
+        return attn
+
+    for a, b in ((0, 41), (41, 42), (42, 46), (46, 62), (62, 109), (109, 110)):
+        x = ids[:, a:b].cuda()
+        copies = cache.clone(), cache.clone()
+        got, _ = model(x, cache)
+        want = []
+        for c, names in zip(copies, (("ks", "vs"), ("vs", "ks"))):
+            with monkeypatch.context() as m:
+                m.setattr(ops, "attn_paged", oracle(c, *names))
+                want.append(model(x, c)[0].float())
+        assert torch.equal(cache.layers[ATTN]["k"].view(torch.uint8), copies[0].layers[ATTN]["k"].view(torch.uint8))
+        ref, past = R.model_forward(W, cfg, ids[:, a:b], past)
+        r16, p16 = R.model_forward(W16, cfg, ids[:, a:b], p16)
+        bar = 2 * float((r16.float() - ref).abs().max()) + 1e-3 * float(ref.abs().max())
+        err = float((got.float() - want[0]).abs().max())
+        assert err <= bar, f"tokens {a} .. {b}: off by {err}, bar {bar}"
+        worst_exchanged = max(worst_exchanged, float((got.float() - want[1]).abs().max()) / bar)
+    assert worst_exchanged > 1, worst_exchanged
