@@ -311,8 +311,8 @@ def _gate_arg(gate, B, T, Hq, D, dev):
         row = seq if B > 1 else Hq * head
     p = gate.data_ptr()
     if one != 1 or (B > 1 and T > 1 and seq != T * row) or head < D or row < (Hq - 1) * head + D \
-            or row % 8 or head % 8 or p & 15:
-        raise ValueError("gate rows must be evenly strided, 16-byte aligned and not overlap")
+            or row % 8 or head % 8 or p & 15 or head > 0x7fffffff:
+        raise ValueError("gate rows must be evenly strided, 16-byte aligned and not overlap, heads within 2^31")
     return p, row, head
 
 

@@ -53,6 +53,20 @@ def test_attn_append_refuses(kw, rc):
     assert append(**kw) == rc
 
 
+def test_gate_strides():
+    """The stride of a head is 32 bits in the C call: a wider one is refused, not cut."""
+    from lollm_amd import ops
+
+    def gate(head):
+        return torch.empty(2 * head, dtype=torch.bfloat16, device="meta").as_strided((1, 1, 2, 256), (1, 1, head, 1))
+
+    for head in (256, 512, 2 ** 31 - 8):
+        assert ops._gate_arg(gate(head), 1, 1, 2, 256, -1) == (0, 2 * head, head)
+    for head in (2 ** 31, 2 ** 32 + 256, 128, 260):
+        with pytest.raises(ValueError):
+            ops._gate_arg(gate(head), 1, 1, 2, 256, -1)
+
+
 def test_workspace_bytes():
     f = _lib.lib().lollm_attn_paged_workspace_bytes
     # one fp32 piece of 32 x 256 values and 2 x 32 sums per workgroup and pair, 16 bytes a pair
