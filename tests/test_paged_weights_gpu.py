@@ -58,3 +58,44 @@ def check(keys, T, nats, at, grid):
 def test_light_keys_beside_a_heavy_one(keys, T, at, grid, nats):
     print(f"case heavy key {at} of {keys} by {nats} nats, T {T} grid {grid}", flush=True)
     check(keys, T, nats, at, grid)
+
+
+@pytest.mark.parametrize("P", [16, 64])
+@pytest.mark.parametrize("nats", [6, 13, 18])
+@pytest.mark.parametrize("keys,T,grid", [(3001, 2, 1), (3001, 2, 0), (733, 70, 0), (5003, 260, 0)])
+def test_random_keys_beside_a_heavy_one(keys, T, grid, nats, P):
+    """Normal scores and values in pages of different scales, and a first key of value 0 above them.
+    The tolerance is the kernel's published bound, term by term."""
+    from lollm_amd import ops
+    print(f"case first of {keys} keys by {nats} nats, T {T} grid {grid} page {P}", flush=True)
+    g = torch.Generator().manual_seed(keys + T + nats)
+    Hq, Hkv, n, f8 = 8, 2, -(-keys // P), torch.float8_e4m3fn
+    q = torch.randn(1, T, Hq, D, generator=g)
+    q[..., 0] = float(nats)
+    k, v = (torch.randn(n, Hkv, P, D, generator=g) for _ in range(2))
+    k[..., 0] = 0.0
+    k[0, :, 0] = 0.0
+    k[0, :, 0, 0] = 16.0
+    v[0, :, 0] = 0.0
+    q, k, v = q.bfloat16(), (k / 0.25).to(f8), (v * 16).to(f8)
+    ks = torch.full((n, Hkv), 0.25)
+    vs = torch.exp2(torch.randint(-6, -1, (n, Hkv), generator=g).float())
+    table = torch.arange(n, dtype=torch.int32)[None].contiguous()
+    lens = torch.tensor([keys], dtype=torch.int32)
+    got = ops.attn_paged(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lens.cuda(), k_scale=ks.cuda(), v_scale=vs.cuda(),
+                         grid=grid).double().cpu().view(T, Hq, D)
+    hidden = torch.arange(keys)[None] > torch.arange(keys - T, keys)[:, None]
+    worst = 0.0
+    for h in range(Hq):
+        kv = h // (Hq // Hkv)
+        kd = (k[:, kv].float().double() * 0.25).reshape(-1, D)[:keys]
+        vd = (v[:, kv].float().double() * vs[:, kv, None, None].double()).reshape(-1, D)[:keys]
+        qd = q[0, :, h].double()
+        p = torch.softmax((qd @ kd.T / 16).masked_fill(hidden, -math.inf), -1)
+        ds = 258 * 2.0 ** -24 * (qd.abs() @ kd.abs().T / 16).amax(-1, keepdim=True)
+        want = p @ vd
+        tol = ((2.0 ** -11 + 2 * ds + keys / 16 * 2.0 ** -24) * (p @ vd.abs())
+               + 2.0 ** -35 * p.amax(-1, keepdim=True) * ((~hidden).double() @ vd.abs())
+               + 2.0 ** -25 * float(vs[:, kv].max()) + (2.0 ** -8 + 2.0 ** -20) * want.abs())
+        worst = max(worst, float(((got[:, h] - want).abs() / tol).max()))
+    assert worst <= 1, worst
