@@ -24,9 +24,11 @@
 // Query heads: a workgroup per token and as many heads as its half-waves take at once where
 // tokens are few, up to 32 heads otherwise.
 //
-// What bounds it: memory for prompts (32 / 4 heads, us and TB/s: 3 x 1500 tokens into bf16 pages 31,
-// 5.9; 2 x 1999 28, 5.8; into 8-bit pages of 16 / 64 / 128 rows 31 / 33 / 37, 5.1 / 4.8 / 4.2, as the
-// rows that a workgroup holds take its registers), the launch for few tokens (4 to 5 us at 1 to 64).
+// What bounds it: memory for prompts (32 / 4 heads, three inputs in turn, us and TB/s: 3 x 1500 tokens
+// into bf16 pages 35, 5.3; 2 x 1999 32, 5.2; into 8-bit pages of 16 / 64 / 128 rows 34 / 39 / 43, 4.5 /
+// 4.0 / 3.6, as the rows that a workgroup holds take its registers; one input again and again, part of
+// it still in the chip's last cache, 31, 28 and 31 / 33 / 38), the launch for few tokens (4 to 5 us at
+// 1 to 64).
 #include "attn_common.h"
 
 namespace lollm {

@@ -24,9 +24,9 @@
 // Weights enter the product with V as hi + lo bf16 (attn_prefill.hip), with 8-bit V as fp16.
 //
 // What bounds it: the KV stream from some ten blocks a workgroup on, a fixed 12 us before.  16 x 4
-// tokens, 32 / 4 heads (us, TB/s of K and V): 128 keys 15.5 (8 bits 14.3), 1024 25.4, 2.6 (21.0,
-// 1.6), 4096 53, 5.0 (35, 3.9), 16384 180, 6.0 (93, 5.8), 65536 663, 6.5 (349, 6.1); pages of 16 to
-// 128 rows alike.  Of the fixed part the two launches are 5, lengths and table before the first
+// tokens, 32 / 4 heads, inputs in turn (us, TB/s of K and V): 128 keys 17 (8 bits 14.3), 1024 25.8, 2.6
+// (22.6, 1.5), 4096 56, 4.8 (36, 3.7), 16384 172, 6.2 (102, 5.3), 65536 638, 6.7 (350, 6.1); pages of 16
+// to 128 rows alike.  Of the fixed part the two launches are 5, lengths and table before the first
 // load 1.5, the last block's products 1.5, the merge of the waves 1.8.  8-bit blocks
 // are half the bytes: K is asked for two blocks ahead, of bf16 one, as a wave has at most 63 loads on
 // its way.

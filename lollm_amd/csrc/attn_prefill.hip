@@ -39,7 +39,8 @@
 // only, where they can two workgroups a CU: 256 registers a wave, for which bf16 pages leave four of
 // Q's 16 operands in LDS and have two sets of rows (80 KB), and O leaves through the sets.  2 x 1999
 // tokens: bf16 pages 223 us (588 TFLOP/s; one workgroup of 256 rows a CU 240, slabs that way 219), 8
-// bits 183 (717; 197).  1024 tokens over 9024 keys: 383 us (745; 433), 8 bits 317 (902; 412).  What
+// bits 189 (694; 183 and 197 while a row's reference had the weight 1, at_f16).  1024 tokens over 9024
+// keys: 383 us (745; 433), 8 bits 317 (901; 412).  What
 // bounds it is the instructions beside the products: 240 of the VALU and 80 of the scalar unit a
 // block and wave of 8-bit pages, half of the former conversions, beside 32 products of 32 cycles.
 // Where tiles are fewer than the chip holds, a tile's keys are dealt out to `parts` workgroups, whose
@@ -780,8 +781,8 @@ int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* p
   // Query tiles, whatever their number (us, tiles / split-K, bf16: 20 tiles of 2070 keys 35 / 38, of
   // 30000 134 / 308; 64 of 8256 123 / 220; 128 of 8289 203 / 418; but 32 of 256 28 / 20), but for few
   // tiles of 8-bit pages, whose codes a tile converts for 32 rows at a time as the split-K does,
-  // without its depth of loads: from 64 full tiles on (32 of 1128 42 / 31, of 4128 53 / 53; 64 of
-  // 1256 47 / 37, of 4256 72 / 79, of 16256 164 / 236; 128 of 512 46 / 42, of 8289 166 / 249).
+  // without its depth of loads: from 64 full tiles on (32 of 1128 33 / 32, of 4128 55 / 54; 64 of
+  // 1256 47 / 39, of 4256 71 / 81, of 16256 171 / 246; 128 of 512 49 / 44, of 8289 168 / 264).
   if (f8 && 4 * pairs * T * n_rep < 128LL * cus) return 0;
   int QB;
   const long long tiles = prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * pairs;
