@@ -73,21 +73,22 @@ __device__ __forceinline__ bf16x8 at_bf16(uint32_t w0, uint32_t w1, float scale)
   return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// The weights of 8-bit pages are fp16 (at_f16), whose steps end at 2^-24: a weight far below its row's
+// largest is held by that step and not by its own bits, while the row's sum counts it whole, and many
+// light keys beside a heavy one (a first token that every query looks at) would be lost from the
+// product alone.  So the row's reference has the weight 2^AT_F16_UP and moves where a block's maximum
+// passes it by more than AT_F16_LAG in the exponent (weights end at 2^15 of fp16's 65504): a weight is
+// off by at most 2^-11 of itself, or by 2^-25 / 2^AT_F16_UP of the row's largest.  What that costs is the
+// moves, of all of O each (us, UP, LAG 0, 15 / 8, 7 / 10, 5 / 12, 3: 2 x 1999 tokens 182 / 184 / 185 / 190,
+// 16 x 1 over 1000 .. 4000 keys 25.4 / 25.5 / 26.2 / 26.9).
+constexpr float AT_F16_UP = 10.f, AT_F16_LAG = 5.f;
+
 // Eight e4m3 codes as fp16, times a power of two of at most 2^7.  With 8-bit values the weights enter
 // their product as fp16, 11 bits of them, in one product, where bf16 values (whose range fp16 lacks)
 // take two of hi + lo bf16 weights.  So that no value leaves fp16's range, a tile of O counts in
 // units of a scale that it has met: codes enter times their page's scale over that (448 * 2^7 is
 // below 2^16), and O is rescaled where one comes that is more than 2^7 of it.  Scales are compared
 // and divided as the bits of powers of two; 0 is no scale (an unmapped page).
-// fp16's steps end at 2^-24, so a weight far below its row's largest is held by that step and not by
-// its own bits, while the row's sum counts it whole: many light keys beside a heavy one (a first
-// token that every query looks at) would be lost from the product alone.  So the row's reference has
-// the weight 2^AT_F16_UP and moves where a block's maximum passes it by more than AT_F16_LAG in the
-// exponent (weights end at 2^15 of fp16's 65504): a weight is off by at most 2^-11 of itself, or by
-// 2^-25 / 2^AT_F16_UP of the row's largest.  What that costs is the moves, of all of O each (us, UP, LAG
-// 0, 15 / 8, 7 / 10, 5 / 12, 3: 2 x 1999 tokens 182 / 184 / 185 / 190, 16 x 1 over 1000 .. 4000 keys 25.4 /
-// 25.5 / 26.2 / 26.9).
-constexpr float AT_F16_UP = 10.f, AT_F16_LAG = 5.f;
 __device__ __forceinline__ f16x8 at_f16(uint32_t w0, uint32_t w1, float ratio) {
   const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, ratio, false);
   const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, ratio, true);
