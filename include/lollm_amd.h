@@ -449,6 +449,28 @@ int lollm_gemm_rows(const void* A, long long lda, const void* Wt, void* C, long 
                     int N, int K, int epilogue, int tile, int splits, void* workspace,
                     long long workspace_bytes, void* stream);
 
+/* Products with 4-bit weights and group scales: W[n, k] = (c[n, k] - z[n, g]) s[n, g], g = k / group.
+ * Replaces: the same nn.Linear projections (src/qwen3_5/blocks.py:199-236,255-262,309-342) over a
+ * quantised weight.
+ *
+ *   codes   (N, K / 2) uint8   even k in the low half of a byte
+ *   scales  (N, K / group) bf16
+ *   zeros   (N, K / group) uint8, or NULL: 8 everywhere
+ * lollm_q4_quantize rounds a bf16 weight (N, K) to these (zeros given: 16 levels over the group's
+ * range, zero included; NULL: -8 .. 7 of max |w| / 7.5).  lollm_q4_pack re-lays them, once, in the order that
+ * lollm_gemm_q4 streams (epilogue 1: W = [gate; up], its rows interleaved 8 by 8), into
+ * lollm_q4_packed_bytes(N, K, group, zeros != NULL) bytes (-1: unsupported).  lollm_gemm_q4:
+ * C = A W^T, or with epilogue 1 silu(gate) * up (N / 2 columns), A (M, K) bf16, fp32 throughout,
+ * one rounding; any number of rows.  N a multiple of 64, K of 128, group 32, 64 or 128, lda of 8,
+ * ldc of 4; A and packed 16-byte aligned, C 8-byte. */
+long long lollm_q4_packed_bytes(int N, int K, int group, int zeros);
+int lollm_q4_quantize(const void* weight, void* codes, void* scales, void* zeros, int N, int K,
+                      int group, void* stream);
+int lollm_q4_pack(const void* codes, const void* scales, const void* zeros, void* packed, int N,
+                  int K, int group, int epilogue, void* stream);
+int lollm_gemm_q4(const void* A, long long lda, const void* packed, int zeros, void* C,
+                  long long ldc, int M, int N, int K, int group, int epilogue, void* stream);
+
 /* Greedy acceptance (temperature 0) without the verify logits: argmax (B, k + 1) int32
  * holds the argmax token of each verify row (lollm_gemm_argmax on the lm_head, same
  * token as lollm_gemm + the greedy sampler); n_accepted[b] = the number of leading drafts

@@ -502,6 +502,97 @@ def gemm_rows(x, tiled, N, K, epilogue, tile, splits=1):
     return out
 
 
+Q4_GROUPS = (32, 64, 128)
+
+
+class Q4Weight:
+    """A 4-bit weight as gemm_q4 streams it (q4_pack): N outputs of K inputs, scales (and zeros,
+    where it has them) of `group` inputs each."""
+
+    __slots__ = ("packed", "N", "K", "group", "zeros", "epilogue")
+
+    def __init__(self, packed, N, K, group, zeros, epilogue):
+        self.packed, self.N, self.K, self.group = packed, N, K, group
+        self.zeros, self.epilogue = zeros, epilogue
+
+    def nbytes(self):
+        return self.packed.numel()
+
+
+def q4_supported(N, K, group=128, epilogue=GEMM_NONE):
+    return gemm_supported(N, K, epilogue) and group in Q4_GROUPS
+
+
+def q4_quantize(weight, group=128, zeros=False):
+    """The (N, K) bf16 weight rounded to 4 bits: (codes (N, K / 2) uint8, even k in the low half of a
+    byte, scales (N, K / group) bf16, zeros (N, K / group) uint8 or None).  W ~ (code - zero) scale;
+    with zeros 16 levels over each group's range (0 among them), else -8 .. 7 of max |w| / 7.5.
+    Values must be finite."""
+    if weight.dim() != 2:
+        raise ValueError("weight must be (N, K)")
+    N, K = weight.shape
+    if not q4_supported(N, K, group):
+        raise ValueError(f"4-bit weights have N a multiple of 64, K of 128 and groups of {Q4_GROUPS}, got {N} x {K}, {group}")
+    dev = torch._C._cuda_getDevice()
+    w = _arg(weight, "weight", torch.bfloat16, (N, K), dev)
+    codes = torch.empty(N, K // 2, dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(N, K // group, dtype=torch.bfloat16, device=weight.device)
+    zero = torch.empty(N, K // group, dtype=torch.uint8, device=weight.device) if zeros else None
+    rc = _lib.lib().lollm_q4_quantize(w, _ptr(codes), _ptr(scales), _ptr(zero), N, K, group, _stream())
+    _lib.check(rc, "lollm_q4_quantize")
+    return codes, scales, zero
+
+
+def q4_pack(codes, scales, zeros=None, epilogue=GEMM_NONE):
+    """A Q4Weight of codes (N, K / 2) uint8, scales (N, K / group) bf16 and zeros (N, K / group)
+    uint8 (None: 8), as q4_quantize gives them.  GEMM_SWIGLU: the weight is [gate; up]."""
+    if codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0] or not scales.shape[1]:
+        raise ValueError("codes must be (N, K / 2) and scales (N, K / group)")
+    N, K = codes.shape[0], 2 * codes.shape[1]
+    group = K // scales.shape[1]
+    if group * scales.shape[1] != K or not q4_supported(N, K, group, epilogue):
+        raise ValueError(f"4-bit weights have N a multiple of 64, K of 128 and groups of {Q4_GROUPS}, got codes "
+                         f"{tuple(codes.shape)} and scales {tuple(scales.shape)}")
+    if epilogue not in (GEMM_NONE, GEMM_SWIGLU):
+        raise ValueError(f"unknown epilogue {epilogue}")
+    dev = torch._C._cuda_getDevice()
+    c = _arg(codes, "codes", torch.uint8, (N, K // 2), dev)
+    s = _arg(scales, "scales", torch.bfloat16, (N, K // group), dev)
+    z = None if zeros is None else _arg(zeros, "zeros", torch.uint8, (N, K // group), dev)
+    packed = torch.empty(_lib.lib().lollm_q4_packed_bytes(N, K, group, z is not None), dtype=torch.uint8,
+                         device=codes.device)
+    rc = _lib.lib().lollm_q4_pack(c, s, z, _ptr(packed), N, K, group, epilogue, _stream())
+    _lib.check(rc, "lollm_q4_pack")
+    return Q4Weight(packed, N, K, group, z is not None, epilogue)
+
+
+def gemm_q4(x, weight, out=None):
+    """y = x W^T for x (..., K) bf16 of any number of rows and a Q4Weight, in fp32 with one
+    rounding: (..., N) bf16, or (..., N / 2) = silu(gate) * up for a GEMM_SWIGLU weight."""
+    N, K = weight.N, weight.K
+    dev = torch._C._cuda_getDevice()
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"x is {tuple(x.shape)}, expected (..., {K})")
+    x = x.contiguous()
+    xp = _arg(x, "x", torch.bfloat16, x.shape, dev)
+    wp = _arg(weight.packed, "weight", torch.uint8, weight.packed.shape, dev)
+    oc = N // 2 if weight.epilogue else N
+    shape = (*x.shape[:-1], oc)
+    if out is None:
+        out = x.new_empty(shape)
+        o = out.data_ptr()
+    else:
+        o = _arg(out, "out", torch.bfloat16, shape, dev)
+    M = x.numel() // K
+    if M == 0:
+        return out
+    rc = _lib.lib().lollm_gemm_q4(xp, K, wp, weight.zeros, o, oc, M, N, K, weight.group, weight.epilogue,
+                                  torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, "lollm_gemm_q4")
+    return out
+
+
 def gemm_argmax(x, tiled, N, K, out=None, grid=0):
     """argmax over the N columns of each row of x W^T (bf16-rounded products, ties to the
     lowest column) without writing the logits (lollm_gemm_argmax).  x (M, K) bf16 with
