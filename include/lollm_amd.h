@@ -124,6 +124,30 @@ int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages, co
                      long long workspace_bytes, int B, int T, int Hq, int Hkv, int D, int grid,
                      float scale, void* stream);
 
+/* A tree of drafted tokens: T <= 64 nodes a sequence, each hanging on a node before it or on the
+ * committed context.  parents (B, T) int32: an entry outside [0, i) hangs node i on the context.
+ * mask (B, T) 64-bit words: bit j of node i's word is set for its ancestors and for itself.
+ * depth (B, T) int32 or NULL: ancestors of a node (its position is the context's length + depth).
+ * No counterpart in the reference, whose draft is a chain (mtp.py:141-155). */
+int lollm_tree_masks(const int32_t* parents, void* mask, int32_t* depth, int B, int T, void* stream);
+
+/* lollm_attn_verify and lollm_attn_paged for a tree of drafts: the T new positions are its nodes, node i
+ * in cache row kv_len[b] - T + i, and query i sees every key before them and, of the nodes up to
+ * itself, those whose bits its word in `tree` (B, T) has.  Values of all nodes must be finite (a
+ * weight of 0 meets them).  Workspaces: lollm_attn_workspace_bytes, and for pages
+ * lollm_attn_paged_tree_workspace_bytes.  T <= 64. */
+int lollm_attn_tree(const void* q, const void* k_cache, const void* v_cache, const int32_t* kv_len,
+                    const void* tree, const void* gate, void* out, void* workspace,
+                    long long workspace_bytes, int B, int T, int Hq, int Hkv, int D, int max_len,
+                    long long seq_stride, long long head_stride, int grid, float scale, void* stream);
+long long lollm_attn_paged_tree_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype, int grid);
+int lollm_attn_paged_tree(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
+                          const float* v_scale, int kv_dtype, const int32_t* table, long long table_stride,
+                          int table_width, int n_pages, int page, const int32_t* kv_len, const void* tree,
+                          const void* gate, long long gate_row, int gate_head, void* out, void* workspace,
+                          long long workspace_bytes, int B, int T, int Hq, int Hkv, int D, int grid,
+                          float scale, void* stream);
+
 /* Speculative-sampling acceptance over the full vocabulary for B sequences with k
  * drafts each, and the residual / bonus draw.
  *

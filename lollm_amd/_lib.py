@@ -36,6 +36,13 @@ SIGNATURES = {
     "lollm_attn_paged": ([_P, _P, _P, _P, _P, _I, _P, ctypes.c_longlong, _I, _I, _I, _P, _P,
                           ctypes.c_longlong, _I, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _I, _I, _F,
                           _P], _I),
+    "lollm_tree_masks": ([_P, _P, _P, _I, _I, _P], _I),
+    "lollm_attn_tree": ([_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _I,
+                         _I, ctypes.c_longlong, ctypes.c_longlong, _I, _F, _P], _I),
+    "lollm_attn_paged_tree_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _I], ctypes.c_longlong),
+    "lollm_attn_paged_tree": ([_P, _P, _P, _P, _P, _I, _P, ctypes.c_longlong, _I, _I, _I, _P, _P, _P,
+                               ctypes.c_longlong, _I, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _I, _I, _F,
+                               _P], _I),
     "lollm_attn_append": ([_P, _P, _P, _P, _P, _P, _I, _P, ctypes.c_longlong, _I, _I, _I, _I, _I, _I, _I,
                            _I, _I, _I, _F, _P, _P, _P, _P, _P, _P], _I),
     "lollm_spec_workspace_bytes": ([_I, _I, _I], ctypes.c_longlong),

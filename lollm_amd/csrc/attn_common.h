@@ -35,6 +35,7 @@ struct AttnArgs {
   // strides of gate in elements: of a token, of a head (Hq * D and D where it is dense)
   long long gate_row;
   int gate_head;
+  const uint64_t* tree;    // (B, T) or null: bit j of query i's word says that it sees new position j
 };
 
 struct PagedArgs {
@@ -119,6 +120,17 @@ __device__ __forceinline__ void at_store4(uint16_t* out, const float (&acc)[4], 
   *reinterpret_cast<uint2*>(out) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
 }
 
+// A tree of drafts: the T new positions are its nodes, and a query sees, of these, the ones whose bit
+// its word has (itself and its ancestors); the cache before them it sees whole.
+constexpr int AT_TREE_MAX = 64;   // nodes: bits of a word
+// Which of the 32 keys from node `first` on (negative: cache before the tree) a word lets through, of
+// those up to key `lim` of the 32 (negative: none); bit k for key k.
+__device__ __forceinline__ uint32_t at_tree_keys(uint64_t word, int first, int lim) {
+  const uint32_t w = first >= 0 ? (first < 64 ? (uint32_t)(word >> first) : 0u)
+                                : (first > -32 ? (uint32_t)(word << -first) | ((1u << -first) - 1u) : ~0u);
+  return lim < 0 ? 0u : w & (lim >= 31 ? ~0u : (2u << lim) - 1u);
+}
+
 constexpr int AW_WAVES = 4;
 constexpr int AW_THREADS = 64 * AW_WAVES;
 constexpr int AT_BLOCK = 128;        // keys per block
@@ -200,7 +212,7 @@ int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st, const Pag
                         int parts = 1);
 // For pages: workgroups of 128-row tiles that share a CU, or 0 for the split-K kernels, and the
 // workgroups that a tile's keys are dealt out to, with the bytes of workspace that takes.
-int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts);
+int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts, bool tree = false);
 long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts);
 
 }  // namespace lollm

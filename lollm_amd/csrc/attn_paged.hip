@@ -91,7 +91,7 @@ __device__ __forceinline__ void pg_read_rows(uint32_t at, u32x2_t (&v)[8]) {
 #undef RD
 }
 
-template <bool F8>
+template <bool F8, bool TREE>
 __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) {
   using Set = PagedSet<F8>;
   const AttnArgs& a = p.a;
@@ -248,6 +248,8 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   };
   // Row r of a pair is position r / n_rep of its query block, head r % n_rep; this thread's rows
   // tid / 32 + 8 i of Q, 16 bytes each.
+  const int lq = (int)(((uint32_t)l32 * p.rep_mul) >> 16);   // the lane's position in its query block
+  uint64_t word_next = 0, word = 0;   // TREE: the lane's query's, of the next pair and of this one
   uint32_t qoff[4];
   int qi[4];
 #pragma unroll
@@ -264,6 +266,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
     for (int i = 0; i < 4; ++i)
       qr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
                                               rs, qi[i] < QB ? qoff[i] : 0x80000000u, 0, 0));
+    if constexpr (TREE) word_next = a.tree[(size_t)X.b * a.T + q0 + min(lq, QB - 1)];
   };
 
   look_up();
@@ -286,7 +289,6 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   float m_ref = -INFINITY, l_s = 0.f;
   int v_ref = 0;          // 8 bits: O counts in units of this scale (bits), at_f16
   constexpr float LAG = F8 ? AT_F16_LAG : 16.f, UP = F8 ? AT_F16_UP : 0.f;
-  const int lq = (int)(((uint32_t)l32 * p.rep_mul) >> 16);   // the lane's position in its query block
   int qpos = 0, rows = 0;
 
   for (uint32_t ub = u0; ub < u1; ub += 2) {
@@ -301,6 +303,10 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       if (seg_first) {
         const int q0 = (C.ph % a.qblocks) * a.QB;
         qpos = C.L - a.T + q0 + lq;
+        if constexpr (TREE) {
+          word = word_next;
+          asm volatile("" : "+v"(word));   // (landed here, with Q)
+        }
         rows = a.n_rep * min(a.QB, a.T - q0);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt)
@@ -360,6 +366,15 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
         const int lim = min(C.L - 1, qpos) - kb;
         const int lim0 = C.page[0] >= 0 ? lim : -1, lim1 = C.page[1] >= 0 ? lim : -1;
         float bm = -INFINITY;
+        if (TREE && (C.j + 1) * AT_BLOCK > C.L - a.T) {
+          const uint32_t seen = at_tree_keys(word, kb - (C.L - a.T), lim);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool there = seen >> (8 * (r >> 2) + (r & 3)) & 1;
+            S[r] = there ? S[r] : -INFINITY;
+            S1[r] = there ? S1[r] : 0.f;
+          }
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int kk = 8 * (r >> 2) + (r & 3);
@@ -614,22 +629,32 @@ static long long paged_ws_bytes(int B, int T, int Hkv, int n_rep, int qblocks, i
   return n > 16 ? n : 16;
 }
 
-LOLLM_API long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype,
-                                                     int grid) {
+static long long paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype, int grid, bool tree) {
   int n_rep, QB, qblocks, parts = 1;
   if (attn_geometry(B, T, Hq, Hkv, D, 1, &n_rep, &QB, &qblocks)) return -1;
   const int nw = attn_grid(grid);
   if (nw <= 0 || nw > 1024 || (kv_dtype != LOLLM_BF16 && kv_dtype != LOLLM_F8)) return -1;
-  const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, kv_dtype == LOLLM_F8, &parts) : 0;
+  const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, kv_dtype == LOLLM_F8, &parts, tree) : 0;
   return paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts);
 }
 
-LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages,
-                               const float* k_scale, const float* v_scale, int kv_dtype,
-                               const int32_t* table, long long table_stride, int table_width, int n_pages,
-                               int page, const int32_t* kv_len, const void* gate, long long gate_row,
-                               int gate_head, void* out, void* workspace, long long workspace_bytes, int B,
-                               int T, int Hq, int Hkv, int D, int grid, float scale, void* stream) {
+LOLLM_API long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype,
+                                                     int grid) {
+  return paged_workspace_bytes(B, T, Hq, Hkv, D, kv_dtype, grid, false);
+}
+
+LOLLM_API long long lollm_attn_paged_tree_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype,
+                                                          int grid) {
+  return T > AT_TREE_MAX ? -1 : paged_workspace_bytes(B, T, Hq, Hkv, D, kv_dtype, grid, true);
+}
+
+// (tree: null for a chain)
+static int attn_paged_call(const void* q, const void* k_pages, const void* v_pages,
+                           const float* k_scale, const float* v_scale, int kv_dtype,
+                           const int32_t* table, long long table_stride, int table_width, int n_pages,
+                           int page, const int32_t* kv_len, const void* tree, const void* gate, long long gate_row,
+                           int gate_head, void* out, void* workspace, long long workspace_bytes, int B,
+                           int T, int Hq, int Hkv, int D, int grid, float scale, void* stream) {
   if (!q || !k_pages || !v_pages || !table || !kv_len || !out) return LOLLM_EINVAL;
   if (kv_dtype != LOLLM_BF16 && kv_dtype != LOLLM_F8) return LOLLM_EUNSUPPORTED;
   const bool f8 = kv_dtype == LOLLM_F8;
@@ -651,7 +676,7 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   const int nw = attn_grid(grid);
   if (nw <= 0 || nw > 1024) return LOLLM_EUNSUPPORTED;
   int parts = 1;
-  const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, f8, &parts) : 0;
+  const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, f8, &parts, tree != nullptr) : 0;
   if (!groups && pairs > 65535) return LOLLM_EUNSUPPORTED;                        // the combine's grid
   if (!groups && pairs * (rows / AT_BLOCK + 1) > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;   // 32-bit block numbers
   if (!workspace || workspace_bytes < paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts)) return LOLLM_EINVAL;
@@ -664,16 +689,40 @@ LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v
   a.max_len = (int)rows; a.nw = nw;
   a.cl2 = scale * 1.4426950408889634f;
   a.gate_row = gate_row; a.gate_head = gate_head;
+  a.tree = (const uint64_t*)tree;
   p.table = table; p.ks = k_scale; p.vs = v_scale; p.table_stride = table_stride;
   p.n_pages = n_pages; p.pshift = pshift;
   p.rep_mul = (uint32_t)((65536 + n_rep - 1) / n_rep);
   hipStream_t st = (hipStream_t)stream;
   if (groups) return attn_prefill_launch(a, groups, st, &p, parts);
-  if (f8)
-    hipLaunchKernelGGL(attn_paged_kernel<true>, dim3(nw), dim3(AW_THREADS), 0, st, p);
-  else
-    hipLaunchKernelGGL(attn_paged_kernel<false>, dim3(nw), dim3(AW_THREADS), 0, st, p);
+  auto* kernel = tree ? (f8 ? attn_paged_kernel<true, true> : attn_paged_kernel<false, true>)
+                      : (f8 ? attn_paged_kernel<true, false> : attn_paged_kernel<false, false>);
+  hipLaunchKernelGGL(kernel, dim3(nw), dim3(AW_THREADS), 0, st, p);
   if ((rc = launch_status())) return rc;
   hipLaunchKernelGGL(attn_paged_combine_kernel, dim3((n_rep * QB + 3) / 4, (unsigned)pairs), dim3(256), 0, st, p);
   return launch_status();
+}
+
+LOLLM_API int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages,
+                               const float* k_scale, const float* v_scale, int kv_dtype,
+                               const int32_t* table, long long table_stride, int table_width, int n_pages,
+                               int page, const int32_t* kv_len, const void* gate, long long gate_row,
+                               int gate_head, void* out, void* workspace, long long workspace_bytes, int B,
+                               int T, int Hq, int Hkv, int D, int grid, float scale, void* stream) {
+  return attn_paged_call(q, k_pages, v_pages, k_scale, v_scale, kv_dtype, table, table_stride, table_width, n_pages,
+                         page, kv_len, nullptr, gate, gate_row, gate_head, out, workspace, workspace_bytes, B, T, Hq,
+                         Hkv, D, grid, scale, stream);
+}
+
+LOLLM_API int lollm_attn_paged_tree(const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
+                                    const float* v_scale, int kv_dtype, const int32_t* table, long long table_stride,
+                                    int table_width, int n_pages, int page, const int32_t* kv_len, const void* tree,
+                                    const void* gate, long long gate_row, int gate_head, void* out, void* workspace,
+                                    long long workspace_bytes, int B, int T, int Hq, int Hkv, int D, int grid,
+                                    float scale, void* stream) {
+  if (!tree || (uintptr_t)tree % 8) return LOLLM_EINVAL;
+  if (T > AT_TREE_MAX) return LOLLM_EUNSUPPORTED;
+  return attn_paged_call(q, k_pages, v_pages, k_scale, v_scale, kv_dtype, table, table_stride, table_width, n_pages,
+                         page, kv_len, tree, gate, gate_row, gate_head, out, workspace, workspace_bytes, B, T, Hq, Hkv,
+                         D, grid, scale, stream);
 }

@@ -87,6 +87,7 @@ struct ApArgs {
   int gate_head, n_pages, pshift, parts;
   uint32_t rep_mul;        // ceil(2^16 / n_rep): r / n_rep = r * rep_mul >> 16 for r < 256
   float cl2;
+  const uint64_t* tree;    // TREE: (B, T) words of ancestors
 };
 
 // S += K Q^T with S in vector registers.  O of 64 rows takes all 256 accumulator registers,
@@ -113,7 +114,8 @@ __device__ __forceinline__ T ap_sload(const T* p, long long i) {
 
 // SETS: of K and V rows in LDS.  Two for bf16 pages where two workgroups share a CU (K two blocks
 // ahead, V one), else three.
-template <int RG, int KV, int SETS>
+// TREE: the new positions are the nodes of a tree of drafts, at_tree_keys.
+template <int RG, int KV, int SETS, bool TREE>
 __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1) void attn_prefill_kernel(ApArgs a) {
   constexpr bool F8 = KV == AP_PAGES8;
   constexpr int ROW = F8 ? AT_D : AT_D * 2;      // bytes of a key's row
@@ -261,12 +263,14 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
   unsigned char* const ql = qlate + (QL ? 1024 * QL * wave + 16 * lane : 0);
   // this lane's rows: position q0 + qi, query head kvh n_rep + hr
   int qpos[RG];
+  uint64_t word[RG];
   bf16x8 Q[RG][16];
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     const int r = 32 * (RG * wave + rg) + l32, qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
     const bool live = qi < QB;
     qpos[rg] = live ? p0 + qi : -1;
+    if constexpr (TREE) word[rg] = a.tree[(size_t)b * a.T + q0 + (live ? qi : 0)];
     const uint16_t* src = a.q + (((size_t)b * a.T + q0 + (live ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D;
 #pragma unroll
     for (int ks = 0; ks < 16; ++ks)   // (8 bits: a lane's 16 codes of K are two k-steps)
@@ -389,6 +393,14 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) ap_mfma_done(S[rg]);
     const int key0 = j * AP_KEYS;
+    if (TREE && key0 + AP_KEYS > L - a.T) {
+#pragma unroll
+      for (int rg = 0; rg < RG; ++rg) {
+        const uint32_t seen = at_tree_keys(word[rg], key0 + 4 * h - (L - a.T), qpos[rg] - key0 - 4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[rg][r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? S[rg][r] : -INFINITY;
+      }
+    }
     if (key0 + AP_KEYS - 1 > wmin || (KV != AP_ROWS && there != 3)) {   // acc r holds key 8 (r / 4) + 4 h + r % 4
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg) {
@@ -774,7 +786,7 @@ static int prefill_tiles(int B, int T, int Hkv, int n_rep, int rg, int* QB) {
   return (T + *QB - 1) / *QB;
 }
 
-int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts) {
+int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts, bool tree) {
   *parts = 1;
   if (T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS) return 0;
   const long long pairs = (long long)B * Hkv;
@@ -818,9 +830,9 @@ long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts) {
   return tiles * parts * AP_PIECE * (long long)sizeof(float) + tiles * 4;
 }
 
-template <int RG, int KV, int SETS>
+template <int RG, int KV, int SETS, bool TREE = false>
 static void prefill_start(const ApArgs& a, unsigned n, hipStream_t st) {
-  hipLaunchKernelGGL((attn_prefill_kernel<RG, KV, SETS>), dim3(n), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((attn_prefill_kernel<RG, KV, SETS, TREE>), dim3(n), dim3(256), 0, st, a);
 }
 
 int attn_prefill_launch(const AttnArgs& v, int groups, hipStream_t st, const PagedArgs* paged, int parts) {
@@ -840,7 +852,12 @@ int attn_prefill_launch(const AttnArgs& v, int groups, hipStream_t st, const Pag
     a.table = paged->table; a.ks = paged->ks; a.vs = paged->vs; a.table_stride = paged->table_stride;
     a.n_pages = paged->n_pages; a.pshift = paged->pshift;
   }
-  if (paged && paged->ks) prefill_start<1, AP_PAGES8, 3>(a, (unsigned)n, st);
+  a.tree = v.tree;
+  if (v.tree) {   // (tiles of 128 rows, one workgroup a CU: attn_paged_groups takes two from 256 tokens on)
+    if (paged && paged->ks) prefill_start<1, AP_PAGES8, 3, true>(a, (unsigned)n, st);
+    else if (paged) prefill_start<1, AP_PAGES, 3, true>(a, (unsigned)n, st);
+    else prefill_start<1, AP_ROWS, 3, true>(a, (unsigned)n, st);
+  } else if (paged && paged->ks) prefill_start<1, AP_PAGES8, 3>(a, (unsigned)n, st);
   else if (paged && groups == 2) prefill_start<1, AP_PAGES, 2>(a, (unsigned)n, st);
   else if (paged) prefill_start<1, AP_PAGES, 3>(a, (unsigned)n, st);
   else if (groups == 2) prefill_start<2, AP_ROWS, 3>(a, (unsigned)n, st);

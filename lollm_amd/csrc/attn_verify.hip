@@ -38,6 +38,9 @@
 //     maximum exceeds it by more than 16 in the exponent.
 // At the end of a pair the four waves' (m, l, O) are merged through the free LDS set
 // into the workgroup's piece.
+//
+// TREE: the new positions are the nodes of a tree of drafts; in the blocks that reach them a query's
+// word of ancestors (fetched with its Q) masks the keys beside the position.
 #include "attn_common.h"
 
 namespace lollm {
@@ -63,6 +66,7 @@ constexpr int AW_QROW = AT_D * 2 + 16;                // padded Q row in LDS
 constexpr int AW_OROW = AT_D / 2 + 4;                 // padded floats per row of an O half-dump
 static_assert(AW_WAVES * AT_ROWS * AW_OROW * 4 <= AW_VSET, "the O dump fits a V set");
 
+template <bool TREE>
 __global__ __launch_bounds__(AW_THREADS, 1) void attn_verify_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned char vs0[AW_VSET];   // V of even units
   __shared__ __attribute__((aligned(16))) unsigned char vs1[AW_VSET];   // V of odd units
@@ -146,6 +150,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_verify_kernel(AttnArgs a) 
   //      chunk t % 32), staged in LDS (padded rows) at the pair's first unit and read as
   //      the S MFMA B operand (lane: row l32, d chunk 2 ks + h)
   u32x4_t kr[16], qr[4];
+  uint64_t word_next = 0, word = 0;   // TREE: the lane's query's, of the next pair and of this one
   auto rsrc_of = [&](const uint16_t* cache, const AtCursor& X, bool live) {
     const int kvh = live ? X.ph / a.qblocks : 0;
     const uint32_t bytes = live ? (uint32_t)__builtin_amdgcn_readfirstlane(len[X.b]) * (AT_D * 2) : 0u;
@@ -181,6 +186,8 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_verify_kernel(AttnArgs a) 
                                     : 0x80000000u;
       qr[ii] = at_bload<0>(rs, qo, 0u);
     }
+    if constexpr (TREE)
+      if (load) word_next = a.tree[(size_t)X.b * a.T + q0_ + l32 % QB_];
   };
 
   AtCursor X1 = advance(C), X2 = advance(X1);
@@ -207,6 +214,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_verify_kernel(AttnArgs a) 
         L = __builtin_amdgcn_readfirstlane(len[b]);
         const int q0 = qb * a.QB, QB = min(a.QB, a.T - q0);
         qpos = L - a.T + q0 + l32 % QB;
+        word = word_next;
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
@@ -241,6 +249,11 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_verify_kernel(AttnArgs a) 
         const int kb = j * AT_BLOCK + AW_WKEYS * wave + 4 * h;
         const int lim = min(L - 1, qpos) - kb;
         float bm = -INFINITY;
+        if (TREE && (j + 1) * AT_BLOCK > L - a.T) {
+          const uint32_t seen = at_tree_keys(word, kb - (L - a.T), lim);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? S[r] : -INFINITY;
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int kk = 8 * (r >> 2) + (r & 3);
@@ -487,11 +500,12 @@ LOLLM_API long long lollm_attn_workspace_bytes(int B, int T, int Hq, int Hkv, in
   return attn_ws_bytes(nw, (long long)B * Hkv * qblocks);
 }
 
-LOLLM_API int lollm_attn_verify(const void* q, const void* k_cache, const void* v_cache,
-                                const int32_t* kv_len, const void* gate, void* out,
-                                void* workspace, long long workspace_bytes, int B, int T, int Hq,
-                                int Hkv, int D, int max_len, long long seq_stride,
-                                long long head_stride, int grid, float scale, void* stream) {
+// (tree: null for a chain)
+static int attn_verify_call(const void* q, const void* k_cache, const void* v_cache,
+                            const int32_t* kv_len, const void* tree, const void* gate, void* out,
+                            void* workspace, long long workspace_bytes, int B, int T, int Hq,
+                            int Hkv, int D, int max_len, long long seq_stride,
+                            long long head_stride, int grid, float scale, void* stream) {
   if (!q || !k_cache || !v_cache || !kv_len || !out) return LOLLM_EINVAL;
   int n_rep, QB, qblocks;
   int rc = attn_geometry(B, T, Hq, Hkv, D, max_len, &n_rep, &QB, &qblocks);
@@ -511,13 +525,35 @@ LOLLM_API int lollm_attn_verify(const void* q, const void* k_cache, const void* 
   a.max_len = max_len; a.nw = nw;
   a.cl2 = scale * 1.4426950408889634f;
   a.gate_row = (long long)Hq * D; a.gate_head = D;
+  a.tree = (const uint64_t*)tree;
   hipStream_t st = (hipStream_t)stream;
   if (grid == 0) {
     const int groups = attn_prefill_groups(B, T, Hkv, n_rep, nw);
-    if (groups) return attn_prefill_launch(a, groups, st);
+    // (a tree's rows are at most 64 n_rep of a sequence: its tiles have 128)
+    if (groups) return attn_prefill_launch(a, tree ? 1 : groups, st);
   }
-  hipLaunchKernelGGL(attn_verify_kernel, dim3(nw), dim3(AW_THREADS), 0, st, a);
+  if (tree) hipLaunchKernelGGL(attn_verify_kernel<true>, dim3(nw), dim3(AW_THREADS), 0, st, a);
+  else hipLaunchKernelGGL(attn_verify_kernel<false>, dim3(nw), dim3(AW_THREADS), 0, st, a);
   if ((rc = launch_status())) return rc;
   hipLaunchKernelGGL(attn_combine_kernel, dim3(AT_ROWS, B * Hkv * qblocks), dim3(256), 0, st, a);
   return launch_status();
+}
+
+LOLLM_API int lollm_attn_verify(const void* q, const void* k_cache, const void* v_cache,
+                                const int32_t* kv_len, const void* gate, void* out,
+                                void* workspace, long long workspace_bytes, int B, int T, int Hq,
+                                int Hkv, int D, int max_len, long long seq_stride,
+                                long long head_stride, int grid, float scale, void* stream) {
+  return attn_verify_call(q, k_cache, v_cache, kv_len, nullptr, gate, out, workspace, workspace_bytes, B, T, Hq, Hkv,
+                          D, max_len, seq_stride, head_stride, grid, scale, stream);
+}
+
+LOLLM_API int lollm_attn_tree(const void* q, const void* k_cache, const void* v_cache, const int32_t* kv_len,
+                              const void* tree, const void* gate, void* out, void* workspace,
+                              long long workspace_bytes, int B, int T, int Hq, int Hkv, int D, int max_len,
+                              long long seq_stride, long long head_stride, int grid, float scale, void* stream) {
+  if (!tree || (uintptr_t)tree % 8) return LOLLM_EINVAL;
+  if (T > AT_TREE_MAX) return LOLLM_EUNSUPPORTED;
+  return attn_verify_call(q, k_cache, v_cache, kv_len, tree, gate, out, workspace, workspace_bytes, B, T, Hq, Hkv, D,
+                          max_len, seq_stride, head_stride, grid, scale, stream);
 }

@@ -152,13 +152,44 @@ def attn_workspace_bytes(B, T, Hq, Hkv, D, max_len, grid=0):
     return n
 
 
+TREE_MAX = 64      # nodes of a tree of drafts
+
+
+def tree_masks(parents):
+    """A tree of drafts as the calls with tree= take it: (mask (B, T) int64, bit j of node i's word
+    for its ancestors and itself; depth (B, T) int32, its number of ancestors).  parents (B, T)
+    int32: the node before it that node i hangs on, -1 (or anything outside [0, i)) for the
+    committed context; T <= TREE_MAX."""
+    if parents.dim() != 2:
+        raise ValueError("parents must be (B, T)")
+    dev = torch._C._cuda_getDevice()
+    B, T = parents.shape
+    if B < 1 or not 1 <= T <= TREE_MAX:
+        raise ValueError(f"a tree has 1..{TREE_MAX} nodes, got parents {tuple(parents.shape)}")
+    p = _arg(parents, "parents", torch.int32, (B, T), dev)
+    mask = torch.empty(B, T, dtype=torch.int64, device=parents.device)
+    depth = torch.empty(B, T, dtype=torch.int32, device=parents.device)
+    rc = _lib.lib().lollm_tree_masks(p, _ptr(mask), _ptr(depth), B, T, _stream())
+    _lib.check(rc, "lollm_tree_masks")
+    return mask, depth
+
+
+def _tree_arg(tree, B, T, dev):
+    """The address of a tree's words (tree_masks) for (B, T) nodes."""
+    if T > TREE_MAX:
+        raise ValueError(f"a tree has at most {TREE_MAX} nodes, got {T}")
+    return _arg(tree, "tree", torch.int64, (B, T), dev)
+
+
 def attn_verify(q, k_cache, v_cache, kv_len, gate=None, *, grid=0, scale=None,
-                workspace=None, out=None):
+                workspace=None, out=None, tree=None):
     """q (B, T, Hq, D) bf16; k_cache / v_cache (B, Hkv, max_len, D) bf16 with the T
     new keys already written at positions kv_len-T .. kv_len-1; kv_len (B,) int32;
     gate (B, T, Hq*D) bf16 or None.  Returns (B, T, Hq*D) bf16.  The key blocks of
     all sequences are dealt out evenly to `grid` workgroups (0: one per CU, or for long calls
-    that fill the chip one workgroup per query tile)."""
+    that fill the chip one workgroup per query tile).  tree: (B, T) int64 of tree_masks, the T
+    positions are the nodes of a tree of drafts, each of which sees the keys before the tree, its
+    ancestors and itself (all nodes' values must be finite)."""
     B, T, Hq, D = q.shape
     _need(q, "q", torch.bfloat16)
     if k_cache.dim() != 4 or k_cache.shape[0] != B or k_cache.shape[3] != D:
@@ -179,6 +210,14 @@ def attn_verify(q, k_cache, v_cache, kv_len, gate=None, *, grid=0, scale=None,
     wbytes = workspace.numel() * workspace.element_size()
     if scale is None:
         scale = D ** -0.5
+    if tree is not None:
+        t = _tree_arg(tree, B, T, q.get_device())
+        rc = _lib.lib().lollm_attn_tree(
+            _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(kv_len), t, _ptr(gate), _ptr(out),
+            _ptr(workspace), wbytes, B, T, Hq, Hkv, D, max_len, Hkv * max_len * D, max_len * D,
+            grid, float(scale), _stream())
+        _lib.check(rc, "lollm_attn_tree")
+        return out
     rc = _lib.lib().lollm_attn_verify(
         _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(kv_len), _ptr(gate), _ptr(out),
         _ptr(workspace), wbytes, B, T, Hq, Hkv, D, max_len, Hkv * max_len * D, max_len * D,
@@ -281,15 +320,17 @@ def attn_append(qkv, q_norm_w, k_norm_w, inv_freq, lengths, table, k_pages, v_pa
     return q_out, qkv.as_strided((B, T, Hq, D), (T * width, width, 2 * D, 1), qkv.storage_offset() + D)
 
 
-def attn_paged_workspace_bytes(B, T, Hq, Hkv, D, dtype=torch.bfloat16, grid=0):
-    """Bytes of attn_paged's workspace over pages of `dtype`, for `grid` workgroups (0: one per CU)."""
+def attn_paged_workspace_bytes(B, T, Hq, Hkv, D, dtype=torch.bfloat16, grid=0, tree=False):
+    """Bytes of attn_paged's workspace over pages of `dtype`, for `grid` workgroups (0: one per CU)
+    and a call with or without a tree."""
     return _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, F8 if dtype is torch.float8_e4m3fn else BF16, grid,
-                                       torch._C._cuda_getDevice() if grid <= 0 else -1)
+                                       torch._C._cuda_getDevice() if grid <= 0 else -1, bool(tree))
 
 
 @functools.lru_cache(maxsize=4096)
-def _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, code, grid, device):
-    n = _lib.lib().lollm_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, code, grid)
+def _attn_paged_workspace_bytes(B, T, Hq, Hkv, D, code, grid, device, tree=False):
+    fn = "lollm_attn_paged_tree_workspace_bytes" if tree else "lollm_attn_paged_workspace_bytes"
+    n = getattr(_lib.lib(), fn)(B, T, Hq, Hkv, D, code, grid)
     if n < 0:
         raise ValueError("unsupported attention geometry")
     return n
@@ -317,11 +358,11 @@ def _gate_arg(gate, B, T, Hq, D, dev):
 
 
 def attn_paged(q, k_pages, v_pages, table, kv_len, gate=None, *, k_scale=None, v_scale=None, grid=0,
-               scale=None, workspace=None, out=None):
+               scale=None, workspace=None, out=None, tree=None):
     """attn_verify over a paged cache: q (B, T, Hq, D) bf16, keys and values in the pages that
     table (B, width) int32 names (as attn_append writes them; keys of unmapped pages do not
     exist), kv_len (B,) int32 with the T new ones included; gate (B, T, Hq, D) bf16, which may be
-    attn_append's view, or (B, T, Hq*D), or None.  Returns (B, T, Hq*D) bf16."""
+    attn_append's view, or (B, T, Hq*D), or None; tree as attn_verify's.  Returns (B, T, Hq*D) bf16."""
     if q.dim() != 4:
         raise ValueError("q must be (B, T, Hq, D)")
     dev = torch._C._cuda_getDevice()
@@ -333,18 +374,26 @@ def attn_paged(q, k_pages, v_pages, table, kv_len, gate=None, *, k_scale=None, v
     x = _arg(q, "q", torch.bfloat16, (B, T, Hq, D), dev)
     ln = _arg(kv_len, "kv_len", torch.int32, (B,), dev)
     g, row, head = _gate_arg(gate, B, T, Hq, D, dev) if gate is not None else (None, 0, 0)
+    words = None if tree is None else _tree_arg(tree, B, T, dev)
     if out is None:
         out = q.new_empty((B, T, Hq * D))
         o = out.data_ptr()
     else:
         o = _arg(out, "out", torch.bfloat16, (B, T, Hq * D), dev)
     if workspace is None:
-        wbytes = attn_paged_workspace_bytes(B, T, Hq, Hkv, D, k_pages.dtype, grid)
+        wbytes = attn_paged_workspace_bytes(B, T, Hq, Hkv, D, k_pages.dtype, grid, tree is not None)
         workspace = q.new_empty(wbytes, dtype=torch.uint8)
         ws = workspace.data_ptr()
     else:
         wbytes = workspace.numel() * workspace.element_size()
         ws = _arg(workspace, "workspace", workspace.dtype, workspace.shape, dev)
+    if tree is not None:
+        rc = _lib.lib().lollm_attn_paged_tree(
+            x, kp, vp, ks, vs, code, tab, stride, cols, n, page, ln, words, g, row, head, o, ws, wbytes, B, T, Hq,
+            Hkv, D, grid, D ** -0.5 if scale is None else scale, torch._C._cuda_getCurrentRawStream(dev))
+        if rc:
+            _lib.check(rc, "lollm_attn_paged_tree")
+        return out
     rc = _lib.lib().lollm_attn_paged(
         x, kp, vp, ks, vs, code, tab, stride, cols, n, page, ln, g, row, head, o, ws, wbytes, B, T, Hq, Hkv, D, grid,
         D ** -0.5 if scale is None else scale, torch._C._cuda_getCurrentRawStream(dev))
