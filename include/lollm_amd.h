@@ -473,6 +473,21 @@ int lollm_gemm_rows(const void* A, long long lda, const void* Wt, void* C, long 
                     int N, int K, int epilogue, int tile, int splits, void* workspace,
                     long long workspace_bytes, void* stream);
 
+/* lollm_gdn_layer over a tree of drafts (lollm_tree_masks): the T positions are its nodes, and node i's
+ * convolution and state continue from its parent's, from the committed ones where it has none.  Every
+ * node's record goes to the other half at the node's own slot and its input to the window's row K - 1
+ * + i, as a short call's; committing a path of the tree is moving its records and rows to the front
+ * (lollm_tree_keep) and then setting the indices as after a short call.  T <= 64, slots >= T, win_rows
+ * >= conv_kernel - 1 + T, conv_kernel 4, Dk == Dv == 128; the words' bits at and past the node itself
+ * count for nothing, and bits that are no tree's give numbers without meaning.  q, k and v are rounded
+ * to bf16 once, after the activation; beta and what follows stay fp32 to the output. */
+int lollm_gdn_layer_tree(const void* proj, long long proj_stride, const void* conv_w,
+                         const float* A_log, const float* dt_bias, const void* norm_w, void* win,
+                         const int32_t* conv_off, int win_rows, float* rec,
+                         const int32_t* rec_half, void* rep, const int32_t* replay, int slots,
+                         int fresh, const void* tree, void* out, int B, int T, int Hk, int Hv,
+                         int Dk, int Dv, int conv_kernel, float eps, void* stream);
+
 /* Products with 4-bit weights and group scales: W[n, k] = (c[n, k] - z[n, g]) s[n, g], g = k / group.
  * Replaces: the same nn.Linear projections (src/qwen3_5/blocks.py:199-236,255-262,309-342) over a
  * quantised weight.

@@ -1056,12 +1056,14 @@ def _check_gdn_state(rec, rec_half, rep, replay, B, Hv, D):
 
 
 def gdn_layer(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half, rep, replay,
-              fresh, B, T, Hk, Hv, D, conv_kernel, eps, out=None, chunked=None):
+              fresh, B, T, Hk, Hv, D, conv_kernel, eps, out=None, chunked=None, tree=None):
     """Fused GDN mixer (include/lollm_amd.h).  proj (B, T, P) bf16; win (B, 2W,
     conv_dim) bf16; rec (B, 2, Hv, D, D) fp32 state halves; rep (B, 2, Hv, S,
     gdn_record_bytes(D)) uint8 replay records; conv_off / rec_half / replay (B,) int32.
     chunked: None = the chunked kernels for long calls of at least GDN_CHUNK_MIN_T tokens
-    that they support, the recurrent kernel otherwise; True / False force one."""
+    that they support, the recurrent kernel otherwise; True / False force one.
+    tree: (B, T) int64 of tree_masks, the T positions are the nodes of a tree of drafts, each of which
+    continues from its parent (lollm_gdn_layer_tree: T <= TREE_MAX and S, the window's rows for it)."""
     P = proj.shape[-1]
     _need(proj, "proj", torch.bfloat16)
     _need(win, "win", torch.bfloat16)
@@ -1073,6 +1075,25 @@ def gdn_layer(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half
     if out is None:
         out = torch.empty(B, T, value_dim, dtype=torch.bfloat16, device=proj.device)
     W = win.shape[1] // 2
+    if tree is not None:
+        dev = torch._C._cuda_getDevice()
+        if T > S or conv_kernel - 1 + T > W or conv_kernel != 4:
+            raise ValueError(f"a tree of {T} nodes needs as many records ({S}) and {conv_kernel - 1 + T} window rows "
+                             f"({W}), and a convolution of 4 taps")
+        C, V = 2 * Hk * D + Hv * D, Hv * D
+        if P < C + V + 2 * Hv or P % 8 or min(B, T, Hk) < 1 or Hv % Hk:
+            raise ValueError(f"proj has rows of {P}, expected at least {C + V + 2 * Hv}, a multiple of 8")
+        words = _tree_arg(tree, B, T, dev)
+        rc = _lib.lib().lollm_gdn_layer_tree(
+            _arg(proj, "proj", torch.bfloat16, (B, T, P), dev), P,
+            _arg(conv_w, "conv_w", torch.bfloat16, (C, conv_kernel), dev), _arg(A_log, "A_log", torch.float32, (Hv,), dev),
+            _arg(dt_bias, "dt_bias", torch.float32, (Hv,), dev), _arg(norm_w, "norm_w", torch.bfloat16, (D,), dev),
+            _arg(win, "win", torch.bfloat16, (B, 2 * W, C), dev), _ptr(conv_off), W, _ptr(rec), _ptr(rec_half),
+            _ptr(rep), _ptr(replay), S, int(bool(fresh)), words, _arg(out, "out", torch.bfloat16, (B, T, V), dev), B, T,
+            Hk, Hv, D, D, conv_kernel, float(eps), torch._C._cuda_getCurrentRawStream(dev))
+        if rc:
+            _lib.check(rc, "lollm_gdn_layer_tree")
+        return out
     if chunked is None:
         chunked = T >= GDN_CHUNK_MIN_T and gdn_chunked_ok(T, S, W, conv_kernel, P)
     fn, ws = "lollm_gdn_layer_chunked" if chunked else "lollm_gdn_layer", ()
