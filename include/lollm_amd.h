@@ -131,6 +131,30 @@ int lollm_attn_paged(const void* q, const void* k_pages, const void* v_pages, co
  * No counterpart in the reference, whose draft is a chain (mtp.py:141-155). */
 int lollm_tree_masks(const int32_t* parents, void* mask, int32_t* depth, int B, int T, void* stream);
 
+/* The accepted path of a tree whose node 0 is the pending token: drawn (B, T) int32 is the token drawn
+ * (or the argmax) at each node, ids (B, T) int32 the nodes' own tokens.  From node 0 the walk goes on
+ * to the child, the lowest node of several, that is the token drawn at its parent, until there is
+ * none: sample-and-match as mtp.py:144-147, whose emitted tokens have the target's distribution
+ * whatever the tree.  path (B, T) int32: the accepted nodes in order, then -1; count (B) >= 1;
+ * next_token (B): drawn at the last of them. */
+int lollm_tree_accept(const int32_t* drawn, const int32_t* ids, const void* mask, int32_t* path,
+                      int32_t* count, int32_t* next_token, int B, int T, void* stream);
+
+/* Commit of a path (B, P) int32 of increasing nodes, count (B) of them: node path[i]'s row moves to
+ * row i of the tree's rows, in one layer's cache.  Nodes below their place or >= T are left where they are, as
+ * are rows without a page.  lollm_tree_keep_kv: bf16 K and V, the tree's rows from lengths[b] on, slabs
+ * (B, Hkv, max_len, D) with table NULL, or pages (n_pages, Hkv, page, D).  lollm_tree_keep_gdn: the
+ * records and window rows that lollm_gdn_layer_tree wrote; rec_half and conv_off are those of that
+ * call.  Afterwards rec_half ^= 1, replay = count, conv_off = the written window half's first row +
+ * count, lengths += count. */
+int lollm_tree_keep_kv(void* k, void* v, const int32_t* lengths, const int32_t* table,
+                       long long table_stride, int table_width, int n_pages, int page,
+                       const int32_t* path, const int32_t* count, int P, int B, int T, int Hkv, int D,
+                       int max_len, void* stream);
+int lollm_tree_keep_gdn(void* rep, void* win, const int32_t* rec_half, const int32_t* conv_off,
+                        const int32_t* path, const int32_t* count, int P, int B, int T, int Hv,
+                        int slots, int win_rows, int conv_dim, int conv_kernel, void* stream);
+
 /* lollm_attn_verify and lollm_attn_paged for a tree of drafts: the T new positions are its nodes, node i
  * in cache row kv_len[b] - T + i, and query i sees every key before them and, of the nodes up to
  * itself, those whose bits its word in `tree` (B, T) has.  Values of all nodes must be finite (a
@@ -477,7 +501,7 @@ int lollm_gemm_rows(const void* A, long long lda, const void* Wt, void* C, long 
  * convolution and state continue from its parent's, from the committed ones where it has none.  Every
  * node's record goes to the other half at the node's own slot and its input to the window's row K - 1
  * + i, as a short call's; committing a path of the tree is moving its records and rows to the front
- * (lollm_tree_keep) and then setting the indices as after a short call.  T <= 64, slots >= T, win_rows
+ * (lollm_tree_keep_gdn) and then setting the indices as after a short call.  T <= 64, slots >= T, win_rows
  * >= conv_kernel - 1 + T, conv_kernel 4, Dk == Dv == 128; the words' bits at and past the node itself
  * count for nothing, and bits that are no tree's give numbers without meaning.  q, k and v are rounded
  * to bf16 once, after the activation; beta and what follows stay fp32 to the output. */

@@ -37,6 +37,9 @@ SIGNATURES = {
                           ctypes.c_longlong, _I, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _I, _I, _F,
                           _P], _I),
     "lollm_tree_masks": ([_P, _P, _P, _I, _I, _P], _I),
+    "lollm_tree_accept": ([_P, _P, _P, _P, _P, _P, _I, _I, _P], _I),
+    "lollm_tree_keep_kv": ([_P, _P, _P, _P, ctypes.c_longlong, _I, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P], _I),
+    "lollm_tree_keep_gdn": ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P], _I),
     "lollm_attn_tree": ([_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _I,
                          _I, ctypes.c_longlong, ctypes.c_longlong, _I, _F, _P], _I),
     "lollm_attn_paged_tree_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _I], ctypes.c_longlong),

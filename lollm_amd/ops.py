@@ -174,6 +174,72 @@ def tree_masks(parents):
     return mask, depth
 
 
+def tree_accept(drawn, ids, tree):
+    """The accepted path of trees whose node 0 is the pending token (lollm_tree_accept): drawn (B, T)
+    int32, the token drawn at each node, ids (B, T) int32, the nodes' tokens, tree of tree_masks.
+    Returns (path (B, T) int32, the accepted nodes, then -1; count (B,) int32, at least 1; next_token
+    (B,) int32, drawn at the last of them)."""
+    if drawn.dim() != 2:
+        raise ValueError("drawn must be (B, T)")
+    dev = torch._C._cuda_getDevice()
+    B, T = drawn.shape
+    d = _arg(drawn, "drawn", torch.int32, (B, T), dev)
+    i = _arg(ids, "ids", torch.int32, (B, T), dev)
+    t = _tree_arg(tree, B, T, dev)
+    path, out = torch.empty_like(drawn), torch.empty(2, B, dtype=torch.int32, device=drawn.device)
+    rc = _lib.lib().lollm_tree_accept(d, i, t, _ptr(path), _ptr(out[0]), _ptr(out[1]), B, T, _stream())
+    _lib.check(rc, "lollm_tree_accept")
+    return path, out[0], out[1]
+
+
+def _path_args(path, count, B, dev):
+    if path.dim() != 2 or path.shape[0] != B or path.shape[1] < 1:
+        raise ValueError(f"path must be ({B}, nodes), got {tuple(path.shape)}")
+    if count.dtype != torch.int32 or count.shape != (B,) or not count.is_contiguous() or count.get_device() != dev:
+        raise ValueError(f"count must be ({B},) int32 on the current device, {dev}")
+    return _arg(path, "path", torch.int32, path.shape, dev), count.data_ptr(), path.shape[1]
+
+
+def tree_keep_kv(k, v, lengths, path, count, T, table=None):
+    """Rows of an accepted path to the front of the tree's T rows, in one layer's bf16 keys and values:
+    row lengths[b] + path[b, i] to lengths[b] + i for i < count[b] (path as tree_accept's).  k, v
+    (B, Hkv, max_len, D), or pages (n_pages, Hkv, page, D) with their table (B, width)."""
+    dev = torch._C._cuda_getDevice()
+    if k.dtype is not torch.bfloat16 or k.dim() != 4:
+        raise TypeError(f"keys and values must be 4-dimensional bf16, not {k.dtype} (8-bit rows share their page's scale)")
+    if not 1 <= T <= TREE_MAX:
+        raise ValueError(f"a tree has 1..{TREE_MAX} nodes, got {T}")
+    B = path.shape[0]
+    p, c, P = _path_args(path, count, B, dev)
+    ln = _arg(lengths, "lengths", torch.int32, (B,), dev)
+    if table is None:
+        kp, vp = _arg(k, "k", k.dtype, (B, *k.shape[1:]), dev), _arg(v, "v", k.dtype, k.shape, dev)
+        at, max_len = (None, 0, 0, 0, 0), k.shape[2]
+    else:
+        n, _, page, _, stride, cols, kp, vp, _, _, tab = _pages(k, v, None, None, table, B, dev)
+        at, max_len = (tab, stride, cols, n, page), 0
+    rc = _lib.lib().lollm_tree_keep_kv(kp, vp, ln, *at, p, c, P, B, T, k.shape[1], k.shape[3], max_len, _stream())
+    _lib.check(rc, "lollm_tree_keep_kv")
+
+
+def tree_keep_gdn(rep, win, rec_half, conv_off, path, count, T, conv_kernel):
+    """Records and window rows of an accepted path to the front, in what gdn_layer(tree=) wrote for T
+    nodes; rec_half and conv_off as in that call (path as tree_accept's)."""
+    dev = torch._C._cuda_getDevice()
+    if rep.dim() != 5 or rep.shape[4] != gdn_record_bytes(128) or win.dim() != 3 or win.shape[1] % 2:
+        raise ValueError(f"rep must be (B, 2, Hv, slots, {gdn_record_bytes(128)}) and win (B, 2 W, conv_dim)")
+    B, _, Hv, S, _ = rep.shape
+    W = win.shape[1] // 2
+    if not 1 <= T <= min(TREE_MAX, S, W - conv_kernel + 1):
+        raise ValueError(f"a tree of {T} nodes does not fit {S} records and {W} window rows")
+    p, c, P = _path_args(path, count, B, dev)
+    rc = _lib.lib().lollm_tree_keep_gdn(
+        _arg(rep, "rep", torch.uint8, (B, 2, Hv, S, rep.shape[4]), dev), _arg(win, "win", torch.bfloat16, (B, 2 * W, win.shape[2]), dev),
+        _arg(rec_half, "rec_half", torch.int32, (B,), dev), _arg(conv_off, "conv_off", torch.int32, (B,), dev), p, c, P, B,
+        T, Hv, S, W, win.shape[2], conv_kernel, _stream())
+    _lib.check(rc, "lollm_tree_keep_gdn")
+
+
 def _tree_arg(tree, B, T, dev):
     """The address of a tree's words (tree_masks) for (B, T) nodes."""
     if T > TREE_MAX:

@@ -153,6 +153,38 @@ class Projection:
         return norm(self(x), residual=residual)
 
 
+class Projection4:
+    """A Projection over a 4-bit weight with group scales (ops.gemm_q4), for any number of rows.
+    The bf16 weight is not kept."""
+
+    tiled = None        # (none for the callers that take the bf16 GEMM's fused forms)
+
+    def __init__(self, weight, epilogue=ops.GEMM_NONE, group=128, zeros=False):
+        codes, scales, zero = ops.q4_quantize(weight.to(torch.bfloat16).contiguous(), group, zeros)
+        self.q4 = ops.q4_pack(codes, scales, zero, epilogue)
+        self.N, self.K, self.epilogue = self.q4.N, self.q4.K, epilogue
+
+    def workspace_bytes(self, rows=ops.GEMM_MAX_ROWS):
+        return 0
+
+    def __call__(self, x):
+        return ops.gemm_q4(x, self.q4)
+
+    def add_norm(self, x, residual, norm):
+        """As Projection.add_norm: (norm(residual + x W^T), residual + x W^T)."""
+        if residual is None:
+            h = self(x)
+            return norm(h), h
+        return norm(self(x), residual=residual)
+
+
+def quantized(p, group=128, zeros=False):
+    """The 4-bit form of a Projection, or `p` itself where the shape has none (or it is 4-bit)."""
+    if isinstance(p, Projection4) or not ops.q4_supported(p.N, p.K, group, p.epilogue):
+        return p
+    return Projection4(p.weight, p.epilogue, group, zeros)
+
+
 _CUS = {}
 
 
@@ -189,6 +221,9 @@ class MLP:
     def projections(self):
         return [self.gate_up, self.down]
 
+    def quantize(self, group=128, zeros=False):
+        self.gate_up, self.down = (quantized(p, group, zeros) for p in self.projections())
+
     def __call__(self, x):
         return self.down(self.gate_up(x))
 
@@ -220,8 +255,11 @@ class GatedDeltaNet:
     def projections(self):
         return [self.in_proj, self.out_proj]
 
-    def core(self, x, cache, layer):
-        """Everything before out_proj (blocks.py:288-325)."""
+    def quantize(self, group=128, zeros=False):
+        self.in_proj, self.out_proj = (quantized(p, group, zeros) for p in self.projections())
+
+    def core(self, x, cache, layer, tree=None):
+        """Everything before out_proj (blocks.py:288-325); tree: the words of a tree of drafts."""
         B, T, _ = x.shape
         cfg = self.cfg
         proj = self.in_proj(x)
@@ -231,7 +269,7 @@ class GatedDeltaNet:
                              cache.fresh, B, T,
                              cfg.linear_num_key_heads, cfg.linear_num_value_heads,
                              cfg.linear_key_head_dim, cfg.linear_conv_kernel_dim,
-                             cfg.rms_norm_eps)
+                             cfg.rms_norm_eps, tree=tree)
 
     @property
     def out(self):
@@ -264,12 +302,15 @@ class GatedAttention:
     def projections(self):
         return [self.qkv, self.o_proj]
 
+    def quantize(self, group=128, zeros=False):
+        self.qkv, self.o_proj = (quantized(p, group, zeros) for p in self.projections())
+
     def core(self, x, k_cache, v_cache, lengths, kv_len, rope_pos=None, grid=0,
-             workspace=None, table=None, k_scale=None, v_scale=None):
+             workspace=None, table=None, k_scale=None, v_scale=None, tree=None):
         """Everything before o_proj (blocks.py:208-235).  rope_pos: None (RoPE at the cache
         rows), (B,) int32 start positions, or (B, T) int32 per-token positions.  table: the caches
         are pages that it names (ops.attn_append, ops.attn_paged), with their scales where they
-        hold 8 bits."""
+        hold 8 bits.  tree: the words of a tree of drafts (ops.tree_masks)."""
         B, T, _ = x.shape
         cfg = self.cfg
         qkv = self.qkv(x)
@@ -278,8 +319,8 @@ class GatedAttention:
                                       v_cache, cfg.num_attention_heads, cfg.rotary_dim, cfg.rms_norm_eps,
                                       k_scale=k_scale, v_scale=v_scale, rope_pos=rope_pos)
             return ops.attn_paged(q, k_cache, v_cache, table, kv_len, gate, k_scale=k_scale,
-                                  v_scale=v_scale, grid=grid, workspace=workspace)
-        if T == 1 and k_cache.shape[2] <= ops.ATTN_SMALL_MAXL:
+                                  v_scale=v_scale, grid=grid, workspace=workspace, tree=tree)
+        if T == 1 and tree is None and k_cache.shape[2] <= ops.ATTN_SMALL_MAXL:
             # one token over a short cache (the MTP head's draft block): prologue fused
             return ops.attn_small(qkv, self.q_norm, self.k_norm, self.inv_freq, lengths, kv_len, B,
                                   cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim,
@@ -289,7 +330,7 @@ class GatedAttention:
                                     cfg.num_attention_heads, cfg.num_key_value_heads,
                                     cfg.head_dim, cfg.rotary_dim, cfg.rms_norm_eps, k_cache,
                                     v_cache, rope_pos=rope_pos)
-        return ops.attn_verify(q, k_cache, v_cache, kv_len, gate, grid=grid, workspace=workspace)
+        return ops.attn_verify(q, k_cache, v_cache, kv_len, gate, grid=grid, workspace=workspace, tree=tree)
 
     @property
     def out(self):

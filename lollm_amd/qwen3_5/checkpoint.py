@@ -41,15 +41,18 @@ def read_checkpoint(path: str):
     return raw_config, weights
 
 
-def load_checkpoint(path: str, device="cuda", with_mtp=True, progress=None):
+def load_checkpoint(path: str, device="cuda", with_mtp=True, progress=None, weight_bits=16, group=128):
     """(model, mtp or None, unused tensor names).  The MTP head is built when asked for
     and the checkpoint carries `mtp.*` tensors; a missing or mis-shaped tensor raises
-    (hard-fail, as the reference's loaders do)."""
+    (hard-fail, as the reference's loaders do).  weight_bits, group: as `load`'s, the MTP head's
+    projections with them."""
     raw_config, weights = read_checkpoint(path)
     if raw_config.get("model_type") is None:
         raise ValueError("config.json has no 'model_type'; cannot route to a family")
-    model = load(raw_config, weights, "hf", device=device, progress=progress)
+    model = load(raw_config, weights, "hf", device=device, progress=progress, weight_bits=weight_bits, group=group)
     mtp = None
     if with_mtp and any(k.startswith("mtp.") for k in weights):
         mtp = load_mtp(model, weights, "hf", device=device)
+        if weight_bits == 4:
+            mtp.quantize(group)
     return model, mtp, sorted(weights)

@@ -67,6 +67,7 @@ class Qwen3_5Cache:
         self.replay = torch.zeros(batch, dtype=torch.int32, device=device)
         self.conv_off = torch.zeros(batch, dtype=torch.int32, device=device)
         self.last_T = 0
+        self.tree_T = 0                   # nodes of a tree that the last forward wrote, uncommitted
         # host-side upper bound of max(lengths): every forward or speculative step adds
         # its T, rollbacks leave it, so capacity is checked without reading the device
         self.len_bound = 0
@@ -111,6 +112,7 @@ class Qwen3_5Cache:
     def grew(self, T: int):
         """Record that a call may have added up to T tokens to every sequence."""
         self.len_bound += T
+        self.tree_T = 0                   # (an earlier tree's rows are no longer behind the tokens)
 
     # -- bookkeeping used by the model's forward -------------------------------------
     def commit_all(self, T: int):
@@ -132,10 +134,44 @@ class Qwen3_5Cache:
         T = self.last_T
         if T > self.spec_slots:
             raise RuntimeError("rollback needs the last forward to have written replay records")
+        self.tree_T = 0
         a = n_accepted.to(torch.int32).clamp(0, T - 1)
         self.lengths.sub_(T - 1 - a)
         self.replay.sub_(T - 1 - a)
         self.conv_off.sub_(T - 1 - a)
+
+    # -- a tree of drafts --------------------------------------------------------------
+    def tree_begins(self, T: int):
+        """Raise unless a forward over a tree of T nodes fits this cache."""
+        if not 1 <= T <= min(self.spec_slots, ops.TREE_MAX):
+            raise ValueError(f"a tree of {T} nodes needs a cache with spec_slots >= {T} (this one has "
+                             f"{self.spec_slots}) and at most {ops.TREE_MAX} nodes")
+        self.tree_T = 0
+
+    def tree_written(self, T: int):
+        """After a forward over a tree of T nodes, which commits nothing."""
+        self.tree_T = T
+
+    def keep_path(self, path: torch.Tensor, count: torch.Tensor):
+        """Commit a path of the tree that the last forward wrote: nodes path[b, :count[b]], increasing,
+        (B, P) and (B,) int32 as ops.tree_accept gives them, become the sequence's next tokens."""
+        T = self.tree_T
+        if not T:
+            raise RuntimeError("keep_path follows a forward over a tree")
+        W, K = self.win_rows, self.cfg.linear_conv_kernel_dim
+        for i, s in enumerate(self.layers):
+            if "rep" in s:
+                ops.tree_keep_gdn(s["rep"], s["win"], self.rec_half, self.conv_off, path, count, T, K)
+            else:
+                ops.tree_keep_kv(s["k"], s["v"], self.lengths, path, count, T, self.kv_args(i).get("table"))
+        n = count.clamp(0, min(T, path.shape[1]))
+        self.fresh = False
+        self.rec_half.bitwise_xor_(1)
+        self.replay.copy_(n)
+        self.conv_off.copy_(torch.where(self.conv_off >= W, 0, W) + n)
+        self.lengths.add_(n)
+        self.grew(min(T, path.shape[1]))
+        self.last_T = self.spec_slots + 1   # (not a call that a rollback shortens)
 
     # -- the reference cache API (kv.py:26-58) ---------------------------------------
     def _uniform_length(self) -> int:
@@ -190,6 +226,7 @@ class Qwen3_5Cache:
         records (the cache holds the same state afterwards)."""
         if self.fresh:
             return
+        self.tree_T = 0
         for s in self.layers:
             if s is not None and "rec" in s:
                 ops.gdn_state(s["rec"], self.rec_half, s["rep"], self.replay, to_other_half=True)
@@ -200,6 +237,7 @@ class Qwen3_5Cache:
         s = self.layers[layer]
         K = self.cfg.linear_conv_kernel_dim
         b = torch.arange(self.batch, device=self.device)
+        self.tree_T = 0
         self.settle()   # the other layers keep their states; this one's is replaced whole
         rows = self.conv_off[:, None].long() + torch.arange(K - 1, device=self.device)[None]
         s["win"][b[:, None], rows] = conv.transpose(1, 2).to(torch.bfloat16)
@@ -289,6 +327,7 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
 
     def grew(self, T: int):
         self._bounds = [n + T for n in self._bounds]
+        self.tree_T = 0
 
     def reserve(self, T: int):
         """Raise RuntimeError unless T more rows fit max_len and the pool; name their pages.  Goes
@@ -343,6 +382,12 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
         self.table.copy_(self._host_table)
 
     # -- the reference cache API -------------------------------------------------------
+    def tree_begins(self, T: int):
+        super().tree_begins(T)
+        if self.kv_dtype != torch.bfloat16:
+            raise ValueError("a tree of drafts takes bf16 pages: the rows of 8-bit pages share their page's scale and "
+                             "cannot be moved alone")
+
     def _rows(self, L):
         if not all(self.live):
             raise RuntimeError("a released sequence has no rows")

@@ -40,6 +40,12 @@ class DecoderLayer:
         self.mlp = MLP(W[p + "mlp.gate_proj.weight"], W[p + "mlp.up_proj.weight"],
                        W[p + "mlp.down_proj.weight"])
 
+    def quantize(self, group=128, zeros=False):
+        """The layer's projections in 4 bits (blocks.Projection4)."""
+        mixer = self.self_attn if self.layer_type == "full_attention" else self.linear_attn
+        mixer.quantize(group, zeros)
+        self.mlp.quantize(group, zeros)
+
 
 class _Embedding:
     def __init__(self, weight):
@@ -79,6 +85,14 @@ class Qwen3_5Model:
             out += mixer.projections() + layer.mlp.projections()
         return out
 
+    def quantize(self, group=128, zeros=False):
+        """The decoder layers' projections rounded to 4 bits with a scale (and with zeros=True a zero) for
+        every `group` inputs, 32, 64 or 128 (ops.q4_quantize); their bf16 weights are let go.  The embedding
+        and the lm_head stay bf16.  Before anything is captured in a graph.  Returns the model."""
+        for layer in self.model.layers:
+            layer.quantize(group, zeros)
+        return self
+
     # ---------------------------------------------------------------------------------
     def new_cache(self, batch, max_len, spec_slots=4, page=None, kv_dtype=None, n_pages=None):
         """A cache of `batch` sequences of up to max_len tokens: one slab per sequence, or, with
@@ -107,26 +121,35 @@ class Qwen3_5Model:
         return ws
 
     @torch.no_grad()
-    def forward(self, input_ids, past=None, return_hidden=False, logits="all"):
+    def forward(self, input_ids, past=None, return_hidden=False, logits="all", tree=None):
+        """tree: the T tokens are the nodes of a tree of drafts behind what the cache holds,
+        (mask, depth) of ops.tree_masks: each node's logits continue its own path.  Nothing is
+        committed: cache.keep_path does that for the accepted path, and without it the cache
+        holds what it held."""
         B, T = input_ids.shape
         cache = past if past is not None else self.new_cache(B, T + self.default_extra_capacity)
+        if tree is not None:
+            cache.tree_begins(T)
         cache.reserve(T)                  # raise before any KV row could land past max_len
-        x, normed = self.hidden_states(input_ids, cache)
+        x, normed = self.hidden_states(input_ids, cache, tree=tree)
         if logits == "last":
             out = self.lm_head(normed[:, -1:])
         else:
             out = self.lm_head(normed)
-        cache.commit_all(T)
+        if tree is not None:
+            cache.tree_written(T)
+        else:
+            cache.commit_all(T)
         return (out, cache, x) if return_hidden else (out, cache)
 
     __call__ = forward
 
-    def hidden_states(self, input_ids, cache, inputs=None):
+    def hidden_states(self, input_ids, cache, inputs=None, tree=None):
         """The decoder stack; returns (pre-norm hidden, final-normed hidden).  Writes
         the KV rows / GDN records of the T new tokens but does not commit them.  The
         caller has checked the capacity (cache.reserve(T)).  inputs: the block's
         (embedding rows, layer 0's input norm of them, lengths + T) when already formed
-        (lollm_verify_input), else they are formed here."""
+        (lollm_verify_input), else they are formed here.  tree: (mask, depth) of ops.tree_masks."""
         B, T = input_ids.shape
         cfg = self.cfg
         lengths = cache.lengths
@@ -142,9 +165,14 @@ class Qwen3_5Model:
               self.attn_workspace(B, T, cache.max_len, keep=T <= max(cache.spec_slots, 1)))
         # a call that can be rolled back (the verify block, as the GDN layers tell it) asks for
         # the split-K attention at any size, where a row's bits do not depend on T
-        grid = self.attn_grid or (_cus() if T <= cache.spec_slots else 0)
+        # (a tree's rows are committed or not as a whole: it takes the form that is fastest for it)
+        grid = self.attn_grid or (_cus() if T <= cache.spec_slots and tree is None else 0)
         # each residual-stream projection (o_proj / out_proj / down_proj) is issued with
         # the residual add and the norm that follows it (modeling_qwen3_5.py:59-60)
+        words, rope = None, {}
+        if tree is not None:
+            words, depth = tree
+            rope = {"rope_pos": lengths[:, None] + depth, "tree": words}
         pending = None   # (down_proj, its input): opens the next layer
         for i, layer in enumerate(self.model.layers):
             if pending is None:
@@ -155,10 +183,10 @@ class Qwen3_5Model:
                 s = cache.layers[i]
                 mixer = layer.self_attn
                 core = mixer.core(h_in, s["k"], s["v"], lengths, kv_len,
-                                  grid=grid, workspace=ws, **cache.kv_args(i))
+                                  grid=grid, workspace=ws, **cache.kv_args(i), **rope)
             else:
                 mixer = layer.linear_attn
-                core = mixer.core(h_in, cache, i)
+                core = mixer.core(h_in, cache, i, words)
             y, x = mixer.out.add_norm(core, x, layer.post_attention_layernorm)
             pending = (layer.mlp.down, layer.mlp.gate_up(y))
         normed, x = pending[0].add_norm(pending[1], x, self.model.norm)

@@ -27,7 +27,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
-from .blocks import Projection, RMSNorm
+from .blocks import Projection, RMSNorm, quantized
 from .kv import capturing
 from .modeling_qwen3_5 import DecoderLayer, Qwen3_5Model
 from .random_init import weight_shapes
@@ -48,6 +48,12 @@ class MTP:
         ops.gemm_workspace(max(p.workspace_bytes() for p in
                                [self.fc] + layer.self_attn.projections() + layer.mlp.projections()),
                            model.device)
+
+    def quantize(self, group=128, zeros=False):
+        """fc and the layer's projections in 4 bits, as Qwen3_5Model.quantize.  Returns the head."""
+        self.fc = quantized(self.fc, group, zeros)
+        self.layers[0].quantize(group, zeros)
+        return self
 
     def _block(self, hidden, k_cache, v_cache, lengths, kv_len, rope_pos, ws, tok=None,
                fc_in=None):

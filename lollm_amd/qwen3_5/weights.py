@@ -51,7 +51,11 @@ def take_weights(cfg, weights: dict, names, device, dtype, progress=None, who="q
 
 
 def load(raw_config: dict, weights: dict, fmt: str, device="cuda", dtype=None,
-         progress=None) -> Qwen3_5Model:
+         progress=None, weight_bits=16, group=128) -> Qwen3_5Model:
+    """weight_bits=4: the decoder layers' projections rounded to 4 bits with a scale for every `group`
+    inputs (Qwen3_5Model.quantize)."""
+    if weight_bits not in (4, 16):
+        raise ValueError(f"weights are held in 16 or 4 bits, not {weight_bits}")
     cfg = build_config(raw_config, fmt)
     dev = torch.device(device)
     if dev.type != "cuda":
@@ -66,4 +70,5 @@ def load(raw_config: dict, weights: dict, fmt: str, device="cuda", dtype=None,
     W = take_weights(cfg, weights, names, dev, dtype, progress)
     if tied:
         W["lm_head.weight"] = W["model.embed_tokens.weight"]
-    return Qwen3_5Model(cfg, W, dev)
+    model = Qwen3_5Model(cfg, W, dev)
+    return model.quantize(group) if weight_bits == 4 else model
