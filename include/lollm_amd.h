@@ -524,15 +524,19 @@ int lollm_gdn_layer_tree(const void* proj, long long proj_stride, const void* co
  * lollm_gemm_q4 streams (epilogue 1: W = [gate; up], its rows interleaved 8 by 8), into
  * lollm_q4_packed_bytes(N, K, group, zeros != NULL) bytes (-1: unsupported).  lollm_gemm_q4:
  * C = A W^T, or with epilogue 1 silu(gate) * up (N / 2 columns), A (M, K) bf16, fp32 throughout,
- * one rounding; any number of rows.  N a multiple of 64, K of 128, group 32, 64 or 128, lda of 8,
- * ldc of 4; A and packed 16-byte aligned, C 8-byte. */
+ * one rounding; any number of rows (workspace: lollm_gemm_q4_workspace_bytes, 0 for few rows, 16-byte
+ * aligned, used only within the call).  A row's bits depend on no other row, nor up to 64 rows on
+ * M; an infinity in A makes its row NaN.  N a multiple of 64, K of 128, group 32, 64 or 128, lda of
+ * 8, ldc of 4; A and packed 16-byte aligned, C 8-byte. */
 long long lollm_q4_packed_bytes(int N, int K, int group, int zeros);
 int lollm_q4_quantize(const void* weight, void* codes, void* scales, void* zeros, int N, int K,
                       int group, void* stream);
 int lollm_q4_pack(const void* codes, const void* scales, const void* zeros, void* packed, int N,
                   int K, int group, int epilogue, void* stream);
+long long lollm_gemm_q4_workspace_bytes(int M, int N, int K, int group);
 int lollm_gemm_q4(const void* A, long long lda, const void* packed, int zeros, void* C,
-                  long long ldc, int M, int N, int K, int group, int epilogue, void* stream);
+                  long long ldc, void* workspace, long long workspace_bytes, int M, int N, int K,
+                  int group, int epilogue, void* stream);
 
 /* Greedy acceptance (temperature 0) without the verify logits: argmax (B, k + 1) int32
  * holds the argmax token of each verify row (lollm_gemm_argmax on the lm_head, same

@@ -92,7 +92,9 @@ SIGNATURES = {
     "lollm_q4_packed_bytes": ([_I, _I, _I, _I], ctypes.c_longlong),
     "lollm_q4_quantize": ([_P, _P, _P, _P, _I, _I, _I, _P], _I),
     "lollm_q4_pack": ([_P, _P, _P, _P, _I, _I, _I, _I, _P], _I),
-    "lollm_gemm_q4": ([_P, ctypes.c_longlong, _P, _I, _P, ctypes.c_longlong, _I, _I, _I, _I, _I, _P], _I),
+    "lollm_gemm_q4_workspace_bytes": ([_I, _I, _I, _I], ctypes.c_longlong),
+    "lollm_gemm_q4": ([_P, ctypes.c_longlong, _P, _I, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _I, _I, _I, _I,
+                       _I, _P], _I),
     "lollm_gemm_rowmax_slots": ([_I], _I),
     "lollm_gemm_logits": ([_P, ctypes.c_longlong, _P, _I, _I, _I, _P, ctypes.c_longlong, _P,
                            ctypes.c_longlong, _P, _I, _P, _I, _I, _I, _F, _P, ctypes.c_longlong,

@@ -681,9 +681,19 @@ def q4_pack(codes, scales, zeros=None, epilogue=GEMM_NONE):
     return Q4Weight(packed, N, K, group, z is not None, epilogue)
 
 
+@functools.lru_cache(maxsize=4096)
+def _q4_workspace_bytes(M, N, K, group, device):
+    n = _lib.lib().lollm_gemm_q4_workspace_bytes(M, N, K, group)
+    if n < 0:
+        raise ValueError(f"unsupported 4-bit product {M} x {N} x {K}, groups of {group}")
+    return n
+
+
 def gemm_q4(x, weight, out=None):
     """y = x W^T for x (..., K) bf16 of any number of rows and a Q4Weight, in fp32 with one
-    rounding: (..., N) bf16, or (..., N / 2) = silu(gate) * up for a GEMM_SWIGLU weight."""
+    rounding: (..., N) bf16, or (..., N / 2) = silu(gate) * up for a GEMM_SWIGLU weight.  A row's
+    bits depend on no other row, and up to 64 rows not on their number (beyond, sizes choose
+    between two orders of the sums).  An infinite x makes its row NaN."""
     N, K = weight.N, weight.K
     dev = torch._C._cuda_getDevice()
     if x.dim() < 1 or x.shape[-1] != K:
@@ -701,7 +711,9 @@ def gemm_q4(x, weight, out=None):
     M = x.numel() // K
     if M == 0:
         return out
-    rc = _lib.lib().lollm_gemm_q4(xp, K, wp, weight.zeros, o, oc, M, N, K, weight.group, weight.epilogue,
+    need = _q4_workspace_bytes(M, N, K, weight.group, dev)
+    ws = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
+    rc = _lib.lib().lollm_gemm_q4(xp, K, wp, weight.zeros, o, oc, ws, need, M, N, K, weight.group, weight.epilogue,
                                   torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, "lollm_gemm_q4")

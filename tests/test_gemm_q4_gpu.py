@@ -103,6 +103,70 @@ def test_gemm_q4_at_the_models_sizes(M, N, K, group, swiglu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("swiglu", (False, True))
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("group", (32, 64, 128))
+def test_gemm_q4_with_many_rows(group, zeros, swiglu):
+    """The form for many rows, chosen by sizes: tiles that end inside (one row, 64 columns), one to nine
+    stages of K, a workspace that the call asks for; the whole sum's room as for few rows, the product over
+    the groups' three-part sums within it."""
+    from lollm_amd import ops
+    N = 6208
+    for M, K in ((513, 1152), (640, 128), (900, 256), (1000, 640)):
+        print(f"case q4 many rows {M} x {N} x {K} group {group} zeros {zeros} swiglu {swiglu}", flush=True)
+        assert ops._q4_workspace_bytes(M, N, K, group, torch.cuda.current_device()) > 0
+        code, scale, zero = weight(N, K, group, zeros, M + K)
+        w = values(code, scale, zero, group).cuda()
+        packed = ops.q4_pack(bytes_of(code).cuda(), scale.cuda(), None if zero is None else zero.cuda(),
+                             ops.GEMM_SWIGLU if swiglu else ops.GEMM_NONE)
+        g = torch.Generator().manual_seed(K)
+        x = (torch.randn(M, 2 * K, generator=g) * torch.where(torch.rand(2 * K, generator=g) < 0.01, 16.0, 1.0)).bfloat16()
+        x = x.cuda()[:, K:]
+        buf = torch.full((M + 1, N // 2 if swiglu else N), 7.0, dtype=torch.bfloat16, device="cuda")
+        got = ops.gemm_q4(x, packed, out=buf[:M])
+        ref, _ = expected(x, w, swiglu)
+        room = (x.double().abs().reshape(M, K // group, group).sum(-1) @ scale.cuda().double().t()) * 32 * 2 ** -18
+        if swiglu:
+            gate, up = (x.double() @ w.t()).chunk(2, -1)
+            rg, ru = room.chunk(2, -1)
+            room = 1.1 * rg * up.abs() + gate.abs() * ru
+        assert ((got.double() - ref).abs() <= ref.abs() * 2 ** -8 + room).all()
+        assert (buf[M:] == 7.0).all() and torch.equal(ops.gemm_q4(x, packed), got)
+
+
+@pytest.mark.gpu
+def test_gemm_q4_many_rows_captured_and_refused_without_a_workspace():
+    from lollm_amd import _lib, ops
+    M, N, K, group = 513, 6208, 256, 128
+    code, scale, _ = weight(N, K, group, False, 6)
+    packed = ops.q4_pack(bytes_of(code).cuda(), scale.cuda())
+    xs = [torch.randn(M, K, generator=torch.Generator().manual_seed(i)).bfloat16().cuda() for i in range(2)]
+    want = [ops.gemm_q4(x, packed).clone() for x in xs]
+    need = _lib.lib().lollm_gemm_q4_workspace_bytes(M, N, K, group)
+    assert need == 6 * M * 32
+    out = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for at, size in ((None, need), (ws.data_ptr(), need - 1), (ws.data_ptr() + 8, need)):
+        assert _lib.lib().lollm_gemm_q4(xs[0].data_ptr(), K, packed.packed.data_ptr(), 0, out.data_ptr(), N, at, size, M, N, K,
+                                        group, 0, None) == 1
+    torch.cuda.synchronize()
+    assert not out.any()
+    buf = xs[0].clone()
+    graphs = []
+    for _ in range(2):      # two graphs, each with its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.gemm_q4(buf, packed)
+        graphs.append((graph, y))
+    for turn in range(4):
+        buf.copy_(xs[turn % 2])
+        for graph, y in graphs:
+            graph.replay()
+            assert torch.equal(y, want[turn % 2])
+        ops.gemm_q4(xs[1 - turn % 2], packed)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("zeros", (False, True))
 def test_gemm_q4_rows_do_not_depend_on_each_other(zeros):
     """A row's bits are the same in calls of any number of rows, and over calls."""
@@ -230,13 +294,13 @@ def test_q4_entry_points_check_before_any_launch():
     for shape in ((60, 256, 128), (64, 200, 128), (64, 256, 16), (0, 256, 32), (64, -128, 32)):
         assert L.lollm_q4_packed_bytes(*shape, 0) == -1
     p = 4096     # an address that no check reads
-    assert L.lollm_gemm_q4(None, 256, p, 0, p, 64, 1, 64, 256, 128, 0, None) == 1
-    assert L.lollm_gemm_q4(p, 256, p, 0, p, 64, 0, 64, 256, 128, 0, None) == 1
-    assert L.lollm_gemm_q4(p, 256, p, 0, p, 64, 1, 64, 256, 96, 0, None) == 2
-    assert L.lollm_gemm_q4(p, 248, p, 0, p, 64, 1, 64, 256, 128, 0, None) == 1
-    assert L.lollm_gemm_q4(p, 256, p, 0, p, 60, 1, 64, 256, 128, 0, None) == 1
-    assert L.lollm_gemm_q4(p, 256, p, 0, p, 64, 1, 64, 256, 128, 2, None) == 1
-    assert L.lollm_gemm_q4(p + 8, 256, p, 0, p, 64, 1, 64, 256, 128, 0, None) == 1
+    assert L.lollm_gemm_q4(None, 256, p, 0, p, 64, None, 0, 1, 64, 256, 128, 0, None) == 1
+    assert L.lollm_gemm_q4(p, 256, p, 0, p, 64, None, 0, 0, 64, 256, 128, 0, None) == 1
+    assert L.lollm_gemm_q4(p, 256, p, 0, p, 64, None, 0, 1, 64, 256, 96, 0, None) == 2
+    assert L.lollm_gemm_q4(p, 248, p, 0, p, 64, None, 0, 1, 64, 256, 128, 0, None) == 1
+    assert L.lollm_gemm_q4(p, 256, p, 0, p, 60, None, 0, 1, 64, 256, 128, 0, None) == 1
+    assert L.lollm_gemm_q4(p, 256, p, 0, p, 64, None, 0, 1, 64, 256, 128, 2, None) == 1
+    assert L.lollm_gemm_q4(p + 8, 256, p, 0, p, 64, None, 0, 1, 64, 256, 128, 0, None) == 1
     assert L.lollm_q4_pack(p, None, None, p, 64, 256, 128, 0, None) == 1
     assert L.lollm_q4_pack(p, p, None, p + 4, 64, 256, 128, 0, None) == 1
     assert L.lollm_q4_quantize(None, p, p, None, 64, 256, 128, None) == 1
