@@ -63,6 +63,7 @@ constexpr int AP_FEW_ROWS = 64;                // tokens of a call that keeps th
 constexpr int AP_KEYS = 32;                    // keys per block
 constexpr int AP_AHEAD = 3;                    // operands read ahead of their products
 constexpr int AP_PART_BLOCKS = 8;              // blocks of a part of a tile's keys at least
+constexpr int AP_TREE_BLOCKS = 3;              // trees, few tiles for the chip: 500 keys of 1 x 16 nodes 22 us, at 8 blocks 41
 constexpr int AP_MAX_PARTS = 64;
 constexpr int AP_PIECE = 2 * 128 + 128 * AT_D; // floats: maxima, sums and O of a part of a 128-row tile
 
@@ -112,6 +113,46 @@ __device__ __forceinline__ T ap_sload(const T* p, long long i) {
   return ((const __attribute__((address_space(4))) T*)p)[i];
 }
 
+// Trees over pages: the workgroups of a (query tile, KV head), a.parts a sequence on average, go to sequences by
+// their lengths (one to each first), as trees come over contexts of any lengths and a call has few tiles: the
+// parts of 4 sequences of 1000 to 30000 keys are then alike within a few per cent, where equal numbers let the
+// longest take twice the mean.
+constexpr int AP_TILE_PARTS = 8;   // bits of a tile's number of parts, before its first one's place
+__device__ __forceinline__ int ap_tree_blocks(const ApArgs& a, int b) {
+  return b < a.B ? (min(max(a.kv_len[b], 0), a.max_len) + AP_KEYS - 1) / AP_KEYS : 0;
+}
+struct ApShare { int b, part, parts; };   // b < 0: a spare one
+__device__ __forceinline__ ApShare ap_tree_share(const ApArgs& a, int s, int lane) {
+  uint64_t total = 0;   // (64 sequences' blocks fit 32 bits)
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    uint32_t n = (uint32_t)ap_tree_blocks(a, b0 + lane);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    total += n;
+  }
+  const int more = a.B * (a.parts - 1);
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const uint64_t n = (uint64_t)ap_tree_blocks(a, b0 + lane) * (uint32_t)more;
+    // (the quotient in 64 bits is never rounded up to a whole number: both are below 2^53 / 2^10)
+    const int mine = b0 + lane >= a.B ? 0 : min(1 + (total ? (int)((double)n / (double)total) : 0), AP_MAX_PARTS);
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += t;
+    }
+    const uint64_t m = __ballot(s < before + upto);
+    if (m) {
+      const int l = __builtin_ctzll(m);
+      const int p = __builtin_amdgcn_readlane(mine, l);
+      return {b0 + l, s - before - __builtin_amdgcn_readlane(upto, l) + p, p};
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {-1, 0, 1};
+}
+
 // SETS: of K and V rows in LDS.  Two for bf16 pages where two workgroups share a CU (K two blocks
 // ahead, V one), else three.
 // TREE: the new positions are the nodes of a tree of drafts, at_tree_keys.
@@ -133,9 +174,16 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
   // 8 pairs, one pair's tiles all run on one XCD and share its L2
   const int pairs = a.B * a.Hkv;
   constexpr bool PARTS = KV != AP_ROWS;   // a tile's keys may go to a.parts workgroups
-  const int turn_ = blockIdx.x / pairs, pair = blockIdx.x % pairs;
-  const int part = PARTS ? turn_ % a.parts : 0;
+  const int turn_ = blockIdx.x / pairs;
+  int pair = blockIdx.x % pairs, part = PARTS ? turn_ % a.parts : 0, most = a.parts;
   const int qt = a.qtiles - 1 - (PARTS ? turn_ / a.parts : turn_);
+  if constexpr (PARTS && TREE) {
+    const ApShare own = ap_tree_share(a, blockIdx.x / a.Hkv % (a.B * a.parts), lane);
+    if (own.b < 0) return;
+    pair = own.b * a.Hkv + blockIdx.x % a.Hkv;
+    part = own.part;
+    most = own.parts;
+  }
   const int b = pair / a.Hkv, kvh = pair % a.Hkv;
   const int q0 = qt * a.QB, QB = min(a.QB, a.T - q0);
   const int L = min(max(a.kv_len[b], 0), a.max_len);
@@ -145,7 +193,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
 
   // The blocks of this workgroup: from the first page that is mapped on (a window leaves none
   // before it), and of these one of `parts` equal parts.  Parts of 8 blocks (10 us) or more, from
-  // 24 blocks on: what a division saves has to pay for the pieces and their merge, some 10 us.
+  // 24 blocks on: what a division saves has to pay for the pieces and their merge, some 10 us.  (Trees: 3, from 6.)
   int j0 = 0, nblk = nall, parts = 1;
   if constexpr (KV != AP_ROWS) {
     const int32_t* row = a.table + b * a.table_stride;
@@ -164,7 +212,8 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
     }
     if constexpr (PARTS) {
       const int n = nall - j0;
-      parts = n < 3 * AP_PART_BLOCKS ? 1 : min(a.parts, n / AP_PART_BLOCKS);
+      constexpr int LEAST = TREE ? AP_TREE_BLOCKS : AP_PART_BLOCKS;
+      parts = n < (TREE ? 2 : 3) * LEAST ? 1 : min(most, n / LEAST);
       if (part >= parts) return;
       nblk = j0 + (int)((long long)n * (part + 1) / parts);
       j0 += (int)((long long)n * part / parts);
@@ -644,14 +693,15 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
     if constexpr (PARTS) {
       if (!whole) {
         const int tile = qt * pairs + pair;
-        piece = a.ws + ((size_t)tile * a.parts + part) * AP_PIECE;
+        piece = a.ws + (TREE ? (size_t)blockIdx.x : (size_t)tile * a.parts + part) * AP_PIECE;
         if (h == 0) {
           piece[32 * wave + l32] = m_ref[0];
           piece[128 + 32 * wave + l32] = l;
         }
       }
       if (tid == 0 && part == 0 && a.parts > 1)
-        reinterpret_cast<int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[qt * pairs + pair] = parts;
+        reinterpret_cast<int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[qt * pairs + pair] =
+            TREE ? (int)blockIdx.x << AP_TILE_PARTS | parts : parts;
     }
 #pragma unroll
     for (int cp = 0; cp < AT_D / COLS; ++cp) {
@@ -717,24 +767,27 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
 }
 
 // Merges the parts of a tile, a wave per row (4 columns a lane), with the gate; tiles of one part
-// are finished already.
+// are finished already.  (Trees: a tile's parts begin at a place of their own, a.Hkv apart.)
+template <bool TREE>
 __global__ __launch_bounds__(256) void attn_parts_combine_kernel(ApArgs a) {
   const int pairs = a.B * a.Hkv, tile = blockIdx.x >> 5, lane = threadIdx.x & 63;
   const int r = 4 * (blockIdx.x & 31) + (threadIdx.x >> 6);
-  const int n = reinterpret_cast<const int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[tile];
+  const int entry = reinterpret_cast<const int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[tile];
+  const int n = TREE ? entry & ((1 << AP_TILE_PARTS) - 1) : entry;
   if (n == 1) return;
   const int qt = tile / pairs, pair = tile - qt * pairs, b = pair / a.Hkv, kvh = pair - b * a.Hkv;
   const int qi = ap_div(r, a.rep_mul), q0 = qt * a.QB;
   if (qi >= min(a.QB, a.T - q0)) return;
   const int head = kvh * a.n_rep + r - qi * a.n_rep;
   const size_t bt = (size_t)b * a.T + q0 + qi;
-  const float* piece = a.ws + (size_t)tile * a.parts * AP_PIECE;
-  const float* mine = piece + (size_t)min(lane, n - 1) * AP_PIECE;
+  const float* piece = a.ws + (TREE ? (size_t)(entry >> AP_TILE_PARTS) : (size_t)tile * a.parts) * AP_PIECE;
+  const size_t next = (size_t)AP_PIECE * (TREE ? a.Hkv : 1);
+  const float* mine = piece + min(lane, n - 1) * next;
   const float m = mine[r], ls = lane < n ? mine[128 + r] : 0.f;
   const float* col = piece + 256 + r * AT_D + 4 * lane;
   float4 v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float4*>(col + (size_t)min(e, n - 1) * AP_PIECE);
+  for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float4*>(col + min(e, n - 1) * next);
   uint2 gv = make_uint2(0, 0);
   if (a.gate)
     gv = *reinterpret_cast<const uint2*>(a.gate + bt * a.gate_row + (size_t)head * a.gate_head + 4 * lane);
@@ -757,7 +810,7 @@ __global__ __launch_bounds__(256) void attn_parts_combine_kernel(ApArgs a) {
     if (s + 4 < n) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        v[e] = *reinterpret_cast<const float4*>(col + (size_t)min(s + 4 + e, n - 1) * AP_PIECE);
+        v[e] = *reinterpret_cast<const float4*>(col + min(s + 4 + e, n - 1) * next);
     }
   }
   at_store4(a.out + (bt * a.Hq + head) * AT_D + 4 * lane, acc, l == 0.f ? 0.f : 1.f / l, a.gate != nullptr, gv);
@@ -788,14 +841,20 @@ static int prefill_tiles(int B, int T, int Hkv, int n_rep, int rg, int* QB) {
 
 int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts, bool tree) {
   *parts = 1;
-  if (T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS) return 0;
+  // Trees: tiles where a (sequence, KV head) has more than the split-K's 32 rows, which reads its keys once for
+  // each 32, and the call a number of rows in all (us, tiles / split-K, 8 rows a head, bf16: 1 x 12 nodes over 2000
+  // keys 25 / 20, over 30000 50 / 68; 1 x 16 26 / 21, 52 / 82; 4 x 7 over 500 23 / 18, over 16000 67 / 85;
+  // 4 x 63 34 / 36, 224 / 439; 8 bits: 1 x 16 over 2000 26 / 18, over 30000 52 / 50; 4 x 16 38 / 25, over 16000
+  // 73 / 86; 1 x 63 40 / 29, over 30000 97 / 137; 16 x 63 over 8000 311 / 614).
+  if (tree && (T * n_rep <= AT_ROWS || (long long)B * T * Hkv * n_rep < (f8 ? 2048 : 512))) return 0;
+  if (!tree && (T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS)) return 0;
   const long long pairs = (long long)B * Hkv;
   // Query tiles, whatever their number (us, tiles / split-K, bf16: 20 tiles of 2070 keys 35 / 38, of
   // 30000 134 / 308; 64 of 8256 123 / 220; 128 of 8289 203 / 418; but 32 of 256 28 / 20), but for few
   // tiles of 8-bit pages, whose codes a tile converts for 32 rows at a time as the split-K does,
   // without its depth of loads: from 64 full tiles on (32 of 1128 33 / 32, of 4128 55 / 54; 64 of
   // 1256 47 / 39, of 4256 71 / 81, of 16256 171 / 246; 128 of 512 49 / 44, of 8289 168 / 264).
-  if (f8 && 4 * pairs * T * n_rep < 128LL * cus) return 0;
+  if (f8 && !tree && 4 * pairs * T * n_rep < 128LL * cus) return 0;
   int QB;
   const long long tiles = prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * pairs;
   // Workgroups of a CU: a wave alone on its SIMD issues a VALU instruction every 8 cycles, two share
@@ -865,7 +924,9 @@ int attn_prefill_launch(const AttnArgs& v, int groups, hipStream_t st, const Pag
   if (parts > 1) {
     const int rc = launch_status();
     if (rc) return rc;
-    hipLaunchKernelGGL(attn_parts_combine_kernel, dim3((unsigned)(n / parts) * 32), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(n / parts) * 32);
+    if (v.tree) hipLaunchKernelGGL(attn_parts_combine_kernel<true>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(attn_parts_combine_kernel<false>, grid, dim3(256), 0, st, a);
   }
   return launch_status();
 }
