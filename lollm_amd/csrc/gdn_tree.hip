@@ -13,20 +13,26 @@
 // The products with S0 are bf16 MFMAs of the rows (bf16 as they are: q, k and v are bf16 tensors, which
 // the records hold) with S0 as hi + lo bf16, 16 bits of it; all sums are fp32.
 //
-// One workgroup of four waves per (sequence, v-head).  Wave w owns value columns 32 w ..: its part of S0
+// One workgroup of eight waves per (sequence, v-head).  Wave w owns value columns 16 w ..: its part of S0
 // lies in registers in the order in which the MFMA takes it as operand (lane 16 g + c: rows 32 s + 8 g
-// + e, columns 32 w + 2 c + t), the triangular solve and the outputs of its columns never leave its
+// + e, column 16 w + c), the triangular solve and the outputs of its columns never leave its
 // accumulators, which hold rows in the order that the next product contracts over.
+//
+// Measured: 8 x 63 nodes, 32 v-heads 28 us, 16 x 16 25 us, 1 x 7 with 16 heads 11 us; the bytes (states in and
+// out, rows, records) take 12.5, 16 and 0.5 at a large copy's rate.  With one workgroup a CU (63 nodes: 108 KB of
+// LDS) its phases follow each other: of 50,000 cycles 13,000 each are the loads' way and the last products
+// (fp32 MFMAs of a 64 x 64 triangle, a chain), 7,700 the convolution (exponentials), 5,500 the two matrices.
+// Four waves of 32 columns took 36 us: each phase had half the waves to hide its latencies.
 #include "gdn_common.h"
 
 namespace lollm {
 
 typedef float gt_f32x4 __attribute__((ext_vector_type(4)));
-typedef float gt_f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 gt_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 gt_bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int GT_MAX = 64;            // nodes
+constexpr int GT_WAVES = 8, GT_THREADS = 64 * GT_WAVES;
 constexpr int GT_K = 4;               // taps of the convolution
 constexpr int GT_PW = GL_DK + 8;      // bf16 pitch of 128-wide rows
 
@@ -50,7 +56,7 @@ struct GtShared {
   uint16_t cw[GL_CH][GT_K];
   uint64_t word[TP];                         // ancestors, without the node itself
   float G[TP], beta[TP], rk[TP], rq[TP], E[TP];
-  float ss[4][TP];
+  float ss[GT_WAVES][TP], rn[TP];
   uint8_t up[TP][4];                         // rows of raw behind the taps 2, 1, 0
 };
 
@@ -67,12 +73,21 @@ __device__ __forceinline__ float gt_sum_groups(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+__device__ __forceinline__ float gt_dot2(uint32_t a, uint32_t b, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(gt_bf16x2, a), __builtin_bit_cast(gt_bf16x2, b), c, false);
+}
 __device__ __forceinline__ gt_bf16x8 gt_row8(const uint16_t* p) {
   return __builtin_bit_cast(gt_bf16x8, *reinterpret_cast<const u32x4_t*>(p));
 }
 
+struct GtRecord {   // of a committed token: k in the lane's rows, v of its column; decay, beta, 1 / |k|
+  u32x4_t k[4];
+  uint16_t v;
+  float4 sc;
+};
+
 template <int MT>
-__global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
+__global__ __launch_bounds__(GT_THREADS, MT < 4 ? 4 : 2) void gdn_tree_kernel(GtArgs ga) {
   using Sh = GtShared<MT>;
   constexpr int TP = Sh::TP;
   __shared__ __attribute__((aligned(16))) Sh sh;
@@ -99,12 +114,12 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
   };
 
   // ---- 1. one batch of loads: the convolution's inputs and weights, the gates; the state last ----
-  constexpr int NX = ((Km1 + TP) * 48 + 255) / 256;
+  constexpr int NX = ((Km1 + TP) * 48 + GT_THREADS - 1) / GT_THREADS;
   const int nx = (Km1 + T) * 48;
   uint4 xv[NX];
 #pragma unroll
   for (int it = 0; it < NX; ++it) {
-    const int id = it * 256 + tid;
+    const int id = it * GT_THREADS + tid;
     xv[it] = make_uint4(0, 0, 0, 0);
     if (id < nx) {
       const int r = id / 48, gi = (id / 16) % 3, part = id % 16;
@@ -119,23 +134,36 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
   const uint16_t bb_raw = a.proj[base_ba + h], aa_raw = a.proj[base_ba + a.Hv + h];
   const uint64_t word_raw = ga.tree[(size_t)b * T + (lane < T ? lane : T - 1)];
   const float a_log = a.A_log[h], dtb = a.dt_bias[h];
-  gt_f32x2 S[4][8];
+  // the first two records, later the next two while one is applied: each in turn from memory costs its way there
+  const uint8_t* rp = a.rep + hin * a.S * GL_REC_BYTES;
+  GtRecord rec2[2];
+  const int col = 16 * wave + c16;
+  auto load_rec = [&](GtRecord& r, int j) {
+    const uint8_t* p = rp + (size_t)min(j, a.S - 1) * GL_REC_BYTES;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) r.k[s] = *reinterpret_cast<const u32x4_t*>(p + 2 * (32 * s + 8 * g4));
+    r.v = *reinterpret_cast<const uint16_t*>(p + 2 * GL_DK + 2 * col);
+    r.sc = *reinterpret_cast<const float4*>(p + 4 * GL_DK);
+  };
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (j < n) load_rec(rec2[j], j);
+  float S[4][8];
   {
     const __amdgpu_buffer_rsrc_t rs = buf_rsrc(a.rec + hin * SS, a.fresh ? 0u : (uint32_t)(SS * sizeof(float)));
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        S[s][e] = __builtin_bit_cast(gt_f32x2, __builtin_amdgcn_raw_buffer_load_b64(
-                                                   rs, (uint32_t)(((32 * s + 8 * g4 + e) * GL_DK + 32 * wave + 2 * c16) * 4),
-                                                   0, 2));
+        S[s][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+            rs, (uint32_t)(((32 * s + 8 * g4 + e) * GL_DK + col) * 4), 0, 2));
   }
   __builtin_amdgcn_sched_barrier(0);   // nothing that waits on a load moves above the state loads
 
   // ---- 2. to LDS, the new conv window to the other half; words, gates and path sums ----
 #pragma unroll
   for (int it = 0; it < NX; ++it) {
-    const int id = it * 256 + tid;
+    const int id = it * GT_THREADS + tid;
     if (id < (Km1 + TP) * 48) {
       const int r = id / 48, gi = (id / 16) % 3, part = id % 16;
       *reinterpret_cast<uint4*>(&sh.raw[r][gi * GL_DK + part * 8]) = xv[it];   // (zeros past the last node)
@@ -148,10 +176,14 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
     const uint64_t above = lane < T ? word_raw & ((1ull << lane) - 1) : 0ull;
     const float g = lane < T ? -__expf(a_log) * softplus_g(bf16_to_f32(aa_raw) + dtb) : 0.f;
     const float beta = lane < T ? 1.f / (1.f + __expf(-bf16_to_f32(bb_raw))) : 0.f;
+    // the path's sum by doubling: from the parent, its sum so far and its own
     float G = g;
-    for (int j = 0; j < T - 1; ++j) {
-      const float gj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), j));
-      G += (above >> j) & 1 ? gj : 0.f;
+    int p = above ? 63 - __clzll((long long)above) : -1;
+    for (int d = 1; d < T; d <<= 1) {
+      const float Gp = __shfl(G, max(p, 0), 64);
+      const int pp = __shfl(p, max(p, 0), 64);
+      G += p >= 0 ? Gp : 0.f;
+      p = p >= 0 ? pp : -1;
     }
     if (lane < TP) {
       sh.word[lane] = above;
@@ -175,25 +207,25 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
     }
   }
   lds_only_barrier();
-  // ---- 3. conv + SiLU: channels 8 o .. of the head's 384, nodes i, i + 5, .. ----
-  if (tid < 240) {
+  // ---- 3. conv + SiLU: channels 8 o .. of the head's 384, nodes i, i + 10, .. ----
+  if (tid < 480) {
     const int o = tid % 48;
     uint16_t* dst = o < 16 ? &sh.q[0][8 * o] : (o < 32 ? &sh.k[0][8 * o - GL_DK] : &sh.v[0][8 * o - 2 * GL_DK]);
-    float w[8][GT_K];
+    uint2 w[8];   // a channel's taps in pairs
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint2 u = *reinterpret_cast<const uint2*>(&sh.cw[8 * o + e][0]);
-      w[e][0] = gt_lo(u.x); w[e][1] = gt_hi(u.x); w[e][2] = gt_lo(u.y); w[e][3] = gt_hi(u.y);
-    }
-    for (int i = tid / 48; i < TP; i += 5) {
+    for (int e = 0; e < 8; ++e) w[e] = *reinterpret_cast<const uint2*>(&sh.cw[8 * o + e][0]);
+    for (int i = tid / 48; i < TP; i += 10) {
       const uint32_t up = *reinterpret_cast<const uint32_t*>(&sh.up[i][0]);
       const int rows[GT_K] = {(int)(up >> 16 & 255), (int)(up >> 8 & 255), (int)(up & 255), Km1 + i};
-      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      u32x4_t x[GT_K];
 #pragma unroll
-      for (int tap = 0; tap < GT_K; ++tap) {
-        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(&sh.raw[rows[tap]][8 * o]);
+      for (int tap = 0; tap < GT_K; ++tap) x[tap] = *reinterpret_cast<const u32x4_t*>(&sh.raw[rows[tap]][8 * o]);
+      float acc[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = fmaf(w[e][tap], e & 1 ? gt_hi(x[e >> 1]) : gt_lo(x[e >> 1]), acc[e]);
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;   // the same half of two rows
+        acc[e] = gt_dot2(__builtin_amdgcn_perm(x[1][e >> 1], x[0][e >> 1], sel), w[e].x, 0.f);
+        acc[e] = gt_dot2(__builtin_amdgcn_perm(x[3][e >> 1], x[2][e >> 1], sel), w[e].y, acc[e]);
       }
       u32x4_t y;
 #pragma unroll
@@ -204,8 +236,8 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
   lds_only_barrier();
   // ---- 4. norms, records ----
   {
-    constexpr int PER = 256 / TP, CH = GL_DK / PER;   // threads of a node, values of a thread
-    const int i = tid / PER, part = tid % PER;
+    constexpr int PER = TP < 64 ? 16 : 8, CH = GL_DK / PER;   // threads of a node, values of a thread
+    const int i = min(tid / PER, TP - 1), part = tid % PER;   // (16 nodes take half the threads)
     float sq = 0.f, sk = 0.f;
 #pragma unroll
     for (int e = 0; e < CH; e += 8) {
@@ -213,8 +245,8 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
       const u32x4_t k = *reinterpret_cast<const u32x4_t*>(&sh.k[i][CH * part + e]);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        sq = fmaf(gt_lo(q[x]), gt_lo(q[x]), sq); sq = fmaf(gt_hi(q[x]), gt_hi(q[x]), sq);
-        sk = fmaf(gt_lo(k[x]), gt_lo(k[x]), sk); sk = fmaf(gt_hi(k[x]), gt_hi(k[x]), sk);
+        sq = gt_dot2(q[x], q[x], sq);
+        sk = gt_dot2(k[x], k[x], sk);
       }
     }
 #pragma unroll
@@ -222,7 +254,7 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
       sq += __shfl_xor(sq, o, 64);
       sk += __shfl_xor(sk, o, 64);
     }
-    if (part == 0) {
+    if (part == 0 && tid < TP * PER) {
       const float rk = rsqrtf(sk + 1e-6f);
       sh.rk[i] = i < T ? rk : 0.f;
       sh.rq[i] = i < T ? rsqrtf(sq + 1e-6f) * rsqrtf((float)GL_DK) : 0.f;
@@ -232,7 +264,7 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
         rec[3] = 0.f;
       }
     }
-    for (int id = tid; id < T * 32; id += 256) {
+    for (int id = tid; id < T * 32; id += GT_THREADS) {
       const int r = id / 32, p = id % 32;
       const uint16_t* src = p < 16 ? &sh.k[r][8 * p] : &sh.v[r][8 * p - GL_DK];
       *reinterpret_cast<uint4*>(a.rep + (hout * a.S + r) * GL_REC_BYTES + 16 * p) = *reinterpret_cast<const uint4*>(src);
@@ -242,7 +274,7 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
   // ---- 5. the two T x T matrices (block rows I, columns J <= I), the diagonal blocks' inverses ----
   {
     constexpr int NT = MT * (MT + 1) / 2;
-    for (int t = wave; t < 2 * NT; t += 4) {
+    for (int t = wave; t < 2 * NT; t += GT_WAVES) {
       const bool qs = t >= NT;
       int I = 0, J = qs ? t - NT : t;
       while (J > I) J -= ++I;
@@ -275,145 +307,122 @@ __global__ __launch_bounds__(256) void gdn_tree_kernel(GtArgs ga) {
       for (int j = 0; j < i; ++j) y = fmaf(sh.m.am[16 * wave + i][16 * wave + j], x[j], y);
       x[i] = y;
       sh.m.tinv[wave][i][lane] = y;
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (or all of the block waits in registers)
     }
   }
   // ---- 6. the committed state: n records on the stored one, to the other half ----
-  const uint8_t* rp = a.rep + hin * a.S * GL_REC_BYTES;
-  for (int j = 0; j < n; ++j, rp += GL_REC_BYTES) {
-    u32x4_t kw[4];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) kw[s] = *reinterpret_cast<const u32x4_t*>(rp + 2 * (32 * s + 8 * g4));
-    const uint32_t v2 = *reinterpret_cast<const uint32_t*>(rp + 2 * GL_DK + 2 * (32 * wave + 2 * c16));
-    const float4 sc = *reinterpret_cast<const float4*>(rp + 4 * GL_DK);
-    float p0 = 0.f, p1 = 0.f;
+  auto apply = [&](const GtRecord& r) {
+    float p[2] = {0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float kk = e & 1 ? gt_hi(kw[s][e >> 1]) : gt_lo(kw[s][e >> 1]);
-        p0 = fmaf(S[s][e].x, kk, p0);
-        p1 = fmaf(S[s][e].y, kk, p1);
-      }
-    p0 = gt_sum_groups(p0);
-    p1 = gt_sum_groups(p1);
-    const float d0 = (gt_lo(v2) - sc.x * p0 * sc.z) * sc.y, d1 = (gt_hi(v2) - sc.x * p1 * sc.z) * sc.y;
+      for (int e = 0; e < 8; ++e) p[s & 1] = fmaf(S[s][e], e & 1 ? gt_hi(r.k[s][e >> 1]) : gt_lo(r.k[s][e >> 1]), p[s & 1]);
+    const float d = (bf16_to_f32(r.v) - r.sc.x * gt_sum_groups(p[0] + p[1]) * r.sc.z) * r.sc.y, kd = d * r.sc.z;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float kk = (e & 1 ? gt_hi(kw[s][e >> 1]) : gt_lo(kw[s][e >> 1])) * sc.z;
-        S[s][e].x = fmaf(kk, d0, sc.x * S[s][e].x);
-        S[s][e].y = fmaf(kk, d1, sc.x * S[s][e].y);
-      }
+      for (int e = 0; e < 8; ++e)
+        S[s][e] = fmaf(e & 1 ? gt_hi(r.k[s][e >> 1]) : gt_lo(r.k[s][e >> 1]), kd, r.sc.x * S[s][e]);
+  };
+  for (int j = 0; j < n; j += 2) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (j + x >= n) break;
+      apply(rec2[x]);
+      if (j + x + 2 < n) load_rec(rec2[x], j + x + 2);
+    }
   }
   {
     float* so = a.rec + hout * SS;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        __builtin_nontemporal_store(S[s][e], reinterpret_cast<gt_f32x2*>(so + (32 * s + 8 * g4 + e) * GL_DK + 32 * wave +
-                                                                         2 * c16));
+      for (int e = 0; e < 8; ++e) __builtin_nontemporal_store(S[s][e], so + (32 * s + 8 * g4 + e) * GL_DK + col);
   }
-  gt_bf16x8 Sh_[2][4], Sl[2][4];
+  gt_bf16x8 Sh_[4], Sl[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x0 = S[s][e].x, x1 = S[s][e].y;
-      Sh_[0][s][e] = (__bf16)x0;
-      Sh_[1][s][e] = (__bf16)x1;
-      Sl[0][s][e] = (__bf16)(x0 - (float)(__bf16)x0);
-      Sl[1][s][e] = (__bf16)(x1 - (float)(__bf16)x1);
+      Sh_[s][e] = (__bf16)S[s][e];
+      Sl[s][e] = (__bf16)(S[s][e] - (float)(__bf16)S[s][e]);
     }
   // ---- 7. u and o, block row by block row; the gate's z on its way ----
   lds_only_barrier();   // the inverses
-  uint32_t z[MT][4];
+  uint16_t z[MT][4];
 #pragma unroll
   for (int I = 0; I < MT; ++I)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = min(16 * I + 4 * g4 + r, T - 1);
-      z[I][r] = *reinterpret_cast<const uint32_t*>(a.proj + ((size_t)b * T + i) * a.P + a.C + (size_t)h * GL_DK +
-                                                   32 * wave + 2 * c16);
+      z[I][r] = a.proj[((size_t)b * T + i) * a.P + a.C + (size_t)h * GL_DK + col];
     }
-  gt_f32x4 U[MT][2], O[MT][2];
+  gt_f32x4 U[MT], O[MT];
 #pragma unroll
   for (int I = 0; I < MT; ++I) {
-    gt_f32x4 ks[2], qs[2];
+    gt_f32x4 ks[2], qs[2];   // with the state's high and low parts
 #pragma unroll
     for (int t = 0; t < 2; ++t) ks[t] = qs[t] = gt_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const gt_bf16x8 kr = gt_row8(&sh.k[16 * I + c16][32 * s + 8 * g4]), qr = gt_row8(&sh.q[16 * I + c16][32 * s + 8 * g4]);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        ks[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, Sh_[t][s], ks[t], 0, 0, 0);
-        qs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, Sh_[t][s], qs[t], 0, 0, 0);
-        ks[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, Sl[t][s], ks[t], 0, 0, 0);
-        qs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, Sl[t][s], qs[t], 0, 0, 0);
-      }
+      ks[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, Sh_[s], ks[0], 0, 0, 0);
+      qs[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, Sh_[s], qs[0], 0, 0, 0);
+      ks[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, Sl[s], ks[1], 0, 0, 0);
+      qs[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, Sl[s], qs[1], 0, 0, 0);
     }
-    gt_f32x4 rhs[2];
+    gt_f32x4 rhs;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * I + 4 * g4 + r;
-      const uint32_t v2 = *reinterpret_cast<const uint32_t*>(&sh.v[i][32 * wave + 2 * c16]);
-      const float E = sh.E[i], bet = sh.beta[i], ek = E * sh.rk[i], eq = E * sh.rq[i];
-      rhs[0][r] = bet * (gt_lo(v2) - ek * ks[0][r]);
-      rhs[1][r] = bet * (gt_hi(v2) - ek * ks[1][r]);
-      O[I][0][r] = eq * qs[0][r];
-      O[I][1][r] = eq * qs[1][r];
+      const float E = sh.E[i];
+      rhs[r] = sh.beta[i] * (bf16_to_f32(sh.v[i][col]) - E * sh.rk[i] * (ks[0][r] + ks[1][r]));
+      O[I][r] = E * sh.rq[i] * (qs[0][r] + qs[1][r]);
     }
 #pragma unroll
     for (int J = 0; J < I; ++J) {
       const float4 m = *reinterpret_cast<const float4*>(&sh.m.am[16 * I + c16][16 * J + 4 * g4]);
       const float mm[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) rhs[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[s], U[J][t][s], rhs[t], 0, 0, 0);
+      for (int s = 0; s < 4; ++s) rhs = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[s], U[J][s], rhs, 0, 0, 0);
     }
     {
       const float4 m = *reinterpret_cast<const float4*>(&sh.m.tinv[I][c16][4 * g4]);
       const float mm[4] = {m.x, m.y, m.z, m.w};
+      U[I] = gt_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        U[I][t] = gt_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) U[I][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[s], rhs[t][s], U[I][t], 0, 0, 0);
-      }
+      for (int s = 0; s < 4; ++s) U[I] = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[s], rhs[s], U[I], 0, 0, 0);
     }
 #pragma unroll
     for (int J = 0; J <= I; ++J) {
       const float4 m = *reinterpret_cast<const float4*>(&sh.m.qk[16 * I + c16][16 * J + 4 * g4]);
       const float mm[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) O[I][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[s], U[J][t][s], O[I][t], 0, 0, 0);
+      for (int s = 0; s < 4; ++s) O[I] = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[s], U[J][s], O[I], 0, 0, 0);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float s = sum_lanes16(O[I][0][r] * O[I][0][r] + O[I][1][r] * O[I][1][r]);
+      const float s = sum_lanes16(O[I][r] * O[I][r]);
       if (c16 == 0) sh.ss[wave][16 * I + 4 * g4 + r] = s;
     }
   }
   lds_only_barrier();
   // ---- 8. gated RMSNorm ----
-  const uint32_t w2 = *reinterpret_cast<const uint32_t*>(a.norm_w + 32 * wave + 2 * c16);
+  if (tid < TP) {
+    float ss = 0.f;
+#pragma unroll
+    for (int w = 0; w < GT_WAVES; ++w) ss += sh.ss[w][tid];
+    sh.rn[tid] = rsqrtf(ss / (float)GL_DK + a.eps);
+  }
+  lds_only_barrier();
+  const float nw = bf16_to_f32(a.norm_w[col]);
 #pragma unroll
   for (int I = 0; I < MT; ++I)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * I + 4 * g4 + r;
-      const float ss = sh.ss[0][i] + sh.ss[1][i] + sh.ss[2][i] + sh.ss[3][i];
-      const float rn = rsqrtf(ss / (float)GL_DK + a.eps);
-      const float y0 = O[I][0][r] * rn * gt_lo(w2) * silu_g(gt_lo(z[I][r]));
-      const float y1 = O[I][1][r] * rn * gt_hi(w2) * silu_g(gt_hi(z[I][r]));
-      if (i < T)
-        *reinterpret_cast<uint32_t*>(a.out + ((size_t)b * T + i) * a.value_dim + (size_t)h * GL_DK + 32 * wave + 2 * c16) =
-            gt_pack(y0, y1);
+      const float y = O[I][r] * sh.rn[i] * nw * silu_g(bf16_to_f32(z[I][r]));
+      if (i < T) a.out[((size_t)b * T + i) * a.value_dim + (size_t)h * GL_DK + col] = f32_to_bf16(y);
     }
 }
 
@@ -448,7 +457,7 @@ LOLLM_API int lollm_gdn_layer_tree(const void* proj, long long proj_stride, cons
   a.eps = eps;
   ga.tree = (const uint64_t*)tree;
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 g(B * Hv), t(256);
+  const dim3 g(B * Hv), t(GT_THREADS);
   if (T <= 16) hipLaunchKernelGGL(gdn_tree_kernel<1>, g, t, 0, st, ga);
   else if (T <= 32) hipLaunchKernelGGL(gdn_tree_kernel<2>, g, t, 0, st, ga);
   else hipLaunchKernelGGL(gdn_tree_kernel<4>, g, t, 0, st, ga);
