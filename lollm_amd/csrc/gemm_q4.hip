@@ -9,7 +9,7 @@
 // tile share (many rows: after the loop, by a product over the groups).  The group's scale then meets an
 // fp32 sum, so weights are never rounded.  What the detour costs: partial sums of at most 32 sum |x| in
 // fp32, 2^-24 of that against a group's typical 52 |x| is 1e-5 of it, below a bf16 output's 2^-9.  An
-// infinite x gives NaN in its row.
+// x that is infinite, or so large (2^116) that these sums are, makes its row NaN.
 //
 // Layout (lollm_q4_pack, once per weight).  1 KB blocks of 16 rows x 128 k in operand order: lane
 // 16 g + r holds row r's codes of k 32 j + 8 g .. + 8 in word j, even k in the low half and odd k in
@@ -318,28 +318,31 @@ __global__ __launch_bounds__(Q4_THREADS) void gemm_q4_wide_kernel(Q4Args a) {
   // column tile j with COUNT of the held stages: their chains of products side by side
   auto tile = [&](const Q4Weights<HELD, GPS>& d, int j, auto count) {
     constexpr int COUNT = decltype(count)::value;
+    q4_f32x4 v[COUNT][GPS];
 #pragma unroll
-    for (int g = 0; g < GPS; ++g) {
-      q4_f32x4 v[COUNT];
+    for (int h = 0; h < COUNT; ++h)
 #pragma unroll
-      for (int h = 0; h < COUNT; ++h)
+      for (int g = 0; g < GPS; ++g)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          v[h][e] = ZERO ? c0[h][g] * (-16.f - (float)((d.z[h][g] >> (8 * e)) & 0xffu)) : c0[h][g];
+          v[h][g][e] = ZERO ? c0[h][g] * (-16.f - (float)((d.z[h][g] >> (8 * e)) & 0xffu)) : c0[h][g];
 #pragma unroll
-      for (int q = 0; q < KPG; ++q)
-#pragma unroll
-        for (int h = 0; h < COUNT; ++h)
-          v[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_frag(d.w[h][g * KPG + q], kc),
-                                                         __builtin_bit_cast(q4_bf16x8, x[h][g * KPG + q]), v[h], 0, 0, 0);
+    for (int q = 0; q < KPG; ++q)
 #pragma unroll
       for (int h = 0; h < COUNT; ++h)
+#pragma unroll
+        for (int g = 0; g < GPS; ++g)
+          v[h][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_frag(d.w[h][g * KPG + q], kc),
+                                                            __builtin_bit_cast(q4_bf16x8, x[h][g * KPG + q]), v[h][g], 0, 0, 0);
+#pragma unroll
+    for (int h = 0; h < COUNT; ++h)   // (a stage's groups, then the next one's: the order of all few-row kernels)
+#pragma unroll
+      for (int g = 0; g < GPS; ++g)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t b = d.s[h][g][e >> 1];
-          tot[j][e] = fmaf(__uint_as_float(e & 1 ? b & 0xffff0000u : b << 16), v[h][e], tot[j][e]);
+          tot[j][e] = fmaf(__uint_as_float(e & 1 ? b & 0xffff0000u : b << 16), v[h][g][e], tot[j][e]);
         }
-    }
   };
   for (int c = 0; c < n; c += HELD) {
 #pragma unroll

@@ -182,6 +182,23 @@ def test_gemm_q4_rows_do_not_depend_on_each_other(zeros):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("N,K", [(4224, 1152), (12352, 640), (24640, 1152), (33088, 2432), (4096, 5504)])
+def test_gemm_q4_a_rows_bits_at_any_number_of_columns(N, K, group, zeros):
+    """The same over the forms that the number of columns chooses: one or several column tiles a
+    workgroup, whole and partial sets of the stages that a wave holds."""
+    from lollm_amd import ops
+    code, scale, zero = weight(N, K, group, zeros, N + group)
+    packed = ops.q4_pack(bytes_of(code).cuda(), scale.cuda(), None if zero is None else zero.cuda())
+    x = torch.randn(64, K, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    whole = ops.gemm_q4(x, packed)
+    for lo, hi in ((0, 1), (5, 9), (16, 32), (30, 47), (17, 49), (0, 33)):
+        print(f"case q4 {N} x {K} group {group} zeros {zeros} rows {lo}:{hi}", flush=True)
+        assert torch.equal(ops.gemm_q4(x[lo:hi], packed), whole[lo:hi])
+
+
+@pytest.mark.gpu
 def test_gemm_q4_leading_shapes_strides_and_no_rows():
     from lollm_amd import ops
     N, K = 128, 256
