@@ -503,7 +503,8 @@ int lollm_gemm_rows(const void* A, long long lda, const void* Wt, void* C, long 
  * + i, as a short call's; committing a path of the tree is moving its records and rows to the front
  * (lollm_tree_keep_gdn) and then setting the indices as after a short call.  T <= 64, slots >= T, win_rows
  * >= conv_kernel - 1 + T, conv_kernel 4, Dk == Dv == 128; the words' bits at and past the node itself
- * count for nothing, and bits that are no tree's give numbers without meaning.  q, k and v are rounded
+ * count for nothing, and bits that are no tree's give numbers without meaning; what all nodes bring
+ * must be finite (a weight of 0 meets it in the others' sums).  q, k and v are rounded
  * to bf16 once, after the activation; beta and what follows stay fp32 to the output. */
 int lollm_gdn_layer_tree(const void* proj, long long proj_stride, const void* conv_w,
                          const float* A_log, const float* dt_bias, const void* norm_w, void* win,
@@ -526,7 +527,7 @@ int lollm_gdn_layer_tree(const void* proj, long long proj_stride, const void* co
  * C = A W^T, or with epilogue 1 silu(gate) * up (N / 2 columns), A (M, K) bf16, fp32 throughout,
  * one rounding; any number of rows (workspace: lollm_gemm_q4_workspace_bytes, 0 for few rows, 16-byte
  * aligned, used only within the call).  A row's bits depend on no other row, nor up to 64 rows on
- * M; an infinity in A makes its row NaN.  N a multiple of 64, K of 128, group 32, 64 or 128, lda of
+ * M; an infinity in A, or a value beyond 2^116, makes its row NaN.  N a multiple of 64, K of 128, group 32, 64 or 128, lda of
  * 8, ldc of 4; A and packed 16-byte aligned, C 8-byte. */
 long long lollm_q4_packed_bytes(int N, int K, int group, int zeros);
 int lollm_q4_quantize(const void* weight, void* codes, void* scales, void* zeros, int N, int K,

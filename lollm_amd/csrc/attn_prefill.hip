@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
   const int turn_ = blockIdx.x / pairs;
   int pair = blockIdx.x % pairs, part = PARTS ? turn_ % a.parts : 0, most = a.parts;
   const int qt = a.qtiles - 1 - (PARTS ? turn_ / a.parts : turn_);
-  if constexpr (PARTS && TREE) {
+  if (PARTS && TREE && a.parts > 1) {
     const ApShare own = ap_tree_share(a, blockIdx.x / a.Hkv % (a.B * a.parts), lane);
     if (own.b < 0) return;
     pair = own.b * a.Hkv + blockIdx.x % a.Hkv;

@@ -186,10 +186,10 @@ def tree_accept(drawn, ids, tree):
     d = _arg(drawn, "drawn", torch.int32, (B, T), dev)
     i = _arg(ids, "ids", torch.int32, (B, T), dev)
     t = _tree_arg(tree, B, T, dev)
-    path, out = torch.empty_like(drawn), torch.empty(2, B, dtype=torch.int32, device=drawn.device)
-    rc = _lib.lib().lollm_tree_accept(d, i, t, _ptr(path), _ptr(out[0]), _ptr(out[1]), B, T, _stream())
+    path, count, token = torch.empty_like(drawn), drawn.new_empty(B), drawn.new_empty(B)
+    rc = _lib.lib().lollm_tree_accept(d, i, t, _ptr(path), _ptr(count), _ptr(token), B, T, _stream())
     _lib.check(rc, "lollm_tree_accept")
-    return path, out[0], out[1]
+    return path, count, token
 
 
 def _path_args(path, count, B, dev):
@@ -277,7 +277,11 @@ def attn_verify(q, k_cache, v_cache, kv_len, gate=None, *, grid=0, scale=None,
     if scale is None:
         scale = D ** -0.5
     if tree is not None:
-        t = _tree_arg(tree, B, T, q.get_device())
+        dev = torch._C._cuda_getDevice()
+        t = _tree_arg(tree, B, T, dev)
+        _arg(q, "q", torch.bfloat16, q.shape, dev)
+        _arg(k_cache, "k_cache", torch.bfloat16, k_cache.shape, dev)
+        _arg(kv_len, "kv_len", torch.int32, (B,), dev)
         rc = _lib.lib().lollm_attn_tree(
             _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(kv_len), t, _ptr(gate), _ptr(out),
             _ptr(workspace), wbytes, B, T, Hq, Hkv, D, max_len, Hkv * max_len * D, max_len * D,
@@ -693,7 +697,7 @@ def gemm_q4(x, weight, out=None):
     """y = x W^T for x (..., K) bf16 of any number of rows and a Q4Weight, in fp32 with one
     rounding: (..., N) bf16, or (..., N / 2) = silu(gate) * up for a GEMM_SWIGLU weight.  A row's
     bits depend on no other row, and up to 64 rows not on their number (beyond, sizes choose
-    between two orders of the sums).  An infinite x makes its row NaN."""
+    between two orders of the sums).  An x that is infinite or beyond 2^116 makes its row NaN."""
     N, K = weight.N, weight.K
     dev = torch._C._cuda_getDevice()
     if x.dim() < 1 or x.shape[-1] != K:
@@ -1141,7 +1145,8 @@ def gdn_layer(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half
     chunked: None = the chunked kernels for long calls of at least GDN_CHUNK_MIN_T tokens
     that they support, the recurrent kernel otherwise; True / False force one.
     tree: (B, T) int64 of tree_masks, the T positions are the nodes of a tree of drafts, each of which
-    continues from its parent (lollm_gdn_layer_tree: T <= TREE_MAX and S, the window's rows for it)."""
+    continues from its parent (lollm_gdn_layer_tree: T <= TREE_MAX and S, the window's rows for it;
+    what all nodes bring must be finite)."""
     P = proj.shape[-1]
     _need(proj, "proj", torch.bfloat16)
     _need(win, "win", torch.bfloat16)
@@ -1166,8 +1171,10 @@ def gdn_layer(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half
             _arg(proj, "proj", torch.bfloat16, (B, T, P), dev), P,
             _arg(conv_w, "conv_w", torch.bfloat16, (C, conv_kernel), dev), _arg(A_log, "A_log", torch.float32, (Hv,), dev),
             _arg(dt_bias, "dt_bias", torch.float32, (Hv,), dev), _arg(norm_w, "norm_w", torch.bfloat16, (D,), dev),
-            _arg(win, "win", torch.bfloat16, (B, 2 * W, C), dev), _ptr(conv_off), W, _ptr(rec), _ptr(rec_half),
-            _ptr(rep), _ptr(replay), S, int(bool(fresh)), words, _arg(out, "out", torch.bfloat16, (B, T, V), dev), B, T,
+            _arg(win, "win", torch.bfloat16, (B, 2 * W, C), dev), _arg(conv_off, "conv_off", torch.int32, (B,), dev), W,
+            _arg(rec, "rec", torch.float32, rec.shape, dev), _arg(rec_half, "rec_half", torch.int32, (B,), dev),
+            _arg(rep, "rep", torch.uint8, rep.shape, dev), _arg(replay, "replay", torch.int32, (B,), dev), S,
+            int(bool(fresh)), words, _arg(out, "out", torch.bfloat16, (B, T, V), dev), B, T,
             Hk, Hv, D, D, conv_kernel, float(eps), torch._C._cuda_getCurrentRawStream(dev))
         if rc:
             _lib.check(rc, "lollm_gdn_layer_tree")

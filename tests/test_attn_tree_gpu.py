@@ -155,6 +155,30 @@ def test_attn_tree_many_nodes(B, T, hq, hkv, kind):
     close(got, *reference(q, kh, vh, None, lens, words))
 
 
+RAGGED = [(70, 12, 8, 1, [12 + (b * b * 7) % 300 if b % 5 else 0 for b in range(70)]),       # more sequences than lanes
+          (4, 63, 32, 4, [0, 63, 900, 5000]), (3, 33, 16, 2, [33, 2000, 40]), (1, 64, 32, 4, [3000]),
+          (2, 24, 32, 4, [24, 24]), (65, 17, 8, 1, [17] * 64 + [1500])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ((16, 16), (128, 16), (16, 8), (128, 8)), ids=str)
+@pytest.mark.parametrize("case", RAGGED, ids=lambda c: f"{c[0]}x{c[1]}")
+def test_attn_tree_keys_dealt_out_by_length(case, kind):
+    """Query tiles whose keys go to workgroups by the sequences' lengths: none, few and many keys, empty
+    sequences between, one that takes nearly all."""
+    B, T, hq, hkv, lens = case
+    print("case tree attention by length", B, T, hq, hkv, kind, flush=True)
+    q, k, v, gate = inputs(B, T, hq, hkv, lens, 8)
+    _, words = tree(B, T, 9, 3)
+    got, kh, vh = run(kind, q, k, v, gate, lens, words)
+    again, _, _ = run(kind, q, k, v, gate, lens, words)
+    assert torch.equal(got, again)
+    close(got, *reference(q, kh, vh, gate, lens, words))
+    for b in range(B):
+        if lens[b] == 0:
+            assert (got[b] == 0).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS, ids=str)
 def test_attn_tree_any_words(kind):
