@@ -502,7 +502,12 @@ __global__ __launch_bounds__(256) void q4_sums_kernel(const uint16_t* __restrict
   float v = 0.f;
   if (g < groups) {
     const uint16_t* p = x + (size_t)m * ldx + (size_t)g * G + l * (G / 16);
-    for (int i = 0; i < G / 16; ++i) v += bf16_to_f32(p[i]);
+    u32x4_t w = {0, 0, 0, 0};   // the thread's 8, 4 or 2 values
+    if (G == 128) w = *reinterpret_cast<const u32x4_t*>(p);
+    else if (G == 64) { const uint2 t = *reinterpret_cast<const uint2*>(p); w.x = t.x; w.y = t.y; }
+    else w.x = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v += __uint_as_float(w[i] << 16) + __uint_as_float(w[i] & 0xffff0000u);
   }
   v = sum_lanes16(v) * factor;
   if (l < 3) {
