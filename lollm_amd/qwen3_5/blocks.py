@@ -8,6 +8,7 @@ between them.  A GEMM over at most 64 rows (the verify and draft passes) streams
 tiled copy of its weight through lollm_gemm, with SiLU(gate) * up fused into the
 gate|up GEMM; longer calls (the prefill) take lollm_gemm_rows on the same copy, SwiGLU
 fused too, where its tiles (or its parts of a long K) fill the chip, else hipBLASLt on the row-major weight.
+Projection4 holds a weight in 4 bits instead, for any number of rows.
 """
 
 from __future__ import annotations

@@ -23,6 +23,9 @@ for the MI355X kernels:
 
 Qwen3_5PagedCache holds the full-attention layers' keys and values in pages instead, in bf16
 or in 8 bits: a sequence takes the pages it fills, and gives them back.
+
+A forward over a tree of drafts writes its nodes' rows and records behind the committed ones and
+commits nothing; keep_path moves the accepted path's to the front and sets the indices.
 """
 
 from __future__ import annotations
