@@ -715,7 +715,7 @@ def gemm_q4(x, weight, out=None):
     M = x.numel() // K
     if M == 0:
         return out
-    need = _q4_workspace_bytes(M, N, K, weight.group, dev)
+    need = _q4_workspace_bytes(M, N, K, weight.group, dev) if M > 64 else 0
     ws = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
     rc = _lib.lib().lollm_gemm_q4(xp, K, wp, weight.zeros, o, oc, ws, need, M, N, K, weight.group, weight.epilogue,
                                   torch._C._cuda_getCurrentRawStream(dev))
@@ -1137,6 +1137,40 @@ def _check_gdn_state(rec, rec_half, rep, replay, B, Hv, D):
     return rep.shape[3]
 
 
+def _gdn_layer_tree(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half, rep, replay, fresh, B, T, Hk,
+                    Hv, D, conv_kernel, eps, out, tree):
+    """gdn_layer with a tree (one look at each operand: a call of few nodes is host time)."""
+    dev = torch._C._cuda_getDevice()
+    if rep.dim() != 5 or win.dim() != 3 or win.shape[1] % 2:
+        raise ValueError(f"rep must be (B, 2, Hv, slots, {gdn_record_bytes(D)}) and win (B, 2 W, conv_dim)")
+    if min(B, T, Hk) < 1 or Hv % Hk:
+        raise ValueError(f"{B} sequences of {T} nodes with {Hk} and {Hv} heads")
+    S, W, P = rep.shape[3], win.shape[1] // 2, proj.shape[-1]
+    if T > S or conv_kernel - 1 + T > W or conv_kernel != 4:
+        raise ValueError(f"a tree of {T} nodes needs as many records ({S}) and {conv_kernel - 1 + T} window rows "
+                         f"({W}), and a convolution of 4 taps")
+    V = Hv * D
+    C = 2 * Hk * D + V
+    if P < C + V + 2 * Hv or P % 8:
+        raise ValueError(f"proj has rows of {P}, expected at least {C + V + 2 * Hv}, a multiple of 8")
+    f32, i32, bf16, row = torch.float32, torch.int32, torch.bfloat16, (B,)
+    words = _tree_arg(tree, B, T, dev)
+    if out is None:
+        out = proj.new_empty((B, T, V))
+    rc = _lib.lib().lollm_gdn_layer_tree(
+        _arg(proj, "proj", bf16, (B, T, P), dev), P, _arg(conv_w, "conv_w", bf16, (C, conv_kernel), dev),
+        _arg(A_log, "A_log", f32, (Hv,), dev), _arg(dt_bias, "dt_bias", f32, (Hv,), dev),
+        _arg(norm_w, "norm_w", bf16, (D,), dev), _arg(win, "win", bf16, (B, 2 * W, C), dev),
+        _arg(conv_off, "conv_off", i32, row, dev), W, _arg(rec, "rec", f32, (B, 2, Hv, D, D), dev),
+        _arg(rec_half, "rec_half", i32, row, dev),
+        _arg(rep, "rep", torch.uint8, (B, 2, Hv, S, gdn_record_bytes(D)), dev), _arg(replay, "replay", i32, row, dev), S,
+        1 if fresh else 0, words, _arg(out, "out", bf16, (B, T, V), dev), B, T, Hk, Hv, D, D, conv_kernel, eps,
+        torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, "lollm_gdn_layer_tree")
+    return out
+
+
 def gdn_layer(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half, rep, replay,
               fresh, B, T, Hk, Hv, D, conv_kernel, eps, out=None, chunked=None, tree=None):
     """Fused GDN mixer (include/lollm_amd.h).  proj (B, T, P) bf16; win (B, 2W,
@@ -1147,6 +1181,9 @@ def gdn_layer(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half
     tree: (B, T) int64 of tree_masks, the T positions are the nodes of a tree of drafts, each of which
     continues from its parent (lollm_gdn_layer_tree: T <= TREE_MAX and S, the window's rows for it;
     what all nodes bring must be finite)."""
+    if tree is not None:
+        return _gdn_layer_tree(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half, rep, replay, fresh,
+                               B, T, Hk, Hv, D, conv_kernel, eps, out, tree)
     P = proj.shape[-1]
     _need(proj, "proj", torch.bfloat16)
     _need(win, "win", torch.bfloat16)
@@ -1158,27 +1195,6 @@ def gdn_layer(proj, conv_w, A_log, dt_bias, norm_w, win, conv_off, rec, rec_half
     if out is None:
         out = torch.empty(B, T, value_dim, dtype=torch.bfloat16, device=proj.device)
     W = win.shape[1] // 2
-    if tree is not None:
-        dev = torch._C._cuda_getDevice()
-        if T > S or conv_kernel - 1 + T > W or conv_kernel != 4:
-            raise ValueError(f"a tree of {T} nodes needs as many records ({S}) and {conv_kernel - 1 + T} window rows "
-                             f"({W}), and a convolution of 4 taps")
-        C, V = 2 * Hk * D + Hv * D, Hv * D
-        if P < C + V + 2 * Hv or P % 8 or min(B, T, Hk) < 1 or Hv % Hk:
-            raise ValueError(f"proj has rows of {P}, expected at least {C + V + 2 * Hv}, a multiple of 8")
-        words = _tree_arg(tree, B, T, dev)
-        rc = _lib.lib().lollm_gdn_layer_tree(
-            _arg(proj, "proj", torch.bfloat16, (B, T, P), dev), P,
-            _arg(conv_w, "conv_w", torch.bfloat16, (C, conv_kernel), dev), _arg(A_log, "A_log", torch.float32, (Hv,), dev),
-            _arg(dt_bias, "dt_bias", torch.float32, (Hv,), dev), _arg(norm_w, "norm_w", torch.bfloat16, (D,), dev),
-            _arg(win, "win", torch.bfloat16, (B, 2 * W, C), dev), _arg(conv_off, "conv_off", torch.int32, (B,), dev), W,
-            _arg(rec, "rec", torch.float32, rec.shape, dev), _arg(rec_half, "rec_half", torch.int32, (B,), dev),
-            _arg(rep, "rep", torch.uint8, rep.shape, dev), _arg(replay, "replay", torch.int32, (B,), dev), S,
-            int(bool(fresh)), words, _arg(out, "out", torch.bfloat16, (B, T, V), dev), B, T,
-            Hk, Hv, D, D, conv_kernel, float(eps), torch._C._cuda_getCurrentRawStream(dev))
-        if rc:
-            _lib.check(rc, "lollm_gdn_layer_tree")
-        return out
     if chunked is None:
         chunked = T >= GDN_CHUNK_MIN_T and gdn_chunked_ok(T, S, W, conv_kernel, P)
     fn, ws = "lollm_gdn_layer_chunked" if chunked else "lollm_gdn_layer", ()
