@@ -210,6 +210,7 @@ int attn_grid(int grid);
 int attn_prefill_groups(int B, int T, int Hkv, int n_rep, int cus);
 int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st, const PagedArgs* paged = nullptr,
                         int parts = 1);
+int attn_slab_tree(const AttnArgs& a, hipStream_t st);   // attn_paged.hip's kernels over slabs
 // For pages: workgroups of 128-row tiles that share a CU, or 0 for the split-K kernels, and the
 // workgroups that a tile's keys are dealt out to, with the bytes of workspace that takes.
 int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts, bool tree = false);

@@ -91,7 +91,8 @@ __device__ __forceinline__ void pg_read_rows(uint32_t at, u32x2_t (&v)[8]) {
 #undef RD
 }
 
-template <bool F8, bool TREE>
+// SLAB: the rows of (sequence, KV head) lie in one run at its strides, a "page" is the sequence.
+template <bool F8, bool TREE, bool SLAB>
 __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) {
   using Set = PagedSet<F8>;
   const AttnArgs& a = p.a;
@@ -159,8 +160,12 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
     for (int g = 0; g < 2; ++g) {
       const int key = tj * AT_BLOCK + PG_WKEYS * wave + 16 * g;
       const bool in = key >= 0 && key < tL;   // (a table of 2^31 rows: a last block's keys may wrap)
-      const int id = in ? p.table[(long long)lo * p.table_stride + (key >> p.pshift)] : -1;
-      tp[g] = id >= 0 && id < p.n_pages ? id : -1;
+      if constexpr (SLAB) {
+        tp[g] = in ? lo : -1;
+      } else {
+        const int id = in ? p.table[(long long)lo * p.table_stride + (key >> p.pshift)] : -1;
+        tp[g] = id >= 0 && id < p.n_pages ? id : -1;
+      }
     }
   };
   auto look_up_scales = [&]() {
@@ -207,15 +212,17 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
   constexpr int KAHEAD = F8 ? 2 : 1;  // blocks that K is asked for ahead of its products
   u32x4_t kr[KAHEAD][KL], qr[4];
   const int pmask = (1 << p.pshift) - 1;
-  auto row_of = [&](const PgUnit& X, int page, int key) {   // the pool's row of a key in that page
+  auto byte_of = [&](const PgUnit& X, int page, int key) {   // of a key's row in that page, in the pool
     const int kvh = X.ph / a.qblocks;
-    return (((long long)page * a.Hkv + kvh) << p.pshift) + (key & pmask);
+    if constexpr (SLAB) return (page * a.seq_stride + kvh * a.head_stride) * 2 + (long long)key * Set::ROW;
+    else return ((((long long)page * a.Hkv + kvh) << p.pshift) + (key & pmask)) * Set::ROW;
   };
   auto issue_k = [&](u32x4_t (&to)[KL], const PgUnit& X) {
     const int key0 = X.j * AT_BLOCK + PG_WKEYS * wave;
-    const long long r0 = row_of(X, max(X.page[0], 0), key0), r1 = row_of(X, max(X.page[1], 0), key0 + 16);
-    // (without a page all lanes read the pool's first bytes, one line an instruction)
-    const long long at = (l32 < 16 ? r0 : r1) * Set::ROW + (l32 & 15) * Set::ROW + 16 * h;
+    const long long r0 = byte_of(X, max(X.page[0], 0), key0), r1 = byte_of(X, max(X.page[1], 0), key0 + 16);
+    // (without a page all lanes read the pool's first bytes, one line an instruction; a slab ends anywhere)
+    const int row = SLAB ? min(key0 + l32, a.max_len - 1) - key0 - (l32 & 16) : l32 & 15;
+    const long long at = (l32 < 16 ? r0 : r1) + row * Set::ROW + 16 * h;
     const unsigned char* src =
         reinterpret_cast<const unsigned char*>(a.kc) + ((l32 < 16 ? X.page[0] : X.page[1]) >= 0 ? at : 0);
 #pragma unroll
@@ -229,7 +236,7 @@ __global__ __launch_bounds__(AW_THREADS, 1) void attn_paged_kernel(PagedArgs p) 
       const int key = key0 + 16 * g;
       const int rows = X.page[g] >= 0 ? min(X.L - key, 16) : 0;   // (a mapped group begins before L)
       const __amdgpu_buffer_rsrc_t rs =
-          buf_rsrc(reinterpret_cast<const unsigned char*>(a.vc) + row_of(X, max(X.page[g], 0), key) * Set::ROW,
+          buf_rsrc(reinterpret_cast<const unsigned char*>(a.vc) + byte_of(X, max(X.page[g], 0), key),
                    (uint32_t)(rows * Set::ROW));
       if constexpr (F8) {
         // four rows a DMA: lane -> row 4 i + lane / 16, chunk (lane % 16) ^ row
@@ -619,6 +626,19 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedArgs p) {
   at_store4(a.out + (bt * a.Hq + h) * AT_D + 4 * lane, acc, l == 0.f ? 0.f : 1.f / l, a.gate != nullptr, gv);
 }
 
+// A tree over slabs (attn_verify.hip says when).  The workspace is attn_verify's, which is laid out alike.
+int attn_slab_tree(const AttnArgs& a, hipStream_t st) {
+  PagedArgs p = {};
+  p.a = a;
+  p.rep_mul = (uint32_t)((65536 + a.n_rep - 1) / a.n_rep);
+  hipLaunchKernelGGL((attn_paged_kernel<false, true, true>), dim3(a.nw), dim3(AW_THREADS), 0, st, p);
+  const int rc = launch_status();
+  if (rc) return rc;
+  hipLaunchKernelGGL(attn_paged_combine_kernel, dim3((a.n_rep * a.QB + 3) / 4, (unsigned)(a.B * a.Hkv * a.qblocks)),
+                     dim3(256), 0, st, p);
+  return launch_status();
+}
+
 }  // namespace lollm
 
 using namespace lollm;
@@ -695,8 +715,8 @@ static int attn_paged_call(const void* q, const void* k_pages, const void* v_pag
   p.rep_mul = (uint32_t)((65536 + n_rep - 1) / n_rep);
   hipStream_t st = (hipStream_t)stream;
   if (groups) return attn_prefill_launch(a, groups, st, &p, parts);
-  auto* kernel = tree ? (f8 ? attn_paged_kernel<true, true> : attn_paged_kernel<false, true>)
-                      : (f8 ? attn_paged_kernel<true, false> : attn_paged_kernel<false, false>);
+  auto* kernel = tree ? (f8 ? attn_paged_kernel<true, true, false> : attn_paged_kernel<false, true, false>)
+                      : (f8 ? attn_paged_kernel<true, false, false> : attn_paged_kernel<false, false, false>);
   hipLaunchKernelGGL(kernel, dim3(nw), dim3(AW_THREADS), 0, st, p);
   if ((rc = launch_status())) return rc;
   hipLaunchKernelGGL(attn_paged_combine_kernel, dim3((n_rep * QB + 3) / 4, (unsigned)pairs), dim3(256), 0, st, p);

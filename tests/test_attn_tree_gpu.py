@@ -324,3 +324,22 @@ def test_tree_entry_points_check_before_any_launch():
     assert L.lollm_attn_paged_tree(*head, None, None, 0, 0, p, p, 1 << 30, 1, 4, 4, 2, D, 8, 0.0625, None) == 1
     assert L.lollm_attn_paged_tree(*head, p, None, 0, 0, p, p, 1 << 30, 1, 65, 4, 2, D, 8, 0.0625, None) == 2
     assert L.lollm_attn_paged_tree_workspace_bytes(1, 65, 4, 2, D, 0, 8) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,hq,hkv,lens,max_len", [(2, 5, 8, 2, [131, 40], 131), (1, 16, 32, 4, [600], 9001),
+                                                     (3, 7, 8, 1, [7, 0, 1021], 1021), (1, 3, 2, 2, [3], 3)], ids=str)
+def test_attn_tree_slabs_that_end_anywhere(B, T, hq, hkv, lens, max_len):
+    """Capacities that no block divides, sequences that fill them, long slabs with few keys; rows past the
+    lengths are NaN."""
+    from lollm_amd import ops
+    print("case tree attention, slabs of", max_len, lens, flush=True)
+    q, k, v, gate = inputs(B, T, hq, hkv, [max_len] * B, 4)
+    _, words = tree(B, T, 4, 2)
+    kc, vc = k.clone(), v.clone()
+    for b in range(B):
+        kc[b, :, lens[b]:] = float("nan")
+        vc[b, :, lens[b]:] = float("nan")
+    got = ops.attn_verify(q.cuda(), kc.cuda(), vc.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                          gate.reshape(B, T, hq * D).cuda(), tree=words.cuda())
+    close(got, *reference(q, k, v, gate, lens, words))
