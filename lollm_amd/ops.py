@@ -247,6 +247,38 @@ def _tree_arg(tree, B, T, dev):
     return _arg(tree, "tree", torch.int64, (B, T), dev)
 
 
+@functools.lru_cache(maxsize=4096)
+def _attn_tree_workspace_bytes(B, T, Hq, Hkv, D, max_len, grid, device):
+    return attn_workspace_bytes(B, T, Hq, Hkv, D, max_len, grid)
+
+
+def _attn_tree(q, k_cache, v_cache, kv_len, gate, grid, scale, workspace, out, tree):
+    """attn_verify with a tree (one look at each operand, as _arg)."""
+    dev = torch._C._cuda_getDevice()
+    if q.dim() != 4 or k_cache.dim() != 4:
+        raise ValueError("q must be (B, T, Hq, D) and k_cache (B, Hkv, max_len, D)")
+    B, T, Hq, D = q.shape
+    Hkv, max_len = k_cache.shape[1], k_cache.shape[2]
+    bf16, rows = torch.bfloat16, (B, Hkv, max_len, D)
+    words = _tree_arg(tree, B, T, dev)
+    x, k, v = _arg(q, "q", bf16, q.shape, dev), _arg(k_cache, "k_cache", bf16, rows, dev), _arg(v_cache, "v_cache", bf16, rows, dev)
+    ln = _arg(kv_len, "kv_len", torch.int32, (B,), dev)
+    g = None if gate is None else _arg(gate, "gate", bf16, (B, T, Hq * D), dev)
+    if out is None:
+        out = q.new_empty((B, T, Hq * D))
+    o = _arg(out, "out", bf16, (B, T, Hq * D), dev)
+    if workspace is None:
+        workspace = q.new_empty(_attn_tree_workspace_bytes(B, T, Hq, Hkv, D, max_len, grid, dev if grid <= 0 else -1),
+                                dtype=torch.uint8)
+    ws = _arg(workspace, "workspace", workspace.dtype, workspace.shape, dev)
+    rc = _lib.lib().lollm_attn_tree(x, k, v, ln, words, g, o, ws, workspace.numel() * workspace.element_size(), B, T, Hq,
+                                    Hkv, D, max_len, Hkv * max_len * D, max_len * D, grid,
+                                    D ** -0.5 if scale is None else float(scale), torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, "lollm_attn_tree")
+    return out
+
+
 def attn_verify(q, k_cache, v_cache, kv_len, gate=None, *, grid=0, scale=None,
                 workspace=None, out=None, tree=None):
     """q (B, T, Hq, D) bf16; k_cache / v_cache (B, Hkv, max_len, D) bf16 with the T
@@ -256,6 +288,8 @@ def attn_verify(q, k_cache, v_cache, kv_len, gate=None, *, grid=0, scale=None,
     that fill the chip one workgroup per query tile).  tree: (B, T) int64 of tree_masks, the T
     positions are the nodes of a tree of drafts, each of which sees the keys before the tree, its
     ancestors and itself (all nodes' values must be finite)."""
+    if tree is not None:
+        return _attn_tree(q, k_cache, v_cache, kv_len, gate, grid, scale, workspace, out, tree)
     B, T, Hq, D = q.shape
     _need(q, "q", torch.bfloat16)
     if k_cache.dim() != 4 or k_cache.shape[0] != B or k_cache.shape[3] != D:
@@ -276,18 +310,6 @@ def attn_verify(q, k_cache, v_cache, kv_len, gate=None, *, grid=0, scale=None,
     wbytes = workspace.numel() * workspace.element_size()
     if scale is None:
         scale = D ** -0.5
-    if tree is not None:
-        dev = torch._C._cuda_getDevice()
-        t = _tree_arg(tree, B, T, dev)
-        _arg(q, "q", torch.bfloat16, q.shape, dev)
-        _arg(k_cache, "k_cache", torch.bfloat16, k_cache.shape, dev)
-        _arg(kv_len, "kv_len", torch.int32, (B,), dev)
-        rc = _lib.lib().lollm_attn_tree(
-            _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(kv_len), t, _ptr(gate), _ptr(out),
-            _ptr(workspace), wbytes, B, T, Hq, Hkv, D, max_len, Hkv * max_len * D, max_len * D,
-            grid, float(scale), _stream())
-        _lib.check(rc, "lollm_attn_tree")
-        return out
     rc = _lib.lib().lollm_attn_verify(
         _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(kv_len), _ptr(gate), _ptr(out),
         _ptr(workspace), wbytes, B, T, Hq, Hkv, D, max_len, Hkv * max_len * D, max_len * D,
