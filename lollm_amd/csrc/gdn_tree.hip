@@ -357,7 +357,8 @@ __global__ __launch_bounds__(GT_THREADS, MT < 4 ? 4 : 2) void gdn_tree_kernel(Gt
       const int i = min(16 * I + 4 * g4 + r, T - 1);
       z[I][r] = a.proj[((size_t)b * T + i) * a.P + a.C + (size_t)h * GL_DK + col];
     }
-  gt_f32x4 U[MT], O[MT];
+  // the products with the state of all rows first: the chain below waits for none of them
+  gt_f32x4 U[MT], O[MT];   // (U: the right sides until solved)
 #pragma unroll
   for (int I = 0; I < MT; ++I) {
     gt_f32x4 ks[2], qs[2];   // with the state's high and low parts
@@ -371,14 +372,17 @@ __global__ __launch_bounds__(GT_THREADS, MT < 4 ? 4 : 2) void gdn_tree_kernel(Gt
       ks[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, Sl[s], ks[1], 0, 0, 0);
       qs[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, Sl[s], qs[1], 0, 0, 0);
     }
-    gt_f32x4 rhs;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * I + 4 * g4 + r;
       const float E = sh.E[i];
-      rhs[r] = sh.beta[i] * (bf16_to_f32(sh.v[i][col]) - E * sh.rk[i] * (ks[0][r] + ks[1][r]));
+      U[I][r] = sh.beta[i] * (bf16_to_f32(sh.v[i][col]) - E * sh.rk[i] * (ks[0][r] + ks[1][r]));
       O[I][r] = E * sh.rq[i] * (qs[0][r] + qs[1][r]);
     }
+  }
+#pragma unroll
+  for (int I = 0; I < MT; ++I) {
+    gt_f32x4 rhs = U[I];
 #pragma unroll
     for (int J = 0; J < I; ++J) {
       const float4 m = *reinterpret_cast<const float4*>(&sh.m.am[16 * I + c16][16 * J + 4 * g4]);
