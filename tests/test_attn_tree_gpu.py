@@ -343,3 +343,19 @@ def test_attn_tree_slabs_that_end_anywhere(B, T, hq, hkv, lens, max_len):
     got = ops.attn_verify(q.cuda(), kc.cuda(), vc.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
                           gate.reshape(B, T, hq * D).cuda(), tree=words.cuda())
     close(got, *reference(q, k, v, gate, lens, words))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", (16, 8))
+def test_attn_tree_parts_of_rows_of_any_size(bits):
+    """Keys dealt out in parts whose values differ by powers of two from part to part and head to head, from
+    2^-40 to 2^60 in bf16: a part's pieces are in units of their own."""
+    B, T, hq, hkv, lens = 2, 24, 32, 4, [1500, 777]
+    print("case tree attention, sizes of values", bits, flush=True)
+    q, k, v, gate = inputs(B, T, hq, hkv, lens, 21)
+    step = torch.arange(1500) // 96
+    size = (step * 7 % 11 - 4) * (10 if bits == 16 else 1)
+    v = (v.float() * torch.exp2(size.float())[None, None, :, None] * torch.tensor([1.0, 2.0 ** 10, 2.0 ** -10, 1.0])[None, :, None, None]).bfloat16()
+    _, words = tree(B, T, 6, 5)
+    got, kh, vh = run((64, bits), q, k, v, gate, lens, words)
+    close(got, *reference(q, kh, vh, gate, lens, words))
