@@ -129,8 +129,10 @@ __device__ __forceinline__ int ap_tree_blocks(const ApArgs& a, int b) {
 struct ApShare { int b, part, parts; };   // b < 0: a spare one
 __device__ __forceinline__ ApShare ap_tree_share(const ApArgs& a, int s, int lane) {
   uint64_t total = 0;   // (64 sequences' blocks fit 32 bits)
+  int blocks = 0;       // the lane's, of the last 64
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    uint32_t n = (uint32_t)ap_tree_blocks(a, b0 + lane);
+    blocks = ap_tree_blocks(a, b0 + lane);
+    uint32_t n = (uint32_t)blocks;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
     total += n;
@@ -138,7 +140,8 @@ __device__ __forceinline__ ApShare ap_tree_share(const ApArgs& a, int s, int lan
   const int more = a.B * (a.parts - 1);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const uint64_t n = (uint64_t)ap_tree_blocks(a, b0 + lane) * (uint32_t)more;
+    if (a.B > 64) blocks = ap_tree_blocks(a, b0 + lane);
+    const uint64_t n = (uint64_t)blocks * (uint32_t)more;
     // (the quotient in 64 bits is never rounded up to a whole number: both are below 2^53 / 2^10)
     const int mine = b0 + lane >= a.B ? 0 : min(1 + (total ? (int)((double)n / (double)total) : 0), AP_MAX_PARTS);
     int upto = mine;
@@ -192,6 +195,23 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
   }
   const int b = pair / a.Hkv, kvh = pair % a.Hkv;
   const int q0 = qt * a.QB, QB = min(a.QB, a.T - q0);
+  // this lane's rows: position q0 + qi, query head kvh n_rep + hr
+  uint64_t word[RG];
+  bf16x8 Q[RG][16];
+  auto load_q = [&]() {
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+      const int r = 32 * (RG * wave + rg) + l32, qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
+      const bool live = qi < QB;
+      if constexpr (TREE) word[rg] = a.tree[(size_t)b * a.T + q0 + (live ? qi : 0)];
+      const uint16_t* src = a.q + (((size_t)b * a.T + q0 + (live ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D;
+#pragma unroll
+      for (int ks = 0; ks < 16; ++ks)   // (8 bits: a lane's 16 codes of K are two k-steps)
+        Q[rg][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(
+                                                   src + (F8 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1) : 16 * ks + 8 * h)));
+    }
+  };
+  if constexpr (TREE) load_q();   // (on its way while the lengths and the table are read)
   const int L = min(max(a.kv_len[b], 0), a.max_len);
   const int p0 = L - a.T + q0;                       // position of the tile's first query
   const int keys = min(max(p0 + QB, 0), L);          // keys any row of the tile sees
@@ -316,21 +336,12 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
   constexpr int QL = SETS == 2 ? 4 : 0;
   __shared__ __attribute__((aligned(16))) unsigned char qlate[QL ? AP_WAVES * QL * 1024 : 16];
   unsigned char* const ql = qlate + (QL ? 1024 * QL * wave + 16 * lane : 0);
-  // this lane's rows: position q0 + qi, query head kvh n_rep + hr
+  if constexpr (!TREE) load_q();
   int qpos[RG];
-  uint64_t word[RG];
-  bf16x8 Q[RG][16];
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
-    const int r = 32 * (RG * wave + rg) + l32, qi = ap_div(r, a.rep_mul), hr = r - qi * a.n_rep;
-    const bool live = qi < QB;
-    qpos[rg] = live ? p0 + qi : -1;
-    if constexpr (TREE) word[rg] = a.tree[(size_t)b * a.T + q0 + (live ? qi : 0)];
-    const uint16_t* src = a.q + (((size_t)b * a.T + q0 + (live ? qi : 0)) * a.Hq + kvh * a.n_rep + hr) * AT_D;
-#pragma unroll
-    for (int ks = 0; ks < 16; ++ks)   // (8 bits: a lane's 16 codes of K are two k-steps)
-      Q[rg][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_t*>(
-                                                 src + (F8 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1) : 16 * ks + 8 * h)));
+    const int qi = ap_div(32 * (RG * wave + rg) + l32, a.rep_mul);
+    qpos[rg] = qi < QB ? p0 + qi : -1;
 #pragma unroll
     for (int i = 0; i < QL; ++i) *reinterpret_cast<bf16x8*>(ql + 1024 * i) = Q[rg][16 - QL + i];
   }
@@ -882,7 +893,7 @@ int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* p
   // keys 25 / 20, over 30000 50 / 68; 1 x 16 26 / 21, 52 / 82; 4 x 7 over 500 23 / 18, over 16000 67 / 85;
   // 4 x 63 34 / 36, 224 / 439; 8 bits: 1 x 16 over 2000 26 / 18, over 30000 52 / 50; 4 x 16 38 / 25, over 16000
   // 73 / 86; 1 x 63 40 / 29, over 30000 97 / 137; 16 x 63 over 8000 311 / 614).
-  if (tree && (T * n_rep <= AT_ROWS || (long long)B * T * Hkv * n_rep < (f8 ? 2048 : 512))) return 0;
+  if (tree && (T * n_rep <= AT_ROWS || (long long)B * T * Hkv * n_rep < (f8 ? 1536 : 512))) return 0;
   if (!tree && (T < AP_MIN_T || (long long)B * T <= AP_FEW_ROWS)) return 0;
   const long long pairs = (long long)B * Hkv;
   // Query tiles, whatever their number (us, tiles / split-K, bf16: 20 tiles of 2070 keys 35 / 38, of
