@@ -159,7 +159,8 @@ int lollm_tree_keep_gdn(void* rep, void* win, const int32_t* rec_half, const int
  * in cache row kv_len[b] - T + i, and query i sees every key before them and, of the nodes up to
  * itself, those whose bits its word in `tree` (B, T) has.  Values of all nodes must be finite (a
  * weight of 0 meets them).  Workspaces: lollm_attn_workspace_bytes, and for pages
- * lollm_attn_paged_tree_workspace_bytes.  T <= 64. */
+ * lollm_attn_paged_tree_workspace_bytes.  T <= 64.  Given a grid, a chain's bits are those of the plain
+ * call with that grid; with 0 the call takes the form that is fastest for its rows. */
 int lollm_attn_tree(const void* q, const void* k_cache, const void* v_cache, const int32_t* kv_len,
                     const void* tree, const void* gate, void* out, void* workspace,
                     long long workspace_bytes, int B, int T, int Hq, int Hkv, int D, int max_len,

@@ -22,6 +22,9 @@
 //      become bf16 with v_cvt_scalef32_pk_bf16_fp8, which applies the scale; V is read with the
 //      transposing 8-bit LDS read and becomes fp16 (at_f16).
 // Weights enter the product with V as hi + lo bf16 (attn_prefill.hip), with 8-bit V as fp16.
+// TREE: the new positions are the nodes of a tree of drafts; in the blocks that reach them a query's word of
+// ancestors masks the keys beside the position (1 x 7 nodes over 138 keys 14.5 us, 16 x 7 over 2000, 8 rows a head,
+// 43; SLAB, the same over slabs: 14.5 and 52).
 //
 // What bounds it: the KV stream from some ten blocks a workgroup on, a fixed 12 us before.  16 x 4
 // tokens, 32 / 4 heads, inputs in turn (us, TB/s of K and V): 128 keys 17 (8 bits 14.3), 1024 25.8, 2.6
