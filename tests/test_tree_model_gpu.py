@@ -287,6 +287,54 @@ def test_4_bit_speculative_decoder_replayed(micro):
 
 
 @pytest.mark.gpu
+def test_load_checkpoint_in_4_bits(tmp_path):
+    """A checkpoint loaded with weight_bits=4 is the loaded model quantised: the same bits."""
+    from lollm_amd.qwen3_5 import load, load_checkpoint
+    from lollm_amd.qwen3_5.blocks import Projection4
+    from test_checkpoint import micro_weights, write_checkpoint
+    raw, W = micro_weights(seed=6)
+    write_checkpoint(str(tmp_path), raw, W)
+    model, mtp, unused = load_checkpoint(str(tmp_path), weight_bits=4, group=64)
+    assert unused == [] and isinstance(model.model.layers[0].mlp.down, Projection4)
+    assert isinstance(mtp.layers[0].mlp.down, Projection4) and model.model.layers[0].mlp.down.q4.group == 64
+    ref = load(raw, dict(W), "hf", device="cuda").quantize(64)
+    ids = torch.randint(0, raw["vocab_size"], (2, 7), generator=torch.Generator().manual_seed(1)).cuda()
+    print("case checkpoint in 4 bits", flush=True)
+    assert torch.equal(model(ids, model.new_cache(2, 32))[0], ref(ids, ref.new_cache(2, 32))[0])
+
+
+@pytest.mark.gpu
+def test_tree_beside_a_released_sequence(micro):
+    """A released sequence's nodes mean nothing, take no pages and leave the others' tree as it is, over several
+    trees; the others' numbers at the model tests' bar (keys are dealt out by all sequences' lengths)."""
+    from lollm_amd import ops
+    model, _, _, cfg = micro
+    g = torch.Generator().manual_seed(12)
+    prompt = torch.randint(0, cfg.vocab_size, (2, 20), generator=g).cuda()
+    nodes = [torch.randint(0, cfg.vocab_size, (2, 13), generator=g).cuda() for _ in range(3)]
+    mask, depth = ops.tree_masks(torch.tensor(PARENTS, dtype=torch.int32).cuda())
+    path = torch.tensor([[0, 1, 3], [0, 1, 2]], dtype=torch.int32).cuda()
+    count = torch.tensor([3, 2], dtype=torch.int32).cuda()
+    out = []
+    for released in (False, True):
+        cache = model.new_cache(2, 96, spec_slots=13, page=16)
+        model(prompt, cache)
+        if released:
+            cache.release(0)
+        rows = []
+        print("case tree beside a released sequence", released, flush=True)
+        for ids in nodes:
+            rows.append(model(ids, cache, tree=(mask, depth))[0][1].float())
+            cache.keep_path(path, count)
+        if released:
+            assert cache.held[0] == 0
+        assert int(cache.lengths[1]) == 20 + 3 * 2
+        out.append(torch.cat(rows))
+    cs = torch.nn.functional.cosine_similarity
+    assert (1 - cs(out[0], out[1], dim=-1)).max().item() <= 1e-3
+
+
+@pytest.mark.gpu
 def test_tree_refusals(micro):
     from lollm_amd import ops
     model = micro[0]
