@@ -475,7 +475,7 @@ __global__ __launch_bounds__(Q4_THREADS) void gemm_q4_lds_kernel(Q4Args a) {
 // that nothing is lost; s (16 + z) has 13 bits and needs two).  In the loop that leaves the decoding
 // (7 instructions for 8 codes), the products and, a group's end, its scale: 192 VALU instructions a stage
 // beside 64 products of 16 cycles.
-// 1999 x 18432 x 4096, groups of 128: 303 us, 995 TF (64: 423, 32: 453), 63% of what a bf16 product of 8192^3
+// 1999 x 18432 x 4096, groups of 128: 300 to 316 us by the card, 955 to 1000 TF (64: 379, 32: 454), 63% of what a bf16 product of 8192^3
 // reaches here.  The decoding is what is left: it and the products of two waves share a SIMD's issue.
 constexpr int QR_BM = 128, QR_BN = 256;
 constexpr int QR_CODES = QR_BM * 256, QR_SCALES = QR_CODES + QR_BN * 64;   // a slot: rows, codes, scales
@@ -577,16 +577,18 @@ __global__ __launch_bounds__(512, 1) void gemm_q4_rows_kernel(Q4Args a) {
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int g = 0; g < GPS; ++g) sc[j][g] = {0, 0};
-  auto take = [&](int g) {   // a finished group's sums, with its scales
+  auto take_tile = [&](int j, int g) {   // a finished group's sums, with its scales
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t b = sc[j][g][e >> 1];
+      const float f = __uint_as_float(e & 1 ? b & 0xffff0000u : b << 16);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t b = sc[j][g][e >> 1];
-        const float f = __uint_as_float(e & 1 ? b & 0xffff0000u : b << 16);
+      for (int i = 0; i < 4; ++i) tot[j][i][e] = fmaf(f, c[j][i][e], tot[j][i][e]);
+    }
+  };
+  auto take = [&](int g) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tot[j][i][e] = fmaf(f, c[j][i][e], tot[j][i][e]);
-      }
+    for (int j = 0; j < 4; ++j) take_tile(j, g);
   };
   const int ar = (64 * wm + l16) * 256;
   auto stage = [&](auto at, int st) {
@@ -612,9 +614,9 @@ __global__ __launch_bounds__(512, 1) void gemm_q4_rows_kernel(Q4Args a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           x[(q + 1) & 1][i] = *reinterpret_cast<const u32x4_t*>(slot + ar + 4096 * i + 16 * ((4 * (q + 1) + g4) ^ l16));
-      if (q && q % KPG == 0) take(q / KPG - 1);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        if (q && q % KPG == 0) take_tile(j, q / KPG - 1);   // (while the last tile's products run)
         const q4_bf16x8 f = q4_frag(w[j][q], kc);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
