@@ -738,9 +738,9 @@ def gemm_q4(x, weight, out=None):
     if M == 0:
         return out
     need = _q4_workspace_bytes(M, N, K, weight.group, dev) if M > 64 else 0
-    ws = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
-    rc = _lib.lib().lollm_gemm_q4(xp, K, wp, weight.zeros, o, oc, ws, need, M, N, K, weight.group, weight.epilogue,
-                                  torch._C._cuda_getCurrentRawStream(dev))
+    workspace = x.new_empty(need, dtype=torch.uint8) if need else None   # (held until the launches are on the stream)
+    rc = _lib.lib().lollm_gemm_q4(xp, K, wp, weight.zeros, o, oc, _ptr(workspace), need, M, N, K, weight.group,
+                                  weight.epilogue, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, "lollm_gemm_q4")
     return out
