@@ -8,7 +8,6 @@ namespace lollm {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -213,9 +212,8 @@ int attn_prefill_launch(const AttnArgs& a, int groups, hipStream_t st, const Pag
                         int parts = 1);
 int attn_slab_tree(const AttnArgs& a, hipStream_t st);   // attn_paged.hip's kernels over slabs
 // For pages: workgroups of 128-row tiles that share a CU, or 0 for the split-K kernels, and the
-// workgroups that a tile's keys are dealt out to, with the bytes of workspace that takes (half: of trees
-// over bf16 pages).
+// workgroups that a tile's keys are dealt out to, with the bytes of workspace that takes.
 int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* parts, bool tree = false);
-long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts, bool half);
+long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts);
 
 }  // namespace lollm

@@ -647,8 +647,8 @@ int attn_slab_tree(const AttnArgs& a, hipStream_t st) {
 using namespace lollm;
 
 // Workspace of a call: the split-K's pieces, or the parts' of query tiles.
-static long long paged_ws_bytes(int B, int T, int Hkv, int n_rep, int qblocks, int nw, int groups, int parts, bool half) {
-  const long long n = groups ? attn_parts_bytes(B, T, Hkv, n_rep, parts, half) : attn_ws_bytes(nw, (long long)B * Hkv * qblocks);
+static long long paged_ws_bytes(int B, int T, int Hkv, int n_rep, int qblocks, int nw, int groups, int parts) {
+  const long long n = groups ? attn_parts_bytes(B, T, Hkv, n_rep, parts) : attn_ws_bytes(nw, (long long)B * Hkv * qblocks);
   return n > 16 ? n : 16;
 }
 
@@ -658,7 +658,7 @@ static long long paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int
   const int nw = attn_grid(grid);
   if (nw <= 0 || nw > 1024 || (kv_dtype != LOLLM_BF16 && kv_dtype != LOLLM_F8)) return -1;
   const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, kv_dtype == LOLLM_F8, &parts, tree) : 0;
-  return paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts, tree && kv_dtype == LOLLM_BF16);
+  return paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts);
 }
 
 LOLLM_API long long lollm_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int kv_dtype,
@@ -702,7 +702,7 @@ static int attn_paged_call(const void* q, const void* k_pages, const void* v_pag
   const int groups = grid == 0 ? attn_paged_groups(B, T, Hkv, n_rep, nw, f8, &parts, tree != nullptr) : 0;
   if (!groups && pairs > 65535) return LOLLM_EUNSUPPORTED;                        // the combine's grid
   if (!groups && pairs * (rows / AT_BLOCK + 1) > 0x7fffffffLL) return LOLLM_EUNSUPPORTED;   // 32-bit block numbers
-  if (!workspace || workspace_bytes < paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts, tree && !f8)) return LOLLM_EINVAL;
+  if (!workspace || workspace_bytes < paged_ws_bytes(B, T, Hkv, n_rep, qblocks, nw, groups, parts)) return LOLLM_EINVAL;
   PagedArgs p;
   AttnArgs& a = p.a;
   a.q = (const uint16_t*)q; a.kc = (const uint16_t*)k_pages; a.vc = (const uint16_t*)v_pages;

@@ -65,12 +65,9 @@ constexpr int AP_AHEAD = 3;                    // operands read ahead of their p
 constexpr int AP_PART_BLOCKS = 8;              // blocks of a part of a tile's keys at least
 constexpr int AP_TREE_BLOCKS = 3;              // trees, few tiles for the chip: 500 keys of 1 x 16 nodes 22 us, at 8 blocks 41
 constexpr int AP_MAX_PARTS = 64;
-// Floats of a part of a 128-row tile: maxima, sums and O.  Trees over bf16 pages, whose few tiles have many parts:
-// maxima, sums, a power of two and O in units of it as fp16, off by 2^-12 of a value or 2^-25 of the row's largest
-// (16 x 16 nodes over 2000 keys 48 us, with pieces in 32 bits 52; 8-bit pages, whose kernel has half the registers,
-// spilled 43 of them for it and took 323 us where they take 245).
-constexpr int AP_PIECE = 2 * 128 + 128 * AT_D, AP_PIECE_HALF = 3 * 128 + 128 * AT_D / 2;
-constexpr int ap_piece(bool half) { return half ? AP_PIECE_HALF : AP_PIECE; }
+// Floats of a part of a 128-row tile: maxima, sums and O, all in 32 bits.  (O as fp16 in a unit of its row saves a
+// twelfth of the time of a tree over bf16 pages, and loses a row's small columns beside its large ones.)
+constexpr int AP_PIECE = 2 * 128 + 128 * AT_D;
 
 // Where the keys are: AP_ROWS one slab per (sequence, KV head); AP_PAGES, AP_PAGES8 pages that a
 // table names (attn_paged.hip), in bf16 or as e4m3 codes with scales.
@@ -166,8 +163,7 @@ __device__ __forceinline__ ApShare ap_tree_share(const ApArgs& a, int s, int lan
 // TREE: the new positions are the nodes of a tree of drafts, at_tree_keys.
 template <int RG, int KV, int SETS, bool TREE>
 __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1) void attn_prefill_kernel(ApArgs a) {
-  constexpr bool F8 = KV == AP_PAGES8, HALF = TREE && KV == AP_PAGES;
-  constexpr int PIECE = ap_piece(HALF);
+  constexpr bool F8 = KV == AP_PAGES8;
   constexpr int ROW = F8 ? AT_D : AT_D * 2;      // bytes of a key's row
   constexpr int AP_SET = AP_KEYS * ROW;          // K or V rows of a block
   // separate arrays, so that the reads of one set are not ordered after the DMA into another
@@ -708,30 +704,16 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
     if constexpr (F8) inv *= __int_as_float(v_ref);
     float* piece = nullptr;
     if constexpr (PARTS) {
-      float unit = 1.f;
-      if (HALF && !whole) {   // 2^up, the row's largest value below it
-        float top = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(O[rg][dt][r]));
-        const auto st = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(st[0]), __uint_as_float(st[1])) * inv;
-        const int up = top > 0.f && top < INFINITY ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 127) : 0;
-        inv = ldexpf(inv, -up);
-        unit = ldexpf(1.f, up);
-      }
       if (!whole) {
         const int tile = qt * pairs + pair;
-        piece = a.ws + (TREE ? (size_t)blockIdx.x : (size_t)tile * a.parts + part) * PIECE;
+        piece = a.ws + (TREE ? (size_t)blockIdx.x : (size_t)tile * a.parts + part) * AP_PIECE;
         if (h == 0) {
           piece[32 * wave + l32] = m_ref[0];
           piece[128 + 32 * wave + l32] = l;
-          if (HALF) piece[256 + 32 * wave + l32] = unit;
         }
       }
       if (tid == 0 && part == 0 && a.parts > 1)
-        reinterpret_cast<int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * PIECE)[qt * pairs + pair] =
+        reinterpret_cast<int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[qt * pairs + pair] =
             TREE ? (int)blockIdx.x << AP_TILE_PARTS | parts : parts;
     }
 #pragma unroll
@@ -770,14 +752,7 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
           y[4 * u] = f.x; y[4 * u + 1] = f.y; y[4 * u + 2] = f.z; y[4 * u + 3] = f.w;
         }
         if (!whole) {
-          if constexpr (HALF) {
-            if (live[it]) {
-              f16x8 t;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) t[e] = (_Float16)y[e];
-              *reinterpret_cast<f16x8*>(piece + 384 + ((32 * wave + rr) * AT_D + COLS * cp + 8 * c8) / 2) = t;
-            }
-          } else if (live[it]) {
+          if (live[it]) {
             float* to = piece + 256 + (32 * wave + rr) * AT_D + COLS * cp + 8 * c8;
             *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
             *reinterpret_cast<float4*>(to + 4) = make_float4(y[4], y[5], y[6], y[7]);
@@ -806,12 +781,11 @@ __global__ __launch_bounds__(64 * AP_WAVES, KV == AP_PAGES8 || SETS == 2 ? 2 : 1
 
 // Merges the parts of a tile, a wave per row (4 columns a lane), with the gate; tiles of one part
 // are finished already.  (Trees: a tile's parts begin at a place of their own, a.Hkv apart.)
-template <bool TREE, bool HALF>
+template <bool TREE>
 __global__ __launch_bounds__(256) void attn_parts_combine_kernel(ApArgs a) {
   const int pairs = a.B * a.Hkv, tile = blockIdx.x >> 5, lane = threadIdx.x & 63;
   const int r = 4 * (blockIdx.x & 31) + (threadIdx.x >> 6);
-  constexpr int PIECE = ap_piece(HALF);
-  const int entry = reinterpret_cast<const int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * PIECE)[tile];
+  const int entry = reinterpret_cast<const int*>(a.ws + (size_t)a.qtiles * pairs * a.parts * AP_PIECE)[tile];
   const int n = TREE ? entry & ((1 << AP_TILE_PARTS) - 1) : entry;
   if (n == 1) return;
   const int qt = tile / pairs, pair = tile - qt * pairs, b = pair / a.Hkv, kvh = pair - b * a.Hkv;
@@ -819,23 +793,14 @@ __global__ __launch_bounds__(256) void attn_parts_combine_kernel(ApArgs a) {
   if (qi >= min(a.QB, a.T - q0)) return;
   const int head = kvh * a.n_rep + r - qi * a.n_rep;
   const size_t bt = (size_t)b * a.T + q0 + qi;
-  const float* piece = a.ws + (TREE ? (size_t)(entry >> AP_TILE_PARTS) : (size_t)tile * a.parts) * PIECE;
-  const size_t next = (size_t)PIECE * (TREE ? a.Hkv : 1);
+  const float* piece = a.ws + (TREE ? (size_t)(entry >> AP_TILE_PARTS) : (size_t)tile * a.parts) * AP_PIECE;
+  const size_t next = (size_t)AP_PIECE * (TREE ? a.Hkv : 1);
   const float* mine = piece + min(lane, n - 1) * next;
   const float m = mine[r], ls = lane < n ? mine[128 + r] : 0.f;
-  const float unit = HALF ? mine[256 + r] : 1.f;
-  const float* col = piece + (HALF ? 384 + (r * AT_D + 4 * lane) / 2 : 256 + r * AT_D + 4 * lane);
-  auto load = [&](int s) {
-    if constexpr (HALF) {
-      const f16x4 t = *reinterpret_cast<const f16x4*>(col + min(s, n - 1) * next);
-      return make_float4((float)t[0], (float)t[1], (float)t[2], (float)t[3]);
-    } else {
-      return *reinterpret_cast<const float4*>(col + min(s, n - 1) * next);
-    }
-  };
+  const float* col = piece + 256 + r * AT_D + 4 * lane;
   float4 v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = load(e);
+  for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float4*>(col + min(e, n - 1) * next);
   uint2 gv = make_uint2(0, 0);
   if (a.gate)
     gv = *reinterpret_cast<const uint2*>(a.gate + bt * a.gate_row + (size_t)head * a.gate_head + 4 * lane);
@@ -851,13 +816,14 @@ __global__ __launch_bounds__(256) void attn_parts_combine_kernel(ApArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (s + e < n) {
-        const float x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt * unit), s + e));
+        const float x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), s + e));
         acc[0] += x * v[e].x; acc[1] += x * v[e].y; acc[2] += x * v[e].z; acc[3] += x * v[e].w;
       }
     }
     if (s + 4 < n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = load(s + 4 + e);
+      for (int e = 0; e < 4; ++e)
+        v[e] = *reinterpret_cast<const float4*>(col + min(s + 4 + e, n - 1) * next);
     }
   }
   at_store4(a.out + (bt * a.Hq + head) * AT_D + 4 * lane, acc, l == 0.f ? 0.f : 1.f / l, a.gate != nullptr, gv);
@@ -929,11 +895,11 @@ int attn_paged_groups(int B, int T, int Hkv, int n_rep, int cus, bool f8, int* p
   return per_cu;
 }
 
-long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts, bool half) {
+long long attn_parts_bytes(int B, int T, int Hkv, int n_rep, int parts) {
   int QB;
   if (parts <= 1) return 0;
   const long long tiles = (long long)prefill_tiles(B, T, Hkv, n_rep, 1, &QB) * B * Hkv;
-  return tiles * parts * ap_piece(half) * (long long)sizeof(float) + tiles * 4;
+  return tiles * parts * AP_PIECE * (long long)sizeof(float) + tiles * 4;
 }
 
 template <int RG, int KV, int SETS, bool TREE = false>
@@ -972,9 +938,8 @@ int attn_prefill_launch(const AttnArgs& v, int groups, hipStream_t st, const Pag
     const int rc = launch_status();
     if (rc) return rc;
     const dim3 grid((unsigned)(n / parts) * 32);
-    if (v.tree && paged->ks) hipLaunchKernelGGL((attn_parts_combine_kernel<true, false>), grid, dim3(256), 0, st, a);
-    else if (v.tree) hipLaunchKernelGGL((attn_parts_combine_kernel<true, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((attn_parts_combine_kernel<false, false>), grid, dim3(256), 0, st, a);
+    if (v.tree) hipLaunchKernelGGL(attn_parts_combine_kernel<true>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(attn_parts_combine_kernel<false>, grid, dim3(256), 0, st, a);
   }
   return launch_status();
 }
