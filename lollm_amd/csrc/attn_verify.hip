@@ -531,14 +531,13 @@ static int attn_verify_call(const void* q, const void* k_cache, const void* v_ca
     const int groups = attn_prefill_groups(B, T, Hkv, n_rep, nw);
     // (a tree's rows are at most 64 n_rep of a sequence: its tiles have 128)
     if (groups) return attn_prefill_launch(a, tree ? 1 : groups, st);
-    // Trees: the kernels for pages, within their limits, which start sooner and hold a weight in 16 bits; but for
-    // several query blocks of few (sequence, KV head)s over long slabs, as their hi + lo weights cost more than
-    // the start saves (us, pages' / these, 8 rows a head: 1 x 7 nodes over 130 keys 14 / 19, 16 x 7 over 2000 52 / 59,
-    // 16 x 16 over 8000 311 / 318, 1 x 1 over 30000 37 / 37; but 1 x 16 over 30000 84 / 66, 4 x 16 over 16000
-    // 162 / 122).  Given a grid, these: a chain's bits are then the plain call's.
+    // Trees: the kernels for pages, within their limits, which start sooner and hold a weight in 16 bits (us, pages' /
+    // these, 8 rows a head: 1 x 7 nodes over 130 keys 14 / 19, 16 x 7 over 2000 52 / 59, 16 x 16 over 8000 311 / 318,
+    // 1 x 1 over 30000 37 / 37; 1 x 16 over 30000 84 / 66, 4 x 16 over 16000 162 / 122, but these hold a weight in
+    // 8 bits, outputs within 2.0e-3 where those are within 1.66e-3, and the host knows a slab's capacity, not its
+    // keys).  Given a grid, these: a chain's bits are then the plain call's.
     const long long pairs = (long long)B * Hkv * qblocks;
-    const bool long_few = qblocks > 1 && B * Hkv <= 32 && max_len > 8192;
-    if (tree && !long_few && scale > 0.f && scale < INFINITY && Hkv <= 65535 && pairs <= 65535 &&
+    if (tree && scale > 0.f && scale < INFINITY && Hkv <= 65535 && pairs <= 65535 &&
         pairs * (max_len / AT_BLOCK + 1) <= 0x7fffffffLL)
       return attn_slab_tree(a, st);
   }
