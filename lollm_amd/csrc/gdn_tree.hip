@@ -11,7 +11,8 @@
 // The left side is a unit lower triangular matrix (a parent comes before its node): 16 x 16
 // blocks on its diagonal are inverted by the recurrence, the rest is block substitution in fp32 MFMA.
 // The products with S0 are bf16 MFMAs of the rows (bf16 as they are: q, k and v are bf16 tensors, which
-// the records hold) with S0 as hi + lo bf16, 16 bits of it; all sums are fp32.
+// the records hold) with S0 as hi + lo bf16, 16 bits of it (2^-17 of a term, the output keeps 2^-9); all sums
+// are fp32, those of the decays 64 bits, as their differences count.
 //
 // One workgroup of eight waves per (sequence, v-head).  Wave w owns value columns 16 w ..: its part of S0
 // lies in registers in the order in which the MFMA takes it as operand (lane 16 g + c: rows 32 s + 8 g
@@ -55,7 +56,8 @@ struct GtShared {
   uint16_t q[TP][GT_PW], k[TP][GT_PW], v[TP][GT_PW];
   uint16_t cw[GL_CH][GT_K];
   uint64_t word[TP];                         // ancestors, without the node itself
-  float G[TP], beta[TP], rk[TP], rq[TP], E[TP];
+  double G[TP];
+  float beta[TP], rk[TP], rq[TP], E[TP];
   float ss[GT_WAVES][TP], rn[TP];
   uint8_t up[TP][4];                         // rows of raw behind the taps 2, 1, 0
 };
@@ -176,19 +178,21 @@ __global__ __launch_bounds__(GT_THREADS, MT < 4 ? 4 : 2) void gdn_tree_kernel(Gt
     const uint64_t above = lane < T ? word_raw & ((1ull << lane) - 1) : 0ull;
     const float g = lane < T ? -__expf(a_log) * softplus_g(bf16_to_f32(aa_raw) + dtb) : 0.f;
     const float beta = lane < T ? 1.f / (1.f + __expf(-bf16_to_f32(bb_raw))) : 0.f;
-    // the path's sum by doubling: from the parent, its sum so far and its own
-    float G = g;
+    // the path's sum by doubling: from the parent, its sum so far and its own.  In 64 bits: the weights are
+    // differences of these sums, and a strong decay above both nodes (of 10^6 half a unit of the last place in 32
+    // bits is 0.03) cancels in them.  Past 10^6, infinity among them, e^g is 0 all the same.
+    double G = g < -1e6f ? -1e6f : g;
     int p = above ? 63 - __clzll((long long)above) : -1;
     for (int d = 1; d < T; d <<= 1) {
-      const float Gp = __shfl(G, max(p, 0), 64);
+      const double Gp = __shfl(G, max(p, 0), 64);
       const int pp = __shfl(p, max(p, 0), 64);
-      G += p >= 0 ? Gp : 0.f;
+      G += p >= 0 ? Gp : 0.;
       p = p >= 0 ? pp : -1;
     }
     if (lane < TP) {
       sh.word[lane] = above;
       sh.G[lane] = G;
-      sh.E[lane] = lane < T ? __expf(G) : 0.f;
+      sh.E[lane] = lane < T ? __expf((float)G) : 0.f;
       sh.beta[lane] = beta;
       // the rows of the last three inputs before the node's own: nearest ancestors, then the window's
       uint64_t m = above;
@@ -285,14 +289,15 @@ __global__ __launch_bounds__(GT_THREADS, MT < 4 ? 4 : 2) void gdn_tree_kernel(Gt
             gt_row8(qs ? &sh.q[16 * I + c16][32 * s + 8 * g4] : &sh.k[16 * I + c16][32 * s + 8 * g4]),
             gt_row8(&sh.k[16 * J + c16][32 * s + 8 * g4]), acc, 0, 0, 0);
       const int j = 16 * J + c16;
-      const float Gj = sh.G[j], rkj = sh.rk[j];
+      const double Gj = sh.G[j];
+      const float rkj = sh.rk[j];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * I + 4 * g4 + r;
         const uint64_t w = sh.word[i];
         const bool on = ((w >> j) & 1) || (qs && i == j);
         // (of a tree's words G_i <= G_j)
-        const float f = on ? __expf(fminf(sh.G[i] - Gj, 0.f)) * rkj * (qs ? sh.rq[i] : -sh.beta[i] * sh.rk[i]) : 0.f;
+        const float f = on ? __expf(fminf((float)(sh.G[i] - Gj), 0.f)) * rkj * (qs ? sh.rq[i] : -sh.beta[i] * sh.rk[i]) : 0.f;
         (qs ? sh.m.qk : sh.m.am)[i][j] = on ? acc[r] * f : 0.f;
       }
     }
