@@ -724,15 +724,16 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const uint16_t* __rest
     hi = fmaxf(hi, __shfl_xor(hi, o, 32));
   }
   const float s = round_bf16(zero ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.5f);
-  const float inv = s > 0.f ? 1.f / s : 0.f;
-  const float z = zero ? fminf(fmaxf(rintf(-lo * inv), 0.f), 15.f) : 8.f;
+  // (a scale below 2^-128 has no finite reciprocal: it and the values are then taken 2^100 times)
+  const float up = s < 0x1p-100f ? 0x1p100f : 1.f, inv = s > 0.f ? 1.f / (s * up) : 0.f;
+  const float z = zero ? fminf(fmaxf(rintf(-lo * up * inv), 0.f), 15.f) : 8.f;
   if (l == 0) {
     scale[g] = f32_to_bf16(s);
     if (zero) zero[g] = (uint8_t)z;
   }
   // a thread's 1, 2 or 4 codes: bytes of two; with one each, the even lanes write
   uint32_t c = 0;
-  for (int i = 0; i < per; ++i) c |= (uint32_t)fminf(fmaxf(rintf(v[i] * inv) + z, 0.f), 15.f) << (4 * i);
+  for (int i = 0; i < per; ++i) c |= (uint32_t)fminf(fmaxf(rintf(v[i] * up * inv) + z, 0.f), 15.f) << (4 * i);
   uint8_t* d = codes + (g * G + l * per) / 2;
   if (per == 1) {
     const uint32_t o = __shfl_down(c, 1, 32);
