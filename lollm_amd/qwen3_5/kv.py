@@ -199,6 +199,8 @@ class Qwen3_5Cache:
         t = k.shape[2]
         if L + t > self.max_len:
             raise RuntimeError("KV cache capacity exceeded")
+        if t:
+            self.tree_T = 0               # (written over)
         s["k"][:, :, L:L + t] = k
         s["v"][:, :, L:L + t] = v
         return s["k"][:, :, :L + t], s["v"][:, :, :L + t]
@@ -407,6 +409,7 @@ class Qwen3_5PagedCache(Qwen3_5Cache):
             raise RuntimeError("KV cache capacity exceeded")
         if t:
             self.reserve(t)
+            self.tree_T = 0
             page, slot = self._rows(L + t)
             s["k"][page[:, L:], :, slot[L:]] = k.transpose(1, 2).to(torch.bfloat16)
             s["v"][page[:, L:], :, slot[L:]] = v.transpose(1, 2).to(torch.bfloat16)

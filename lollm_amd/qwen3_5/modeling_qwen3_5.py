@@ -152,6 +152,7 @@ class Qwen3_5Model:
         (lollm_verify_input), else they are formed here.  tree: (mask, depth) of ops.tree_masks."""
         B, T = input_ids.shape
         cfg = self.cfg
+        cache.tree_T = 0                  # (an earlier tree's rows and records are written over)
         lengths = cache.lengths
         if inputs is None:
             x = self.model.embed_tokens(input_ids.to(self.device))
