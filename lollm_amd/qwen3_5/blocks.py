@@ -179,8 +179,20 @@ class Projection4:
         return norm(self(x), residual=residual)
 
 
+def check_quantized(projections, group, zeros):
+    """Raise ValueError unless quantized() takes them all: a group that weights have, and what is in 4 bits
+    already in the same form (its bf16 weight is gone)."""
+    if group not in ops.Q4_GROUPS:
+        raise ValueError(f"4-bit weights have groups of {', '.join(map(str, ops.Q4_GROUPS))}, not {group}")
+    for p in projections:
+        if isinstance(p, Projection4) and (p.q4.group, p.q4.zeros) != (group, bool(zeros)):
+            raise ValueError(f"a weight is in 4 bits already, in groups of {p.q4.group} "
+                             f"{'with' if p.q4.zeros else 'without'} zeros")
+
+
 def quantized(p, group=128, zeros=False):
-    """The 4-bit form of a Projection, or `p` itself where the shape has none (or it is 4-bit)."""
+    """The 4-bit form of a Projection, or `p` itself where the shape has none (or it is in this form)."""
+    check_quantized([p], group, zeros)
     if isinstance(p, Projection4) or not ops.q4_supported(p.N, p.K, group, p.epilogue):
         return p
     return Projection4(p.weight, p.epilogue, group, zeros)

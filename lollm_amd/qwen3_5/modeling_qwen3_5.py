@@ -17,7 +17,8 @@ import torch
 import torch.nn.functional as F
 
 from .. import ops
-from .blocks import MLP, GatedAttention, GatedDeltaNet, Projection, RMSNorm, _cus, rope_inv_freq
+from .blocks import (MLP, GatedAttention, GatedDeltaNet, Projection, RMSNorm, _cus, check_quantized,
+                     rope_inv_freq)
 from .config import Qwen3_5Config
 from .kv import Qwen3_5Cache, Qwen3_5PagedCache
 
@@ -40,10 +41,17 @@ class DecoderLayer:
         self.mlp = MLP(W[p + "mlp.gate_proj.weight"], W[p + "mlp.up_proj.weight"],
                        W[p + "mlp.down_proj.weight"])
 
+    @property
+    def mixer(self):
+        return self.self_attn if self.layer_type == "full_attention" else self.linear_attn
+
+    def projections(self):
+        return self.mixer.projections() + self.mlp.projections()
+
     def quantize(self, group=128, zeros=False):
         """The layer's projections in 4 bits (blocks.Projection4)."""
-        mixer = self.self_attn if self.layer_type == "full_attention" else self.linear_attn
-        mixer.quantize(group, zeros)
+        check_quantized(self.projections(), group, zeros)
+        self.mixer.quantize(group, zeros)
         self.mlp.quantize(group, zeros)
 
 
@@ -81,14 +89,15 @@ class Qwen3_5Model:
         """Every weight GEMM of the decoder (for workspace sizing)."""
         out = [self.lm_head]
         for layer in self.model.layers:
-            mixer = layer.self_attn if layer.layer_type == "full_attention" else layer.linear_attn
-            out += mixer.projections() + layer.mlp.projections()
+            out += layer.projections()
         return out
 
     def quantize(self, group=128, zeros=False):
         """The decoder layers' projections rounded to 4 bits with a scale (and with zeros=True a zero) for
         every `group` inputs, 32, 64 or 128 (ops.q4_quantize); their bf16 weights are let go.  The embedding
-        and the lm_head stay bf16.  Before anything is captured in a graph.  Returns the model."""
+        and the lm_head stay bf16, and projections whose shape has no 4-bit form (ops.q4_supported).  Before
+        anything is captured in a graph.  Returns the model."""
+        check_quantized(self.projections(), group, zeros)
         for layer in self.model.layers:
             layer.quantize(group, zeros)
         return self

@@ -27,7 +27,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
-from .blocks import Projection, RMSNorm, quantized
+from .blocks import Projection, RMSNorm, check_quantized, quantized
 from .kv import capturing
 from .modeling_qwen3_5 import DecoderLayer, Qwen3_5Model
 from .random_init import weight_shapes
@@ -45,12 +45,11 @@ class MTP:
         self.layers = [DecoderLayer(cfg, W, "mtp.layers.0.", "full_attention", model.inv_freq)]
         self.norm = RMSNorm(W["mtp.norm.weight"], eps)
         layer = self.layers[0]
-        ops.gemm_workspace(max(p.workspace_bytes() for p in
-                               [self.fc] + layer.self_attn.projections() + layer.mlp.projections()),
-                           model.device)
+        ops.gemm_workspace(max(p.workspace_bytes() for p in [self.fc] + layer.projections()), model.device)
 
     def quantize(self, group=128, zeros=False):
         """fc and the layer's projections in 4 bits, as Qwen3_5Model.quantize.  Returns the head."""
+        check_quantized([self.fc] + self.layers[0].projections(), group, zeros)
         self.fc = quantized(self.fc, group, zeros)
         self.layers[0].quantize(group, zeros)
         return self

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 
+from .blocks import check_quantized
 from .config import build_config
 from .modeling_qwen3_5 import Qwen3_5Model
 from .random_init import weight_shapes
@@ -56,6 +57,8 @@ def load(raw_config: dict, weights: dict, fmt: str, device="cuda", dtype=None,
     inputs (Qwen3_5Model.quantize)."""
     if weight_bits not in (4, 16):
         raise ValueError(f"weights are held in 16 or 4 bits, not {weight_bits}")
+    if weight_bits == 4:
+        check_quantized([], group, False)   # (before anything is loaded)
     cfg = build_config(raw_config, fmt)
     dev = torch.device(device)
     if dev.type != "cuda":

@@ -6,6 +6,9 @@ import pytest
 import torch
 
 from lollm_amd import _lib, ops
+from lollm_amd.qwen3_5 import MTP, Qwen3_5Model, blocks, load
+from lollm_amd.qwen3_5.config import micro_config_dict
+from lollm_amd.qwen3_5.modeling_qwen3_5 import DecoderLayer
 
 
 @pytest.fixture
@@ -44,3 +47,59 @@ def test_gemm_q4_of_few_rows_takes_no_workspace(library):
     ops.gemm_q4(torch.zeros(64, 128, dtype=torch.bfloat16), w)
     (args, _), = library.calls
     assert args[6] is None and args[7] == 0
+
+
+def linear(N=128, K=256):
+    return blocks.Projection(torch.zeros(N, K))
+
+
+def held(group=64, zeros=False, N=128, K=256):
+    p = blocks.Projection4.__new__(blocks.Projection4)
+    p.q4 = ops.Q4Weight(torch.empty(0, dtype=torch.uint8), N, K, group, zeros, ops.GEMM_NONE)
+    p.N, p.K, p.epilogue = N, K, ops.GEMM_NONE
+    return p
+
+
+@pytest.mark.parametrize("group", (0, 16, 48, 100, 256))
+def test_quantized_refuses_groups_that_no_weight_has(group):
+    """(Instead of leaving everything in bf16.)"""
+    with pytest.raises(ValueError, match="32, 64, 128"):
+        blocks.quantized(linear(), group)
+    with pytest.raises(ValueError, match="32, 64, 128"):
+        load(micro_config_dict(), {}, "hf", weight_bits=4, group=group)
+
+
+def test_quantized_refuses_another_group_or_zeros_for_what_is_in_4_bits():
+    p = held(64, False)
+    assert blocks.quantized(p, 64) is p and blocks.quantized(p, 64, zeros=False) is p
+    for group, zeros in ((128, False), (64, True), (32, True)):
+        with pytest.raises(ValueError, match="groups of 64 without zeros"):
+            blocks.quantized(p, group, zeros)
+    odd = linear(100, 256)
+    assert blocks.quantized(odd, 64) is odd        # no 4-bit form: bf16 as it was
+
+
+def test_a_refused_quantize_changes_nothing():
+    """The projections are looked over before the first of them is rounded."""
+    model = Qwen3_5Model.__new__(Qwen3_5Model)
+    model.model = type("Inner", (), {})()
+    layers = []
+    for late in (linear(), held(64)):
+        mlp = blocks.MLP.__new__(blocks.MLP)
+        mlp.gate_up, mlp.down = linear(), late
+        mixer = blocks.GatedDeltaNet.__new__(blocks.GatedDeltaNet)
+        mixer.in_proj, mixer.out_proj = linear(), linear()
+        layer = DecoderLayer.__new__(DecoderLayer)
+        layer.layer_type, layer.linear_attn, layer.mlp = "linear_attention", mixer, mlp
+        layers.append(layer)
+    model.model.layers, model.lm_head = layers, linear()
+    before = model.projections()
+    with pytest.raises(ValueError, match="groups of 64"):
+        model.quantize(128)
+    assert all(a is b for a, b in zip(before, model.projections()))
+    mtp = MTP.__new__(MTP)
+    mtp.fc, mtp.layers = linear(), layers[1:]
+    fc = mtp.fc
+    with pytest.raises(ValueError, match="groups of 64"):
+        mtp.quantize(32)
+    assert mtp.fc is fc
