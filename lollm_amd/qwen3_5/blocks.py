@@ -179,15 +179,18 @@ class Projection4:
         return norm(self(x), residual=residual)
 
 
-def check_quantized(projections, group, zeros):
+def check_quantized(projections, group, zeros, in_graph=False):
     """Raise ValueError unless quantized() takes them all: a group that weights have, and what is in 4 bits
-    already in the same form (its bf16 weight is gone)."""
+    already in the same form (its bf16 weight is gone).  in_graph: their weights may be read by a graph's
+    replays; RuntimeError then, unless there is nothing left to round."""
     if group not in ops.Q4_GROUPS:
         raise ValueError(f"4-bit weights have groups of {', '.join(map(str, ops.Q4_GROUPS))}, not {group}")
     for p in projections:
         if isinstance(p, Projection4) and (p.q4.group, p.q4.zeros) != (group, bool(zeros)):
             raise ValueError(f"a weight is in 4 bits already, in groups of {p.q4.group} "
                              f"{'with' if p.q4.zeros else 'without'} zeros")
+        if in_graph and isinstance(p, Projection) and ops.q4_supported(p.N, p.K, group, p.epilogue):
+            raise RuntimeError("these weights were captured in a graph, whose replays read them: quantize before that")
 
 
 def quantized(p, group=128, zeros=False):

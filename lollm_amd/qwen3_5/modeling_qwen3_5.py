@@ -68,6 +68,8 @@ class _Inner:
 
 
 class Qwen3_5Model:
+    in_graph = False     # a graph has been captured over the layers' weights
+
     def __init__(self, cfg: Qwen3_5Config, W: dict, device="cuda"):
         """W: canonical (`model.*`, `lm_head.weight`) bf16 tensors on the device."""
         self.cfg = cfg
@@ -95,9 +97,10 @@ class Qwen3_5Model:
     def quantize(self, group=128, zeros=False):
         """The decoder layers' projections rounded to 4 bits with a scale (and with zeros=True a zero) for
         every `group` inputs, 32, 64 or 128 (ops.q4_quantize); their bf16 weights are let go.  The embedding
-        and the lm_head stay bf16, and projections whose shape has no 4-bit form (ops.q4_supported).  Before
-        anything is captured in a graph.  Returns the model."""
-        check_quantized(self.projections(), group, zeros)
+        and the lm_head stay bf16, and projections whose shape has no 4-bit form (ops.q4_supported).  Raises
+        RuntimeError once a forward has been captured in a graph, which reads the weights where they were.
+        Returns the model."""
+        check_quantized(self.projections()[1:], group, zeros, self.in_graph)
         for layer in self.model.layers:
             layer.quantize(group, zeros)
         return self
@@ -161,6 +164,7 @@ class Qwen3_5Model:
         (lollm_verify_input), else they are formed here.  tree: (mask, depth) of ops.tree_masks."""
         B, T = input_ids.shape
         cfg = self.cfg
+        self.in_graph = self.in_graph or torch.cuda.is_current_stream_capturing()
         cache.tree_T = 0                  # (an earlier tree's rows and records are written over)
         lengths = cache.lengths
         if inputs is None:

@@ -35,6 +35,8 @@ from .weights import take_weights, to_raw
 
 
 class MTP:
+    in_graph = False     # as the model's
+
     def __init__(self, model: Qwen3_5Model, W: dict):
         cfg = model.cfg
         self.cfg, self.model = cfg, model
@@ -49,7 +51,7 @@ class MTP:
 
     def quantize(self, group=128, zeros=False):
         """fc and the layer's projections in 4 bits, as Qwen3_5Model.quantize.  Returns the head."""
-        check_quantized([self.fc] + self.layers[0].projections(), group, zeros)
+        check_quantized([self.fc] + self.layers[0].projections(), group, zeros, self.in_graph)
         self.fc = quantized(self.fc, group, zeros)
         self.layers[0].quantize(group, zeros)
         return self
@@ -59,6 +61,7 @@ class MTP:
         """Returns (MTP layer output before the final norm, normed output).  The fc input is
         `fc_in`, or from the next tokens' ids `tok` (B,) int32: the lookup, both pre-fc norms
         and the concatenation run as one kernel (lollm_mtp_input)."""
+        self.in_graph = self.in_graph or torch.cuda.is_current_stream_capturing()
         if fc_in is None:
             B = tok.numel()
             fc_in = ops.mtp_input(tok, hidden, self.model.model.embed_tokens.weight,
