@@ -156,7 +156,8 @@ class Projection:
 
 class Projection4:
     """A Projection over a 4-bit weight with group scales (ops.gemm_q4), for any number of rows.
-    The bf16 weight is not kept."""
+    The bf16 weight is not kept.  For inference: where a gradient, a function transform or a trace would
+    have to follow the call, it raises RuntimeError."""
 
     tiled = None        # (none for the callers that take the bf16 GEMM's fused forms)
 
@@ -169,6 +170,12 @@ class Projection4:
         return 0
 
     def __call__(self, x):
+        # (Projection takes F.linear there past 64 rows; no bf16 weight is left for it)
+        if ((x.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0
+                or torch._C._functorch.peek_interpreter_stack() is not None
+                or torch._C._get_tracing_state() is not None or torch.compiler.is_compiling()):
+            raise RuntimeError("a product with a 4-bit weight has no derivative and cannot be traced: call it on x.detach() "
+                               "or under torch.no_grad(), outside function transforms and traces")
         return ops.gemm_q4(x, self.q4)
 
     def add_norm(self, x, residual, norm):

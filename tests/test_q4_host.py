@@ -103,3 +103,26 @@ def test_a_refused_quantize_changes_nothing():
     with pytest.raises(ValueError, match="groups of 64"):
         mtp.quantize(32)
     assert mtp.fc is fc
+
+
+def test_a_product_in_4_bits_refuses_what_would_have_to_follow_it(library):
+    """A gradient that would silently be lost, a function transform, a trace."""
+    p = held(64, False, 64, 128)
+    p.q4.packed = torch.empty(64 * 64 + 64 * 4, dtype=torch.uint8)
+    x = torch.zeros(3, 128, dtype=torch.bfloat16)
+    p(x)
+    leaf = x.clone().requires_grad_()
+    with torch.no_grad():
+        p(leaf)
+    p(leaf.detach())
+    assert len(library.calls) == 3
+
+    def dual():
+        with torch.autograd.forward_ad.dual_level():
+            p(torch.autograd.forward_ad.make_dual(x, x))
+
+    for call in (lambda: p(leaf), dual, lambda: torch.func.vmap(p)(x[None]), lambda: torch.func.jvp(p, (x,), (x,)),
+                 lambda: torch.jit.trace(p.__call__, (x,))):
+        with pytest.raises(RuntimeError, match="4-bit weight"):
+            call()
+    assert len(library.calls) == 3
