@@ -273,6 +273,8 @@ class GatedDeltaNet:
 
     @property
     def w_in(self):
+        if isinstance(self.in_proj, Projection4):
+            raise AttributeError("the in-projection is in 4 bits: its bf16 weight is gone")
         return self.in_proj.weight
 
     def projections(self):

@@ -126,3 +126,12 @@ def test_a_product_in_4_bits_refuses_what_would_have_to_follow_it(library):
         with pytest.raises(RuntimeError, match="4-bit weight"):
             call()
     assert len(library.calls) == 3
+
+
+def test_the_in_projections_weight_is_gone_in_4_bits():
+    mixer = blocks.GatedDeltaNet.__new__(blocks.GatedDeltaNet)
+    mixer.in_proj = linear()
+    assert mixer.w_in is mixer.in_proj.weight
+    mixer.in_proj = held()
+    with pytest.raises(AttributeError, match="in 4 bits"):
+        mixer.w_in
