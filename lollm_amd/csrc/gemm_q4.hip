@@ -242,7 +242,7 @@ __device__ __forceinline__ void q4_finish(const Q4Args& a, const q4_f32x4 (&tot)
 // operands straight to registers, two stages ahead; the waves' sums meet in LDS in a fixed order at the end.
 // All few-row kernels share these sums' order, so that a row's bits do not depend on the number of rows.
 // (Eight stages ahead cost 8% more: the code is longer, and every launch starts with it out of the cache.)
-// 1 x 4096 x 12288 at groups of 64: 10.9 us, 2.3 TB/s; 16 rows 15.4 us, where every workgroup fetches all of x,
+// 1 x 4096 x 12288 at groups of 64: 9.7 us, 2.6 TB/s of codes; 16 rows 15.4 us, where every workgroup fetches all of x,
 // four times the weights in all, from L2.
 template <int GPS, bool ZERO, bool SWIGLU>
 __global__ __launch_bounds__(Q4_THREADS) void gemm_q4_kernel(Q4Args a) {
@@ -283,8 +283,8 @@ __global__ __launch_bounds__(Q4_THREADS) void gemm_q4_kernel(Q4Args a) {
 // At most 16 rows and several column tiles a workgroup: the rows' operands of a few stages stay in
 // registers while the weights of one column tile after the other stream past them, two tiles ahead.
 // (Fetched again for every tile, as above, they and their sums cost more than the weights.)
-// 1 x 24576 x 4096 with SwiGLU and zeros, groups of 128: 15.9 us, 3.2 TB/s; 16 rows 17.4 us; 1 x 151936 x 4096
-// 77 us, 4.0 TB/s.
+// 1 x 24576 x 4096 with SwiGLU and zeros, groups of 128: 15.5 us, 3.3 TB/s; 16 rows 18 us; 1 x 151936 x 4096
+// 78 us, 4.0 TB/s.
 template <int NT, int GPS, bool ZERO, bool SWIGLU>
 __global__ __launch_bounds__(Q4_THREADS) void gemm_q4_wide_kernel(Q4Args a) {
   constexpr int KPG = 4 / GPS, HELD = GPS == 4 ? 2 : 4;   // (stages held)
@@ -393,6 +393,7 @@ __global__ __launch_bounds__(Q4_THREADS) void gemm_q4_wide_kernel(Q4Args a) {
 // products, so the next stage's rows are on their way into the same buffer meanwhile.
 // 61 x 12352 x 4096 with zeros, groups of 128: 19 us, 1.3 TB/s, 316 TF: bound by the rows' way from L2 to LDS,
 // once for each 64 columns (without it two thirds of the time remain), and by products behind their decoding.
+// Four column tiles of 64 rows with zeros spill 6 registers (2.4 MB written for these 61 rows).
 typedef __attribute__((address_space(3))) void q4_lds_t;
 
 template <int MT, int NT, int P, int GPS, bool ZERO, bool SWIGLU>
@@ -477,6 +478,7 @@ __global__ __launch_bounds__(Q4_THREADS) void gemm_q4_lds_kernel(Q4Args a) {
 // beside 64 products of 16 cycles.
 // 1999 x 18432 x 4096, groups of 128: 300 to 316 us by the card, 955 to 1000 TF (64: 379, 32: 454), 63% of what a bf16 product of 8192^3
 // reaches here.  The decoding is what is left: it and the products of two waves share a SIMD's issue.
+// (Groups of 64 spill 5 or 6 registers.)
 constexpr int QR_BM = 128, QR_BN = 256;
 constexpr int QR_CODES = QR_BM * 256, QR_SCALES = QR_CODES + QR_BN * 64;   // a slot: rows, codes, scales
 
@@ -795,9 +797,12 @@ static void q4_rows(const Q4Args& a, hipStream_t st) {
 }
 
 // Whether the 128 x 256 tiles are the faster ones: their rounds of the chip at 1.8 us a stage against those
-// of 64 x 64 tiles at 0.4 us a stage (eight waves share them) and 3 us each.  us, large / small tiles: 129 x
-// 4096 x 4096 59 / 17, 512 x 4096 x 4096 63 / 33, 512 x 18432 x 4096 125 / 148, 1000 x 4096 x 12288 177 / 154,
-// 1000 x 24576 x 4096 212 / 392.
+// of 64 x 64 tiles at 0.4 us a stage (eight waves share them) and 3 us each, the costs of groups of 128.  Smaller
+// groups raise both alike, so one rule serves all (us, large / small tiles, at groups of 128; 64; 32: 129 x 4096 x
+// 4096 59 / 17; 72 / 22; 88 / 25, 512 x 4096 x 4096 59 / 31; 75 / 45; 91 / 51, 700 x 4096 x 8192 114 / 80; 144 / 114;
+// 179 / 133, 1000 x 4096 x 12288 167 / 156; 215 / 223; 271 / 258; but 300 x 12352 x 4096 60 / 64; 76 / 87; 92 / 100,
+// 512 x 18432 x 4096 120 / 140; 151 / 193; 181 / 225, 1000 x 24576 x 4096 189 / 365; 234 / 503; 281 / 585.  With
+// zeros 1000 x 4096 x 12288 170 / 174 and 278 / 272 at 128 and 32: where the rule errs it is a tie).
 static bool q4_many_rows(int M, int N, int K, int cus) {
   if (M <= 64) return false;
   const long long large = (long long)((M + QR_BM - 1) / QR_BM) * ((N + QR_BN - 1) / QR_BN);
