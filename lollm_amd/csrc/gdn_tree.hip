@@ -11,15 +11,16 @@
 // The left side is a unit lower triangular matrix (a parent comes before its node): 16 x 16
 // blocks on its diagonal are inverted by the recurrence, the rest is block substitution in fp32 MFMA.
 // The products with S0 are bf16 MFMAs of the rows (bf16 as they are: q, k and v are bf16 tensors, which
-// the records hold) with S0 as hi + lo bf16, 16 bits of it (2^-17 of a term, the output keeps 2^-9); all sums
-// are fp32, those of the decays 64 bits, as their differences count.
+// the records hold) with S0 as three bf16 parts, all of its bits: queries that cancel most of a state, and a norm
+// behind them that scales the rest up, leave none to spare (with two parts outputs were off by 2^-17 of the terms).
+// All sums are fp32, those of the decays 64 bits, as their differences count.
 //
 // One workgroup of eight waves per (sequence, v-head).  Wave w owns value columns 16 w ..: its part of S0
 // lies in registers in the order in which the MFMA takes it as operand (lane 16 g + c: rows 32 s + 8 g
 // + e, column 16 w + c), the triangular solve and the outputs of its columns never leave its
 // accumulators, which hold rows in the order that the next product contracts over.
 //
-// Measured: 8 x 63 nodes, 32 v-heads 28 us, 16 x 16 25 us, 1 x 7 with 16 heads 11 us; the bytes (states in and
+// Measured: 8 x 63 nodes, 32 v-heads 30 us, 16 x 16 26 us, 1 x 7 with 16 heads 11 us; the bytes (states in and
 // out, rows, records) take 12.5, 16 and 0.5 at a large copy's rate.  With one workgroup a CU (63 nodes: 108 KB of
 // LDS) its phases follow each other: of 50,000 cycles 13,000 each are the loads' way and the last products
 // (fp32 MFMAs of a 64 x 64 triangle, a chain), 7,700 the convolution (exponentials), 5,500 the two matrices.
@@ -344,13 +345,15 @@ __global__ __launch_bounds__(GT_THREADS, MT < 4 ? 4 : 2) void gdn_tree_kernel(Gt
 #pragma unroll
       for (int e = 0; e < 8; ++e) __builtin_nontemporal_store(S[s][e], so + (32 * s + 8 * g4 + e) * GL_DK + col);
   }
-  gt_bf16x8 Sh_[4], Sl[4];
+  gt_bf16x8 S3[3][4];   // (each the rest of what is before it: together all of S0's 24 bits)
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      Sh_[s][e] = (__bf16)S[s][e];
-      Sl[s][e] = (__bf16)(S[s][e] - (float)(__bf16)S[s][e]);
+      S3[0][s][e] = (__bf16)S[s][e];
+      const float rest = S[s][e] - (float)S3[0][s][e];
+      S3[1][s][e] = (__bf16)rest;
+      S3[2][s][e] = (__bf16)(rest - (float)S3[1][s][e]);
     }
   // ---- 7. u and o, block row by block row; the gate's z on its way ----
   lds_only_barrier();   // the inverses
@@ -366,16 +369,17 @@ __global__ __launch_bounds__(GT_THREADS, MT < 4 ? 4 : 2) void gdn_tree_kernel(Gt
   gt_f32x4 U[MT], O[MT];   // (U: the right sides until solved)
 #pragma unroll
   for (int I = 0; I < MT; ++I) {
-    gt_f32x4 ks[2], qs[2];   // with the state's high and low parts
+    gt_f32x4 ks[2], qs[2];   // with the state's first part, with the others
 #pragma unroll
     for (int t = 0; t < 2; ++t) ks[t] = qs[t] = gt_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const gt_bf16x8 kr = gt_row8(&sh.k[16 * I + c16][32 * s + 8 * g4]), qr = gt_row8(&sh.q[16 * I + c16][32 * s + 8 * g4]);
-      ks[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, Sh_[s], ks[0], 0, 0, 0);
-      qs[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, Sh_[s], qs[0], 0, 0, 0);
-      ks[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, Sl[s], ks[1], 0, 0, 0);
-      qs[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, Sl[s], qs[1], 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        ks[t > 0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, S3[t][s], ks[t > 0], 0, 0, 0);
+        qs[t > 0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr, S3[t][s], qs[t > 0], 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
